@@ -26,7 +26,8 @@ SCALARS = {"uint32_t": "u32", "uint64_t": "u64", "int": "c_int", "float": "f32",
 POINTEE = {"void": "c_void", "float": "f32", "uint16_t": "u16", "uint32_t": "u32", "uint64_t": "u64",
            "char": "c_char", "int64_t": "i64", "double": "f64", "uint8_t": "u8"}
 OPAQUE = {"rt_ctx": "RtCtx", "rt_event": "RtEvent", "rt_graph": "RtGraph", "rt_gguf": "RtGguf",
-          "rt_step": "RtStep", "rt_step_model": "RtStepModel", "rt_step_layer": "RtStepLayer"}
+          "rt_step": "RtStep", "rt_step_model": "RtStepModel", "rt_step_layer": "RtStepLayer",
+          "rt_paged_batch": "RtPagedBatch"}
 MANUAL_PREFIXES = ("rt_ctx_", "rt_flush", "rt_last_error", "rt_global_last_error", "rt_malloc",
                    "rt_free", "rt_upload", "rt_download", "rt_memset", "rt_copy_d2d", "rt_event_",
                    "rt_capture_", "rt_graph_", "rt_gguf_", "rt_decode_step_", "rt_has_kernel",
@@ -109,6 +110,15 @@ def ffi_rs(funcs) -> str:
            "    pub layer: *const RtStepLayer,",
            "    pub token_embd: *const c_void, pub lm_head: *const c_void,",
            "    pub output_norm: *const f32, pub token: *mut u32, pub logits: *mut f32,",
+           "}",
+           "/// rt_paged_batch (include/runit_hip.h)",
+           "#[repr(C)] #[derive(Clone, Copy)]",
+           "pub struct RtPagedBatch {",
+           "    pub k_pages: *mut c_void, pub v_pages: *mut c_void,",
+           "    pub f16: u32, pub num_pages: u32, pub page_size: u32, pub num_kv_heads: u32,",
+           "    pub head_dim: u32, pub table_stride: u32, pub n_seqs: u32, pub rows: u32,",
+           "    pub page_stride: u64,",
+           "    pub table: *const u32, pub row_start: *const u32, pub kv_len: *const u32,",
            "}", "", "extern \"C\" {"]
     for ret, name, params in funcs:
         args = ", ".join(f"{ident(n)}: {rust_type(c, b, s)}" for c, b, s, n in params)
@@ -144,6 +154,9 @@ def dispatch_rs(funcs) -> str:
                 sig.append(f"{ident(pn)}: &Buffer")
                 cast = rust_type(c, b, 1)
                 call.append(f"{ident(pn)}.as_ptr() as {cast}")
+            elif s == 1 and b == "rt_paged_batch":
+                sig.append(f"{ident(pn)}: &ffi::RtPagedBatch")
+                call.append(ident(pn))
             elif s == 0 and b in SCALARS:
                 sig.append(f"{ident(pn)}: {SCALARS[b]}")
                 call.append(ident(pn))

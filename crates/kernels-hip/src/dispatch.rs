@@ -449,6 +449,21 @@ pub fn silu_mul_f32(ctx: &HipContext, gate: &Buffer, up: &Buffer, out: &Buffer, 
 pub fn argmax_rows_first_f32(ctx: &HipContext, in_: &Buffer, result: &Buffer, rows: u32, n: u32) -> Result<()> {
     status(ctx.raw(), unsafe { ffi::rt_argmax_rows_first_f32(ctx.raw(), in_.as_ptr() as *const f32, result.as_ptr() as *mut u32, rows, n) })
 }
+pub fn rope_kv_append_paged_f32(ctx: &HipContext, batch: &ffi::RtPagedBatch, q: &Buffer, k: &Buffer, v: &Buffer, q_out: &Buffer, num_heads: u32, theta: f32) -> Result<()> {
+    status(ctx.raw(), unsafe { ffi::rt_rope_kv_append_paged_f32(ctx.raw(), batch, q.as_ptr() as *const f32, k.as_ptr() as *const f32, v.as_ptr() as *const f32, q_out.as_ptr() as *mut f32, num_heads, theta) })
+}
+pub fn paged_attention_f32(ctx: &HipContext, batch: &ffi::RtPagedBatch, q: &Buffer, out: &Buffer, num_heads: u32) -> Result<()> {
+    status(ctx.raw(), unsafe { ffi::rt_paged_attention_f32(ctx.raw(), batch, q.as_ptr() as *const f32, out.as_ptr() as *mut f32, num_heads) })
+}
+pub fn shared_prefix_attention_f32(ctx: &HipContext, batch: &ffi::RtPagedBatch, q: &Buffer, out: &Buffer, num_heads: u32, shared_table: &Buffer, shared_len: u32) -> Result<()> {
+    status(ctx.raw(), unsafe { ffi::rt_shared_prefix_attention_f32(ctx.raw(), batch, q.as_ptr() as *const f32, out.as_ptr() as *mut f32, num_heads, shared_table.as_ptr() as *const u32, shared_len) })
+}
+pub fn token_logprobs_f32(ctx: &HipContext, logits: &Buffer, tokens: &Buffer, rows: u32, n: u32, row_stride: u64, logprob: &Buffer, entropy: &Buffer, rank: &Buffer, top: u32, top_ids: &Buffer, top_logprobs: &Buffer) -> Result<()> {
+    status(ctx.raw(), unsafe { ffi::rt_token_logprobs_f32(ctx.raw(), logits.as_ptr() as *const f32, tokens.as_ptr() as *const u32, rows, n, row_stride, logprob.as_ptr() as *mut f32, entropy.as_ptr() as *mut f32, rank.as_ptr() as *mut u32, top, top_ids.as_ptr() as *mut u32, top_logprobs.as_ptr() as *mut f32) })
+}
+pub fn token_logprobs_f16(ctx: &HipContext, logits: &Buffer, tokens: &Buffer, rows: u32, n: u32, row_stride: u64, logprob: &Buffer, entropy: &Buffer, rank: &Buffer, top: u32, top_ids: &Buffer, top_logprobs: &Buffer) -> Result<()> {
+    status(ctx.raw(), unsafe { ffi::rt_token_logprobs_f16(ctx.raw(), logits.as_ptr() as *const u16, tokens.as_ptr() as *const u32, rows, n, row_stride, logprob.as_ptr() as *mut f32, entropy.as_ptr() as *mut f32, rank.as_ptr() as *mut u32, top, top_ids.as_ptr() as *mut u32, top_logprobs.as_ptr() as *mut f32) })
+}
 pub fn embed_q8_0_f32(ctx: &HipContext, table: &Buffer, token: &Buffer, out: &Buffer, k: u32) -> Result<()> {
     status(ctx.raw(), unsafe { ffi::rt_embed_q8_0_f32(ctx.raw(), table.as_ptr() as *const c_void, token.as_ptr() as *const u32, out.as_ptr() as *mut f32, k) })
 }

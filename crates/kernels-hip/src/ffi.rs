@@ -28,6 +28,15 @@ pub struct RtStepModel {
     pub token_embd: *const c_void, pub lm_head: *const c_void,
     pub output_norm: *const f32, pub token: *mut u32, pub logits: *mut f32,
 }
+/// rt_paged_batch (include/runit_hip.h)
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct RtPagedBatch {
+    pub k_pages: *mut c_void, pub v_pages: *mut c_void,
+    pub f16: u32, pub num_pages: u32, pub page_size: u32, pub num_kv_heads: u32,
+    pub head_dim: u32, pub table_stride: u32, pub n_seqs: u32, pub rows: u32,
+    pub page_stride: u64,
+    pub table: *const u32, pub row_start: *const u32, pub kv_len: *const u32,
+}
 
 extern "C" {
     pub fn rt_ctx_create(out: *mut *mut RtCtx, code_object_path: *const c_char) -> c_int;
@@ -202,6 +211,11 @@ extern "C" {
     pub fn rt_add_f32(ctx: *mut RtCtx, a: *const f32, b: *const f32, out: *mut f32, n: u32) -> c_int;
     pub fn rt_silu_mul_f32(ctx: *mut RtCtx, gate: *const f32, up: *const f32, out: *mut f32, n: u32) -> c_int;
     pub fn rt_argmax_rows_first_f32(ctx: *mut RtCtx, in_: *const f32, result: *mut u32, rows: u32, n: u32) -> c_int;
+    pub fn rt_rope_kv_append_paged_f32(ctx: *mut RtCtx, batch: *const RtPagedBatch, q: *const f32, k: *const f32, v: *const f32, q_out: *mut f32, num_heads: u32, theta: f32) -> c_int;
+    pub fn rt_paged_attention_f32(ctx: *mut RtCtx, batch: *const RtPagedBatch, q: *const f32, out: *mut f32, num_heads: u32) -> c_int;
+    pub fn rt_shared_prefix_attention_f32(ctx: *mut RtCtx, batch: *const RtPagedBatch, q: *const f32, out: *mut f32, num_heads: u32, shared_table: *const u32, shared_len: u32) -> c_int;
+    pub fn rt_token_logprobs_f32(ctx: *mut RtCtx, logits: *const f32, tokens: *const u32, rows: u32, n: u32, row_stride: u64, logprob: *mut f32, entropy: *mut f32, rank: *mut u32, top: u32, top_ids: *mut u32, top_logprobs: *mut f32) -> c_int;
+    pub fn rt_token_logprobs_f16(ctx: *mut RtCtx, logits: *const u16, tokens: *const u32, rows: u32, n: u32, row_stride: u64, logprob: *mut f32, entropy: *mut f32, rank: *mut u32, top: u32, top_ids: *mut u32, top_logprobs: *mut f32) -> c_int;
     pub fn rt_embed_q8_0_f32(ctx: *mut RtCtx, table: *const c_void, token: *const u32, out: *mut f32, k: u32) -> c_int;
     pub fn rt_embed_q4_0_f32(ctx: *mut RtCtx, table: *const c_void, token: *const u32, out: *mut f32, k: u32) -> c_int;
     pub fn rt_embed_q4k_f32(ctx: *mut RtCtx, table: *const c_void, token: *const u32, out: *mut f32, k: u32) -> c_int;

@@ -716,6 +716,75 @@ int rt_silu_mul_f32(rt_ctx* ctx, const float* gate, const float* up, float* out,
 int rt_argmax_rows_first_f32(rt_ctx* ctx, const float* in, uint32_t* result, uint32_t rows,
                              uint32_t n);
 
+/* ─────────────── batches over a paged cache (new) ───────────────
+ * No counterpart in the reference, whose KvCache holds one sequence
+ * (kv_cache.rs).  A pool of pages holds the keys and the values of many
+ * sequences; page p starts at element p·page_stride and holds
+ * [num_kv_heads][page_size][head_dim], the layout of a cache of page_size
+ * positions.  Position j of sequence s is in page table[s·table_stride +
+ * j / page_size]; an id ≥ num_pages (~0u) is no page: its positions are neither
+ * stored nor seen.  Sequence s brings the rows row_start[s] ..
+ * row_start[s + 1] − 1 of the batch's activations (row_start[0] = 0, in
+ * order; any number, none too), its last positions: with n rows, row i of it
+ * is at position kv_len[s] − n + i, so kv_len counts them.  table, row_start
+ * and kv_len are device arrays, read by the kernels: a captured graph follows
+ * them.  Rows behind the last sequence's are left as they are, here and in the
+ * outputs.  Positions from table_stride·page_size on are neither stored nor
+ * seen, nor are rows at positions below 0 (kv_len[s] < n). */
+typedef struct {
+    void *k_pages, *v_pages;     /* device, 16-byte aligned */
+    uint32_t f16;                /* elements of a page: 0 f32, 1 f16 */
+    uint32_t num_pages, page_size;    /* page_size: a power of two, 16 or more */
+    uint32_t num_kv_heads, head_dim;  /* head_dim 64, 128 or 256 */
+    uint32_t table_stride, n_seqs;
+    uint32_t rows;               /* rows of the activations (at least row_start[n_seqs]) */
+    uint64_t page_stride;        /* elements, a multiple of 8; 0: pages one after another */
+    const uint32_t* table;       /* device [n_seqs][table_stride] */
+    const uint32_t* row_start;   /* device [n_seqs + 1]; NULL: one row a sequence */
+    const uint32_t* kv_len;      /* device [n_seqs] */
+} rt_paged_batch;
+/* RoPE of q [rows][num_heads][head_dim] into q_out (may alias q) and of k
+ * [rows][num_kv_heads][head_dim] at the rows' positions (pairs (d, d +
+ * head_dim/2), the angles reduced in 64 bits), k and v (as k) stored into the
+ * pages (f16: rounded to nearest even).  Rows that several sequences store in one place
+ * leave either's elements there: a shared page is copied before it is written. */
+int rt_rope_kv_append_paged_f32(rt_ctx* ctx, const rt_paged_batch* batch, const float* q,
+                                const float* k, const float* v, float* q_out, uint32_t num_heads,
+                                float theta);
+/* Causal attention of the batch's rows, q and out [rows][num_heads][head_dim],
+ * scale 1/sqrt(head_dim), f32 sums: a row at position p sees the positions ≤ p
+ * of its sequence.  A row that sees none gives zeros.  What is behind a
+ * sequence's length in its pages, and what a row does not see, may hold
+ * anything.  Workspace as rt_flash_attention_f32's: sized by the first call of
+ * a size, before it is captured. */
+int rt_paged_attention_f32(rt_ctx* ctx, const rt_paged_batch* batch, const float* q, float* out,
+                           uint32_t num_heads);
+/* rt_paged_attention_f32 where the first shared_len positions of every
+ * sequence are the same: they are read through shared_table (device,
+ * ceil(shared_len / page_size) page ids), once for all rows of the batch, and
+ * the sequences' own tables from position shared_len on.  kv_len counts them. */
+int rt_shared_prefix_attention_f32(rt_ctx* ctx, const rt_paged_batch* batch, const float* q,
+                                   float* out, uint32_t num_heads, const uint32_t* shared_table,
+                                   uint32_t shared_len);
+/* Log probabilities of given tokens (new; the reference samples on the CPU and
+ * reports none).  logits [rows] of n values, row r at logits + r·row_stride;
+ * tokens [rows]:
+ *   logprob[r] = x_t − ln Σ e^x     (−inf for a token id ≥ n)
+ *   entropy[r] = −Σ p·ln p          (nats; may be NULL)
+ *   rank[r]    = logits above x_t   (may be NULL)
+ *   top_ids, top_logprobs [rows][top]: the `top` (0 .. 64, ≤ n) most probable
+ *                tokens in order, equal ones by id (NULL at top 0).
+ * A logit of −inf has probability 0.  A row with a NaN or +inf, or of −inf
+ * alone, has no distribution: NaN for all but ids and rank; NaN ranks as −inf
+ * there.  Workspace: as above. */
+int rt_token_logprobs_f32(rt_ctx* ctx, const float* logits, const uint32_t* tokens, uint32_t rows,
+                          uint32_t n, uint64_t row_stride, float* logprob, float* entropy,
+                          uint32_t* rank, uint32_t top, uint32_t* top_ids, float* top_logprobs);
+int rt_token_logprobs_f16(rt_ctx* ctx, const uint16_t* logits, const uint32_t* tokens,
+                          uint32_t rows, uint32_t n, uint64_t row_stride, float* logprob,
+                          float* entropy, uint32_t* rank, uint32_t top, uint32_t* top_ids,
+                          float* top_logprobs);
+
 /* New: out = dequant(table row *token) for a [vocab, k] table in the named
  * block format (reference or ggml layout, or plain f16 / f32 rows, as
  * token_embd.weight is stored); the token id is read from device memory

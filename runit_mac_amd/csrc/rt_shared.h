@@ -45,3 +45,60 @@ constexpr uint32_t RT_STEP_MAX_WGS = 1024;
 #define RT_STEP_THREADS 512
 constexpr uint32_t RT_STEP_SYNC_BYTES = 2048;  // StepSync (k_step.hip)
 constexpr uint32_t RT_STEP_STATUS_OFF = 1280;  // its status word
+
+// Attention over paged caches (k_paged.hip): the rows of a block, the positions
+// of a tile (page sizes are multiples of it), the waves of a workgroup.
+constexpr uint32_t RT_PAGED_ROWS = 16;
+constexpr uint32_t RT_PAGED_TILE = 16;
+constexpr uint32_t RT_PAGED_WAVES = 4;
+
+// One batch over a paged cache, as rt_paged_batch describes it.
+struct PagedBatch {
+    void* k;                    // page p at p·page_stride elements: [KVH][page size][head size]
+    void* v;
+    const uint32_t* table;      // [n_seqs][table_stride] page ids
+    const uint32_t* row_start;  // [n_seqs + 1], or null: one row a sequence
+    const uint32_t* kv_len;     // [n_seqs]
+    uint64_t page_stride;
+    uint32_t num_pages, ps_shift, table_stride, n_seqs, rows, KVH;
+};
+struct PagedAppendArgs {
+    PagedBatch b;
+    const float* q;  // [rows][H][head size]
+    const float* k;  // [rows][KVH][head size]
+    const float* v;
+    float* q_out;
+    double log2_theta;
+    uint32_t H;
+};
+struct PagedAttnArgs {
+    PagedBatch b;
+    const float* q;  // [rows][H][head size]
+    float* out;
+    const uint32_t* shared_table;  // positions below shared_len are read through it
+    float* part;     // [jobs][KVH][RT_PAGED_ROWS][head size] unnormalised outputs
+    float* ml;       // [jobs][KVH][RT_PAGED_ROWS][max, sum]
+    uint32_t* info;  // [rows][H][2 parts][first job, chunks · 16 + row of its block]
+    uint32_t H, shared_len;
+    uint32_t jobs;    // jobs of a KV head (at most)
+    uint32_t target;  // its chunks beyond one a block (at most; 0: blocks are not split)
+    uint32_t min_chunk;  // tiles of a chunk (at least)
+    float scale;
+};
+
+// Token log probabilities (k_logprobs.hip).
+constexpr uint32_t RT_LOGPROBS_TOP_MAX = 64;   // alternatives (at most): one a lane
+constexpr uint32_t RT_LOGPROBS_SEG_MAX = 64;   // segments of a row (at most): one a lane of the merge
+struct LogprobsArgs {
+    const void* x;  // [rows][row_stride]
+    const uint32_t* tokens;
+    float* logprob;
+    float* entropy;   // or null
+    uint32_t* rank;   // or null
+    uint32_t* top_ids;
+    float* top_logprobs;
+    float* part;      // segs > 1: [rows][segs][4]: max, Σe, Σe·(max − x), rank
+    uint64_t* keys;   //           [rows][segs][top]: the largest, in order
+    uint64_t row_stride;
+    uint32_t n, top, segs, seg_len;
+};

@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <string>
@@ -182,6 +183,13 @@ const char* const kKernelNames[] = {
     "k_gemm3_q6kg_mg4", "k_gemm3_q6k_mg1_w8", "k_gemm3_q6kg_mg1_w8", "k_gemm3_q6k_mg2_w8", "k_gemm3_q6k_mg4_w8", "k_gemm3_q6kg_mg2_w8",
     "k_gemm3_q6kg_mg4_w8",
     "k_gemm_xh_prep_mg1", "k_gemm_xh_prep_mg2", "k_gemm_xh_prep_mg4",
+    "k_paged_append_f32_hd64", "k_paged_append_f32_hd128", "k_paged_append_f32_hd256",
+    "k_paged_append_f16_hd64", "k_paged_append_f16_hd128", "k_paged_append_f16_hd256",
+    "k_paged_attn_f32_hd64", "k_paged_attn_f32_hd128", "k_paged_attn_f32_hd256",
+    "k_paged_attn_f16_hd64", "k_paged_attn_f16_hd128", "k_paged_attn_f16_hd256",
+    "k_paged_merge_hd64", "k_paged_merge_hd128", "k_paged_merge_hd256",
+    "k_logprobs_f32", "k_logprobs_f16", "k_logprobs_top_f32", "k_logprobs_top_f16",
+    "k_logprobs_merge_f32", "k_logprobs_merge_f16",
 };
 
 // Kernels of the LDS-streamed GEMV body: <base>_ls<NI>, NI = 1..3 global→LDS
@@ -4132,6 +4140,190 @@ int rt_flash_attention_f32(rt_ctx* c, const float* q, const float* k, const floa
     if (mq != kLsDecline) return mq;
     snprintf(kn, sizeof kn, "k_decode_attention_f32_hd%u", head_dim);
     return attn_launch(c, kn, a, (uint32_t)rows);
+}
+
+// ───────────────────────── batches over a paged cache ─────────────────────────
+
+static int paged_check(rt_ctx* c, const rt_paged_batch* b, uint32_t num_heads, const char* who, PagedBatch& d) {
+    if (!b) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: null batch", who);
+    const int st = attn_check(c, num_heads, b->num_kv_heads, b->head_dim);
+    if (st != RT_OK) return st;
+    if (num_heads == 0) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: num_heads=0", who);
+    if (b->f16 > 1)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: f16=%u is neither 0 nor 1", who, b->f16);
+    if (b->page_size < RT_PAGED_TILE || (b->page_size & (b->page_size - 1)))
+        return fail(c, RT_ERR_DISPATCH,
+                    "kernel dispatch error: %s: page_size=%u must be a power of two, %u or more", who,
+                    b->page_size, RT_PAGED_TILE);
+    if (b->num_pages == 0 || b->num_pages > 0x7fffffffu)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: num_pages=%u", who, b->num_pages);
+    const uint64_t page = (uint64_t)b->num_kv_heads * b->page_size * b->head_dim;
+    const uint64_t stride = b->page_stride ? b->page_stride : page;
+    if (stride < page || stride % 8)
+        return fail(c, RT_ERR_DISPATCH,
+                    "kernel dispatch error: %s: page_stride=%llu must be a multiple of 8, at least %llu", who,
+                    (unsigned long long)stride, (unsigned long long)page);
+    if (stride > (1ull << 60) / b->num_pages)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: the pool exceeds the address space", who);
+    if ((uint64_t)b->table_stride * b->page_size > 0x10000000u)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: %u pages of %u positions exceed 2^28", who,
+                    b->table_stride, b->page_size);
+    if ((uint64_t)b->rows * num_heads > 0x1000000u || b->n_seqs > 0x100000u)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: rows=%u of %u heads, %u sequences are too many",
+                    who, b->rows, num_heads, b->n_seqs);
+    if (b->n_seqs && b->rows &&
+        (!b->k_pages || !b->v_pages || !b->kv_len || (!b->table && b->table_stride)))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: null buffer", who);
+    if (!aligned(b->k_pages, 16) || !aligned(b->v_pages, 16))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: pages must be 16-byte aligned", who);
+    if (!b->row_start && b->rows < b->n_seqs)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: %u rows for %u sequences of one", who,
+                    b->rows, b->n_seqs);
+    d = PagedBatch{b->k_pages, b->v_pages, b->table, b->row_start, b->kv_len, stride, b->num_pages,
+                   (uint32_t)__builtin_ctz(b->page_size), b->table_stride, b->n_seqs, b->rows, b->num_kv_heads};
+    return RT_OK;
+}
+
+int rt_rope_kv_append_paged_f32(rt_ctx* c, const rt_paged_batch* batch, const float* q, const float* k,
+                                const float* v, float* q_out, uint32_t num_heads, float theta) {
+    if (!c) return fail(nullptr, RT_ERR_DISPATCH, "kernel dispatch error: null context");
+    PagedAppendArgs a{};
+    const int st = paged_check(c, batch, num_heads, "rope_kv_append_paged", a.b);
+    if (st != RT_OK) return st;
+    if (a.b.n_seqs == 0 || a.b.rows == 0) return RT_OK;
+    if (!q || !k || !v || !q_out)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: rope_kv_append_paged: null buffer");
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(q_out, 16))
+        return fail(c, RT_ERR_DISPATCH,
+                    "kernel dispatch error: rope_kv_append_paged: activations must be 16-byte aligned");
+    if (!(theta > 0.0f) || theta > 3.4e38f)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: rope_kv_append_paged: theta=%g must be positive",
+                    theta);
+    a.q = q, a.k = k, a.v = v, a.q_out = q_out;
+    a.log2_theta = log2((double)theta);
+    a.H = num_heads;
+    char name[48];
+    snprintf(name, sizeof name, "k_paged_append_%s_hd%u", batch->f16 ? "f16" : "f32", batch->head_dim);
+    const uint32_t rows = a.b.row_start ? a.b.rows : a.b.n_seqs;
+    const uint32_t per = 2048 / batch->head_dim;  // heads of a pass
+    const uint32_t passes = (num_heads + 2 * a.b.KVH + per - 1) / per;
+    void* params[] = {&a};
+    return launch(c, name, dim3(rows, passes), dim3(256), 0, params);
+}
+
+static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* q, float* out, uint32_t num_heads,
+                           const uint32_t* shared_table, uint32_t shared_len, const char* who) {
+    if (!c) return fail(nullptr, RT_ERR_DISPATCH, "kernel dispatch error: null context");
+    PagedAttnArgs a{};
+    int st = paged_check(c, batch, num_heads, who, a.b);
+    if (st != RT_OK) return st;
+    if (shared_len > (uint64_t)a.b.table_stride * batch->page_size)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: shared_len=%u exceeds the tables' %llu positions",
+                    who, shared_len, (unsigned long long)a.b.table_stride * batch->page_size);
+    if (a.b.n_seqs == 0 || a.b.rows == 0) return RT_OK;
+    if (!q || !out || (shared_len && !shared_table))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: null buffer", who);
+    if (!aligned(q, 16) || !aligned(out, 16))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: activations must be 16-byte aligned", who);
+    if (q == out) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: out must not alias q", who);
+    const uint32_t hd = batch->head_dim, G = num_heads / a.b.KVH;
+    const uint32_t rows = a.b.row_start ? a.b.rows : a.b.n_seqs;
+    a.q = q, a.out = out, a.shared_table = shared_table, a.shared_len = shared_len, a.H = num_heads;
+    a.scale = 1.0f / std::sqrt((float)hd);
+    a.min_chunk = 8;
+    // blocks of a KV head (at most), and the chunks that its share of two
+    // workgroups a CU leaves beyond one a block
+    const uint64_t cols = (uint64_t)rows * G, R = RT_PAGED_ROWS;
+    uint64_t blocks = a.b.row_start ? cols / R + a.b.n_seqs : (uint64_t)a.b.n_seqs * ((G + R - 1) / R);
+    if (shared_len) blocks += (cols + R - 1) / R;
+    const uint64_t slots = std::max<uint64_t>(1, 2 * (uint64_t)c->cu_count / a.b.KVH);
+    if ((blocks + slots) * a.b.KVH > 0xffffffu)  // (2^32 threads a launch)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: too many rows (%u of %u heads)", who, rows,
+                    num_heads);
+    a.target = (uint32_t)(blocks >= 8 * slots ? 0 : blocks < slots / 2 ? slots - blocks : slots);
+    a.jobs = (uint32_t)(blocks + a.target);
+    const size_t nslot = (size_t)a.jobs * a.b.KVH * R;
+    const bool merge = shared_len || a.target;
+    if (merge) {
+        const size_t pb = nslot * hd * 4, mb = nslot * 8, ib = (size_t)rows * num_heads * 16;
+        st = ensure_ws(c, pb + mb + ib, who);
+        if (st != RT_OK) return st;
+        a.part = (float*)c->ws;
+        a.ml = (float*)((char*)c->ws + pb);
+        a.info = (uint32_t*)((char*)c->ws + pb + mb);
+    }
+    char name[48];
+    snprintf(name, sizeof name, "k_paged_attn_%s_hd%u", batch->f16 ? "f16" : "f32", hd);
+    void* params[] = {&a};
+    st = launch(c, name, dim3(a.jobs * a.b.KVH), dim3(64 * RT_PAGED_WAVES), 0, params);
+    if (st != RT_OK || !merge) return st;
+    snprintf(name, sizeof name, "k_paged_merge_hd%u", hd);
+    return launch(c, name, dim3((uint32_t)(((size_t)rows * num_heads * (hd / 4) + 255) / 256)), dim3(256), 0, params);
+}
+
+int rt_paged_attention_f32(rt_ctx* c, const rt_paged_batch* batch, const float* q, float* out,
+                           uint32_t num_heads) {
+    return paged_attention(c, batch, q, out, num_heads, nullptr, 0, "paged_attention");
+}
+int rt_shared_prefix_attention_f32(rt_ctx* c, const rt_paged_batch* batch, const float* q, float* out,
+                                   uint32_t num_heads, const uint32_t* shared_table, uint32_t shared_len) {
+    return paged_attention(c, batch, q, out, num_heads, shared_table, shared_len, "shared_prefix_attention");
+}
+
+// ───────────────────────── token log probabilities ─────────────────────────
+
+static int token_logprobs(rt_ctx* c, const char* type, uint32_t el, const void* x, const uint32_t* tokens,
+                          uint32_t rows, uint32_t n, uint64_t row_stride, float* logprob, float* entropy,
+                          uint32_t* rank, uint32_t top, uint32_t* top_ids, float* top_logprobs) {
+    if (!c) return fail(nullptr, RT_ERR_DISPATCH, "kernel dispatch error: null context");
+    if (rows == 0) return RT_OK;
+    if (n == 0 || n > 0x7fffffffu || row_stride < n)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: token_logprobs: rows of n=%u, row_stride=%llu", n,
+                    (unsigned long long)row_stride);
+    if (rows > 65535)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: token_logprobs: rows=%u exceeds 65535", rows);
+    if (top > RT_LOGPROBS_TOP_MAX || top > n)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: token_logprobs: top=%u exceeds %u or n=%u", top,
+                    RT_LOGPROBS_TOP_MAX, n);
+    if (!x || !tokens || !logprob || (top && (!top_ids || !top_logprobs)))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: token_logprobs: null buffer");
+    if (!aligned(x, el))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: token_logprobs: misaligned logits");
+    LogprobsArgs a{};
+    a.x = x, a.tokens = tokens, a.logprob = logprob, a.entropy = entropy, a.rank = rank;
+    a.top_ids = top_ids, a.top_logprobs = top_logprobs, a.row_stride = row_stride, a.n = n, a.top = top;
+    // segments of a row: about four workgroups a CU, each of 4096 values or more
+    const uint32_t want = (uint32_t)(4 * c->cu_count + rows - 1) / rows;
+    const uint32_t segs = std::max(1u, std::min({want, RT_LOGPROBS_SEG_MAX, n / 4096}));
+    a.seg_len = ((n + segs - 1) / segs + 2047) / 2048 * 2048;
+    a.segs = (n + a.seg_len - 1) / a.seg_len;
+    if (a.segs > 1) {
+        const size_t nk = (size_t)rows * a.segs;
+        const int st = ensure_ws(c, nk * (16 + 8 * top), "token_logprobs");
+        if (st != RT_OK) return st;
+        a.part = (float*)c->ws;
+        a.keys = (uint64_t*)((char*)c->ws + nk * 16);
+    }
+    char name[48];
+    snprintf(name, sizeof name, "k_logprobs_%s%s", top ? "top_" : "", type);
+    void* params[] = {&a};
+    const int st = launch(c, name, dim3(a.segs, rows), dim3(256), 0, params);
+    if (st != RT_OK || a.segs == 1) return st;
+    snprintf(name, sizeof name, "k_logprobs_merge_%s", type);
+    return launch(c, name, dim3(rows), dim3(64), 0, params);
+}
+
+int rt_token_logprobs_f32(rt_ctx* c, const float* logits, const uint32_t* tokens, uint32_t rows, uint32_t n,
+                          uint64_t row_stride, float* logprob, float* entropy, uint32_t* rank, uint32_t top,
+                          uint32_t* top_ids, float* top_logprobs) {
+    return token_logprobs(c, "f32", 4, logits, tokens, rows, n, row_stride, logprob, entropy, rank, top, top_ids,
+                          top_logprobs);
+}
+int rt_token_logprobs_f16(rt_ctx* c, const uint16_t* logits, const uint32_t* tokens, uint32_t rows, uint32_t n,
+                          uint64_t row_stride, float* logprob, float* entropy, uint32_t* rank, uint32_t top,
+                          uint32_t* top_ids, float* top_logprobs) {
+    return token_logprobs(c, "f16", 2, logits, tokens, rows, n, row_stride, logprob, entropy, rank, top, top_ids,
+                          top_logprobs);
 }
 
 static int embed_launch(rt_ctx* c, const char* kname, uint32_t blk_el, const void* table,

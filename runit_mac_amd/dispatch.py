@@ -167,6 +167,11 @@ _SIGS = {
     "rt_rms_norm_fused_qkv_bias_q4k_q6k_f32": [_P, _P, _P, _P, _P, _P, _F] + [_P] * 6 + [_U32] * 3,
     "rt_rms_norm_fused_ffn_q4k_f32": [_P, _P, _P, _P, _P, _F, _P, _U32, _U32],
     "rt_rms_norm_gemv_q6k_f32in_f32out": [_P, _P, _P, _P, _F, _P, _U32, _U32],
+    "rt_rope_kv_append_paged_f32": [_P] + [_P] * 5 + [_U32, _F],
+    "rt_paged_attention_f32": [_P, _P, _P, _P, _U32],
+    "rt_shared_prefix_attention_f32": [_P, _P, _P, _P, _U32, _P, _U32],
+    **{f"rt_token_logprobs_{_t}": [_P, _P, _P, _U32, _U32, _U64, _P, _P, _P, _U32, _P, _P]
+       for _t in ("f32", "f16")},
     "rt_stream_read": [_P, _P, c_size_t, _P, c_size_t],
     "rt_stream_copy": [_P, _P, _P, c_size_t],
     "rt_synth_normal_f32": [_P, _P, _U64, _U64, _F, _F],
@@ -290,6 +295,27 @@ def _ptr(b) -> int | None:
     if isinstance(b, bool) or not isinstance(b, (int, np.integer)):
         raise TypeError(f"device pointer expected, got {type(b).__name__}")
     return int(b)
+
+
+class PagedBatch(ctypes.Structure):
+    """rt_paged_batch (include/runit_hip.h): a batch of sequences over a pool
+    of key / value pages, dtype "f32" or "f16".  Buffers are Buffer objects or
+    device pointers; keep the object for as long as pool and tables stay."""
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p)] + \
+               [(n, c_uint32) for n in ("f16", "num_pages", "page_size", "num_kv_heads", "head_dim",
+                                        "table_stride", "n_seqs", "rows")] + \
+               [("page_stride", c_uint64)] + \
+               [(n, c_void_p) for n in ("table", "row_start", "kv_len")]
+
+    def __init__(self, k_pages, v_pages, dtype, num_pages, page_size, num_kv_heads, head_dim, table,
+                 table_stride, n_seqs, kv_len, rows=None, row_start=None, page_stride=0):
+        if dtype not in ("f32", "f16"):
+            raise ValueError(f"pages of dtype {dtype!r}: 'f32' or 'f16' expected")
+        super().__init__(_ptr(k_pages), _ptr(v_pages), int(dtype == "f16"), num_pages, page_size,
+                         num_kv_heads, head_dim, table_stride, n_seqs, n_seqs if rows is None else rows,
+                         page_stride, _ptr(table), _ptr(row_start), _ptr(kv_len))
+        self._held = (k_pages, v_pages, table, row_start, kv_len)  # (a Buffer is freed with its object)
+        self.ref = ctypes.addressof(self)
 
 
 # ───────────────────────────── context / buffers ─────────────────────────────
@@ -879,6 +905,42 @@ def silu_mul_f32(ctx, gate, up, out, n):
 def argmax_rows_first_f32(ctx, input, result, rows, n):
     """verify_draft's per-row argmax (forward.rs:2283-2293): first max wins."""
     _call(ctx, "rt_argmax_rows_first_f32", _ptr(input), _ptr(result), rows, n)
+
+
+# ──────────────────── batches over a paged cache, log probabilities ────────────────────
+
+def rope_kv_append_paged_f32(ctx, batch, q, k, v, q_out, num_heads, theta):
+    """RoPE of the batch's q (into q_out, which may be q) and k at their rows'
+    positions, k and v stored into the pages (new)."""
+    _call(ctx, "rt_rope_kv_append_paged_f32", batch.ref, _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), num_heads,
+          theta)
+
+
+def paged_attention_f32(ctx, batch, q, out, num_heads):
+    """Causal attention of the batch's rows over its pages (new)."""
+    _call(ctx, "rt_paged_attention_f32", batch.ref, _ptr(q), _ptr(out), num_heads)
+
+
+def shared_prefix_attention_f32(ctx, batch, q, out, num_heads, shared_table, shared_len):
+    """paged_attention_f32 where all sequences begin with the same shared_len
+    positions, in the pages of shared_table, read once for all (new)."""
+    _call(ctx, "rt_shared_prefix_attention_f32", batch.ref, _ptr(q), _ptr(out), num_heads, _ptr(shared_table),
+          shared_len)
+
+
+def _token_logprobs(name):
+    def fn(ctx, logits, tokens, rows, n, logprob, entropy=None, rank=None, top=0, top_ids=None,
+           top_logprobs=None, row_stride=None):
+        _call(ctx, "rt_" + name, _ptr(logits), _ptr(tokens), rows, n, n if row_stride is None else row_stride,
+              _ptr(logprob), _ptr(entropy), _ptr(rank), top, _ptr(top_ids), _ptr(top_logprobs))
+    fn.__name__ = name
+    fn.__doc__ = ("Log probabilities of the given tokens (u32 ids), the rows' entropies, the tokens' ranks and "
+                  f"the `top` most probable alternatives, from {name[-3:]} logits (new).")
+    return fn
+
+
+token_logprobs_f32 = _token_logprobs("token_logprobs_f32")
+token_logprobs_f16 = _token_logprobs("token_logprobs_f16")
 
 
 def embed_q8_0_f32(ctx, table, token, out, k):
