@@ -205,6 +205,12 @@ struct PagedTile {
     }
 };
 
+RT_DEV uint64_t pair_of(float lo, float hi) {
+    return (uint64_t)__builtin_bit_cast(uint32_t, hi) << 32 | __builtin_bit_cast(uint32_t, lo);
+}
+RT_DEV float pair_lo(uint64_t p) { return __builtin_bit_cast(float, (uint32_t)p); }
+RT_DEV float pair_hi(uint64_t p) { return __builtin_bit_cast(float, (uint32_t)(p >> 32)); }
+
 template <int HD, class T>
 RT_DEV void paged_attn(const PagedAttnArgs& a) {
     typedef PagedTile<HD, T> Tile;
@@ -285,13 +291,24 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
         for (uint32_t e = 0; e < VW; ++e) acc[i][e] = f32x4{0, 0, 0, 0};
     const float NEG = -__builtin_huge_valf(), scale2 = a.scale * 1.44269504f;
     float m = NEG, l = 0.0f;  // (in units of log 2)
+    // the next tile's operands are loaded while one is computed, its page id
+    // before that
+    auto entry = [&](uint32_t t) { return t < t1 ? table[(tb + t) * RT_PAGED_TILE >> b.ps_shift] : b.num_pages; };
+    auto place = [&](uint32_t t, uint32_t page) {
+        return page * b.page_stride + (size_t)((tb + t) * RT_PAGED_TILE & ((1u << b.ps_shift) - 1)) * HD;
+    };
+    constexpr bool AHEAD = HD < 256;  // (256: two tiles' operands are more registers than there are)
+    Tile kv, nx;
+    uint32_t page = entry(j.tile0 + w), pnext = entry(j.tile0 + w + NW);
+    if (AHEAD && page < b.num_pages) kv.load(kbase + place(j.tile0 + w, page), vbase + place(j.tile0 + w, page), lane);
     for (uint32_t t = j.tile0 + w; t < t1; t += NW) {
-        const uint32_t p0 = (tb + t) * RT_PAGED_TILE;
-        const uint32_t page = table[p0 >> b.ps_shift];
-        if (page >= b.num_pages) continue;
-        const size_t off = page * b.page_stride + (size_t)(p0 & ((1u << b.ps_shift) - 1)) * HD;
-        Tile kv;
-        kv.load(kbase + off, vbase + off, lane);
+        const uint32_t p0 = (tb + t) * RT_PAGED_TILE, pthis = page;
+        page = pnext;
+        if (AHEAD && page < b.num_pages) nx.load(kbase + place(t + NW, page), vbase + place(t + NW, page), lane);
+        if (!AHEAD && pthis < b.num_pages) kv.load(kbase + place(t, pthis), vbase + place(t, pthis), lane);
+        pnext = entry(t + 2 * NW);
+        if (pthis < b.num_pages) {
+        const size_t off = place(t, pthis);
         f32x4 sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
 #pragma unroll
         for (uint32_t i = 0; i < KN; ++i)
@@ -367,6 +384,8 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
                                 acc[i][e][x] = fmaf(pp, (float)vp[i * 16 * VW + x * VW + e], acc[i][e][x]);
                 }
         }
+        }
+        if constexpr (AHEAD) kv = nx;
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -403,19 +422,100 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
         const size_t slot = ((size_t)job * b.KVH + kvh) * RT_PAGED_ROWS + k;
         if (alone) {
             *(f32x4*)(a.out + ((size_t)row * a.H + hd) * HD + d) = M == NEG ? f32x4{0, 0, 0, 0} : o / L;
-        } else {
+        } else if (a.shared_len) {
             *(f32x4*)(a.part + slot * HD + d) = o;
             if (d == 0) {
                 a.ml[2 * slot] = M;
                 a.ml[2 * slot + 1] = L;
             }
+        } else {
+#pragma unroll
+            for (uint32_t x = 0; x < 4; x += 2) dev_store((uint64_t*)(a.part + slot * HD + d + x), pair_of(o[x], o[x + 1]));
+            if (d == 0) dev_store((uint64_t*)(a.ml + 2 * slot), pair_of(M, L));
         }
-        if (d == 0 && j.chunk == 0 && a.info) {
+        if (a.shared_len && d == 0 && j.chunk == 0) {
             uint32_t* in = a.info + (((size_t)row * a.H + hd) * 2 + (pre ? 1 : 0)) * 2;
             in[0] = j.first;
             in[1] = j.chunks * 16 + k;
         }
     }
+    if (alone || a.shared_len) return;
+    // The block's last workgroup to arrive puts its chunks together; of more
+    // than 12, the last of each group of about √chunks those of the group first.
+    __shared__ uint32_t turn;
+    auto last_of = [&](uint32_t* counter, uint32_t n) {
+        dev_stores_done();
+        __syncthreads();
+        if (tid == 0) {
+            turn = arrive(counter);
+            if (turn == n - 1) dev_store(counter, 0u);
+        }
+        __syncthreads();
+        return turn == n - 1;
+    };
+    auto slot_of = [&](uint32_t jb) { return ((size_t)jb * b.KVH + kvh) * RT_PAGED_ROWS; };
+    // jobs at, at + step, ... (n of them), in their order: into the outputs, or the first one's place
+    auto meet = [&](uint32_t at, uint32_t step, uint32_t n, bool out) {
+        constexpr uint32_t PW = HD / 2, PT = 16 * PW / (64 * NW);  // pairs a row, a thread
+        float o[PT][2], L[PT], M[PT];
+#pragma unroll
+        for (uint32_t u = 0; u < PT; ++u) o[u][0] = o[u][1] = L[u] = 0.0f, M[u] = NEG;
+        for (uint32_t x0 = 0; x0 < n; x0 += 8) {
+#pragma unroll
+            for (uint32_t u = 0; u < PT; ++u) {
+                const uint32_t i = tid + u * 64 * NW, k = i / PW, d = i % PW * 2;
+                if (k >= ncl) break;
+                uint64_t v[8], ml[8];
+#pragma unroll
+                for (uint32_t x = 0; x < 8; ++x) {
+                    const size_t slot = slot_of(at + min(x0 + x, n - 1) * step) + k;
+                    ml[x] = dev_load((const uint64_t*)(a.ml + 2 * slot));
+                    v[x] = dev_load((const uint64_t*)(a.part + slot * HD + d));
+                }
+                float mx = M[u];
+#pragma unroll
+                for (uint32_t x = 0; x < 8; ++x) mx = fmaxf(mx, pair_lo(ml[x]));
+                const float md = mx == NEG ? 0.0f : mx, f0 = __builtin_amdgcn_exp2f(M[u] - md);
+                o[u][0] *= f0, o[u][1] *= f0, L[u] *= f0;
+                M[u] = mx;
+#pragma unroll
+                for (uint32_t x = 0; x < 8; ++x) {
+                    if (x0 + x >= n || pair_lo(ml[x]) == NEG) continue;
+                    const float f = __builtin_amdgcn_exp2f(pair_lo(ml[x]) - md);
+                    L[u] = fmaf(f, pair_hi(ml[x]), L[u]);
+                    o[u][0] = fmaf(f, pair_lo(v[x]), o[u][0]);
+                    o[u][1] = fmaf(f, pair_hi(v[x]), o[u][1]);
+                }
+            }
+        }
+        if (!out) __syncthreads();  // (all have read the place that is written now)
+#pragma unroll
+        for (uint32_t u = 0; u < PT; ++u) {
+            const uint32_t i = tid + u * 64 * NW, k = i / PW, d = i % PW * 2;
+            if (k >= ncl) break;
+            if (out) {
+                float* op = a.out + ((size_t)row_of(k) * a.H + kvh * G + (col0 + k) % G) * HD + d;
+                op[0] = M[u] == NEG ? 0.0f : o[u][0] / L[u];
+                op[1] = M[u] == NEG ? 0.0f : o[u][1] / L[u];
+            } else {
+                const size_t slot = slot_of(at) + k;
+                dev_store((uint64_t*)(a.part + slot * HD + d), pair_of(o[u][0], o[u][1]));
+                if (d == 0) dev_store((uint64_t*)(a.ml + 2 * slot), pair_of(M[u], L[u]));
+            }
+        }
+    };
+    uint32_t* whole = a.counters + 2 * (j.first * b.KVH + kvh);
+    uint32_t step = 1, n = j.chunks;
+    if (n > 12) {
+        step = (uint32_t)ceilf(sqrtf((float)n));
+        const uint32_t grp = j.chunk / step, gn = min(step, n - grp * step), at = j.first + grp * step;
+        if (gn > 1) {
+            if (!last_of(a.counters + 2 * (at * b.KVH + kvh) + 1, gn)) return;
+            meet(at, 1, gn, false);
+        }
+        n = (n + step - 1) / step;
+    }
+    if (last_of(whole, n)) meet(j.first, step, n, true);
 }
 
 // o = Σ o_c·2^(m_c − M) / Σ l_c·2^(m_c − M) over a row's chunks, in their order
@@ -428,8 +528,7 @@ RT_DEV void paged_merge(const PagedAttnArgs& a) {
     if (rh >= rows * a.H) return;
     const uint32_t kvh = rh % a.H / (a.H / b.KVH);
     const uint32_t* in = a.info + (size_t)rh * 4;
-    const uint32_t parts = a.shared_len ? 2 : 1;
-    if (parts == 1 && in[1] / 16 == 1) return;  // (written whole)
+    constexpr uint32_t parts = 2;  // the prefix, the sequence's own positions
     const float NEG = -__builtin_huge_valf();
     float M = NEG;
     for (uint32_t p = 0; p < parts; ++p) {
@@ -460,10 +559,10 @@ RT_DEV void paged_merge(const PagedAttnArgs& a) {
     extern "C" __global__ void __launch_bounds__(256) k_paged_append_f16_hd##HD(PagedAppendArgs a) {     \
         paged_append<HD, _Float16>(a);                                                                    \
     }                                                                                                     \
-    extern "C" __global__ void __launch_bounds__(256) k_paged_attn_f32_hd##HD(PagedAttnArgs a) {         \
+    extern "C" __global__ void __launch_bounds__(256, 2) k_paged_attn_f32_hd##HD(PagedAttnArgs a) {         \
         paged_attn<HD, float>(a);                                                                         \
     }                                                                                                     \
-    extern "C" __global__ void __launch_bounds__(256) k_paged_attn_f16_hd##HD(PagedAttnArgs a) {         \
+    extern "C" __global__ void __launch_bounds__(256, 2) k_paged_attn_f16_hd##HD(PagedAttnArgs a) {         \
         paged_attn<HD, _Float16>(a);                                                                      \
     }                                                                                                     \
     extern "C" __global__ void __launch_bounds__(256) k_paged_merge_hd##HD(PagedAttnArgs a) {            \

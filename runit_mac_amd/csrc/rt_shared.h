@@ -78,7 +78,8 @@ struct PagedAttnArgs {
     const uint32_t* shared_table;  // positions below shared_len are read through it
     float* part;     // [jobs][KVH][RT_PAGED_ROWS][head size] unnormalised outputs
     float* ml;       // [jobs][KVH][RT_PAGED_ROWS][max, sum]
-    uint32_t* info;  // [rows][H][2 parts][first job, chunks · 16 + row of its block]
+    uint32_t* info;  // shared prefix: [rows][H][own, prefix][first job, chunks · 16 + row of its block]
+    uint32_t* counters;  // else: [jobs][KVH][2] arrivals at the block's and the group's first job, 0 between launches
     uint32_t H, shared_len;
     uint32_t jobs;    // jobs of a KV head (at most)
     uint32_t target;  // its chunks beyond one a block (at most; 0: blocks are not split)

@@ -1476,6 +1476,7 @@ int rt_ctx_create(rt_ctx** out, const char* code_object_path) {
             e = hipModuleGetGlobal(&p, &bytes, m, "scratch");
             if (e == hipSuccess && p) break;
         }
+        (void)hipGetLastError();  // the modules without one: another library's next call would report it
         if (e != hipSuccess || !p || bytes != RT_SCRATCH_BYTES) {
             hipFree(c->aux);
             unload(c);
@@ -4243,20 +4244,21 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     a.target = (uint32_t)(blocks >= 8 * slots ? 0 : blocks < slots / 2 ? slots - blocks : slots);
     a.jobs = (uint32_t)(blocks + a.target);
     const size_t nslot = (size_t)a.jobs * a.b.KVH * R;
-    const bool merge = shared_len || a.target;
-    if (merge) {
-        const size_t pb = nslot * hd * 4, mb = nslot * 8, ib = (size_t)rows * num_heads * 16;
+    if (2 * (uint64_t)a.jobs * a.b.KVH > kAttnCounters) a.target = 0, a.jobs = (uint32_t)blocks;
+    if (shared_len || a.target) {
+        const size_t pb = nslot * hd * 4, mb = nslot * 8, ib = shared_len ? (size_t)rows * num_heads * 16 : 0;
         st = ensure_ws(c, pb + mb + ib, who);
         if (st != RT_OK) return st;
         a.part = (float*)c->ws;
         a.ml = (float*)((char*)c->ws + pb);
         a.info = (uint32_t*)((char*)c->ws + pb + mb);
+        a.counters = c->counters;
     }
     char name[48];
     snprintf(name, sizeof name, "k_paged_attn_%s_hd%u", batch->f16 ? "f16" : "f32", hd);
     void* params[] = {&a};
     st = launch(c, name, dim3(a.jobs * a.b.KVH), dim3(64 * RT_PAGED_WAVES), 0, params);
-    if (st != RT_OK || !merge) return st;
+    if (st != RT_OK || !shared_len) return st;
     snprintf(name, sizeof name, "k_paged_merge_hd%u", hd);
     return launch(c, name, dim3((uint32_t)(((size_t)rows * num_heads * (hd / 4) + 255) / 256)), dim3(256), 0, params);
 }
