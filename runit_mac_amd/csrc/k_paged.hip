@@ -98,10 +98,30 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 // ───────────────────────────── attention ─────────────────────────────
 //
 // The rows of a sequence's KV head — (row, head of the group) pairs, row-major
-// — are taken in blocks of 16 columns of the f32 matrix cores, and its
-// positions in tiles of 16.  A job is a block over a chunk of tiles, one
-// workgroup; its four waves take every fourth tile, each with a softmax of its
-// own, and meet in LDS.  Chunks meet in k_paged_merge.
+// — are columns of Sᵀ = K·Qᵀ and Oᵀ = Vᵀ·Pᵀ on the matrix cores: a lane has four
+// positions of one column in registers, in the order that the second product
+// takes them, so that scores never leave their registers.  A job is a block of
+// columns over a chunk of positions, one workgroup.
+//
+// Narrow blocks (16 columns; decoding rows): the four waves take the chunk's
+// tiles in turn, keys and values straight from the pages into registers, each
+// with a softmax of its own, and meet in LDS.  Bound by the pages' bytes.
+// Wide blocks (f16 pages; prompt chunks, a shared prefix): each wave has 16·RT
+// columns of its own and all take every tile, from LDS.  Bound by the f16
+// matrix cores and, beside them, the softmax's vector operations.
+//
+// f32 pages use the f32 matrix cores.  f16 pages use the f16 ones, keys and
+// values as they are, queries and weights as pairs of f16 (x = hi + lo: 22
+// bits): queries scaled by a power of two to [2^14, 2^15) a column, weights by
+// 2^15, so that those down to 2^-17 of the largest keep their 22 bits and
+// smaller ones are off by at most 2^-40 of it.  A job whose sums come out not
+// finite (a value that is not, in places that only some of its columns see; the
+// pairs make NaN of ∞ too) is computed again on the f32 matrix cores.
+
+template <int HD>
+constexpr uint32_t paged_rt() { return HD == 256 ? 1 : 2; }
+template <int HD, bool WIDE>
+constexpr uint32_t paged_slot_rows() { return WIDE ? RT_PAGED_WAVES * 16 * paged_rt<HD>() : RT_PAGED_ROWS; }
 
 // The jobs of one KV head: blocks × chunks of every sequence in turn (and, with
 // a shared prefix, before them those of all rows over it).  The chunk length
@@ -119,6 +139,9 @@ RT_DEV uint32_t paged_tiles(const PagedAttnArgs& a, uint32_t s) {  // a sequence
     const uint32_t t1 = (L + RT_PAGED_TILE - 1) / RT_PAGED_TILE;
     return L > a.shared_len ? t1 - t0 : 0;
 }
+// columns of a block of a sequence (or of all rows) with so many
+template <int HD, bool WIDE>
+RT_DEV uint32_t paged_block(uint32_t cols) { return WIDE && cols > 32 ? paged_slot_rows<HD, WIDE>() : RT_PAGED_ROWS; }
 RT_DEV uint32_t wave_scan_add(uint32_t v) {  // inclusive
     const uint32_t lane = threadIdx.x & 63;
     for (uint32_t o = 1; o < 64; o *= 2) {
@@ -127,21 +150,24 @@ RT_DEV uint32_t wave_scan_add(uint32_t v) {  // inclusive
     }
     return v;
 }
+template <int HD, bool WIDE>
 RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
     const uint32_t lane = threadIdx.x & 63, G = a.H / a.b.KVH, n = a.b.n_seqs;
+    auto blocks_of = [&](uint32_t rows) {
+        const uint32_t bc = paged_block<HD, WIDE>(rows * G);
+        return (rows * G + bc - 1) / bc;
+    };
     const uint32_t rows = a.b.row_start ? min(a.b.row_start[n], a.b.rows) : min(n, a.b.rows);
-    const uint32_t pb = a.shared_len ? (rows * G + RT_PAGED_ROWS - 1) / RT_PAGED_ROWS : 0;
+    const uint32_t pb = a.shared_len ? blocks_of(rows) : 0;
     const uint32_t pt = (a.shared_len + RT_PAGED_TILE - 1) / RT_PAGED_TILE;
-    // (tiles × blocks of 2^28 positions in all: below 2^64)
     uint64_t work = 0;
-    for (uint32_t s = lane; s < n; s += 64)
-        work += (uint64_t)((seq_rows(a.b, s).n * G + RT_PAGED_ROWS - 1) / RT_PAGED_ROWS) * paged_tiles(a, s);
+    for (uint32_t s = lane; s < n; s += 64) work += (uint64_t)blocks_of(seq_rows(a.b, s).n) * paged_tiles(a, s);
     for (uint32_t o = 32; o; o /= 2) work += __shfl_xor((unsigned long long)work, o, 64);
     work += (uint64_t)pb * pt;
     PagedJob j{};
     uint64_t len = a.target ? (work + a.target - 1) / a.target : 0x7fffffffu;
-    len = max((uint64_t)a.min_chunk, (len + RT_PAGED_WAVES - 1) / RT_PAGED_WAVES * RT_PAGED_WAVES);
-    j.len = (uint32_t)min(len, (uint64_t)0x7ffffffc);
+    len = max((uint64_t)a.min_chunk, (len + 7) / 8 * 8);
+    j.len = (uint32_t)min(len, (uint64_t)0x7ffffff8);
     auto chunks = [&](uint32_t tiles) { return max(1u, tiles / j.len + (tiles % j.len ? 1u : 0u)); };
     auto found = [&](uint32_t seq, uint32_t base, uint32_t nc) {
         const uint32_t k = job - base;
@@ -167,7 +193,7 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
         uint32_t mine = 0, nc = 1;
         if (s < n) {
             nc = chunks(paged_tiles(a, s));
-            mine = (seq_rows(a.b, s).n * G + RT_PAGED_ROWS - 1) / RT_PAGED_ROWS * nc;
+            mine = blocks_of(seq_rows(a.b, s).n) * nc;
         }
         const uint32_t upto = base + wave_scan_add(mine);
         const uint64_t hit = __ballot(job < upto);
@@ -181,9 +207,34 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
     return j;
 }
 
-// Operands of a tile.  Keys: lane l holds position l % 16, W of every 4W
-// elements from W·(l / 16) on; values: of the positions 4(l / 16) + t, W of
-// every 16W elements from W·(l % 16) on.
+RT_DEV uint64_t pair_of(float lo, float hi) {
+    return (uint64_t)__builtin_bit_cast(uint32_t, hi) << 32 | __builtin_bit_cast(uint32_t, lo);
+}
+RT_DEV float pair_lo(uint64_t p) { return __builtin_bit_cast(float, (uint32_t)p); }
+RT_DEV float pair_hi(uint64_t p) { return __builtin_bit_cast(float, (uint32_t)(p >> 32)); }
+RT_DEV f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+RT_DEV f32x4 mfma32(h8_t a, h8_t b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Where a job's columns and positions are.
+template <class T>
+struct PagedView {
+    const T *k, *v;         // the KV head's part of page 0
+    const uint32_t* table;
+    uint64_t page_stride;
+    uint32_t num_pages, ps_shift;
+    uint32_t tb, t1;        // tile 0 of the job's numbering, the end of the chunk
+    uint32_t lo;            // first position seen
+    RT_DEV uint32_t page(uint32_t t) const {  // (no page behind the end)
+        return t < t1 ? table[(tb + t) * RT_PAGED_TILE >> ps_shift] : num_pages;
+    }
+    RT_DEV size_t place(uint32_t t, uint32_t page, uint32_t hd) const {
+        return page * page_stride + (size_t)((tb + t) * RT_PAGED_TILE & ((1u << ps_shift) - 1)) * hd;
+    }
+};
+
+// Operands of a tile.  Keys: lane l holds position l % 16, KW of every 4·KW
+// elements from KW·(l / 16) on; values: of the positions 4(l / 16) + r, VW of
+// every 16·VW elements from VW·(l % 16) on.
 template <int HD, class T>
 struct PagedTile {
     static constexpr uint32_t KW = sizeof(T) == 4 ? 4 : 8, KN = HD / (4 * KW);
@@ -197,166 +248,137 @@ struct PagedTile {
 #pragma unroll
         for (uint32_t i = 0; i < KN; ++i) k[i] = *(const kvec*)(kp + i * 4 * KW);
 #pragma unroll
-        for (uint32_t t = 0; t < 4; ++t) {
-            const T* vp = vb + (size_t)(4 * (lane >> 4) + t) * HD + (lane & 15) * VW;
+        for (uint32_t r = 0; r < 4; ++r) {
+            const T* vp = vb + (size_t)(4 * (lane >> 4) + r) * HD + (lane & 15) * VW;
 #pragma unroll
-            for (uint32_t i = 0; i < VN; ++i) v[t][i] = *(const vvec*)(vp + i * 16 * VW);
+            for (uint32_t i = 0; i < VN; ++i) v[r][i] = *(const vvec*)(vp + i * 16 * VW);
         }
+    }
+    RT_DEV void none() {
+#pragma unroll
+        for (uint32_t i = 0; i < KN; ++i) k[i] = kvec{};
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r)
+#pragma unroll
+            for (uint32_t i = 0; i < VN; ++i) v[r][i] = vvec{};
+    }
+    // positions that no column sees may hold anything: zeros
+    RT_DEV void clear(uint32_t pos0, uint32_t lo, uint32_t limx) {
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r)
+#pragma unroll
+            for (uint32_t i = 0; i < VN; ++i) v[r][i] = pos0 + r < lo || pos0 + r >= limx ? vvec{} : v[r][i];
     }
 };
 
-RT_DEV uint64_t pair_of(float lo, float hi) {
-    return (uint64_t)__builtin_bit_cast(uint32_t, hi) << 32 | __builtin_bit_cast(uint32_t, lo);
-}
-RT_DEV float pair_lo(uint64_t p) { return __builtin_bit_cast(float, (uint32_t)p); }
-RT_DEV float pair_hi(uint64_t p) { return __builtin_bit_cast(float, (uint32_t)(p >> 32)); }
-
+// 16 columns' running maximum (in units of log 2), sum and outputs.  Lane (c =
+// l % 16, g = l / 16) has column c's outputs VW·(4g + x) + e of every 16·VW.
 template <int HD, class T>
-RT_DEV void paged_attn(const PagedAttnArgs& a) {
+struct PagedAcc {
     typedef PagedTile<HD, T> Tile;
-    constexpr uint32_t KW = Tile::KW, KN = Tile::KN, VW = Tile::VW, VN = Tile::VN, NW = RT_PAGED_WAVES;
-    __shared__ float olds[NW][16][HD + 4];
-    __shared__ float mlds[NW][16], llds[NW][16];
-    const PagedBatch& b = a.b;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t c = lane & 15, g = lane >> 4, kvh = blockIdx.x % b.KVH, job = blockIdx.x / b.KVH;
-    const PagedJob j = paged_job(a, job);
-    if (!j.any) return;
-    const uint32_t G = a.H / b.KVH, cap = b.table_stride << b.ps_shift;
-    const bool pre = j.seq == b.n_seqs;
-    // a column's row, head, and the positions it sees: [lo, lim)
-    uint32_t ncol, row0, lo, hi;
-    const uint32_t* table;
-    if (pre) {
-        row0 = 0;
-        ncol = (b.row_start ? min(b.row_start[b.n_seqs], b.rows) : min(b.n_seqs, b.rows)) * G;
-        lo = 0;
-        hi = a.shared_len;
-        table = a.shared_table;
-    } else {
-        const SeqRows sr = seq_rows(b, j.seq);
-        row0 = sr.first;
-        ncol = sr.n * G;
-        lo = a.shared_len;
-        hi = min(b.kv_len[j.seq], cap);
-        table = b.table + (size_t)j.seq * b.table_stride;
+    static constexpr uint32_t VW = Tile::VW, VN = Tile::VN;
+    static constexpr float BIAS = sizeof(T) == 2 ? 15.0f : 0.0f;  // weights are 2^BIAS·e^(s − m)
+    f32x4 o[VN][VW];
+    float m, l;
+    RT_DEV void start() {
+#pragma unroll
+        for (uint32_t i = 0; i < VN; ++i)
+#pragma unroll
+            for (uint32_t e = 0; e < VW; ++e) o[i][e] = f32x4{0, 0, 0, 0};
+        m = -__builtin_huge_valf();
+        l = 0.0f;
     }
-    const uint32_t col0 = j.rb * RT_PAGED_ROWS, ncl = min(RT_PAGED_ROWS, ncol - col0);  // columns of the block
-    auto row_of = [&](uint32_t cc) { return row0 + (col0 + cc) / G; };
-    auto lim_of = [&](uint32_t cc) {
-        const uint32_t row = row_of(cc);
-        uint32_t s = j.seq;
-        if (pre) {  // the row's sequence
-            if (!b.row_start) {
-                s = row;
-            } else {
-                uint32_t x = 0, y = b.n_seqs;
-                while (y - x > 1) {
-                    const uint32_t mid = (x + y) / 2;
-                    if (b.row_start[mid] <= row) x = mid; else y = mid;
-                }
-                s = x;
-            }
+    // scores (NEG: unseen) to weights
+    template <uint32_t N>
+    RT_DEV void weigh(float (&p)[N]) {
+        const float NEG = -__builtin_huge_valf();
+        float tmax = NEG;
+#pragma unroll
+        for (uint32_t r = 0; r < N; ++r) tmax = fmaxf(tmax, p[r]);
+        tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
+        tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+        if (__ballot(tmax > m)) {
+            const float mn = fmaxf(m, tmax), md = mn == NEG ? 0.0f : mn, f = __builtin_amdgcn_exp2f(m - md);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (uint32_t i = 0; i < VN; ++i)
+#pragma unroll
+                for (uint32_t e = 0; e < VW; ++e) o[i][e] *= f;
         }
-        const SeqRows sr = seq_rows(b, s);
-        const uint32_t back = sr.n - (row - sr.first), len = b.kv_len[s];
-        return back <= len ? min(len - back + 1, hi) : 0u;
-    };
-    const uint32_t cc = min(c, ncl - 1), head = kvh * G + (col0 + cc) % G;
-    const uint32_t lim = lim_of(cc);
-    uint32_t limx = lim, limn = lim;  // of the block's rows: the largest, the smallest
-    for (uint32_t o = 1; o < 16; o *= 2) {
-        limx = max(limx, __shfl_xor(limx, o, 64));
-        limn = min(limn, __shfl_xor(limn, o, 64));
+        const float md = (m == NEG ? 0.0f : m) - BIAS;
+#pragma unroll
+        for (uint32_t r = 0; r < N; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(p[r] - md);
+            l += p[r];
+        }
     }
-    limx = __builtin_amdgcn_readfirstlane(limx);
-    limn = __builtin_amdgcn_readfirstlane(limn);
-    const uint32_t tb = lo / RT_PAGED_TILE;
-    const uint32_t tend = limx > lo ? (limx + RT_PAGED_TILE - 1) / RT_PAGED_TILE - tb : 0;
-    const uint32_t t1 = min(tend, j.tile0 + j.len);
-    const T* kbase = (const T*)b.k + (((size_t)kvh << b.ps_shift) * HD);
-    const T* vbase = (const T*)b.v + (((size_t)kvh << b.ps_shift) * HD);
+    RT_DEV void join() {  // the sum over the four lanes of a column
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+    }
+    RT_DEV bool finite() const {
+        bool bad = !(l < __builtin_huge_valf());
+#pragma unroll
+        for (uint32_t i = 0; i < VN; ++i)
+#pragma unroll
+            for (uint32_t e = 0; e < VW; ++e)
+#pragma unroll
+                for (uint32_t x = 0; x < 4; ++x) bad |= !(fabsf(o[i][e][x]) < __builtin_huge_valf());
+        return !__ballot(bad);
+    }
+};
 
+// The tiles t0, t0 + step, ... of a chunk (RUN 2: pairs of tiles there) for 16
+// columns on the f32 matrix cores: q is the lane's column, [0, lim) what it sees, limn / limx the
+// smallest and largest lim of the columns.
+template <int HD, class T, uint32_t RUN = 1>
+RT_DEV void paged_f32(PagedAcc<HD, T>& acc, const PagedView<T>& v, const float* q, float scale2, uint32_t t0,
+                      uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx) {
+    typedef PagedTile<HD, T> Tile;
+    constexpr uint32_t KW = Tile::KW, KN = Tile::KN, VW = Tile::VW, VN = Tile::VN;
+    const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     float qf[KN][KW];
-    const float* qp = a.q + ((size_t)row_of(cc) * a.H + head) * HD;
 #pragma unroll
     for (uint32_t i = 0; i < KN; ++i)
 #pragma unroll
-        for (uint32_t e = 0; e < KW; e += 4)
-            *(f32x4*)&qf[i][e] = *(const f32x4*)(qp + i * 4 * KW + g * KW + e);
-    f32x4 acc[VN][VW];
-#pragma unroll
-    for (uint32_t i = 0; i < VN; ++i)
-#pragma unroll
-        for (uint32_t e = 0; e < VW; ++e) acc[i][e] = f32x4{0, 0, 0, 0};
-    const float NEG = -__builtin_huge_valf(), scale2 = a.scale * 1.44269504f;
-    float m = NEG, l = 0.0f;  // (in units of log 2)
-    // the next tile's operands are loaded while one is computed, its page id
-    // before that
-    auto entry = [&](uint32_t t) { return t < t1 ? table[(tb + t) * RT_PAGED_TILE >> b.ps_shift] : b.num_pages; };
-    auto place = [&](uint32_t t, uint32_t page) {
-        return page * b.page_stride + (size_t)((tb + t) * RT_PAGED_TILE & ((1u << b.ps_shift) - 1)) * HD;
-    };
-    constexpr bool AHEAD = HD < 256;  // (256: two tiles' operands are more registers than there are)
-    Tile kv, nx;
-    uint32_t page = entry(j.tile0 + w), pnext = entry(j.tile0 + w + NW);
-    if (AHEAD && page < b.num_pages) kv.load(kbase + place(j.tile0 + w, page), vbase + place(j.tile0 + w, page), lane);
-    for (uint32_t t = j.tile0 + w; t < t1; t += NW) {
-        const uint32_t p0 = (tb + t) * RT_PAGED_TILE, pthis = page;
-        page = pnext;
-        if (AHEAD && page < b.num_pages) nx.load(kbase + place(t + NW, page), vbase + place(t + NW, page), lane);
-        if (!AHEAD && pthis < b.num_pages) kv.load(kbase + place(t, pthis), vbase + place(t, pthis), lane);
-        pnext = entry(t + 2 * NW);
-        if (pthis < b.num_pages) {
-        const size_t off = place(t, pthis);
+        for (uint32_t e = 0; e < KW; e += 4) *(f32x4*)&qf[i][e] = *(const f32x4*)(q + i * 4 * KW + g * KW + e);
+    acc.start();
+    auto after = [&](uint32_t t) { return RUN == 2 && t % 2 == 0 ? t + 1 : t + step - (RUN - 1); };
+    uint32_t next = v.page(t0);
+    for (uint32_t t = t0; t < v.t1; t = after(t)) {
+        const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE, page = next;
+        next = v.page(after(t));
+        if (page >= v.num_pages) continue;
+        const size_t off = v.place(t, page, HD);
+        Tile kv;
+        kv.load(v.k + off, v.v + off, lane);
         f32x4 sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
 #pragma unroll
         for (uint32_t i = 0; i < KN; ++i)
 #pragma unroll
             for (uint32_t e = 0; e < KW; e += 2) {
-                sa = __builtin_amdgcn_mfma_f32_16x16x4f32((float)kv.k[i][e], qf[i][e], sa, 0, 0, 0);
-                sb = __builtin_amdgcn_mfma_f32_16x16x4f32((float)kv.k[i][e + 1], qf[i][e + 1], sb, 0, 0, 0);
+                sa = mfma4((float)kv.k[i][e], qf[i][e], sa);
+                sb = mfma4((float)kv.k[i][e + 1], qf[i][e + 1], sb);
             }
-        float p[4], tmax = NEG;
-        const bool edge = p0 < lo || p0 + RT_PAGED_TILE > limn;
+        const bool edge = p0 < v.lo || p0 + RT_PAGED_TILE > limn;
+        float p[4];
 #pragma unroll
         for (uint32_t r = 0; r < 4; ++r) {
-            p[r] = (sa[r] + sb[r]) * scale2;
             const uint32_t pos = p0 + 4 * g + r;
-            if (edge && (pos < lo || pos >= lim)) p[r] = NEG;
-            tmax = fmaxf(tmax, p[r]);
+            p[r] = edge && (pos < v.lo || pos >= lim) ? -__builtin_huge_valf() : (sa[r] + sb[r]) * scale2;
         }
-        tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
-        tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
-        const float mn = fmaxf(m, tmax), md = mn == NEG ? 0.0f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - md);
-        m = mn;
-        l *= alpha;
-#pragma unroll
-        for (uint32_t r = 0; r < 4; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(p[r] - md);
-            l += p[r];
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < VN; ++i)
-#pragma unroll
-            for (uint32_t e = 0; e < VW; ++e) acc[i][e] *= alpha;
+        acc.weigh(p);
         bool bad = false;
         if (edge) {
-            // positions that no row sees may hold anything: zeros; one that only
-            // later rows see must not reach the earlier ones as 0·∞
+            // what only later columns see must not reach the earlier ones as 0·∞
+            kv.clear(p0 + 4 * g, v.lo, limx);
 #pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) {
-                const uint32_t pos = p0 + 4 * g + r;
-                const bool none = pos < lo || pos >= limx;
+            for (uint32_t r = 0; r < 4; ++r)
 #pragma unroll
                 for (uint32_t i = 0; i < VN; ++i)
 #pragma unroll
-                    for (uint32_t e = 0; e < VW; ++e) {
-                        if (none) kv.v[r][i][e] = (T)0.0f;
-                        bad |= !(fabsf((float)kv.v[r][i][e]) < __builtin_huge_valf());
-                    }
-            }
+                    for (uint32_t e = 0; e < VW; ++e) bad |= !(fabsf((float)kv.v[r][i][e]) < __builtin_huge_valf());
         }
         if (!__ballot(bad)) {
 #pragma unroll
@@ -364,8 +386,7 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
 #pragma unroll
                 for (uint32_t i = 0; i < VN; ++i)
 #pragma unroll
-                    for (uint32_t e = 0; e < VW; ++e)
-                        acc[i][e] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)kv.v[r][i][e], p[r], acc[i][e], 0, 0, 0);
+                    for (uint32_t e = 0; e < VW; ++e) acc.o[i][e] = mfma4((float)kv.v[r][i][e], p[r], acc.o[i][e]);
         } else {
 #pragma unroll
             for (uint32_t r = 0; r < 4; ++r)
@@ -373,35 +394,232 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
                 for (uint32_t h = 0; h < 4; ++h) {
                     const float pp = __shfl(p[r], h * 16 + c, 64);
                     const uint32_t pos = p0 + 4 * h + r;
-                    if (pos < lo || pos >= lim) continue;
-                    const T* vp = vbase + off + (size_t)(4 * h + r) * HD + 4 * g * VW;
+                    if (pos < v.lo || pos >= lim) continue;
+                    const T* vp = v.v + off + (size_t)(4 * h + r) * HD + 4 * g * VW;
 #pragma unroll
                     for (uint32_t i = 0; i < VN; ++i)
 #pragma unroll
                         for (uint32_t e = 0; e < VW; ++e)
 #pragma unroll
                             for (uint32_t x = 0; x < 4; ++x)
-                                acc[i][e][x] = fmaf(pp, (float)vp[i * 16 * VW + x * VW + e], acc[i][e][x]);
+                                acc.o[i][e][x] = fmaf(pp, (float)vp[i * 16 * VW + x * VW + e], acc.o[i][e][x]);
                 }
         }
-        }
-        if constexpr (AHEAD) kv = nx;
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    // lane (c, g) holds column c's elements VW·(4g + x) + e of every 16·VW
+    acc.join();
+}
+
+// A column's query as pairs of f16, x·2^e = hi + lo; returns scale2·2^-e.
+template <int HD>
+RT_DEV float paged_query(const float* q, float scale2, h8_t (&qh)[HD / 32], h8_t (&ql)[HD / 32]) {
+    const uint32_t g = (threadIdx.x & 63) >> 4;
+    float x[HD / 32][8], mx = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < HD / 32; ++i)
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k += 4) {
+            const f32x4 v = *(const f32x4*)(q + 32 * i + 8 * g + k);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                x[i][k + e] = v[e];
+                mx = fmaxf(mx, fabsf(v[e]));
+            }
+        }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    // (at most 126: 2^-e stays a normal number)
+    const int e = mx > 0.0f ? min(126, 15 - __builtin_amdgcn_frexp_expf(mx)) : 0;
+    const float f = ldexpf(1.0f, e);
+#pragma unroll
+    for (uint32_t i = 0; i < HD / 32; ++i)
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            const float y = x[i][k] * f;
+            qh[i][k] = (_Float16)y;
+            ql[i][k] = (_Float16)(y - (float)qh[i][k]);
+        }
+    return scale2 * ldexpf(1.0f, -e);
+}
+template <uint32_t N>
+RT_DEV void split_weights(const float (&p)[N], h8_t& hi, h8_t& lo) {
+#pragma unroll
+    for (uint32_t r = 0; r < 8; ++r) {
+        hi[r] = (_Float16)p[r];
+        lo[r] = (_Float16)(p[r] - (float)hi[r]);
+    }
+}
+
+// The same for f16 pages on the f16 matrix cores, two tiles at a time: t0, t0 +
+// 1, t0 + step, ...
+template <int HD>
+RT_DEV void paged_f16(PagedAcc<HD, _Float16>& acc, const PagedView<_Float16>& v, const float* q, float scale2,
+                      uint32_t t0, uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx) {
+    typedef PagedTile<HD, _Float16> Tile;
+    constexpr uint32_t KN = Tile::KN, VW = Tile::VW, VN = Tile::VN;
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
+    h8_t qh[KN], ql[KN];
+    const float qs = paged_query<HD>(q, scale2, qh, ql);
+    acc.start();
+    uint32_t next[2] = {v.page(t0), v.page(t0 + 1)};
+    for (uint32_t t = t0; t < v.t1; t += step) {
+        const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE;
+        const bool there[2] = {next[0] < v.num_pages, next[1] < v.num_pages};
+        Tile kv[2];
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            if (there[u]) {
+                const size_t off = v.place(t + u, next[u], HD);
+                kv[u].load(v.k + off, v.v + off, lane);
+            } else {
+                kv[u].none();
+            }
+        }
+        next[0] = v.page(t + step), next[1] = v.page(t + step + 1);
+        float p[8];
+        const bool edge = p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn || !there[0] || !there[1];
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            f32x4 sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t i = 0; i < KN; ++i) {
+                sa = mfma32(kv[u].k[i], qh[i], sa);
+                sb = mfma32(kv[u].k[i], ql[i], sb);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) p[4 * u + r] = (sa[r] + sb[r]) * qs;
+        }
+        if (edge) {
+#pragma unroll
+            for (uint32_t r = 0; r < 8; ++r) {
+                const uint32_t pos = p0 + 16 * (r / 4) + 4 * g + r % 4;
+                if (pos < v.lo || pos >= lim || !there[r / 4]) p[r] = -__builtin_huge_valf();
+            }
+            kv[0].clear(p0 + 4 * g, v.lo, limx);
+            kv[1].clear(p0 + 16 + 4 * g, v.lo, limx);
+        }
+        acc.weigh(p);
+        h8_t ph, pl;
+        split_weights(p, ph, pl);
+#pragma unroll
+        for (uint32_t i = 0; i < VN; ++i)
+#pragma unroll
+            for (uint32_t e = 0; e < VW; ++e) {
+                h8_t a;
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r) a[r] = kv[r / 4].v[r % 4][i][e];
+                acc.o[i][e] = mfma32(a, ph, acc.o[i][e]);
+                acc.o[i][e] = mfma32(a, pl, acc.o[i][e]);
+            }
+    }
+    acc.join();
+}
+
+// What a job's workgroup knows of its columns.
+template <int HD, class T>
+struct PagedCols {
+    const PagedAttnArgs& a;
+    PagedView<T> v;
+    uint32_t kvh, G, row0, col0, ncl, hi, tile0;
+    bool pre;
+    uint32_t seq;
+    RT_DEV uint32_t row(uint32_t cc) const { return row0 + (col0 + cc) / G; }
+    RT_DEV uint32_t head(uint32_t cc) const { return kvh * G + (col0 + cc) % G; }
+    RT_DEV const float* q(uint32_t cc) const { return a.q + ((size_t)row(cc) * a.H + head(cc)) * HD; }
+    // positions below it are what a column sees; every lane of the wave calls it
+    RT_DEV uint32_t lim(uint32_t cc) const {
+        const PagedBatch& b = a.b;
+        const uint32_t r = row(cc);
+        uint32_t s = seq;
+        if (pre) {
+            s = r;
+            if (b.row_start) {  // the sequences that end at or before the row
+                s = 0;
+                for (uint32_t s0 = 0; s0 < b.n_seqs; s0 += 64) {
+                    const uint32_t n = min(64u, b.n_seqs - s0), e = b.row_start[s0 + min(threadIdx.x & 63, n - 1) + 1];
+                    for (uint32_t x = 0; x < n; ++x) s += (uint32_t)__builtin_amdgcn_readlane(e, x) <= r;
+                }
+                s = min(s, b.n_seqs - 1);
+            }
+        }
+        const SeqRows sr = seq_rows(b, s);
+        const uint32_t back = sr.n - (r - sr.first), len = b.kv_len[s];
+        return back <= len ? min(len - back + 1, hi) : 0u;
+    }
+    // a column's part of a chunk: outputs at d = i·16·VW + 4·g·VW + ...
+    template <uint32_t SR>
+    RT_DEV void put(const PagedAcc<HD, T>& acc, const PagedJob& j, uint32_t job, uint32_t cc, bool alone) const {
+        constexpr uint32_t VW = PagedTile<HD, T>::VW, VN = PagedTile<HD, T>::VN;
+        if (cc >= ncl) return;
+        const uint32_t g = (threadIdx.x & 63) >> 4;
+        const size_t slot = ((size_t)job * a.b.KVH + kvh) * SR + cc, rh = (size_t)row(cc) * a.H + head(cc);
+        float* o = (alone ? a.out + rh * HD : a.part + slot * HD) + 4 * g * VW;
+        const float f = !alone ? 1.0f : acc.m == -__builtin_huge_valf() ? 0.0f : 1.0f / acc.l;
+#pragma unroll
+        for (uint32_t i = 0; i < VN; ++i)
+#pragma unroll
+            for (uint32_t x = 0; x < 4; ++x)
+#pragma unroll
+                for (uint32_t e = 0; e < VW; e += 4) {
+                    f32x4 y;
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) y[k] = acc.o[i][e + k][x] * f;
+                    *(f32x4*)(o + i * 16 * VW + x * VW + e) = y;
+                }
+        if (g == 0) {
+            if (!alone) {
+                a.ml[2 * slot] = acc.m;
+                a.ml[2 * slot + 1] = acc.l;
+            }
+            if (j.chunk == 0) note<SR>(j, rh, cc);
+        }
+    }
+    template <uint32_t SR>
+    RT_DEV void note(const PagedJob& j, size_t rh, uint32_t cc) const {
+        uint32_t* in = a.info + (rh * 2 + (pre ? 1 : 0)) * 2;
+        in[0] = j.first;
+        in[1] = j.chunks * SR + cc;
+    }
+};
+
+template <int HD, class T, bool WIDE>
+RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, const PagedJob& j, uint32_t job,
+                         float* lds) {
+    constexpr uint32_t NW = RT_PAGED_WAVES, SR = paged_slot_rows<HD, WIDE>();
+    constexpr uint32_t VW = PagedTile<HD, T>::VW, VN = PagedTile<HD, T>::VN;
+    float (*olds)[16][HD + 4] = (float (*)[16][HD + 4])lds;
+    float (*mlds)[16] = (float (*)[16])(lds + NW * 16 * (HD + 4)), (*llds)[16] = mlds + NW;
+    const PagedBatch& b = a.b;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t c = lane & 15, g = lane >> 4, ncl = co.ncl, cc = min(c, ncl - 1), lim = co.lim(cc);
+    uint32_t limx = lim, limn = lim;  // of the block's columns: the largest, the smallest
+    for (uint32_t o = 1; o < 16; o *= 2) {
+        limx = max(limx, __shfl_xor(limx, o, 64));
+        limn = min(limn, __shfl_xor(limn, o, 64));
+    }
+    limx = __builtin_amdgcn_readfirstlane(limx);
+    limn = __builtin_amdgcn_readfirstlane(limn);
+    PagedView<T> v = co.v;
+    v.t1 = min(v.t1, limx > v.lo ? (limx + RT_PAGED_TILE - 1) / RT_PAGED_TILE - v.tb : 0u);
+    const float NEG = -__builtin_huge_valf(), scale2 = a.scale * 1.44269504f;
+    PagedAcc<HD, T> acc;
+    if constexpr (sizeof(T) == 2) {
+        paged_f16<HD>(acc, v, co.q(cc), scale2, co.tile0 + 2 * w, 2 * NW, lim, limn, limx);
+        if (!acc.finite()) paged_f32<HD, T, 2>(acc, v, co.q(cc), scale2, co.tile0 + 2 * w, 2 * NW, lim, limn, limx);
+    } else {
+        paged_f32<HD, T>(acc, v, co.q(cc), scale2, co.tile0 + w, NW, lim, limn, limx);
+    }
 #pragma unroll
     for (uint32_t i = 0; i < VN; ++i)
 #pragma unroll
         for (uint32_t x = 0; x < 4; ++x)
 #pragma unroll
-            for (uint32_t e = 0; e < VW; ++e) olds[w][c][i * 16 * VW + (4 * g + x) * VW + e] = acc[i][e][x];
+            for (uint32_t e = 0; e < VW; ++e) olds[w][c][i * 16 * VW + (4 * g + x) * VW + e] = acc.o[i][e][x];
     if (g == 0) {
-        mlds[w][c] = m;
-        llds[w][c] = l;
+        mlds[w][c] = acc.m;
+        llds[w][c] = acc.l;
     }
     __syncthreads();
-    const bool alone = j.chunks == 1 && !a.shared_len;
+    const bool noted = WIDE || a.shared_len, alone = j.chunks == 1 && !a.shared_len;
     for (uint32_t i = tid; i < 16 * HD / 4; i += 64 * NW) {
         const uint32_t k = i / (HD / 4), d = i % (HD / 4) * 4;
         if (k >= ncl) break;
@@ -418,11 +636,10 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
             L += f * llds[u][k];
             o += f * *(const f32x4*)&olds[u][k][d];
         }
-        const uint32_t row = row_of(k), hd = kvh * G + (col0 + k) % G;
-        const size_t slot = ((size_t)job * b.KVH + kvh) * RT_PAGED_ROWS + k;
+        const size_t slot = ((size_t)job * b.KVH + co.kvh) * SR + k, rh = (size_t)co.row(k) * a.H + co.head(k);
         if (alone) {
-            *(f32x4*)(a.out + ((size_t)row * a.H + hd) * HD + d) = M == NEG ? f32x4{0, 0, 0, 0} : o / L;
-        } else if (a.shared_len) {
+            *(f32x4*)(a.out + rh * HD + d) = M == NEG ? f32x4{0, 0, 0, 0} : o / L;
+        } else if (noted) {
             *(f32x4*)(a.part + slot * HD + d) = o;
             if (d == 0) {
                 a.ml[2 * slot] = M;
@@ -433,13 +650,9 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
             for (uint32_t x = 0; x < 4; x += 2) dev_store((uint64_t*)(a.part + slot * HD + d + x), pair_of(o[x], o[x + 1]));
             if (d == 0) dev_store((uint64_t*)(a.ml + 2 * slot), pair_of(M, L));
         }
-        if (a.shared_len && d == 0 && j.chunk == 0) {
-            uint32_t* in = a.info + (((size_t)row * a.H + hd) * 2 + (pre ? 1 : 0)) * 2;
-            in[0] = j.first;
-            in[1] = j.chunks * 16 + k;
-        }
+        if (noted && d == 0 && j.chunk == 0) co.template note<SR>(j, rh, k);
     }
-    if (alone || a.shared_len) return;
+    if (alone || noted) return;
     // The block's last workgroup to arrive puts its chunks together; of more
     // than 12, the last of each group of about √chunks those of the group first.
     __shared__ uint32_t turn;
@@ -453,7 +666,7 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
         __syncthreads();
         return turn == n - 1;
     };
-    auto slot_of = [&](uint32_t jb) { return ((size_t)jb * b.KVH + kvh) * RT_PAGED_ROWS; };
+    auto slot_of = [&](uint32_t jb) { return ((size_t)jb * b.KVH + co.kvh) * SR; };
     // jobs at, at + step, ... (n of them), in their order: into the outputs, or the first one's place
     auto meet = [&](uint32_t at, uint32_t step, uint32_t n, bool out) {
         constexpr uint32_t PW = HD / 2, PT = 16 * PW / (64 * NW);  // pairs a row, a thread
@@ -465,26 +678,26 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
             for (uint32_t u = 0; u < PT; ++u) {
                 const uint32_t i = tid + u * 64 * NW, k = i / PW, d = i % PW * 2;
                 if (k >= ncl) break;
-                uint64_t v[8], ml[8];
+                uint64_t x[8], ml[8];
 #pragma unroll
-                for (uint32_t x = 0; x < 8; ++x) {
-                    const size_t slot = slot_of(at + min(x0 + x, n - 1) * step) + k;
-                    ml[x] = dev_load((const uint64_t*)(a.ml + 2 * slot));
-                    v[x] = dev_load((const uint64_t*)(a.part + slot * HD + d));
+                for (uint32_t y = 0; y < 8; ++y) {
+                    const size_t slot = slot_of(at + min(x0 + y, n - 1) * step) + k;
+                    ml[y] = dev_load((const uint64_t*)(a.ml + 2 * slot));
+                    x[y] = dev_load((const uint64_t*)(a.part + slot * HD + d));
                 }
                 float mx = M[u];
 #pragma unroll
-                for (uint32_t x = 0; x < 8; ++x) mx = fmaxf(mx, pair_lo(ml[x]));
+                for (uint32_t y = 0; y < 8; ++y) mx = fmaxf(mx, pair_lo(ml[y]));
                 const float md = mx == NEG ? 0.0f : mx, f0 = __builtin_amdgcn_exp2f(M[u] - md);
                 o[u][0] *= f0, o[u][1] *= f0, L[u] *= f0;
                 M[u] = mx;
 #pragma unroll
-                for (uint32_t x = 0; x < 8; ++x) {
-                    if (x0 + x >= n || pair_lo(ml[x]) == NEG) continue;
-                    const float f = __builtin_amdgcn_exp2f(pair_lo(ml[x]) - md);
-                    L[u] = fmaf(f, pair_hi(ml[x]), L[u]);
-                    o[u][0] = fmaf(f, pair_lo(v[x]), o[u][0]);
-                    o[u][1] = fmaf(f, pair_hi(v[x]), o[u][1]);
+                for (uint32_t y = 0; y < 8; ++y) {
+                    if (x0 + y >= n || pair_lo(ml[y]) == NEG) continue;
+                    const float f = __builtin_amdgcn_exp2f(pair_lo(ml[y]) - md);
+                    L[u] = fmaf(f, pair_hi(ml[y]), L[u]);
+                    o[u][0] = fmaf(f, pair_lo(x[y]), o[u][0]);
+                    o[u][1] = fmaf(f, pair_hi(x[y]), o[u][1]);
                 }
             }
         }
@@ -494,7 +707,7 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
             const uint32_t i = tid + u * 64 * NW, k = i / PW, d = i % PW * 2;
             if (k >= ncl) break;
             if (out) {
-                float* op = a.out + ((size_t)row_of(k) * a.H + kvh * G + (col0 + k) % G) * HD + d;
+                float* op = a.out + ((size_t)co.row(k) * a.H + co.head(k)) * HD + d;
                 op[0] = M[u] == NEG ? 0.0f : o[u][0] / L[u];
                 op[1] = M[u] == NEG ? 0.0f : o[u][1] / L[u];
             } else {
@@ -504,13 +717,13 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
             }
         }
     };
-    uint32_t* whole = a.counters + 2 * (j.first * b.KVH + kvh);
+    uint32_t* whole = a.counters + 2 * (j.first * b.KVH + co.kvh);
     uint32_t step = 1, n = j.chunks;
     if (n > 12) {
         step = (uint32_t)ceilf(sqrtf((float)n));
         const uint32_t grp = j.chunk / step, gn = min(step, n - grp * step), at = j.first + grp * step;
         if (gn > 1) {
-            if (!last_of(a.counters + 2 * (at * b.KVH + kvh) + 1, gn)) return;
+            if (!last_of(a.counters + 2 * (at * b.KVH + co.kvh) + 1, gn)) return;
             meet(at, 1, gn, false);
         }
         n = (n + step - 1) / step;
@@ -518,35 +731,234 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
     if (last_of(whole, n)) meet(j.first, step, n, true);
 }
 
-// o = Σ o_c·2^(m_c − M) / Σ l_c·2^(m_c − M) over a row's chunks, in their order
+// Two tiles in LDS: the key operands [2][HD / 32] of 64 lanes' 16 bytes, the
+// value operands [HD / 16]; the next two are brought while they are computed,
+// keys straight to LDS, values through registers, where pairs of positions are
+// put side by side.
 template <int HD>
+RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co, const PagedJob& j, uint32_t job,
+                       h8_t* lds) {
+    typedef PagedTile<HD, _Float16> Tile;
+    typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+    typedef const __attribute__((address_space(1))) uint32_t* gptr_t;
+    typedef __attribute__((address_space(3))) uint32_t* lptr_t;
+    constexpr uint32_t RT = paged_rt<HD>(), NW = RT_PAGED_WAVES, SR = paged_slot_rows<HD, true>();
+    constexpr uint32_t KN = Tile::KN, VW = Tile::VW, VN = Tile::VN;
+    constexpr uint32_t KOPS = 2 * KN * 64, STAGE = KOPS + VN * VW * 64;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t c = lane & 15, g = lane >> 4, x = g, sub = x >> 1;
+    const float NEG = -__builtin_huge_valf(), scale2 = a.scale * 1.44269504f;
+    PagedView<_Float16> v = co.v;
+    // the block's and the wave's columns: what the last (the most) and the first of them see
+    uint32_t lim[RT], limx_w = 0, limn_w = 0xffffffffu;
+#pragma unroll
+    for (uint32_t u = 0; u < RT; ++u) {
+        lim[u] = co.lim(min(16 * (RT * w + u) + c, co.ncl - 1));
+        uint32_t mx = lim[u], mn = lim[u];
+        for (uint32_t o = 1; o < 16; o *= 2) {
+            mx = max(mx, __shfl_xor(mx, o, 64));
+            mn = min(mn, __shfl_xor(mn, o, 64));
+        }
+        limx_w = max(limx_w, (uint32_t)__builtin_amdgcn_readfirstlane(mx));
+        limn_w = min(limn_w, (uint32_t)__builtin_amdgcn_readfirstlane(mn));
+    }
+    const bool idle = 16 * RT * w >= co.ncl;  // (brings tiles, computes none)
+    const uint32_t limx = co.pre ? co.hi : __builtin_amdgcn_readfirstlane(co.lim(co.ncl - 1));
+    v.t1 = min(v.t1, limx > v.lo ? (limx + RT_PAGED_TILE - 1) / RT_PAGED_TILE - v.tb : 0u);
+    h8_t qh[RT][KN], ql[RT][KN];
+    float qs[RT];
+    PagedAcc<HD, _Float16> acc[RT];
+#pragma unroll
+    for (uint32_t u = 0; u < RT; ++u) {
+        qs[u] = paged_query<HD>(co.q(min(16 * (RT * w + u) + c, co.ncl - 1)), scale2, qh[u], ql[u]);
+        acc[u].start();
+    }
+    typename Tile::vvec vr[2][VN];
+    auto bring = [&](uint32_t t, const uint32_t (&page)[2], uint32_t buf) {
+        const bool none[2] = {page[0] >= v.num_pages, page[1] >= v.num_pages};
+        const size_t off[2] = {v.place(t, none[0] ? 0 : page[0], HD), v.place(t + 1, none[1] ? 0 : page[1], HD)};
+#pragma unroll
+        for (uint32_t i = 0; i < 2 * KN / NW; ++i) {
+            const uint32_t kc = i * NW + w;
+            const _Float16* kp = v.k + (kc / KN ? off[1] : off[0]) + (size_t)c * HD + 8 * g + kc % KN * 32;
+            __builtin_amdgcn_global_load_lds((gptr_t)kp, (lptr_t)(lds + buf * STAGE + kc * 64), 16, 0, 0);
+        }
+        const uint32_t p = 4 * w + 2 * (x & 1), pos = (v.tb + t + sub) * RT_PAGED_TILE + p;
+        const _Float16* vp = v.v + (sub ? off[1] : off[0]) + (size_t)p * HD + c * VW;
+#pragma unroll
+        for (uint32_t r = 0; r < 2; ++r)
+#pragma unroll
+            for (uint32_t i = 0; i < VN; ++i) vr[r][i] = *(const typename Tile::vvec*)(vp + r * HD + i * 16 * VW);
+        // positions that no column sees may hold anything: zeros
+        if ((v.tb + t) * RT_PAGED_TILE < v.lo || (v.tb + t + 2) * RT_PAGED_TILE > limx || none[0] || none[1]) {
+#pragma unroll
+            for (uint32_t r = 0; r < 2; ++r)
+#pragma unroll
+                for (uint32_t i = 0; i < VN; ++i)
+                    if (pos + r < v.lo || pos + r >= limx || (sub ? none[1] : none[0])) vr[r][i] = typename Tile::vvec{};
+        }
+    };
+    auto store = [&](uint32_t buf) {
+        uint32_t* d = (uint32_t*)(lds + buf * STAGE + KOPS) + (w * 16 + c) * 4 + x;
+#pragma unroll
+        for (uint32_t i = 0; i < VN; ++i)
+#pragma unroll
+            for (uint32_t e = 0; e < VW; ++e)
+                d[(i * VW + e) * 256] = __builtin_bit_cast(uint32_t, h2_t{vr[0][i][e], vr[1][i][e]});
+    };
+    auto meet = [&]() {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+    };
+    uint32_t page[2] = {v.page(co.tile0), v.page(co.tile0 + 1)}, next[2] = {v.page(co.tile0 + 2), v.page(co.tile0 + 3)};
+    uint32_t buf = 0;
+    if (co.tile0 < v.t1) {
+        bring(co.tile0, page, 0);
+        store(0);
+    }
+    meet();
+    for (uint32_t t = co.tile0; t < v.t1; t += 2, buf ^= 1) {
+        const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE;
+        const bool there[2] = {page[0] < v.num_pages, page[1] < v.num_pages}, more = t + 2 < v.t1;
+        page[0] = next[0], page[1] = next[1];
+        if (more) bring(t + 2, page, buf ^ 1);
+        next[0] = v.page(t + 4), next[1] = v.page(t + 5);
+        if (!idle && p0 < limx_w) {
+            const h8_t* op = lds + buf * STAGE + lane;
+            f32x4 s[RT][2];
+#pragma unroll
+            for (uint32_t u = 0; u < RT; ++u) s[u][0] = s[u][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t i = 0; i < KN; ++i)
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    const h8_t k = op[(h * KN + i) * 64];
+#pragma unroll
+                    for (uint32_t u = 0; u < RT; ++u) s[u][h] = mfma32(k, qh[u][i], s[u][h]);
+#pragma unroll
+                    for (uint32_t u = 0; u < RT; ++u) s[u][h] = mfma32(k, ql[u][i], s[u][h]);
+                }
+            h8_t ph[RT], pl[RT];
+#pragma unroll
+            for (uint32_t u = 0; u < RT; ++u) {
+                float p[8];
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r) p[r] = s[u][r / 4][r % 4] * qs[u];
+                if (p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn_w || !there[0] || !there[1]) {
+#pragma unroll
+                    for (uint32_t r = 0; r < 8; ++r) {
+                        const uint32_t pos = p0 + 16 * (r / 4) + 4 * g + r % 4;
+                        if (pos < v.lo || pos >= lim[u] || !there[r / 4]) p[r] = NEG;
+                    }
+                }
+                acc[u].weigh(p);
+                split_weights(p, ph[u], pl[u]);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < VN; ++i)
+#pragma unroll
+                for (uint32_t e = 0; e < VW; ++e) {
+                    const h8_t y = op[KOPS + (i * VW + e) * 64];
+#pragma unroll
+                    for (uint32_t u = 0; u < RT; ++u) acc[u].o[i][e] = mfma32(y, ph[u], acc[u].o[i][e]);
+#pragma unroll
+                    for (uint32_t u = 0; u < RT; ++u) acc[u].o[i][e] = mfma32(y, pl[u], acc[u].o[i][e]);
+                }
+        }
+        if (more) store(buf ^ 1);
+        meet();
+    }
+    if (idle) return;
+    const bool alone = j.chunks == 1 && !a.shared_len;
+#pragma unroll
+    for (uint32_t u = 0; u < RT; ++u) {
+        const uint32_t cc = 16 * (RT * w + u) + c;
+        acc[u].join();
+        if (!acc[u].finite())
+            paged_f32<HD, _Float16>(acc[u], v, co.q(min(cc, co.ncl - 1)), scale2, co.tile0, 1, lim[u], limn_w, limx_w);
+        co.template put<SR>(acc[u], j, job, cc, alone);
+    }
+}
+
+template <int HD, class T, bool WIDE>
+RT_DEV void paged_attn(const PagedAttnArgs& a) {
+    constexpr uint32_t NARROW = RT_PAGED_WAVES * 16 * (HD + 4 + 2) * 4;  // (two stages of a wide block are less)
+    static_assert(NARROW >= 2 * 128 * HD, "LDS");
+    __shared__ f32x4 lds[NARROW / 16];
+    const PagedBatch& b = a.b;
+    const uint32_t kvh = blockIdx.x % b.KVH, job = blockIdx.x / b.KVH;
+    const PagedJob j = paged_job<HD, WIDE>(a, job);
+    if (!j.any) return;
+    const uint32_t G = a.H / b.KVH, cap = b.table_stride << b.ps_shift;
+    const bool pre = j.seq == b.n_seqs;
+    uint32_t rows, row0 = 0, lo = 0, hi = a.shared_len;
+    const uint32_t* table = a.shared_table;
+    if (pre) {
+        rows = b.row_start ? min(b.row_start[b.n_seqs], b.rows) : min(b.n_seqs, b.rows);
+    } else {
+        const SeqRows sr = seq_rows(b, j.seq);
+        rows = sr.n;
+        row0 = sr.first;
+        lo = a.shared_len;
+        hi = min(b.kv_len[j.seq], cap);
+        table = b.table + (size_t)j.seq * b.table_stride;
+    }
+    const uint32_t bc = paged_block<HD, WIDE>(rows * G), col0 = j.rb * bc;
+    const size_t head = ((size_t)kvh << b.ps_shift) * HD;
+    const uint32_t tb = lo / RT_PAGED_TILE, tend = hi > lo ? (hi + RT_PAGED_TILE - 1) / RT_PAGED_TILE - tb : 0;
+    const PagedView<T> v{(const T*)b.k + head, (const T*)b.v + head, table, b.page_stride, b.num_pages, b.ps_shift,
+                         tb, min(tend, j.tile0 + j.len), lo};
+    const PagedCols<HD, T> co{a, v, kvh, G, row0, col0, min(bc, rows * G - col0), hi, j.tile0, pre, j.seq};
+    if constexpr (WIDE) {
+        if (bc > RT_PAGED_ROWS) {
+            paged_wide<HD>(a, co, j, job, (h8_t*)lds);
+            return;
+        }
+    }
+    paged_narrow<HD, T, WIDE>(a, co, j, job, (float*)lds);
+}
+
+// o = Σ o_c·2^(m_c − M) / Σ l_c·2^(m_c − M) over a row's chunks, in their order,
+// the prefix's after the sequence's own
+template <int HD, bool WIDE>
 RT_DEV void paged_merge(const PagedAttnArgs& a) {
-    constexpr uint32_t TH = HD / 4;
+    constexpr uint32_t TH = HD / 4, SR = paged_slot_rows<HD, WIDE>();
     const PagedBatch& b = a.b;
     const uint32_t i = blockIdx.x * 256 + threadIdx.x, rh = i / TH, d = i % TH * 4;
     const uint32_t rows = b.row_start ? min(b.row_start[b.n_seqs], b.rows) : min(b.n_seqs, b.rows);
     if (rh >= rows * a.H) return;
     const uint32_t kvh = rh % a.H / (a.H / b.KVH);
     const uint32_t* in = a.info + (size_t)rh * 4;
-    constexpr uint32_t parts = 2;  // the prefix, the sequence's own positions
+    const uint32_t parts = a.shared_len ? 2 : 1;
+    if (parts == 1 && in[1] / SR == 1) return;  // (written whole)
     const float NEG = -__builtin_huge_valf();
-    float M = NEG;
-    for (uint32_t p = 0; p < parts; ++p) {
-        const uint32_t first = in[2 * p], n = in[2 * p + 1] / 16, k = in[2 * p + 1] % 16;
-        if (first >= a.jobs || n > a.jobs - first) return;
-        for (uint32_t u = 0; u < n; ++u)
-            M = fmaxf(M, a.ml[2 * (((size_t)(first + u) * b.KVH + kvh) * RT_PAGED_ROWS + k)]);
-    }
-    const float md = M == NEG ? 0.0f : M;
-    float L = 0.0f;
+    float M = NEG, L = 0.0f;
     f32x4 o = {0, 0, 0, 0};
     for (uint32_t p = 0; p < parts; ++p) {
-        const uint32_t first = in[2 * p], n = in[2 * p + 1] / 16, k = in[2 * p + 1] % 16;
-        for (uint32_t u = 0; u < n; ++u) {
-            const size_t slot = ((size_t)(first + u) * b.KVH + kvh) * RT_PAGED_ROWS + k;
-            const float mc = a.ml[2 * slot], f = mc == NEG ? 0.0f : __builtin_amdgcn_exp2f(mc - md);
-            L += f * a.ml[2 * slot + 1];
-            o += f * *(const f32x4*)(a.part + slot * HD + d);
+        const uint32_t first = in[2 * p], n = in[2 * p + 1] / SR, k = in[2 * p + 1] % SR;
+        if (first >= a.jobs || n > a.jobs - first) return;
+        for (uint32_t x0 = 0; x0 < n; x0 += 4) {
+            float mc[4], lc[4], mx = M;
+            f32x4 oc[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+                const size_t slot = ((size_t)(first + min(x0 + u, n - 1)) * b.KVH + kvh) * SR + k;
+                mc[u] = a.ml[2 * slot], lc[u] = a.ml[2 * slot + 1];
+                oc[u] = *(const f32x4*)(a.part + slot * HD + d);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) mx = fmaxf(mx, mc[u]);
+            const float md = mx == NEG ? 0.0f : mx, f0 = __builtin_amdgcn_exp2f(M - md);
+            M = mx;
+            L *= f0;
+            o *= f0;
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+                if (x0 + u >= n || mc[u] == NEG) continue;
+                const float f = __builtin_amdgcn_exp2f(mc[u] - md);
+                L = fmaf(f, lc[u], L);
+                o += f * oc[u];
+            }
         }
     }
     *(f32x4*)(a.out + (size_t)rh * HD + d) = M == NEG ? f32x4{0, 0, 0, 0} : o / L;
@@ -559,14 +971,20 @@ RT_DEV void paged_merge(const PagedAttnArgs& a) {
     extern "C" __global__ void __launch_bounds__(256) k_paged_append_f16_hd##HD(PagedAppendArgs a) {     \
         paged_append<HD, _Float16>(a);                                                                    \
     }                                                                                                     \
-    extern "C" __global__ void __launch_bounds__(256, 2) k_paged_attn_f32_hd##HD(PagedAttnArgs a) {         \
-        paged_attn<HD, float>(a);                                                                         \
+    extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_paged_attn_f32_hd##HD(PagedAttnArgs a) {      \
+        paged_attn<HD, float, false>(a);                                                                  \
     }                                                                                                     \
-    extern "C" __global__ void __launch_bounds__(256, 2) k_paged_attn_f16_hd##HD(PagedAttnArgs a) {         \
-        paged_attn<HD, _Float16>(a);                                                                      \
+    extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_paged_attn_f16_hd##HD(PagedAttnArgs a) {      \
+        paged_attn<HD, _Float16, false>(a);                                                               \
+    }                                                                                                     \
+    extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_paged_attn_f16w_hd##HD(PagedAttnArgs a) {     \
+        paged_attn<HD, _Float16, true>(a);                                                                \
     }                                                                                                     \
     extern "C" __global__ void __launch_bounds__(256) k_paged_merge_hd##HD(PagedAttnArgs a) {            \
-        paged_merge<HD>(a);                                                                               \
+        paged_merge<HD, false>(a);                                                                        \
+    }                                                                                                     \
+    extern "C" __global__ void __launch_bounds__(256) k_paged_mergew_hd##HD(PagedAttnArgs a) {           \
+        paged_merge<HD, true>(a);                                                                         \
     }
 RT_PAGED_KERNELS(64)
 RT_PAGED_KERNELS(128)

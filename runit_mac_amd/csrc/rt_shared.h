@@ -46,8 +46,8 @@ constexpr uint32_t RT_STEP_MAX_WGS = 1024;
 constexpr uint32_t RT_STEP_SYNC_BYTES = 2048;  // StepSync (k_step.hip)
 constexpr uint32_t RT_STEP_STATUS_OFF = 1280;  // its status word
 
-// Attention over paged caches (k_paged.hip): the rows of a block, the positions
-// of a tile (page sizes are multiples of it), the waves of a workgroup.
+// Attention over paged caches (k_paged.hip): the columns of a narrow block, the
+// positions of a tile (page sizes are multiples of it), the waves of a workgroup.
 constexpr uint32_t RT_PAGED_ROWS = 16;
 constexpr uint32_t RT_PAGED_TILE = 16;
 constexpr uint32_t RT_PAGED_WAVES = 4;
@@ -76,9 +76,11 @@ struct PagedAttnArgs {
     const float* q;  // [rows][H][head size]
     float* out;
     const uint32_t* shared_table;  // positions below shared_len are read through it
-    float* part;     // [jobs][KVH][RT_PAGED_ROWS][head size] unnormalised outputs
-    float* ml;       // [jobs][KVH][RT_PAGED_ROWS][max, sum]
-    uint32_t* info;  // shared prefix: [rows][H][own, prefix][first job, chunks · 16 + row of its block]
+    float* part;     // [jobs][KVH][rows of a slot][head size] unnormalised outputs
+    float* ml;       // [jobs][KVH][rows of a slot][max, sum]
+    // where chunks meet in a launch of their own (wide blocks, a shared prefix):
+    // [rows][H][own, prefix][first job, chunks · rows of a slot + row in its block]
+    uint32_t* info;
     uint32_t* counters;  // else: [jobs][KVH][2] arrivals at the block's and the group's first job, 0 between launches
     uint32_t H, shared_len;
     uint32_t jobs;    // jobs of a KV head (at most)

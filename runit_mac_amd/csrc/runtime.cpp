@@ -187,7 +187,9 @@ const char* const kKernelNames[] = {
     "k_paged_append_f16_hd64", "k_paged_append_f16_hd128", "k_paged_append_f16_hd256",
     "k_paged_attn_f32_hd64", "k_paged_attn_f32_hd128", "k_paged_attn_f32_hd256",
     "k_paged_attn_f16_hd64", "k_paged_attn_f16_hd128", "k_paged_attn_f16_hd256",
+    "k_paged_attn_f16w_hd64", "k_paged_attn_f16w_hd128", "k_paged_attn_f16w_hd256",
     "k_paged_merge_hd64", "k_paged_merge_hd128", "k_paged_merge_hd256",
+    "k_paged_mergew_hd64", "k_paged_mergew_hd128", "k_paged_mergew_hd256",
     "k_logprobs_f32", "k_logprobs_f16", "k_logprobs_top_f32", "k_logprobs_top_f16",
     "k_logprobs_merge_f32", "k_logprobs_merge_f16",
 };
@@ -4232,34 +4234,39 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     a.q = q, a.out = out, a.shared_table = shared_table, a.shared_len = shared_len, a.H = num_heads;
     a.scale = 1.0f / std::sqrt((float)hd);
     a.min_chunk = 8;
-    // blocks of a KV head (at most), and the chunks that its share of two
-    // workgroups a CU leaves beyond one a block
-    const uint64_t cols = (uint64_t)rows * G, R = RT_PAGED_ROWS;
-    uint64_t blocks = a.b.row_start ? cols / R + a.b.n_seqs : (uint64_t)a.b.n_seqs * ((G + R - 1) / R);
-    if (shared_len) blocks += (cols + R - 1) / R;
-    const uint64_t slots = std::max<uint64_t>(1, 2 * (uint64_t)c->cu_count / a.b.KVH);
+    // blocks of a KV head (at most), and the chunks that its share of the resident
+    // workgroups leaves beyond one a block; the kernel with wide blocks
+    // where one sequence's rows, or all over the prefix, may fill one
+    const uint64_t cols = (uint64_t)rows * G, n = a.b.n_seqs;
+    const bool wide = batch->f16 && cols > 32 && (shared_len || (rows >= n && (rows - n + 1) * G > 32));
+    const uint64_t SR = wide ? (hd == 256 ? 64 : 128) : RT_PAGED_ROWS;
+    uint64_t blocks = a.b.row_start ? cols / RT_PAGED_ROWS + n : n * ((G + RT_PAGED_ROWS - 1) / RT_PAGED_ROWS);
+    if (wide) blocks = std::min(blocks, 2 * n + cols / SR);
+    if (shared_len) blocks += (cols + SR - 1) / SR + 1;
+    char name[48];
+    snprintf(name, sizeof name, "k_paged_attn_%s_hd%u", wide ? "f16w" : batch->f16 ? "f16" : "f32", hd);
+    const uint64_t slots =
+        std::max<uint64_t>(1, (uint64_t)occupancy(c, name, 64 * RT_PAGED_WAVES, 0) * c->cu_count / a.b.KVH);
     if ((blocks + slots) * a.b.KVH > 0xffffffu)  // (2^32 threads a launch)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: too many rows (%u of %u heads)", who, rows,
                     num_heads);
     a.target = (uint32_t)(blocks >= 8 * slots ? 0 : blocks < slots / 2 ? slots - blocks : slots);
+    const bool noted = wide || shared_len;  // (chunks meet in a launch of their own)
+    if (!noted && 2 * (blocks + a.target) * a.b.KVH > kAttnCounters) a.target = 0;
     a.jobs = (uint32_t)(blocks + a.target);
-    const size_t nslot = (size_t)a.jobs * a.b.KVH * R;
-    if (2 * (uint64_t)a.jobs * a.b.KVH > kAttnCounters) a.target = 0, a.jobs = (uint32_t)blocks;
-    if (shared_len || a.target) {
-        const size_t pb = nslot * hd * 4, mb = nslot * 8, ib = shared_len ? (size_t)rows * num_heads * 16 : 0;
-        st = ensure_ws(c, pb + mb + ib, who);
+    if (noted || a.target) {
+        const size_t nslot = (size_t)a.jobs * a.b.KVH * SR, pb = nslot * hd * 4, mb = nslot * 8;
+        st = ensure_ws(c, pb + mb + (noted ? (size_t)rows * num_heads * 16 : 0), who);
         if (st != RT_OK) return st;
         a.part = (float*)c->ws;
         a.ml = (float*)((char*)c->ws + pb);
         a.info = (uint32_t*)((char*)c->ws + pb + mb);
         a.counters = c->counters;
     }
-    char name[48];
-    snprintf(name, sizeof name, "k_paged_attn_%s_hd%u", batch->f16 ? "f16" : "f32", hd);
     void* params[] = {&a};
     st = launch(c, name, dim3(a.jobs * a.b.KVH), dim3(64 * RT_PAGED_WAVES), 0, params);
-    if (st != RT_OK || !shared_len) return st;
-    snprintf(name, sizeof name, "k_paged_merge_hd%u", hd);
+    if (st != RT_OK || !noted) return st;
+    snprintf(name, sizeof name, "k_paged_merge%s_hd%u", wide ? "w" : "", hd);
     return launch(c, name, dim3((uint32_t)(((size_t)rows * num_heads * (hd / 4) + 255) / 256)), dim3(256), 0, params);
 }
 
