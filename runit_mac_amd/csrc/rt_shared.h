@@ -91,7 +91,7 @@ struct PagedAttnArgs {
 
 // Token log probabilities (k_logprobs.hip).
 constexpr uint32_t RT_LOGPROBS_TOP_MAX = 64;   // alternatives (at most): one a lane
-constexpr uint32_t RT_LOGPROBS_SEG_MAX = 64;   // segments of a row (at most): one a lane of the merge
+constexpr uint32_t RT_LOGPROBS_SEG_MAX = 64;   // segments of a row (at most): one a lane where they meet
 struct LogprobsArgs {
     const void* x;  // [rows][row_stride]
     const uint32_t* tokens;
@@ -100,8 +100,9 @@ struct LogprobsArgs {
     uint32_t* rank;   // or null
     uint32_t* top_ids;
     float* top_logprobs;
-    float* part;      // segs > 1: [rows][segs][4]: max, Σe, Σe·(max − x), rank
-    uint64_t* keys;   //           [rows][segs][top]: the largest, in order
+    uint64_t* part;      // segs > 1: [rows][segs][2]: max and Σe, Σe·(x − max) / ln 2 and rank
+    uint64_t* keys;      //           [rows][segs][top]: the largest, in order
+    uint32_t* counters;  //           [rows] arrivals, 0 between launches
     uint64_t row_stride;
     uint32_t n, top, segs, seg_len;
 };
