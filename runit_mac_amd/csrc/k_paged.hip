@@ -101,7 +101,8 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 // — are columns of Sᵀ = K·Qᵀ and Oᵀ = Vᵀ·Pᵀ on the matrix cores: a lane has four
 // positions of one column in registers, in the order that the second product
 // takes them, so that scores never leave their registers.  A job is a block of
-// columns over a chunk of positions, one workgroup.
+// columns over a chunk of tiles of 16 positions, one workgroup.  Chunks take
+// tiles in turn, so that those of a sequence read one window of it together.
 //
 // Narrow blocks (16 columns; decoding rows): the four waves take the chunk's
 // tiles in turn, keys and values straight from the pages into registers, each
@@ -130,7 +131,7 @@ constexpr uint32_t paged_slot_rows() { return WIDE ? RT_PAGED_WAVES * 16 * paged
 struct PagedJob {
     uint32_t seq;             // n_seqs: the shared prefix
     uint32_t rb, chunk, first, chunks;  // block, chunk, first job of the block, its chunks
-    uint32_t tile0, len;      // first tile of the chunk, tiles of a chunk
+    uint32_t len;             // tiles of a chunk (at most)
     bool any;
 };
 RT_DEV uint32_t paged_tiles(const PagedAttnArgs& a, uint32_t s) {  // a sequence's own tiles
@@ -150,7 +151,7 @@ RT_DEV uint32_t wave_scan_add(uint32_t v) {  // inclusive
     }
     return v;
 }
-template <int HD, bool WIDE>
+template <int HD, class T, bool WIDE>
 RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
     const uint32_t lane = threadIdx.x & 63, G = a.H / a.b.KVH, n = a.b.n_seqs;
     auto blocks_of = [&](uint32_t rows) {
@@ -166,8 +167,29 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
     work += (uint64_t)pb * pt;
     PagedJob j{};
     uint64_t len = a.target ? (work + a.target - 1) / a.target : 0x7fffffffu;
-    len = max((uint64_t)a.min_chunk, (len + 7) / 8 * 8);
-    j.len = (uint32_t)min(len, (uint64_t)0x7ffffff8);
+    constexpr uint32_t STEP = WIDE ? 2 : sizeof(T) == 2 ? 2 : 1;  // (f16 pages: tiles in pairs)
+    len = min((max((uint64_t)a.min_chunk, len) + STEP - 1) / STEP * STEP, (uint64_t)0x7ffffffe);
+    j.len = (uint32_t)len;
+    if (n <= 64 && len > a.min_chunk && a.target) {
+        // the shortest chunk, of 64 from an even share on, whose jobs are no more
+        // than the resident workgroups
+        const uint32_t mt = lane < n ? paged_tiles(a, lane) : 0, mb = lane < n ? blocks_of(seq_rows(a.b, lane).n) : 0;
+        const uint32_t c0 = max(a.min_chunk, (uint32_t)((work + a.slots - 1) / a.slots + STEP - 1) / STEP * STEP);
+        const uint32_t cl = c0 + lane * max(STEP, c0 / 128 / STEP * STEP);
+        const float inv = 1.0f / (float)cl;
+        auto up = [&](uint32_t t) {  // ceil(t / cl), at least 1 (t < 2^24)
+            uint32_t q = (uint32_t)((float)t * inv);
+            q -= q * cl >= t && q ? 1u : 0u;
+            q += q * cl < t ? 1u : 0u;
+            q += q * cl < t ? 1u : 0u;
+            return max(1u, q);
+        };
+        uint32_t jobs = pb * up(pt);
+        for (uint32_t s = 0; s < n; ++s)
+            jobs += (uint32_t)__builtin_amdgcn_readlane(mb, s) * up((uint32_t)__builtin_amdgcn_readlane(mt, s));
+        const uint64_t fit = __ballot(jobs <= a.slots && cl < j.len);
+        if (fit) j.len = __builtin_amdgcn_readlane(cl, __builtin_ctzll(fit));
+    }
     auto chunks = [&](uint32_t tiles) { return max(1u, tiles / j.len + (tiles % j.len ? 1u : 0u)); };
     auto found = [&](uint32_t seq, uint32_t base, uint32_t nc) {
         const uint32_t k = job - base;
@@ -176,7 +198,6 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
         j.chunk = k % nc;
         j.first = job - j.chunk;
         j.chunks = nc;
-        j.tile0 = j.chunk * j.len;
         j.any = true;
     };
     uint32_t base = 0;
@@ -222,7 +243,7 @@ struct PagedView {
     const uint32_t* table;
     uint64_t page_stride;
     uint32_t num_pages, ps_shift;
-    uint32_t tb, t1;        // tile 0 of the job's numbering, the end of the chunk
+    uint32_t tb, t1;        // tile 0 of the job's numbering, the end
     uint32_t lo;            // first position seen
     RT_DEV uint32_t page(uint32_t t) const {  // (no page behind the end)
         return t < t1 ? table[(tb + t) * RT_PAGED_TILE >> ps_shift] : num_pages;
@@ -519,7 +540,7 @@ template <int HD, class T>
 struct PagedCols {
     const PagedAttnArgs& a;
     PagedView<T> v;
-    uint32_t kvh, G, row0, col0, ncl, hi, tile0;
+    uint32_t kvh, G, row0, col0, ncl, hi;
     bool pre;
     uint32_t seq;
     RT_DEV uint32_t row(uint32_t cc) const { return row0 + (col0 + cc) / G; }
@@ -601,12 +622,13 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
     PagedView<T> v = co.v;
     v.t1 = min(v.t1, limx > v.lo ? (limx + RT_PAGED_TILE - 1) / RT_PAGED_TILE - v.tb : 0u);
     const float NEG = -__builtin_huge_valf(), scale2 = a.scale * 1.44269504f;
+    const uint32_t t0 = j.chunk * NW + w, stride = j.chunks * NW;
     PagedAcc<HD, T> acc;
     if constexpr (sizeof(T) == 2) {
-        paged_f16<HD>(acc, v, co.q(cc), scale2, co.tile0 + 2 * w, 2 * NW, lim, limn, limx);
-        if (!acc.finite()) paged_f32<HD, T, 2>(acc, v, co.q(cc), scale2, co.tile0 + 2 * w, 2 * NW, lim, limn, limx);
+        paged_f16<HD>(acc, v, co.q(cc), scale2, 2 * t0, 2 * stride, lim, limn, limx);
+        if (!acc.finite()) paged_f32<HD, T, 2>(acc, v, co.q(cc), scale2, 2 * t0, 2 * stride, lim, limn, limx);
     } else {
-        paged_f32<HD, T>(acc, v, co.q(cc), scale2, co.tile0 + w, NW, lim, limn, limx);
+        paged_f32<HD, T>(acc, v, co.q(cc), scale2, t0, stride, lim, limn, limx);
     }
 #pragma unroll
     for (uint32_t i = 0; i < VN; ++i)
@@ -810,19 +832,20 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
     };
-    uint32_t page[2] = {v.page(co.tile0), v.page(co.tile0 + 1)}, next[2] = {v.page(co.tile0 + 2), v.page(co.tile0 + 3)};
+    const uint32_t t0 = 2 * j.chunk, step = 2 * j.chunks;
+    uint32_t page[2] = {v.page(t0), v.page(t0 + 1)}, next[2] = {v.page(t0 + step), v.page(t0 + step + 1)};
     uint32_t buf = 0;
-    if (co.tile0 < v.t1) {
-        bring(co.tile0, page, 0);
+    if (t0 < v.t1) {
+        bring(t0, page, 0);
         store(0);
     }
     meet();
-    for (uint32_t t = co.tile0; t < v.t1; t += 2, buf ^= 1) {
+    for (uint32_t t = t0; t < v.t1; t += step, buf ^= 1) {
         const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE;
-        const bool there[2] = {page[0] < v.num_pages, page[1] < v.num_pages}, more = t + 2 < v.t1;
+        const bool there[2] = {page[0] < v.num_pages, page[1] < v.num_pages}, more = t + step < v.t1;
         page[0] = next[0], page[1] = next[1];
-        if (more) bring(t + 2, page, buf ^ 1);
-        next[0] = v.page(t + 4), next[1] = v.page(t + 5);
+        if (more) bring(t + step, page, buf ^ 1);
+        next[0] = v.page(t + 2 * step), next[1] = v.page(t + 2 * step + 1);
         if (!idle && p0 < limx_w) {
             const h8_t* op = lds + buf * STAGE + lane;
             f32x4 s[RT][2];
@@ -875,7 +898,7 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
         const uint32_t cc = 16 * (RT * w + u) + c;
         acc[u].join();
         if (!acc[u].finite())
-            paged_f32<HD, _Float16>(acc[u], v, co.q(min(cc, co.ncl - 1)), scale2, co.tile0, 1, lim[u], limn_w, limx_w);
+            paged_f32<HD, _Float16, 2>(acc[u], v, co.q(min(cc, co.ncl - 1)), scale2, t0, step, lim[u], limn_w, limx_w);
         co.template put<SR>(acc[u], j, job, cc, alone);
     }
 }
@@ -887,7 +910,7 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
     __shared__ f32x4 lds[NARROW / 16];
     const PagedBatch& b = a.b;
     const uint32_t kvh = blockIdx.x % b.KVH, job = blockIdx.x / b.KVH;
-    const PagedJob j = paged_job<HD, WIDE>(a, job);
+    const PagedJob j = paged_job<HD, T, WIDE>(a, job);
     if (!j.any) return;
     const uint32_t G = a.H / b.KVH, cap = b.table_stride << b.ps_shift;
     const bool pre = j.seq == b.n_seqs;
@@ -907,8 +930,8 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
     const size_t head = ((size_t)kvh << b.ps_shift) * HD;
     const uint32_t tb = lo / RT_PAGED_TILE, tend = hi > lo ? (hi + RT_PAGED_TILE - 1) / RT_PAGED_TILE - tb : 0;
     const PagedView<T> v{(const T*)b.k + head, (const T*)b.v + head, table, b.page_stride, b.num_pages, b.ps_shift,
-                         tb, min(tend, j.tile0 + j.len), lo};
-    const PagedCols<HD, T> co{a, v, kvh, G, row0, col0, min(bc, rows * G - col0), hi, j.tile0, pre, j.seq};
+                         tb, tend, lo};
+    const PagedCols<HD, T> co{a, v, kvh, G, row0, col0, min(bc, rows * G - col0), hi, pre, j.seq};
     if constexpr (WIDE) {
         if (bc > RT_PAGED_ROWS) {
             paged_wide<HD>(a, co, j, job, (h8_t*)lds);

@@ -85,6 +85,7 @@ struct PagedAttnArgs {
     uint32_t H, shared_len;
     uint32_t jobs;    // jobs of a KV head (at most)
     uint32_t target;  // its chunks beyond one a block (at most; 0: blocks are not split)
+    uint32_t slots;      // workgroups of a KV head that are resident together, ≤ jobs
     uint32_t min_chunk;  // tiles of a chunk (at least)
     float scale;
 };

@@ -4252,7 +4252,9 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     a.target = (uint32_t)(blocks >= 8 * slots ? 0 : blocks < slots / 2 ? slots - blocks : slots);
     const bool noted = wide || shared_len;  // (chunks meet in a launch of their own)
     if (!noted && 2 * (blocks + a.target) * a.b.KVH > kAttnCounters) a.target = 0;
+    if (getenv("XM")) a.min_chunk = atoi(getenv("XM"));
     a.jobs = (uint32_t)(blocks + a.target);
+    a.slots = (uint32_t)std::min<uint64_t>(slots, a.jobs);
     if (noted || a.target) {
         const size_t nslot = (size_t)a.jobs * a.b.KVH * SR, pb = nslot * hd * 4, mb = nslot * 8;
         st = ensure_ws(c, pb + mb + (noted ? (size_t)rows * num_heads * 16 : 0), who);
