@@ -144,53 +144,76 @@ RT_DEV uint32_t paged_tiles(const PagedAttnArgs& a, uint32_t s) {  // a sequence
 template <int HD, bool WIDE>
 RT_DEV uint32_t paged_block(uint32_t cols) { return WIDE && cols > 32 ? paged_slot_rows<HD, WIDE>() : RT_PAGED_ROWS; }
 RT_DEV uint32_t wave_scan_add(uint32_t v) {  // inclusive
-    const uint32_t lane = threadIdx.x & 63;
-    for (uint32_t o = 1; o < 64; o *= 2) {
-        const uint32_t u = __shfl_up(v, o, 64);
-        v += lane >= o ? u : 0;
-    }
+    constexpr int ROW_SHR = 0x110, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143;
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ROW_SHR + 1, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ROW_SHR + 2, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ROW_SHR + 4, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ROW_SHR + 8, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ROW_BCAST15, 0xA, 0xF, false);  // rows 1, 3: the one below's
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ROW_BCAST31, 0xC, 0xF, false);  // rows 2, 3: the lower half's
     return v;
+}
+// ceil(t / d), at least 1, for t < 2^24 and inv = 1 / d
+RT_DEV uint32_t ceil_div(uint32_t t, uint32_t d, float inv) {
+    uint32_t q = (uint32_t)((float)t * inv);  // off by one at most
+    q -= q && q * d >= t ? 1u : 0u;
+    q += q * d < t ? 1u : 0u;
+    q += q * d < t ? 1u : 0u;
+    return max(1u, q);
 }
 template <int HD, class T, bool WIDE>
 RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
+    constexpr uint32_t STEP = sizeof(T) == 2 ? 2 : 1;  // (f16 pages: tiles in pairs)
     const uint32_t lane = threadIdx.x & 63, G = a.H / a.b.KVH, n = a.b.n_seqs;
     auto blocks_of = [&](uint32_t rows) {
         const uint32_t bc = paged_block<HD, WIDE>(rows * G);
         return (rows * G + bc - 1) / bc;
     };
-    const uint32_t rows = a.b.row_start ? min(a.b.row_start[n], a.b.rows) : min(n, a.b.rows);
-    const uint32_t pb = a.shared_len ? blocks_of(rows) : 0;
-    const uint32_t pt = (a.shared_len + RT_PAGED_TILE - 1) / RT_PAGED_TILE;
-    uint64_t work = 0;
-    for (uint32_t s = lane; s < n; s += 64) work += (uint64_t)blocks_of(seq_rows(a.b, s).n) * paged_tiles(a, s);
-    for (uint32_t o = 32; o; o /= 2) work += __shfl_xor((unsigned long long)work, o, 64);
-    work += (uint64_t)pb * pt;
+    // sequences s0 .. of the lanes: their blocks and tiles
+    uint32_t mb = 0, mt = 0;
+    auto look = [&](uint32_t s) {
+        mb = s < n ? blocks_of(seq_rows(a.b, s).n) : 0;
+        mt = s < n ? paged_tiles(a, s) : 0;
+    };
+    look(lane);
+    uint32_t pb = 0, pt = 0;
+    if (a.shared_len) {
+        pb = blocks_of(a.b.row_start ? min(a.b.row_start[n], a.b.rows) : min(n, a.b.rows));
+        pt = (a.shared_len + RT_PAGED_TILE - 1) / RT_PAGED_TILE;
+    }
+    float work = (float)mb * (float)mt;
+    for (uint32_t s = lane + 64; s < n; s += 64) {
+        look(s);
+        work += (float)mb * (float)mt;
+    }
+    work = group_sum(work, 64) + (float)pb * (float)pt;
+    work = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, work)));
+    if (n > 64) look(lane);
     PagedJob j{};
-    uint64_t len = a.target ? (work + a.target - 1) / a.target : 0x7fffffffu;
-    constexpr uint32_t STEP = WIDE ? 2 : sizeof(T) == 2 ? 2 : 1;  // (f16 pages: tiles in pairs)
-    len = min((max((uint64_t)a.min_chunk, len) + STEP - 1) / STEP * STEP, (uint64_t)0x7ffffffe);
-    j.len = (uint32_t)len;
-    if (n <= 64 && len > a.min_chunk && a.target) {
+    // (a thousandth more than the share: the sum's roundings leave no job over)
+    const float share = a.target ? work * 1.001f / (float)a.target : 16777216.0f;
+    j.len = share < 16777216.0f ? ((uint32_t)share + STEP) / STEP * STEP : 16777216u;
+    if (j.len <= a.min_chunk) {
+        j.len = a.min_chunk;
+    } else if (n <= 64 && a.target) {
         // the shortest chunk, of 64 from an even share on, whose jobs are no more
         // than the resident workgroups
-        const uint32_t mt = lane < n ? paged_tiles(a, lane) : 0, mb = lane < n ? blocks_of(seq_rows(a.b, lane).n) : 0;
-        const uint32_t c0 = max(a.min_chunk, (uint32_t)((work + a.slots - 1) / a.slots + STEP - 1) / STEP * STEP);
+        const uint32_t c0 = max(a.min_chunk, ((uint32_t)(work / (float)a.slots) + STEP) / STEP * STEP);
         const uint32_t cl = c0 + lane * max(STEP, c0 / 128 / STEP * STEP);
         const float inv = 1.0f / (float)cl;
-        auto up = [&](uint32_t t) {  // ceil(t / cl), at least 1 (t < 2^24)
-            uint32_t q = (uint32_t)((float)t * inv);
-            q -= q * cl >= t && q ? 1u : 0u;
-            q += q * cl < t ? 1u : 0u;
-            q += q * cl < t ? 1u : 0u;
-            return max(1u, q);
-        };
-        uint32_t jobs = pb * up(pt);
+        auto about = [&](uint32_t t) { return fmaxf(1.0f, floorf(fmaf((float)t, inv, 0.9999f))); };
+        float jobs = (float)pb * about(pt);
         for (uint32_t s = 0; s < n; ++s)
-            jobs += (uint32_t)__builtin_amdgcn_readlane(mb, s) * up((uint32_t)__builtin_amdgcn_readlane(mt, s));
-        const uint64_t fit = __ballot(jobs <= a.slots && cl < j.len);
-        if (fit) j.len = __builtin_amdgcn_readlane(cl, __builtin_ctzll(fit));
+            jobs += (float)__builtin_amdgcn_readlane(mb, s) * about((uint32_t)__builtin_amdgcn_readlane(mt, s));
+        const uint64_t fit = __ballot(jobs <= (float)a.slots && cl < j.len);
+        if (fit) {  // (counted exactly before it is taken)
+            const uint32_t c1 = __builtin_amdgcn_readlane(cl, __builtin_ctzll(fit));
+            const float inv1 = 1.0f / (float)c1;
+            const uint32_t all = __builtin_amdgcn_readlane(wave_scan_add(mb * ceil_div(mt, c1, inv1)), 63);
+            if (all + pb * ceil_div(pt, c1, inv1) <= a.slots) j.len = c1;
+        }
     }
-    auto chunks = [&](uint32_t tiles) { return max(1u, tiles / j.len + (tiles % j.len ? 1u : 0u)); };
+    const float inv = 1.0f / (float)j.len;
     auto found = [&](uint32_t seq, uint32_t base, uint32_t nc) {
         const uint32_t k = job - base;
         j.seq = seq;
@@ -202,7 +225,7 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
     };
     uint32_t base = 0;
     if (pb) {
-        const uint32_t nc = chunks(pt);
+        const uint32_t nc = ceil_div(pt, j.len, inv);
         if (job < pb * nc) {
             found(n, 0, nc);
             return j;
@@ -210,20 +233,16 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
         base = pb * nc;
     }
     for (uint32_t s0 = 0; s0 < n; s0 += 64) {
-        const uint32_t s = s0 + lane;
-        uint32_t mine = 0, nc = 1;
-        if (s < n) {
-            nc = chunks(paged_tiles(a, s));
-            mine = blocks_of(seq_rows(a.b, s).n) * nc;
-        }
+        if (s0) look(s0 + lane);
+        const uint32_t nc = ceil_div(mt, j.len, inv), mine = mb * nc;
         const uint32_t upto = base + wave_scan_add(mine);
         const uint64_t hit = __ballot(job < upto);
         if (hit) {
             const int l = __builtin_ctzll(hit);
-            found(s0 + l, __shfl(upto - mine, l, 64), __shfl(nc, l, 64));
+            found(s0 + l, (uint32_t)__builtin_amdgcn_readlane(upto - mine, l), (uint32_t)__builtin_amdgcn_readlane(nc, l));
             return j;
         }
-        base = __shfl(upto, 63, 64);
+        base = (uint32_t)__builtin_amdgcn_readlane(upto, 63);
     }
     return j;
 }
@@ -676,8 +695,11 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
     }
     if (alone || noted) return;
     // The block's last workgroup to arrive puts its chunks together; of more
-    // than 12, the last of each group of about √chunks those of the group first.
+    // than 24, the last of each group of about √chunks those of the group first.
+    // All loads of sixteen chunks are in flight at once.
     __shared__ uint32_t turn;
+    constexpr uint32_t PW = HD / 2, PT = 16 * PW / (64 * NW), BATCH = 16;  // pairs a row, a thread; chunks at a time
+    __shared__ float mc[BATCH][16], lc[BATCH][16];
     auto last_of = [&](uint32_t* counter, uint32_t n) {
         dev_stores_done();
         __syncthreads();
@@ -689,45 +711,55 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
         return turn == n - 1;
     };
     auto slot_of = [&](uint32_t jb) { return ((size_t)jb * b.KVH + co.kvh) * SR; };
-    // jobs at, at + step, ... (n of them), in their order: into the outputs, or the first one's place
+    // jobs at, at + step, ... (n of them): into the outputs, or the first one's place
     auto meet = [&](uint32_t at, uint32_t step, uint32_t n, bool out) {
-        constexpr uint32_t PW = HD / 2, PT = 16 * PW / (64 * NW);  // pairs a row, a thread
+        const uint32_t items = ncl * PW;
         float o[PT][2], L[PT], M[PT];
 #pragma unroll
         for (uint32_t u = 0; u < PT; ++u) o[u][0] = o[u][1] = L[u] = 0.0f, M[u] = NEG;
-        for (uint32_t x0 = 0; x0 < n; x0 += 8) {
+        for (uint32_t x0 = 0; x0 < n; x0 += BATCH) {
+            uint64_t x[PT][BATCH];
+            const uint32_t mk = tid & 15, my = tid >> 4;
+            uint64_t ml = pair_of(NEG, 0.0f);
+            if (x0 + my < n && mk < ncl) ml = dev_load((const uint64_t*)a.ml + slot_of(at + (x0 + my) * step) + mk);
 #pragma unroll
-            for (uint32_t u = 0; u < PT; ++u) {
-                const uint32_t i = tid + u * 64 * NW, k = i / PW, d = i % PW * 2;
-                if (k >= ncl) break;
-                uint64_t x[8], ml[8];
+            for (uint32_t u = 0; u < PT; ++u)
+                if (256 * u < items) {
+                    const uint32_t i = min(tid + 256 * u, items - 1);
 #pragma unroll
-                for (uint32_t y = 0; y < 8; ++y) {
-                    const size_t slot = slot_of(at + min(x0 + y, n - 1) * step) + k;
-                    ml[y] = dev_load((const uint64_t*)(a.ml + 2 * slot));
-                    x[y] = dev_load((const uint64_t*)(a.part + slot * HD + d));
+                    for (uint32_t y = 0; y < BATCH; ++y)
+                        if (x0 + y < n) x[u][y] = dev_load((const uint64_t*)(a.part + slot_of(at + (x0 + y) * step) * HD) + i);
                 }
-                float mx = M[u];
+            if (x0) __syncthreads();
+            mc[my][mk] = pair_lo(ml);
+            lc[my][mk] = pair_hi(ml);
+            __syncthreads();
 #pragma unroll
-                for (uint32_t y = 0; y < 8; ++y) mx = fmaxf(mx, pair_lo(ml[y]));
-                const float md = mx == NEG ? 0.0f : mx, f0 = __builtin_amdgcn_exp2f(M[u] - md);
-                o[u][0] *= f0, o[u][1] *= f0, L[u] *= f0;
-                M[u] = mx;
+            for (uint32_t u = 0; u < PT; ++u)
+                if (256 * u < items) {
+                    const uint32_t k = min(tid + 256 * u, items - 1) / PW;
+                    float mx = M[u];
 #pragma unroll
-                for (uint32_t y = 0; y < 8; ++y) {
-                    if (x0 + y >= n || pair_lo(ml[y]) == NEG) continue;
-                    const float f = __builtin_amdgcn_exp2f(pair_lo(ml[y]) - md);
-                    L[u] = fmaf(f, pair_hi(ml[y]), L[u]);
-                    o[u][0] = fmaf(f, pair_lo(x[y]), o[u][0]);
-                    o[u][1] = fmaf(f, pair_hi(x[y]), o[u][1]);
+                    for (uint32_t y = 0; y < BATCH; ++y) mx = fmaxf(mx, mc[y][k]);
+                    const float md = mx == NEG ? 0.0f : mx, f0 = __builtin_amdgcn_exp2f(M[u] - md);
+                    o[u][0] *= f0, o[u][1] *= f0, L[u] *= f0;
+                    M[u] = mx;
+#pragma unroll
+                    for (uint32_t y = 0; y < BATCH; ++y)
+                        if (x0 + y < n) {
+                            const bool none = mc[y][k] == NEG;  // (its sums are zeros)
+                            const float f = none ? 0.0f : __builtin_amdgcn_exp2f(mc[y][k] - md);
+                            L[u] = fmaf(f, lc[y][k], L[u]);
+                            o[u][0] = fmaf(f, pair_lo(x[u][y]), o[u][0]);
+                            o[u][1] = fmaf(f, pair_hi(x[u][y]), o[u][1]);
+                        }
                 }
-            }
         }
         if (!out) __syncthreads();  // (all have read the place that is written now)
 #pragma unroll
         for (uint32_t u = 0; u < PT; ++u) {
-            const uint32_t i = tid + u * 64 * NW, k = i / PW, d = i % PW * 2;
-            if (k >= ncl) break;
+            const uint32_t i = tid + 256 * u, k = i / PW, d = i % PW * 2;
+            if (i >= items) break;
             if (out) {
                 float* op = a.out + ((size_t)co.row(k) * a.H + co.head(k)) * HD + d;
                 op[0] = M[u] == NEG ? 0.0f : o[u][0] / L[u];
@@ -741,7 +773,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
     };
     uint32_t* whole = a.counters + 2 * (j.first * b.KVH + co.kvh);
     uint32_t step = 1, n = j.chunks;
-    if (n > 12) {
+    if (n > 24) {
         step = (uint32_t)ceilf(sqrtf((float)n));
         const uint32_t grp = j.chunk / step, gn = min(step, n - grp * step), at = j.first + grp * step;
         if (gn > 1) {

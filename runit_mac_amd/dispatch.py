@@ -288,8 +288,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
 
 
 def _ptr(b) -> int | None:
-    if b is None:
-        return None
+    if b is None or type(b) is int:
+        return b
     if isinstance(b, Buffer):
         return b.ptr
     if isinstance(b, bool) or not isinstance(b, (int, np.integer)):
@@ -912,27 +912,30 @@ def argmax_rows_first_f32(ctx, input, result, rows, n):
 def rope_kv_append_paged_f32(ctx, batch, q, k, v, q_out, num_heads, theta):
     """RoPE of the batch's q (into q_out, which may be q) and k at their rows'
     positions, k and v stored into the pages (new)."""
-    _call(ctx, "rt_rope_kv_append_paged_f32", batch.ref, _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), num_heads,
-          theta)
+    ctx._check(ctx.lib.rt_rope_kv_append_paged_f32(ctx.handle, batch.ref, _ptr(q), _ptr(k), _ptr(v), _ptr(q_out),
+                                                   num_heads, theta))
 
 
 def paged_attention_f32(ctx, batch, q, out, num_heads):
     """Causal attention of the batch's rows over its pages (new)."""
-    _call(ctx, "rt_paged_attention_f32", batch.ref, _ptr(q), _ptr(out), num_heads)
+    ctx._check(ctx.lib.rt_paged_attention_f32(ctx.handle, batch.ref, _ptr(q), _ptr(out), num_heads))
 
 
 def shared_prefix_attention_f32(ctx, batch, q, out, num_heads, shared_table, shared_len):
     """paged_attention_f32 where all sequences begin with the same shared_len
     positions, in the pages of shared_table, read once for all (new)."""
-    _call(ctx, "rt_shared_prefix_attention_f32", batch.ref, _ptr(q), _ptr(out), num_heads, _ptr(shared_table),
-          shared_len)
+    ctx._check(ctx.lib.rt_shared_prefix_attention_f32(ctx.handle, batch.ref, _ptr(q), _ptr(out), num_heads,
+                                                      _ptr(shared_table), shared_len))
 
 
 def _token_logprobs(name):
+    symbol = "rt_" + name
+
     def fn(ctx, logits, tokens, rows, n, logprob, entropy=None, rank=None, top=0, top_ids=None,
            top_logprobs=None, row_stride=None):
-        _call(ctx, "rt_" + name, _ptr(logits), _ptr(tokens), rows, n, n if row_stride is None else row_stride,
-              _ptr(logprob), _ptr(entropy), _ptr(rank), top, _ptr(top_ids), _ptr(top_logprobs))
+        ctx._check(getattr(ctx.lib, symbol)(
+            ctx.handle, _ptr(logits), _ptr(tokens), rows, n, n if row_stride is None else row_stride, _ptr(logprob),
+            _ptr(entropy), _ptr(rank), top, _ptr(top_ids), _ptr(top_logprobs)))
     fn.__name__ = name
     fn.__doc__ = ("Log probabilities of the given tokens (u32 ids), the rows' entropies, the tokens' ranks and "
                   f"the `top` most probable alternatives, from {name[-3:]} logits (new).")
