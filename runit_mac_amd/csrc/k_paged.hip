@@ -311,6 +311,12 @@ struct PagedTile {
     }
 };
 
+// over the four lanes of a column
+RT_DEV float column_max(float v) {
+    v = fmaxf(v, __builtin_bit_cast(float, lane_xor<16>(__builtin_bit_cast(uint32_t, v))));
+    return fmaxf(v, __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, v))));
+}
+
 // 16 columns' running maximum (in units of log 2), sum and outputs.  Lane (c =
 // l % 16, g = l / 16) has column c's outputs VW·(4g + x) + e of every 16·VW.
 template <int HD, class T>
@@ -328,15 +334,14 @@ struct PagedAcc {
         m = -__builtin_huge_valf();
         l = 0.0f;
     }
-    // scores (NEG: unseen) to weights
+    // products (NEG: unseen), scores times 1 / scale, to weights
     template <uint32_t N>
-    RT_DEV void weigh(float (&p)[N]) {
+    RT_DEV void weigh(float (&p)[N], float scale) {
         const float NEG = -__builtin_huge_valf();
-        float tmax = NEG;
+        float tmax = p[0];
 #pragma unroll
-        for (uint32_t r = 0; r < N; ++r) tmax = fmaxf(tmax, p[r]);
-        tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
-        tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+        for (uint32_t r = 1; r < N; ++r) tmax = fmaxf(tmax, p[r]);
+        tmax = column_max(tmax) * scale;
         if (__ballot(tmax > m)) {
             const float mn = fmaxf(m, tmax), md = mn == NEG ? 0.0f : mn, f = __builtin_amdgcn_exp2f(m - md);
             m = mn;
@@ -349,7 +354,7 @@ struct PagedAcc {
         const float md = (m == NEG ? 0.0f : m) - BIAS;
 #pragma unroll
         for (uint32_t r = 0; r < N; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(p[r] - md);
+            p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], scale, -md));
             l += p[r];
         }
     }
@@ -406,9 +411,9 @@ RT_DEV void paged_f32(PagedAcc<HD, T>& acc, const PagedView<T>& v, const float* 
 #pragma unroll
         for (uint32_t r = 0; r < 4; ++r) {
             const uint32_t pos = p0 + 4 * g + r;
-            p[r] = edge && (pos < v.lo || pos >= lim) ? -__builtin_huge_valf() : (sa[r] + sb[r]) * scale2;
+            p[r] = edge && (pos < v.lo || pos >= lim) ? -__builtin_huge_valf() : sa[r] + sb[r];
         }
-        acc.weigh(p);
+        acc.weigh(p, scale2);
         bool bad = false;
         if (edge) {
             // what only later columns see must not reach the earlier ones as 0·∞
@@ -480,12 +485,17 @@ RT_DEV float paged_query(const float* q, float scale2, h8_t (&qh)[HD / 32], h8_t
         }
     return scale2 * ldexpf(1.0f, -e);
 }
-template <uint32_t N>
-RT_DEV void split_weights(const float (&p)[N], h8_t& hi, h8_t& lo) {
+// (hi towards zero, two at a time; what is left has at most 14 bits, lo the
+// nearest of it)
+RT_DEV void split_weights(const float (&p)[8], h8_t& hi, h8_t& lo) {
+    typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+    typedef float f2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (uint32_t r = 0; r < 8; ++r) {
-        hi[r] = (_Float16)p[r];
-        lo[r] = (_Float16)(p[r] - (float)hi[r]);
+    for (uint32_t r = 0; r < 8; r += 2) {
+        const h2_t h = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(p[r], p[r + 1]));
+        const h2_t l = __builtin_convertvector((f2_t{p[r] - (float)h[0], p[r + 1] - (float)h[1]}), h2_t);
+        hi[r] = h[0], hi[r + 1] = h[1];
+        lo[r] = l[0], lo[r + 1] = l[1];
     }
 }
 
@@ -526,7 +536,7 @@ RT_DEV void paged_f16(PagedAcc<HD, _Float16>& acc, const PagedView<_Float16>& v,
                 sb = mfma32(kv[u].k[i], ql[i], sb);
             }
 #pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) p[4 * u + r] = (sa[r] + sb[r]) * qs;
+            for (uint32_t r = 0; r < 4; ++r) p[4 * u + r] = sa[r] + sb[r];
         }
         if (edge) {
 #pragma unroll
@@ -537,7 +547,7 @@ RT_DEV void paged_f16(PagedAcc<HD, _Float16>& acc, const PagedView<_Float16>& v,
             kv[0].clear(p0 + 4 * g, v.lo, limx);
             kv[1].clear(p0 + 16 + 4 * g, v.lo, limx);
         }
-        acc.weigh(p);
+        acc.weigh(p, qs);
         h8_t ph, pl;
         split_weights(p, ph, pl);
 #pragma unroll
@@ -898,7 +908,7 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
             for (uint32_t u = 0; u < RT; ++u) {
                 float p[8];
 #pragma unroll
-                for (uint32_t r = 0; r < 8; ++r) p[r] = s[u][r / 4][r % 4] * qs[u];
+                for (uint32_t r = 0; r < 8; ++r) p[r] = s[u][r / 4][r % 4];
                 if (p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn_w || !there[0] || !there[1]) {
 #pragma unroll
                     for (uint32_t r = 0; r < 8; ++r) {
@@ -906,7 +916,7 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
                         if (pos < v.lo || pos >= lim[u] || !there[r / 4]) p[r] = NEG;
                     }
                 }
-                acc[u].weigh(p);
+                acc[u].weigh(p, qs[u]);
                 split_weights(p, ph[u], pl[u]);
             }
 #pragma unroll

@@ -126,6 +126,26 @@ RT_DEV int sum4_i(int v) {
     return v;
 }
 
+// The value of lane l ^ X, without LDS: within 16 lanes permutations of four, mirrors of
+// eight and sixteen and pairs of them; beyond, swaps of a register's rows with another's.
+template <uint32_t X>
+RT_DEV uint32_t lane_xor(uint32_t v) {
+    if constexpr (X >= 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);  // both halves the lower, the upper
+        return lane_xor<X - 32>(threadIdx.x & 32 ? r[0] : r[1]);
+    } else if constexpr (X >= 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // pairs of rows the even, the odd
+        return lane_xor<X - 16>(threadIdx.x & 16 ? r[0] : r[1]);
+    } else if constexpr (X >= 8) {
+        return lane_xor<15 - X>((uint32_t)dpp_i<DPP_ROW_MIRROR>((int)v));
+    } else if constexpr (X >= 4) {
+        return lane_xor<7 - X>((uint32_t)dpp_i<DPP_ROW_HALF_MIRROR>((int)v));
+    } else if constexpr (X > 0) {
+        return (uint32_t)dpp_i<DPP_QUAD_PERM(0 ^ X, 1 ^ X, 2 ^ X, 3 ^ X)>((int)v);
+    } else {
+        return v;
+    }
+}
 RT_DEV int sdot4(uint32_t a, uint32_t b, int c) {
     return __builtin_amdgcn_sdot4((int)a, (int)b, c, false);
 }
