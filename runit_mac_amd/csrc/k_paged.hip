@@ -264,8 +264,9 @@ struct PagedView {
     uint32_t num_pages, ps_shift;
     uint32_t tb, t1;        // tile 0 of the job's numbering, the end
     uint32_t lo;            // first position seen
-    RT_DEV uint32_t page(uint32_t t) const {  // (no page behind the end)
-        return t < t1 ? table[(tb + t) * RT_PAGED_TILE >> ps_shift] : num_pages;
+    RT_DEV uint32_t page(uint32_t t) const {  // t: the same in every lane; no page behind the end
+        typedef const __attribute__((address_space(4))) uint32_t* sptr_t;  // (a scalar load)
+        return t < t1 ? ((sptr_t)table)[(tb + t) * RT_PAGED_TILE >> ps_shift] : num_pages;
     }
     RT_DEV size_t place(uint32_t t, uint32_t page, uint32_t hd) const {
         return page * page_stride + (size_t)((tb + t) * RT_PAGED_TILE & ((1u << ps_shift) - 1)) * hd;
@@ -595,26 +596,33 @@ struct PagedCols {
         const uint32_t back = sr.n - (r - sr.first), len = b.kv_len[s];
         return back <= len ? min(len - back + 1, hi) : 0u;
     }
-    // a column's part of a chunk: outputs at d = i·16·VW + 4·g·VW + ...
-    template <uint32_t SR>
+    // a column's part of a chunk; BLK: the outputs are those of wide blocks, o[n]
+    // the elements 16n + 4g ..
+    template <uint32_t SR, bool BLK>
     RT_DEV void put(const PagedAcc<HD, T>& acc, const PagedJob& j, uint32_t job, uint32_t cc, bool alone) const {
         constexpr uint32_t VW = PagedTile<HD, T>::VW, VN = PagedTile<HD, T>::VN;
         if (cc >= ncl) return;
         const uint32_t g = (threadIdx.x & 63) >> 4;
         const size_t slot = ((size_t)job * a.b.KVH + kvh) * SR + cc, rh = (size_t)row(cc) * a.H + head(cc);
-        float* o = (alone ? a.out + rh * HD : a.part + slot * HD) + 4 * g * VW;
+        float* o = alone ? a.out + rh * HD : a.part + slot * HD;
         const float f = !alone ? 1.0f : acc.m == -__builtin_huge_valf() ? 0.0f : 1.0f / acc.l;
 #pragma unroll
-        for (uint32_t i = 0; i < VN; ++i)
+        for (uint32_t i = 0; i < VN; ++i) {
+            if constexpr (BLK) {
 #pragma unroll
-            for (uint32_t x = 0; x < 4; ++x)
+                for (uint32_t e = 0; e < VW; ++e) *(f32x4*)(o + (i * VW + e) * 16 + 4 * g) = acc.o[i][e] * f;
+            } else {
 #pragma unroll
-                for (uint32_t e = 0; e < VW; e += 4) {
-                    f32x4 y;
+                for (uint32_t x = 0; x < 4; ++x)
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) y[k] = acc.o[i][e + k][x] * f;
-                    *(f32x4*)(o + i * 16 * VW + x * VW + e) = y;
-                }
+                    for (uint32_t e = 0; e < VW; e += 4) {
+                        f32x4 y;
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) y[k] = acc.o[i][e + k][x] * f;
+                        *(f32x4*)(o + i * 16 * VW + (4 * g + x) * VW + e) = y;
+                    }
+            }
+        }
         if (g == 0) {
             if (!alone) {
                 a.ml[2 * slot] = acc.m;
@@ -795,22 +803,46 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
     if (last_of(whole, n)) meet(j.first, step, n, true);
 }
 
-// Two tiles in LDS: the key operands [2][HD / 32] of 64 lanes' 16 bytes, the
-// value operands [HD / 16]; the next two are brought while they are computed,
-// keys straight to LDS, values through registers, where pairs of positions are
-// put side by side.
+// Stages of two tiles in LDS, brought three ahead, nothing through registers:
+// the key operands [2][HD / 32] of 64 lanes' 16 bytes, then the values' rows as
+// they are, their 16-byte pieces permuted by the row so that the transposing
+// reads (lane a of 16: element a of four rows) meet all banks.
+template <int HD>
+struct PagedStage {
+    static constexpr uint32_t KOPS = HD / 16 * 64, VROW = HD / 8, LEN = KOPS + 32 * VROW, N = 4;  // in 16 bytes
+    static constexpr uint32_t LOADS = LEN / 64 / RT_PAGED_WAVES;  // of a wave
+    // place of piece p of row r
+    static RT_DEV uint32_t piece(uint32_t r, uint32_t p) {
+        return r * VROW + (p ^ (HD == 64 ? (r & 6) : 2 * (r & 7)));
+    }
+};
+// 16 bytes a lane from p (the lane's own) to LDS, lane 0's at `to`, each next behind it.  No registers
+// receive it, and the compiler knows nothing of it: with the builtin it would wait for all of them at
+// each read of LDS.  stages_left() is the wait.
+RT_DEV void bring16(const void* p, const void* to) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)to);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory", "m0");
+}
+// waits until at most n of the wave's stages are on their way
+template <uint32_t LOADS>
+RT_DEV void stages_left(uint32_t n) {
+    constexpr auto wait = [](uint32_t c) constexpr { return (c & 15) | (c >> 4) << 14 | 7 << 4 | 15 << 8; };
+    if (n >= 2) __builtin_amdgcn_s_waitcnt(wait(2 * LOADS));
+    else if (n == 1) __builtin_amdgcn_s_waitcnt(wait(LOADS));
+    else __builtin_amdgcn_s_waitcnt(wait(0));
+}
+
 template <int HD>
 RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co, const PagedJob& j, uint32_t job,
                        h8_t* lds) {
     typedef PagedTile<HD, _Float16> Tile;
-    typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
-    typedef const __attribute__((address_space(1))) uint32_t* gptr_t;
-    typedef __attribute__((address_space(3))) uint32_t* lptr_t;
+    typedef PagedStage<HD> Stage;
+    typedef short s4_t __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4_t* tptr_t;
     constexpr uint32_t RT = paged_rt<HD>(), NW = RT_PAGED_WAVES, SR = paged_slot_rows<HD, true>();
     constexpr uint32_t KN = Tile::KN, VW = Tile::VW, VN = Tile::VN;
-    constexpr uint32_t KOPS = 2 * KN * 64, STAGE = KOPS + VN * VW * 64;
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t c = lane & 15, g = lane >> 4, x = g, sub = x >> 1;
+    const uint32_t c = lane & 15, g = lane >> 4;
     const float NEG = -__builtin_huge_valf(), scale2 = a.scale * 1.44269504f;
     PagedView<_Float16> v = co.v;
     // the block's and the wave's columns: what the last (the most) and the first of them see
@@ -837,71 +869,68 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
         qs[u] = paged_query<HD>(co.q(min(16 * (RT * w + u) + c, co.ncl - 1)), scale2, qh[u], ql[u]);
         acc[u].start();
     }
-    typename Tile::vvec vr[2][VN];
-    auto bring = [&](uint32_t t, const uint32_t (&page)[2], uint32_t buf) {
-        const bool none[2] = {page[0] >= v.num_pages, page[1] >= v.num_pages};
-        const size_t off[2] = {v.place(t, none[0] ? 0 : page[0], HD), v.place(t + 1, none[1] ? 0 : page[1], HD)};
-#pragma unroll
-        for (uint32_t i = 0; i < 2 * KN / NW; ++i) {
-            const uint32_t kc = i * NW + w;
-            const _Float16* kp = v.k + (kc / KN ? off[1] : off[0]) + (size_t)c * HD + 8 * g + kc % KN * 32;
-            __builtin_amdgcn_global_load_lds((gptr_t)kp, (lptr_t)(lds + buf * STAGE + kc * 64), 16, 0, 0);
-        }
-        const uint32_t p = 4 * w + 2 * (x & 1), pos = (v.tb + t + sub) * RT_PAGED_TILE + p;
-        const _Float16* vp = v.v + (sub ? off[1] : off[0]) + (size_t)p * HD + c * VW;
-#pragma unroll
-        for (uint32_t r = 0; r < 2; ++r)
-#pragma unroll
-            for (uint32_t i = 0; i < VN; ++i) vr[r][i] = *(const typename Tile::vvec*)(vp + r * HD + i * 16 * VW);
-        // positions that no column sees may hold anything: zeros
-        if ((v.tb + t) * RT_PAGED_TILE < v.lo || (v.tb + t + 2) * RT_PAGED_TILE > limx || none[0] || none[1]) {
-#pragma unroll
-            for (uint32_t r = 0; r < 2; ++r)
-#pragma unroll
-                for (uint32_t i = 0; i < VN; ++i)
-                    if (pos + r < v.lo || pos + r >= limx || (sub ? none[1] : none[0])) vr[r][i] = typename Tile::vvec{};
-        }
-    };
-    auto store = [&](uint32_t buf) {
-        uint32_t* d = (uint32_t*)(lds + buf * STAGE + KOPS) + (w * 16 + c) * 4 + x;
-#pragma unroll
-        for (uint32_t i = 0; i < VN; ++i)
-#pragma unroll
-            for (uint32_t e = 0; e < VW; ++e)
-                d[(i * VW + e) * 256] = __builtin_bit_cast(uint32_t, h2_t{vr[0][i][e], vr[1][i][e]});
-    };
-    auto meet = [&]() {
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-    };
     const uint32_t t0 = 2 * j.chunk, step = 2 * j.chunks;
-    uint32_t page[2] = {v.page(t0), v.page(t0 + 1)}, next[2] = {v.page(t0 + step), v.page(t0 + step + 1)};
-    uint32_t buf = 0;
-    if (t0 < v.t1) {
-        bring(t0, page, 0);
-        store(0);
-    }
-    meet();
-    for (uint32_t t = t0; t < v.t1; t += step, buf ^= 1) {
-        const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE;
-        const bool there[2] = {page[0] < v.num_pages, page[1] < v.num_pages}, more = t + step < v.t1;
-        page[0] = next[0], page[1] = next[1];
-        if (more) bring(t + step, page, buf ^ 1);
-        next[0] = v.page(t + 2 * step), next[1] = v.page(t + 2 * step + 1);
+    const uint32_t turns = t0 < v.t1 ? (v.t1 - t0 + step - 1) / step : 0;
+    // turn i's tiles into stage i % N
+    auto bring = [&](uint32_t i, uint32_t pg0, uint32_t pg1) {
+        const uint32_t t = t0 + i * step;
+        const size_t off[2] = {v.place(t, pg0 < v.num_pages ? pg0 : 0, HD), v.place(t + 1, pg1 < v.num_pages ? pg1 : 0, HD)};
+        h8_t* st = lds + i % Stage::N * Stage::LEN;
+#pragma unroll
+        for (uint32_t x = 0; x < 2 * KN / NW; ++x) {
+            const uint32_t kc = x * NW + w;
+            const _Float16* kp = v.k + (kc / KN ? off[1] : off[0]) + (size_t)c * HD + 8 * g + kc % KN * 32;
+            bring16(kp, st + kc * 64);
+        }
+#pragma unroll
+        for (uint32_t x = 0; x < Stage::VROW / 2 / NW; ++x) {
+            const uint32_t n = (x * NW + w) * 64, r = (n + lane) / Stage::VROW, p = (n + lane) % Stage::VROW;
+            const uint32_t from = Stage::piece(r, p) - r * Stage::VROW;  // (a permutation that undoes itself)
+            const _Float16* vp = v.v + (n / Stage::VROW >= 16 ? off[1] : off[0]) + (size_t)(r & 15) * HD + from * 8;
+            bring16(vp, st + Stage::KOPS + n);
+        }
+    };
+    uint32_t pg[Stage::N][2];  // of turns i .. i + 3
+#pragma unroll
+    for (uint32_t i = 0; i < Stage::N; ++i) pg[i][0] = v.page(t0 + i * step), pg[i][1] = v.page(t0 + i * step + 1);
+#pragma unroll
+    for (uint32_t i = 0; i < Stage::N - 1; ++i)
+        if (i < turns) bring(i, pg[i][0], pg[i][1]);
+    for (uint32_t i = 0; i < turns; ++i) {
+        const uint32_t t = t0 + i * step, p0 = (v.tb + t) * RT_PAGED_TILE;
+        const bool there[2] = {pg[0][0] < v.num_pages, pg[0][1] < v.num_pages};
+        h8_t* st = lds + i % Stage::N * Stage::LEN;
+        stages_left<Stage::LOADS>(turns - 1 - i);
+        __builtin_amdgcn_s_barrier();  // (this stage is there, the one before is read)
+        asm volatile("" ::: "memory");
+        if (i + Stage::N - 1 < turns) bring(i + Stage::N - 1, pg[Stage::N - 1][0], pg[Stage::N - 1][1]);
+#pragma unroll
+        for (uint32_t k = 0; k + 1 < Stage::N; ++k) pg[k][0] = pg[k + 1][0], pg[k][1] = pg[k + 1][1];
+        pg[Stage::N - 1][0] = v.page(t + Stage::N * step), pg[Stage::N - 1][1] = v.page(t + Stage::N * step + 1);
+        if (p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limx || !there[0] || !there[1]) {
+            // positions that no column sees may hold anything: zeros
+            for (uint32_t n = tid; n < 32 * Stage::VROW; n += 64 * NW) {
+                const uint32_t r = n / Stage::VROW;
+                if (p0 + r < v.lo || p0 + r >= limx || !(r < 16 ? there[0] : there[1])) st[Stage::KOPS + n] = h8_t{};
+            }
+            __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (LDS)
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        }
         if (!idle && p0 < limx_w) {
-            const h8_t* op = lds + buf * STAGE + lane;
+            const h8_t* op = st + lane;
             f32x4 s[RT][2];
 #pragma unroll
             for (uint32_t u = 0; u < RT; ++u) s[u][0] = s[u][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (uint32_t i = 0; i < KN; ++i)
+            for (uint32_t n = 0; n < KN; ++n)
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
-                    const h8_t k = op[(h * KN + i) * 64];
+                    const h8_t k = op[(h * KN + n) * 64];
 #pragma unroll
-                    for (uint32_t u = 0; u < RT; ++u) s[u][h] = mfma32(k, qh[u][i], s[u][h]);
+                    for (uint32_t u = 0; u < RT; ++u) s[u][h] = mfma32(k, qh[u][n], s[u][h]);
 #pragma unroll
-                    for (uint32_t u = 0; u < RT; ++u) s[u][h] = mfma32(k, ql[u][i], s[u][h]);
+                    for (uint32_t u = 0; u < RT; ++u) s[u][h] = mfma32(k, ql[u][n], s[u][h]);
                 }
             h8_t ph[RT], pl[RT];
 #pragma unroll
@@ -920,18 +949,23 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
                 split_weights(p, ph[u], pl[u]);
             }
 #pragma unroll
-            for (uint32_t i = 0; i < VN; ++i)
+            for (uint32_t n = 0; n < HD / 16; ++n) {
+                s4_t y[2];  // element 16n + c of the positions 4g .. 4g + 3 of either tile
 #pragma unroll
-                for (uint32_t e = 0; e < VW; ++e) {
-                    const h8_t y = op[KOPS + (i * VW + e) * 64];
-#pragma unroll
-                    for (uint32_t u = 0; u < RT; ++u) acc[u].o[i][e] = mfma32(y, ph[u], acc[u].o[i][e]);
-#pragma unroll
-                    for (uint32_t u = 0; u < RT; ++u) acc[u].o[i][e] = mfma32(y, pl[u], acc[u].o[i][e]);
+                for (uint32_t h = 0; h < 2; ++h) {
+                    const uint32_t r = 16 * h + 4 * g + (c >> 2);
+                    const h8_t* row = st + Stage::KOPS + Stage::piece(r, 2 * n + ((c & 3) >> 1));
+                    y[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr_t)((const s4_t*)row + (c & 1)));
                 }
+                const h8_t vv = __builtin_bit_cast(h8_t, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (uint32_t u = 0; u < RT; ++u) acc[u].o[n / VW][n % VW] = mfma32(vv, ph[u], acc[u].o[n / VW][n % VW]);
+#pragma unroll
+                for (uint32_t u = 0; u < RT; ++u) acc[u].o[n / VW][n % VW] = mfma32(vv, pl[u], acc[u].o[n / VW][n % VW]);
+            }
         }
-        if (more) store(buf ^ 1);
-        meet();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (its reads are done before the next barrier)
     }
     if (idle) return;
     const bool alone = j.chunks == 1 && !a.shared_len;
@@ -939,17 +973,20 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
     for (uint32_t u = 0; u < RT; ++u) {
         const uint32_t cc = 16 * (RT * w + u) + c;
         acc[u].join();
-        if (!acc[u].finite())
+        if (acc[u].finite()) {
+            co.template put<SR, true>(acc[u], j, job, cc, alone);
+        } else {
             paged_f32<HD, _Float16, 2>(acc[u], v, co.q(min(cc, co.ncl - 1)), scale2, t0, step, lim[u], limn_w, limx_w);
-        co.template put<SR>(acc[u], j, job, cc, alone);
+            co.template put<SR, false>(acc[u], j, job, cc, alone);
+        }
     }
 }
 
 template <int HD, class T, bool WIDE>
 RT_DEV void paged_attn(const PagedAttnArgs& a) {
-    constexpr uint32_t NARROW = RT_PAGED_WAVES * 16 * (HD + 4 + 2) * 4;  // (two stages of a wide block are less)
-    static_assert(NARROW >= 2 * 128 * HD, "LDS");
-    __shared__ f32x4 lds[NARROW / 16];
+    constexpr uint32_t NARROW = RT_PAGED_WAVES * 16 * (HD + 4 + 2) / 4;  // in 16 bytes
+    constexpr uint32_t STAGES = WIDE ? PagedStage<HD>::N * PagedStage<HD>::LEN : 0;
+    __shared__ f32x4 lds[NARROW > STAGES ? NARROW : STAGES];
     const PagedBatch& b = a.b;
     const uint32_t kvh = blockIdx.x % b.KVH, job = blockIdx.x / b.KVH;
     const PagedJob j = paged_job<HD, T, WIDE>(a, job);
