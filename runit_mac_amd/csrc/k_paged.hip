@@ -113,9 +113,9 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 //
 // f32 pages use the f32 matrix cores.  f16 pages use the f16 ones, keys and
 // values as they are, queries and weights as pairs of f16 (x = hi + lo: 22
-// bits): queries scaled by a power of two to [2^14, 2^15) a column, weights by
-// 2^15, so that those down to 2^-17 of the largest keep their 22 bits and
-// smaller ones are off by at most 2^-40 of it.  A job whose sums come out not
+// bits): queries scaled by a power of two to [2^14, 2^15) a column, weights so
+// that the largest is between 2^12 and 2^15: those down to 2^-14 of it keep
+// their 22 bits, smaller ones are off by at most 2^-37 of it.  A job whose sums come out not
 // finite (a value that is not, in places that only some of its columns see; the
 // pairs make NaN of ∞ too) is computed again on the f32 matrix cores.
 
@@ -131,11 +131,12 @@ constexpr uint32_t paged_slot_rows() { return WIDE ? RT_PAGED_WAVES * 16 * paged
 struct PagedJob {
     uint32_t seq;             // n_seqs: the shared prefix
     uint32_t rb, chunk, first, chunks;  // block, chunk, first job of the block, its chunks
+    uint32_t row0, rows, kv;  // the sequence's rows and length (prefix: all rows, its length)
     uint32_t len;             // tiles of a chunk (at most)
     bool any;
 };
-RT_DEV uint32_t paged_tiles(const PagedAttnArgs& a, uint32_t s) {  // a sequence's own tiles
-    const uint32_t cap = a.b.table_stride << a.b.ps_shift, L = min(a.b.kv_len[s], cap);
+RT_DEV uint32_t paged_tiles(const PagedAttnArgs& a, uint32_t kv) {  // own tiles of a sequence of kv positions
+    const uint32_t cap = a.b.table_stride << a.b.ps_shift, L = min(kv, cap);
     const uint32_t t0 = a.shared_len / RT_PAGED_TILE;
     const uint32_t t1 = (L + RT_PAGED_TILE - 1) / RT_PAGED_TILE;
     return L > a.shared_len ? t1 - t0 : 0;
@@ -169,16 +170,20 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
         const uint32_t bc = paged_block<HD, WIDE>(rows * G);
         return (rows * G + bc - 1) / bc;
     };
-    // sequences s0 .. of the lanes: their blocks and tiles
-    uint32_t mb = 0, mt = 0;
+    // a lane's sequence: its rows, length, blocks and tiles
+    uint32_t mb = 0, mt = 0, mkv = 0;
+    SeqRows mr = {0, 0};
     auto look = [&](uint32_t s) {
-        mb = s < n ? blocks_of(seq_rows(a.b, s).n) : 0;
-        mt = s < n ? paged_tiles(a, s) : 0;
+        mr = s < n ? seq_rows(a.b, s) : SeqRows{0, 0};
+        mkv = s < n ? a.b.kv_len[s] : 0;
+        mb = blocks_of(mr.n);
+        mt = paged_tiles(a, mkv);
     };
     look(lane);
-    uint32_t pb = 0, pt = 0;
+    uint32_t pb = 0, pt = 0, all = 0;
     if (a.shared_len) {
-        pb = blocks_of(a.b.row_start ? min(a.b.row_start[n], a.b.rows) : min(n, a.b.rows));
+        all = a.b.row_start ? min(a.b.row_start[n], a.b.rows) : min(n, a.b.rows);
+        pb = blocks_of(all);
         pt = (a.shared_len + RT_PAGED_TILE - 1) / RT_PAGED_TILE;
     }
     float work = (float)mb * (float)mt;
@@ -209,8 +214,8 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
         if (fit) {  // (counted exactly before it is taken)
             const uint32_t c1 = __builtin_amdgcn_readlane(cl, __builtin_ctzll(fit));
             const float inv1 = 1.0f / (float)c1;
-            const uint32_t all = __builtin_amdgcn_readlane(wave_scan_add(mb * ceil_div(mt, c1, inv1)), 63);
-            if (all + pb * ceil_div(pt, c1, inv1) <= a.slots) j.len = c1;
+            const uint32_t own = __builtin_amdgcn_readlane(wave_scan_add(mb * ceil_div(mt, c1, inv1)), 63);
+            if (own + pb * ceil_div(pt, c1, inv1) <= a.slots) j.len = c1;
         }
     }
     const float inv = 1.0f / (float)j.len;
@@ -228,6 +233,7 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
         const uint32_t nc = ceil_div(pt, j.len, inv);
         if (job < pb * nc) {
             found(n, 0, nc);
+            j.rows = all, j.kv = a.shared_len;
             return j;
         }
         base = pb * nc;
@@ -240,6 +246,8 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
         if (hit) {
             const int l = __builtin_ctzll(hit);
             found(s0 + l, (uint32_t)__builtin_amdgcn_readlane(upto - mine, l), (uint32_t)__builtin_amdgcn_readlane(nc, l));
+            j.row0 = __builtin_amdgcn_readlane(mr.first, l), j.rows = __builtin_amdgcn_readlane(mr.n, l);
+            j.kv = __builtin_amdgcn_readlane(mkv, l);
             return j;
         }
         base = (uint32_t)__builtin_amdgcn_readlane(upto, 63);
@@ -284,10 +292,12 @@ struct PagedTile {
     typedef T vvec __attribute__((ext_vector_type(VW)));
     kvec k[KN];
     vvec v[4][VN];
-    RT_DEV void load(const T* kb, const T* vb, uint32_t lane) {
+    RT_DEV void load_k(const T* kb, uint32_t lane) {
         const T* kp = kb + (size_t)(lane & 15) * HD + (lane >> 4) * KW;
 #pragma unroll
         for (uint32_t i = 0; i < KN; ++i) k[i] = *(const kvec*)(kp + i * 4 * KW);
+    }
+    RT_DEV void load_v(const T* vb, uint32_t lane) {
 #pragma unroll
         for (uint32_t r = 0; r < 4; ++r) {
             const T* vp = vb + (size_t)(4 * (lane >> 4) + r) * HD + (lane & 15) * VW;
@@ -295,9 +305,11 @@ struct PagedTile {
             for (uint32_t i = 0; i < VN; ++i) v[r][i] = *(const vvec*)(vp + i * 16 * VW);
         }
     }
-    RT_DEV void none() {
+    RT_DEV void no_k() {
 #pragma unroll
         for (uint32_t i = 0; i < KN; ++i) k[i] = kvec{};
+    }
+    RT_DEV void no_v() {
 #pragma unroll
         for (uint32_t r = 0; r < 4; ++r)
 #pragma unroll
@@ -318,13 +330,14 @@ RT_DEV float column_max(float v) {
     return fmaxf(v, __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, v))));
 }
 
-// 16 columns' running maximum (in units of log 2), sum and outputs.  Lane (c =
+// 16 columns' running reference, near the maximum (in units of log 2), sum and outputs.  Lane (c =
 // l % 16, g = l / 16) has column c's outputs VW·(4g + x) + e of every 16·VW.
 template <int HD, class T>
 struct PagedAcc {
     typedef PagedTile<HD, T> Tile;
     static constexpr uint32_t VW = Tile::VW, VN = Tile::VN;
-    static constexpr float BIAS = sizeof(T) == 2 ? 15.0f : 0.0f;  // weights are 2^BIAS·e^(s − m)
+    // weights are 2^BIAS·e^(s − m); m follows the maximum when that has grown by 2^GROW
+    static constexpr float GROW = 3.0f, BIAS = sizeof(T) == 2 ? 15.0f - GROW : 0.0f;
     f32x4 o[VN][VW];
     float m, l;
     RT_DEV void start() {
@@ -343,7 +356,7 @@ struct PagedAcc {
 #pragma unroll
         for (uint32_t r = 1; r < N; ++r) tmax = fmaxf(tmax, p[r]);
         tmax = column_max(tmax) * scale;
-        if (__ballot(tmax > m)) {
+        if (__ballot(tmax > m + GROW)) {
             const float mn = fmaxf(m, tmax), md = mn == NEG ? 0.0f : mn, f = __builtin_amdgcn_exp2f(m - md);
             m = mn;
             l *= f;
@@ -384,29 +397,40 @@ RT_DEV void paged_f32(PagedAcc<HD, T>& acc, const PagedView<T>& v, const float* 
     typedef PagedTile<HD, T> Tile;
     constexpr uint32_t KW = Tile::KW, KN = Tile::KN, VW = Tile::VW, VN = Tile::VN;
     const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    auto after = [&](uint32_t t) { return RUN == 2 && t % 2 == 0 ? t + 1 : t + step - (RUN - 1); };
+    // the next tile's keys are on their way while this one's weights are made,
+    // its values from the second product on
+    Tile kv;
+    uint32_t page = v.page(t0);
+    if (page < v.num_pages) {
+        kv.load_k(v.k + v.place(t0, page, HD), lane);
+        kv.load_v(v.v + v.place(t0, page, HD), lane);
+    }
     float qf[KN][KW];
 #pragma unroll
     for (uint32_t i = 0; i < KN; ++i)
 #pragma unroll
         for (uint32_t e = 0; e < KW; e += 4) *(f32x4*)&qf[i][e] = *(const f32x4*)(q + i * 4 * KW + g * KW + e);
     acc.start();
-    auto after = [&](uint32_t t) { return RUN == 2 && t % 2 == 0 ? t + 1 : t + step - (RUN - 1); };
-    uint32_t next = v.page(t0);
+    uint32_t next = v.page(after(t0));
     for (uint32_t t = t0; t < v.t1; t = after(t)) {
-        const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE, page = next;
-        next = v.page(after(t));
-        if (page >= v.num_pages) continue;
-        const size_t off = v.place(t, page, HD);
-        Tile kv;
-        kv.load(v.k + off, v.v + off, lane);
+        const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE, tn = after(t);
+        const bool there = page < v.num_pages, more = next < v.num_pages;
+        const size_t off = v.place(t, there ? page : 0, HD), offn = v.place(tn, more ? next : 0, HD);
+        page = next;
+        next = v.page(after(tn));
         f32x4 sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
+        if (there) {
 #pragma unroll
-        for (uint32_t i = 0; i < KN; ++i)
+            for (uint32_t i = 0; i < KN; ++i)
 #pragma unroll
-            for (uint32_t e = 0; e < KW; e += 2) {
-                sa = mfma4((float)kv.k[i][e], qf[i][e], sa);
-                sb = mfma4((float)kv.k[i][e + 1], qf[i][e + 1], sb);
-            }
+                for (uint32_t e = 0; e < KW; e += 2) {
+                    sa = mfma4((float)kv.k[i][e], qf[i][e], sa);
+                    sb = mfma4((float)kv.k[i][e + 1], qf[i][e + 1], sb);
+                }
+        }
+        if (more) kv.load_k(v.k + offn, lane);
+        if (there) {
         const bool edge = p0 < v.lo || p0 + RT_PAGED_TILE > limn;
         float p[4];
 #pragma unroll
@@ -451,6 +475,8 @@ RT_DEV void paged_f32(PagedAcc<HD, T>& acc, const PagedView<T>& v, const float* 
                                 acc.o[i][e][x] = fmaf(pp, (float)vp[i * 16 * VW + x * VW + e], acc.o[i][e][x]);
                 }
         }
+        }
+        if (more) kv.load_v(v.v + offn, lane);
     }
     acc.join();
 }
@@ -508,24 +534,37 @@ RT_DEV void paged_f16(PagedAcc<HD, _Float16>& acc, const PagedView<_Float16>& v,
     typedef PagedTile<HD, _Float16> Tile;
     constexpr uint32_t KN = Tile::KN, VW = Tile::VW, VN = Tile::VN;
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
+    Tile kv[2];
+    uint32_t page[2] = {v.page(t0), v.page(t0 + 1)};
+    auto keys = [&](const bool (&there)[2], const size_t (&off)[2]) {
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            if (there[u]) kv[u].load_k(v.k + off[u], lane);
+            else kv[u].no_k();
+        }
+    };
+    auto values = [&](const bool (&there)[2], const size_t (&off)[2]) {
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            if (there[u]) kv[u].load_v(v.v + off[u], lane);
+            else kv[u].no_v();
+        }
+    };
+    bool there[2] = {page[0] < v.num_pages, page[1] < v.num_pages};
+    {
+        const size_t off[2] = {v.place(t0, there[0] ? page[0] : 0, HD), v.place(t0 + 1, there[1] ? page[1] : 0, HD)};
+        keys(there, off);
+        values(there, off);
+    }
+    page[0] = v.page(t0 + step), page[1] = v.page(t0 + step + 1);
     h8_t qh[KN], ql[KN];
     const float qs = paged_query<HD>(q, scale2, qh, ql);
     acc.start();
-    uint32_t next[2] = {v.page(t0), v.page(t0 + 1)};
     for (uint32_t t = t0; t < v.t1; t += step) {
-        const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE;
-        const bool there[2] = {next[0] < v.num_pages, next[1] < v.num_pages};
-        Tile kv[2];
-#pragma unroll
-        for (uint32_t u = 0; u < 2; ++u) {
-            if (there[u]) {
-                const size_t off = v.place(t + u, next[u], HD);
-                kv[u].load(v.k + off, v.v + off, lane);
-            } else {
-                kv[u].none();
-            }
-        }
-        next[0] = v.page(t + step), next[1] = v.page(t + step + 1);
+        const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE, tn = t + step;
+        const bool more[2] = {page[0] < v.num_pages, page[1] < v.num_pages};
+        const size_t off[2] = {v.place(tn, more[0] ? page[0] : 0, HD), v.place(tn + 1, more[1] ? page[1] : 0, HD)};
+        page[0] = v.page(tn + step), page[1] = v.page(tn + step + 1);
         float p[8];
         const bool edge = p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn || !there[0] || !there[1];
 #pragma unroll
@@ -539,6 +578,7 @@ RT_DEV void paged_f16(PagedAcc<HD, _Float16>& acc, const PagedView<_Float16>& v,
 #pragma unroll
             for (uint32_t r = 0; r < 4; ++r) p[4 * u + r] = sa[r] + sb[r];
         }
+        keys(more, off);
         if (edge) {
 #pragma unroll
             for (uint32_t r = 0; r < 8; ++r) {
@@ -561,6 +601,8 @@ RT_DEV void paged_f16(PagedAcc<HD, _Float16>& acc, const PagedView<_Float16>& v,
                 acc.o[i][e] = mfma32(a, ph, acc.o[i][e]);
                 acc.o[i][e] = mfma32(a, pl, acc.o[i][e]);
             }
+        values(more, off);
+        there[0] = more[0], there[1] = more[1];
     }
     acc.join();
 }
@@ -572,17 +614,17 @@ struct PagedCols {
     PagedView<T> v;
     uint32_t kvh, G, row0, col0, ncl, hi;
     bool pre;
-    uint32_t seq;
+    uint32_t rows, kv;  // of the sequence (not pre)
     RT_DEV uint32_t row(uint32_t cc) const { return row0 + (col0 + cc) / G; }
     RT_DEV uint32_t head(uint32_t cc) const { return kvh * G + (col0 + cc) % G; }
     RT_DEV const float* q(uint32_t cc) const { return a.q + ((size_t)row(cc) * a.H + head(cc)) * HD; }
     // positions below it are what a column sees; every lane of the wave calls it
     RT_DEV uint32_t lim(uint32_t cc) const {
-        const PagedBatch& b = a.b;
-        const uint32_t r = row(cc);
-        uint32_t s = seq;
+        uint32_t back = rows - (col0 + cc) / G, len = kv;  // the row is its sequence's back-th from the end
         if (pre) {
-            s = r;
+            const PagedBatch& b = a.b;
+            const uint32_t r = row(cc);
+            uint32_t s = r;
             if (b.row_start) {  // the sequences that end at or before the row
                 s = 0;
                 for (uint32_t s0 = 0; s0 < b.n_seqs; s0 += 64) {
@@ -591,9 +633,10 @@ struct PagedCols {
                 }
                 s = min(s, b.n_seqs - 1);
             }
+            const SeqRows sr = seq_rows(b, s);
+            back = sr.n - (r - sr.first);
+            len = b.kv_len[s];
         }
-        const SeqRows sr = seq_rows(b, s);
-        const uint32_t back = sr.n - (r - sr.first), len = b.kv_len[s];
         return back <= len ? min(len - back + 1, hi) : 0u;
     }
     // a column's part of a chunk; BLK: the outputs are those of wide blocks, o[n]
@@ -845,30 +888,9 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
     const uint32_t c = lane & 15, g = lane >> 4;
     const float NEG = -__builtin_huge_valf(), scale2 = a.scale * 1.44269504f;
     PagedView<_Float16> v = co.v;
-    // the block's and the wave's columns: what the last (the most) and the first of them see
-    uint32_t lim[RT], limx_w = 0, limn_w = 0xffffffffu;
-#pragma unroll
-    for (uint32_t u = 0; u < RT; ++u) {
-        lim[u] = co.lim(min(16 * (RT * w + u) + c, co.ncl - 1));
-        uint32_t mx = lim[u], mn = lim[u];
-        for (uint32_t o = 1; o < 16; o *= 2) {
-            mx = max(mx, __shfl_xor(mx, o, 64));
-            mn = min(mn, __shfl_xor(mn, o, 64));
-        }
-        limx_w = max(limx_w, (uint32_t)__builtin_amdgcn_readfirstlane(mx));
-        limn_w = min(limn_w, (uint32_t)__builtin_amdgcn_readfirstlane(mn));
-    }
     const bool idle = 16 * RT * w >= co.ncl;  // (brings tiles, computes none)
     const uint32_t limx = co.pre ? co.hi : __builtin_amdgcn_readfirstlane(co.lim(co.ncl - 1));
     v.t1 = min(v.t1, limx > v.lo ? (limx + RT_PAGED_TILE - 1) / RT_PAGED_TILE - v.tb : 0u);
-    h8_t qh[RT][KN], ql[RT][KN];
-    float qs[RT];
-    PagedAcc<HD, _Float16> acc[RT];
-#pragma unroll
-    for (uint32_t u = 0; u < RT; ++u) {
-        qs[u] = paged_query<HD>(co.q(min(16 * (RT * w + u) + c, co.ncl - 1)), scale2, qh[u], ql[u]);
-        acc[u].start();
-    }
     const uint32_t t0 = 2 * j.chunk, step = 2 * j.chunks;
     const uint32_t turns = t0 < v.t1 ? (v.t1 - t0 + step - 1) / step : 0;
     // turn i's tiles into stage i % N
@@ -896,6 +918,27 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
 #pragma unroll
     for (uint32_t i = 0; i < Stage::N - 1; ++i)
         if (i < turns) bring(i, pg[i][0], pg[i][1]);
+    // the wave's columns: what the last (the most) and the first of them see
+    uint32_t lim[RT], limx_w = 0, limn_w = 0xffffffffu;
+#pragma unroll
+    for (uint32_t u = 0; u < RT; ++u) {
+        lim[u] = co.lim(min(16 * (RT * w + u) + c, co.ncl - 1));
+        uint32_t mx = lim[u], mn = lim[u];
+        for (uint32_t o = 1; o < 16; o *= 2) {
+            mx = max(mx, __shfl_xor(mx, o, 64));
+            mn = min(mn, __shfl_xor(mn, o, 64));
+        }
+        limx_w = max(limx_w, (uint32_t)__builtin_amdgcn_readfirstlane(mx));
+        limn_w = min(limn_w, (uint32_t)__builtin_amdgcn_readfirstlane(mn));
+    }
+    h8_t qh[RT][KN], ql[RT][KN];
+    float qs[RT];
+    PagedAcc<HD, _Float16> acc[RT];
+#pragma unroll
+    for (uint32_t u = 0; u < RT; ++u) {
+        qs[u] = paged_query<HD>(co.q(min(16 * (RT * w + u) + c, co.ncl - 1)), scale2, qh[u], ql[u]);
+        acc[u].start();
+    }
     for (uint32_t i = 0; i < turns; ++i) {
         const uint32_t t = t0 + i * step, p0 = (v.tb + t) * RT_PAGED_TILE;
         const bool there[2] = {pg[0][0] < v.num_pages, pg[0][1] < v.num_pages};
@@ -993,24 +1036,14 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
     if (!j.any) return;
     const uint32_t G = a.H / b.KVH, cap = b.table_stride << b.ps_shift;
     const bool pre = j.seq == b.n_seqs;
-    uint32_t rows, row0 = 0, lo = 0, hi = a.shared_len;
-    const uint32_t* table = a.shared_table;
-    if (pre) {
-        rows = b.row_start ? min(b.row_start[b.n_seqs], b.rows) : min(b.n_seqs, b.rows);
-    } else {
-        const SeqRows sr = seq_rows(b, j.seq);
-        rows = sr.n;
-        row0 = sr.first;
-        lo = a.shared_len;
-        hi = min(b.kv_len[j.seq], cap);
-        table = b.table + (size_t)j.seq * b.table_stride;
-    }
+    const uint32_t rows = j.rows, lo = pre ? 0 : a.shared_len, hi = min(j.kv, cap);
+    const uint32_t* table = pre ? a.shared_table : b.table + (size_t)j.seq * b.table_stride;
     const uint32_t bc = paged_block<HD, WIDE>(rows * G), col0 = j.rb * bc;
     const size_t head = ((size_t)kvh << b.ps_shift) * HD;
     const uint32_t tb = lo / RT_PAGED_TILE, tend = hi > lo ? (hi + RT_PAGED_TILE - 1) / RT_PAGED_TILE - tb : 0;
     const PagedView<T> v{(const T*)b.k + head, (const T*)b.v + head, table, b.page_stride, b.num_pages, b.ps_shift,
                          tb, tend, lo};
-    const PagedCols<HD, T> co{a, v, kvh, G, row0, col0, min(bc, rows * G - col0), hi, pre, j.seq};
+    const PagedCols<HD, T> co{a, v, kvh, G, j.row0, col0, min(bc, rows * G - col0), hi, pre, rows, j.kv};
     if constexpr (WIDE) {
         if (bc > RT_PAGED_ROWS) {
             paged_wide<HD>(a, co, j, job, (h8_t*)lds);

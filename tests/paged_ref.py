@@ -71,8 +71,8 @@ class Batch:
         """The outputs in 64 bits, and a bound of an f32 computation's error:
         scores of hd + 16 roundings of Σ|qk|, a weight and their sum e^ of that
         each, sums of L terms and 64 more roundings, all of Σ w|v|.  f16 pages:
-        weights as pairs of f16 scaled to 2^15, the smaller half's last place
-        2^-24: an absolute 2^-40 of the largest weight, and that of the values."""
+        weights as pairs of f16, the largest scaled to 2^12 or more, the smaller half's last place
+        2^-24: an absolute 2^-37 of the largest weight, and that of the values."""
         H, KVH, hd, G = self.H, self.KVH, self.hd, self.H // self.KVH
         out, tol = np.zeros((self.R, H, hd)), np.zeros((self.R, H, hd))
         for s in range(len(self.seqs)):
@@ -92,7 +92,7 @@ class Batch:
                     mag = (np.abs(k) @ np.abs(q)).max() / np.sqrt(hd)
                     tol[r, h] = w @ np.abs(v) / w.sum() * (2 * (hd + 16) * mag + len(seen) + 64) * F32
                     if self.f16:
-                        tol[r, h] += len(seen) * np.abs(v).max(0) * w.max() / w.sum() * 2.0 ** -40
+                        tol[r, h] += len(seen) * np.abs(v).max(0) * w.max() / w.sum() * 2.0 ** -37
         return out, tol
 
 
