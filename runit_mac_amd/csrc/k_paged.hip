@@ -208,8 +208,17 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
         const float inv = 1.0f / (float)cl;
         auto about = [&](uint32_t t) { return fmaxf(1.0f, floorf(fmaf((float)t, inv, 0.9999f))); };
         float jobs = (float)pb * about(pt);
-        for (uint32_t s = 0; s < n; ++s)
+        // (a quarter of the sequences each wave)
+        __shared__ float sums[RT_PAGED_WAVES][64];
+        const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (w) jobs = 0.0f;
+        for (uint32_t s = w; s < n; s += RT_PAGED_WAVES)
             jobs += (float)__builtin_amdgcn_readlane(mb, s) * about((uint32_t)__builtin_amdgcn_readlane(mt, s));
+        sums[w][lane] = jobs;
+        __syncthreads();
+        jobs = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < RT_PAGED_WAVES; ++k) jobs += sums[k][lane];
         const uint64_t fit = __ballot(jobs <= (float)a.slots && cl < j.len);
         if (fit) {  // (counted exactly before it is taken)
             const uint32_t c1 = __builtin_amdgcn_readlane(cl, __builtin_ctzll(fit));
@@ -912,12 +921,25 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
             bring16(vp, st + Stage::KOPS + n);
         }
     };
-    uint32_t pg[Stage::N][2];  // of turns i .. i + 3
+    // page ids of 64 turns, one a lane (scalar loads in the loop would hold up its LDS reads, which
+    // share their counter)
+    uint32_t ids[2];
+    auto ids_from = [&](uint32_t i0) {
+        const uint32_t t = t0 + (i0 + lane) * step;
 #pragma unroll
-    for (uint32_t i = 0; i < Stage::N; ++i) pg[i][0] = v.page(t0 + i * step), pg[i][1] = v.page(t0 + i * step + 1);
+        for (uint32_t h = 0; h < 2; ++h)
+            ids[h] = i0 + lane < turns && t + h < v.t1 ? v.table[(v.tb + t + h) * RT_PAGED_TILE >> v.ps_shift] : v.num_pages;
+    };
+    auto id = [&](uint32_t i, uint32_t h) { return (uint32_t)__builtin_amdgcn_readlane(ids[h], i & 63); };
+    ids_from(0);
+    uint32_t here = 0;  // a bit a tile: of turns i .. i + 3, whether it has a page
 #pragma unroll
     for (uint32_t i = 0; i < Stage::N - 1; ++i)
-        if (i < turns) bring(i, pg[i][0], pg[i][1]);
+        if (i < turns) {
+            const uint32_t p0 = id(i, 0), p1 = id(i, 1);
+            here |= (p0 < v.num_pages ? 1u : 0u) << 2 * i | (p1 < v.num_pages ? 2u : 0u) << 2 * i;
+            bring(i, p0, p1);
+        }
     // the wave's columns: what the last (the most) and the first of them see
     uint32_t lim[RT], limx_w = 0, limn_w = 0xffffffffu;
 #pragma unroll
@@ -941,15 +963,19 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
     }
     for (uint32_t i = 0; i < turns; ++i) {
         const uint32_t t = t0 + i * step, p0 = (v.tb + t) * RT_PAGED_TILE;
-        const bool there[2] = {pg[0][0] < v.num_pages, pg[0][1] < v.num_pages};
+        const bool there[2] = {(here & 1) != 0, (here & 2) != 0};
         h8_t* st = lds + i % Stage::N * Stage::LEN;
         stages_left<Stage::LOADS>(turns - 1 - i);
         __builtin_amdgcn_s_barrier();  // (this stage is there, the one before is read)
         asm volatile("" ::: "memory");
-        if (i + Stage::N - 1 < turns) bring(i + Stage::N - 1, pg[Stage::N - 1][0], pg[Stage::N - 1][1]);
-#pragma unroll
-        for (uint32_t k = 0; k + 1 < Stage::N; ++k) pg[k][0] = pg[k + 1][0], pg[k][1] = pg[k + 1][1];
-        pg[Stage::N - 1][0] = v.page(t + Stage::N * step), pg[Stage::N - 1][1] = v.page(t + Stage::N * step + 1);
+        here >>= 2;
+        if (i + Stage::N - 1 < turns) {
+            const uint32_t in = i + Stage::N - 1;
+            if (in % 64 == 0) ids_from(in);
+            const uint32_t q0 = id(in, 0), q1 = id(in, 1);
+            here |= (q0 < v.num_pages ? 1u : 0u) << 4 | (q1 < v.num_pages ? 2u : 0u) << 4;
+            bring(in, q0, q1);
+        }
         if (p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limx || !there[0] || !there[1]) {
             // positions that no column sees may hold anything: zeros
             for (uint32_t n = tid; n < 32 * Stage::VROW; n += 64 * NW) {
