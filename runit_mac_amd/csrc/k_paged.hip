@@ -107,9 +107,12 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 // Narrow blocks (16 columns; decoding rows): the four waves take the chunk's
 // tiles in turn, keys and values straight from the pages into registers, each
 // with a softmax of its own, and meet in LDS.  Bound by the pages' bytes.
-// Wide blocks (f16 pages; prompt chunks, a shared prefix): each wave has 16·RT
-// columns of its own and all take every tile, from LDS.  Bound by the f16
-// matrix cores and, beside them, the softmax's vector operations.
+// Wide blocks (f16 pages; prompt chunks, a shared prefix): each of four waves has
+// 32 columns of its own and all take every tile, from LDS, on the 32x32x16 f16
+// matrix cores.  Bound by the instructions that go beside the matrix cores' —
+// they overlap up to about three vector operations a 16 cycles of matrix product
+// (measured) —, so that the 16x16x32 form, with twice the products to issue and
+// a second column's statistics a lane, was slower.
 //
 // f32 pages use the f32 matrix cores.  f16 pages use the f16 ones, keys and
 // values as they are, queries and weights as pairs of f16 (x = hi + lo: 22
@@ -119,10 +122,8 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 // finite (a value that is not, in places that only some of its columns see; the
 // pairs make NaN of ∞ too) is computed again on the f32 matrix cores.
 
-template <int HD>
-constexpr uint32_t paged_rt() { return HD == 256 ? 1 : 2; }
-template <int HD, bool WIDE>
-constexpr uint32_t paged_slot_rows() { return WIDE ? RT_PAGED_WAVES * 16 * paged_rt<HD>() : RT_PAGED_ROWS; }
+template <bool WIDE>
+constexpr uint32_t paged_slot_rows() { return WIDE ? RT_PAGED_WIDE_ROWS : RT_PAGED_ROWS; }
 
 // The jobs of one KV head: blocks × chunks of every sequence in turn (and, with
 // a shared prefix, before them those of all rows over it).  The chunk length
@@ -142,8 +143,8 @@ RT_DEV uint32_t paged_tiles(const PagedAttnArgs& a, uint32_t kv) {  // own tiles
     return L > a.shared_len ? t1 - t0 : 0;
 }
 // columns of a block of a sequence (or of all rows) with so many
-template <int HD, bool WIDE>
-RT_DEV uint32_t paged_block(uint32_t cols) { return WIDE && cols > 32 ? paged_slot_rows<HD, WIDE>() : RT_PAGED_ROWS; }
+template <bool WIDE>
+RT_DEV uint32_t paged_block(uint32_t cols) { return WIDE && cols > 32 ? paged_slot_rows<WIDE>() : RT_PAGED_ROWS; }
 RT_DEV uint32_t wave_scan_add(uint32_t v) {  // inclusive
     constexpr int ROW_SHR = 0x110, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143;
     v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ROW_SHR + 1, 0xF, 0xF, false);
@@ -167,7 +168,7 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
     constexpr uint32_t STEP = sizeof(T) == 2 ? 2 : 1;  // (f16 pages: tiles in pairs)
     const uint32_t lane = threadIdx.x & 63, G = a.H / a.b.KVH, n = a.b.n_seqs;
     auto blocks_of = [&](uint32_t rows) {
-        const uint32_t bc = paged_block<HD, WIDE>(rows * G);
+        const uint32_t bc = paged_block<WIDE>(rows * G);
         return (rows * G + bc - 1) / bc;
     };
     // a lane's sequence: its rows, length, blocks and tiles
@@ -490,7 +491,23 @@ RT_DEV void paged_f32(PagedAcc<HD, T>& acc, const PagedView<T>& v, const float* 
     acc.join();
 }
 
-// A column's query as pairs of f16, x·2^e = hi + lo; returns scale2·2^-e.
+// A column's query as pairs of f16, x·2^e = hi + lo, from the lane's part of it
+// and the column's largest; returns scale2·2^-e.
+template <uint32_t N>
+RT_DEV float split_query(const float (&x)[N][8], float mx, float scale2, h8_t (&qh)[N], h8_t (&ql)[N]) {
+    // (at most 126: 2^-e stays a normal number)
+    const int e = mx > 0.0f ? min(126, 15 - __builtin_amdgcn_frexp_expf(mx)) : 0;
+    const float f = ldexpf(1.0f, e);
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i)
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            const float y = x[i][k] * f;
+            qh[i][k] = (_Float16)y;
+            ql[i][k] = (_Float16)(y - (float)qh[i][k]);
+        }
+    return scale2 * ldexpf(1.0f, -e);
+}
 template <int HD>
 RT_DEV float paged_query(const float* q, float scale2, h8_t (&qh)[HD / 32], h8_t (&ql)[HD / 32]) {
     const uint32_t g = (threadIdx.x & 63) >> 4;
@@ -508,28 +525,19 @@ RT_DEV float paged_query(const float* q, float scale2, h8_t (&qh)[HD / 32], h8_t
         }
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    // (at most 126: 2^-e stays a normal number)
-    const int e = mx > 0.0f ? min(126, 15 - __builtin_amdgcn_frexp_expf(mx)) : 0;
-    const float f = ldexpf(1.0f, e);
-#pragma unroll
-    for (uint32_t i = 0; i < HD / 32; ++i)
-#pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) {
-            const float y = x[i][k] * f;
-            qh[i][k] = (_Float16)y;
-            ql[i][k] = (_Float16)(y - (float)qh[i][k]);
-        }
-    return scale2 * ldexpf(1.0f, -e);
+    return split_query<HD / 32>(x, mx, scale2, qh, ql);
 }
 // (hi towards zero, two at a time; what is left has at most 14 bits, lo the
 // nearest of it)
-RT_DEV void split_weights(const float (&p)[8], h8_t& hi, h8_t& lo) {
+RT_DEV void split_weights(const float* p, h8_t& hi, h8_t& lo) {
+    float minus = -1.0f;  // (known, it would be two conversions and subtractions; so it is one mixed fma each)
+    asm("" : "+s"(minus));
     typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
     typedef float f2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (uint32_t r = 0; r < 8; r += 2) {
         const h2_t h = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(p[r], p[r + 1]));
-        const h2_t l = __builtin_convertvector((f2_t{p[r] - (float)h[0], p[r + 1] - (float)h[1]}), h2_t);
+        const h2_t l = __builtin_convertvector((f2_t{fmaf((float)h[0], minus, p[r]), fmaf((float)h[1], minus, p[r + 1])}), h2_t);
         hi[r] = h[0], hi[r + 1] = h[1];
         lo[r] = l[0], lo[r + 1] = l[1];
     }
@@ -648,40 +656,41 @@ struct PagedCols {
         }
         return back <= len ? min(len - back + 1, hi) : 0u;
     }
-    // a column's part of a chunk; BLK: the outputs are those of wide blocks, o[n]
-    // the elements 16n + 4g ..
-    template <uint32_t SR, bool BLK>
+    // where a column's outputs of a chunk go, whole or in part
+    template <uint32_t SR>
+    RT_DEV float* place(uint32_t job, uint32_t cc, bool alone) const {
+        return alone ? a.out + ((size_t)row(cc) * a.H + head(cc)) * HD
+                     : a.part + (((size_t)job * a.b.KVH + kvh) * SR + cc) * HD;
+    }
+    template <uint32_t SR>
+    RT_DEV void state(const PagedJob& j, uint32_t job, uint32_t cc, float m, float l, bool alone) const {
+        const size_t slot = ((size_t)job * a.b.KVH + kvh) * SR + cc;
+        if (!alone) {
+            a.ml[2 * slot] = m;
+            a.ml[2 * slot + 1] = l;
+        }
+        if (j.chunk == 0) note<SR>(j, (size_t)row(cc) * a.H + head(cc), cc);
+    }
+    // of 16 columns
+    template <uint32_t SR>
     RT_DEV void put(const PagedAcc<HD, T>& acc, const PagedJob& j, uint32_t job, uint32_t cc, bool alone) const {
         constexpr uint32_t VW = PagedTile<HD, T>::VW, VN = PagedTile<HD, T>::VN;
         if (cc >= ncl) return;
         const uint32_t g = (threadIdx.x & 63) >> 4;
-        const size_t slot = ((size_t)job * a.b.KVH + kvh) * SR + cc, rh = (size_t)row(cc) * a.H + head(cc);
-        float* o = alone ? a.out + rh * HD : a.part + slot * HD;
+        float* o = place<SR>(job, cc, alone);
         const float f = !alone ? 1.0f : acc.m == -__builtin_huge_valf() ? 0.0f : 1.0f / acc.l;
 #pragma unroll
-        for (uint32_t i = 0; i < VN; ++i) {
-            if constexpr (BLK) {
+        for (uint32_t i = 0; i < VN; ++i)
 #pragma unroll
-                for (uint32_t e = 0; e < VW; ++e) *(f32x4*)(o + (i * VW + e) * 16 + 4 * g) = acc.o[i][e] * f;
-            } else {
+            for (uint32_t x = 0; x < 4; ++x)
 #pragma unroll
-                for (uint32_t x = 0; x < 4; ++x)
+                for (uint32_t e = 0; e < VW; e += 4) {
+                    f32x4 y;
 #pragma unroll
-                    for (uint32_t e = 0; e < VW; e += 4) {
-                        f32x4 y;
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) y[k] = acc.o[i][e + k][x] * f;
-                        *(f32x4*)(o + i * 16 * VW + (4 * g + x) * VW + e) = y;
-                    }
-            }
-        }
-        if (g == 0) {
-            if (!alone) {
-                a.ml[2 * slot] = acc.m;
-                a.ml[2 * slot + 1] = acc.l;
-            }
-            if (j.chunk == 0) note<SR>(j, rh, cc);
-        }
+                    for (uint32_t k = 0; k < 4; ++k) y[k] = acc.o[i][e + k][x] * f;
+                    *(f32x4*)(o + i * 16 * VW + (4 * g + x) * VW + e) = y;
+                }
+        if (g == 0) state<SR>(j, job, cc, acc.m, acc.l, alone);
     }
     template <uint32_t SR>
     RT_DEV void note(const PagedJob& j, size_t rh, uint32_t cc) const {
@@ -694,7 +703,7 @@ struct PagedCols {
 template <int HD, class T, bool WIDE>
 RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, const PagedJob& j, uint32_t job,
                          float* lds) {
-    constexpr uint32_t NW = RT_PAGED_WAVES, SR = paged_slot_rows<HD, WIDE>();
+    constexpr uint32_t NW = RT_PAGED_WAVES, SR = paged_slot_rows<WIDE>();
     constexpr uint32_t VW = PagedTile<HD, T>::VW, VN = PagedTile<HD, T>::VN;
     float (*olds)[16][HD + 4] = (float (*)[16][HD + 4])lds;
     float (*mlds)[16] = (float (*)[16])(lds + NW * 16 * (HD + 4)), (*llds)[16] = mlds + NW;
@@ -855,24 +864,25 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
     if (last_of(whole, n)) meet(j.first, step, n, true);
 }
 
-// Stages of two tiles in LDS, brought three ahead, nothing through registers:
-// the key operands [2][HD / 32] of 64 lanes' 16 bytes, then the values' rows as
-// they are, their 16-byte pieces permuted by the row so that the transposing
-// reads (lane a of 16: element a of four rows) meet all banks.
+// Stages of two tiles in LDS, brought three ahead, nothing through registers: 32
+// rows of keys, 32 of values, as they are but for their 16-byte pieces, permuted
+// by the row so that the reads (keys: 16 rows' same piece; values, transposing:
+// four pieces of eight rows) meet all banks.
 template <int HD>
 struct PagedStage {
-    static constexpr uint32_t KOPS = HD / 16 * 64, VROW = HD / 8, LEN = KOPS + 32 * VROW, N = 4;  // in 16 bytes
-    static constexpr uint32_t LOADS = LEN / 64 / RT_PAGED_WAVES;  // of a wave
-    // place of piece p of row r
+    static constexpr uint32_t ROW = HD / 8, LEN = 64 * ROW, N = 4;  // in 16 bytes
+    static constexpr uint32_t LOADS = LEN / 64 / RT_PAGED_WAVES;    // of a wave
+    // place of piece p of row r (32 ..: values)
     static RT_DEV uint32_t piece(uint32_t r, uint32_t p) {
-        return r * VROW + (p ^ (HD == 64 ? (r & 6) : 2 * (r & 7)));
+        const uint32_t x = r < 32 ? (HD == 64 ? r >> 1 & 7 : r & 15) : (HD == 64 ? r << 1 & 4 : r << 2 & 12);
+        return r * ROW + (p ^ x);
     }
 };
-// 16 bytes a lane from p (the lane's own) to LDS, lane 0's at `to`, each next behind it.  No registers
-// receive it, and the compiler knows nothing of it: with the builtin it would wait for all of them at
-// each read of LDS.  stages_left() is the wait.
-RT_DEV void bring16(const void* p, const void* to) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)to);
+// 16 bytes a lane from p (the lane's own) to LDS, lane 0's at byte `at`, each
+// next behind it.  No registers receive it, and the compiler knows nothing of
+// it: with the builtin it would wait for all of them at each read of LDS.
+// stages_left() is the wait.
+RT_DEV void bring16(const void* p, uint32_t at) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory", "m0");
 }
 // waits until at most n of the wave's stages are on their way
@@ -887,83 +897,101 @@ RT_DEV void stages_left(uint32_t n) {
 template <int HD>
 RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co, const PagedJob& j, uint32_t job,
                        h8_t* lds) {
-    typedef PagedTile<HD, _Float16> Tile;
     typedef PagedStage<HD> Stage;
+    typedef PagedAcc<HD, _Float16> Acc;
     typedef short s4_t __attribute__((ext_vector_type(4)));
+    typedef float f16v __attribute__((ext_vector_type(16)));
     typedef __attribute__((address_space(3))) s4_t* tptr_t;
-    constexpr uint32_t RT = paged_rt<HD>(), NW = RT_PAGED_WAVES, SR = paged_slot_rows<HD, true>();
-    constexpr uint32_t KN = Tile::KN, VW = Tile::VW, VN = Tile::VN;
+    constexpr uint32_t NW = RT_PAGED_WAVES, SR = RT_PAGED_WIDE_ROWS, KS = HD / 16, NB = HD / 32;
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t c = lane & 15, g = lane >> 4;
+    const uint32_t c = lane & 31, h = lane >> 5;  // column; of its positions and elements 4h .. of every 8
     const float NEG = -__builtin_huge_valf(), scale2 = a.scale * 1.44269504f;
     PagedView<_Float16> v = co.v;
-    const bool idle = 16 * RT * w >= co.ncl;  // (brings tiles, computes none)
+    const bool idle = 32 * w >= co.ncl;  // (brings tiles, computes none)
     const uint32_t limx = co.pre ? co.hi : __builtin_amdgcn_readfirstlane(co.lim(co.ncl - 1));
     v.t1 = min(v.t1, limx > v.lo ? (limx + RT_PAGED_TILE - 1) / RT_PAGED_TILE - v.tb : 0u);
     const uint32_t t0 = 2 * j.chunk, step = 2 * j.chunks;
     const uint32_t turns = t0 < v.t1 ? (v.t1 - t0 + step - 1) / step : 0;
-    // turn i's tiles into stage i % N
-    auto bring = [&](uint32_t i, uint32_t pg0, uint32_t pg1) {
-        const uint32_t t = t0 + i * step;
-        const size_t off[2] = {v.place(t, pg0 < v.num_pages ? pg0 : 0, HD), v.place(t + 1, pg1 < v.num_pages ? pg1 : 0, HD)};
-        h8_t* st = lds + i % Stage::N * Stage::LEN;
-#pragma unroll
-        for (uint32_t x = 0; x < 2 * KN / NW; ++x) {
-            const uint32_t kc = x * NW + w;
-            const _Float16* kp = v.k + (kc / KN ? off[1] : off[0]) + (size_t)c * HD + 8 * g + kc % KN * 32;
-            bring16(kp, st + kc * 64);
-        }
-#pragma unroll
-        for (uint32_t x = 0; x < Stage::VROW / 2 / NW; ++x) {
-            const uint32_t n = (x * NW + w) * 64, r = (n + lane) / Stage::VROW, p = (n + lane) % Stage::VROW;
-            const uint32_t from = Stage::piece(r, p) - r * Stage::VROW;  // (a permutation that undoes itself)
-            const _Float16* vp = v.v + (n / Stage::VROW >= 16 ? off[1] : off[0]) + (size_t)(r & 15) * HD + from * 8;
-            bring16(vp, st + Stage::KOPS + n);
-        }
-    };
-    // page ids of 64 turns, one a lane (scalar loads in the loop would hold up its LDS reads, which
-    // share their counter)
-    uint32_t ids[2];
+    // where the two tiles of 64 turns are, one turn a lane, from the KV head's part of the pool on (~0:
+    // nowhere).  Scalar loads in the loop would hold up its LDS reads, which share their counter.
+    uint64_t at[2];
     auto ids_from = [&](uint32_t i0) {
         const uint32_t t = t0 + (i0 + lane) * step;
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h)
-            ids[h] = i0 + lane < turns && t + h < v.t1 ? v.table[(v.tb + t + h) * RT_PAGED_TILE >> v.ps_shift] : v.num_pages;
+        for (uint32_t u = 0; u < 2; ++u) {
+            const uint32_t page =
+                i0 + lane < turns && t + u < v.t1 ? v.table[(v.tb + t + u) * RT_PAGED_TILE >> v.ps_shift] : v.num_pages;
+            at[u] = page < v.num_pages ? v.place(t + u, page, HD) * 2 : ~0ull;
+        }
     };
-    auto id = [&](uint32_t i, uint32_t h) { return (uint32_t)__builtin_amdgcn_readlane(ids[h], i & 63); };
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const h8_t*)lds);
+    // a wave's parts of a stage, 64 pieces each: what its lanes read from a tile's place on
+    const uint8_t* src[Stage::LOADS];
+#pragma unroll
+    for (uint32_t x = 0; x < Stage::LOADS; ++x) {
+        const uint32_t n = (x * NW + w) * 64 + lane, r = n / Stage::ROW, p = n % Stage::ROW;
+        // (the permutation undoes itself)
+        src[x] = (const uint8_t*)((r < 32 ? v.k : v.v) + (size_t)(r & 15) * HD + (Stage::piece(r, p) - r * Stage::ROW) * 8);
+    }
+    // turn i's tiles into stage i % N; whether they have a page, a bit each
+    auto bring = [&](uint32_t i) {
+        uint64_t off[2];
+        uint32_t there = 0;
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at[u], i & 63);
+            const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(at[u] >> 32), i & 63);
+            there |= hi != 0xffffffffu ? 1u << u : 0u;
+            off[u] = hi != 0xffffffffu ? (uint64_t)hi << 32 | lo : 0;  // (nowhere: the pool's first page)
+        }
+        const uint32_t st = lds0 + i % Stage::N * Stage::LEN * 16;
+#pragma unroll
+        for (uint32_t x = 0; x < Stage::LOADS; ++x) {
+            const uint32_t n = (x * NW + w) * 64;
+            bring16(src[x] + (n / Stage::ROW & 16 ? off[1] : off[0]), st + n * 16);
+        }
+        return there;
+    };
     ids_from(0);
-    uint32_t here = 0;  // a bit a tile: of turns i .. i + 3, whether it has a page
+    uint32_t here = 0;  // bring()'s bits of turns i .. i + 3
 #pragma unroll
     for (uint32_t i = 0; i < Stage::N - 1; ++i)
-        if (i < turns) {
-            const uint32_t p0 = id(i, 0), p1 = id(i, 1);
-            here |= (p0 < v.num_pages ? 1u : 0u) << 2 * i | (p1 < v.num_pages ? 2u : 0u) << 2 * i;
-            bring(i, p0, p1);
-        }
-    // the wave's columns: what the last (the most) and the first of them see
-    uint32_t lim[RT], limx_w = 0, limn_w = 0xffffffffu;
-#pragma unroll
-    for (uint32_t u = 0; u < RT; ++u) {
-        lim[u] = co.lim(min(16 * (RT * w + u) + c, co.ncl - 1));
-        uint32_t mx = lim[u], mn = lim[u];
-        for (uint32_t o = 1; o < 16; o *= 2) {
-            mx = max(mx, __shfl_xor(mx, o, 64));
-            mn = min(mn, __shfl_xor(mn, o, 64));
-        }
-        limx_w = max(limx_w, (uint32_t)__builtin_amdgcn_readfirstlane(mx));
-        limn_w = min(limn_w, (uint32_t)__builtin_amdgcn_readfirstlane(mn));
+        if (i < turns) here |= bring(i) << 2 * i;
+    // the column's limit, and what the last (the most) and the first of the wave's see
+    const uint32_t cc = min(32 * w + c, co.ncl - 1), lim = co.lim(cc);
+    uint32_t limx_w = lim, limn_w = lim;
+    for (uint32_t o = 1; o < 32; o *= 2) {
+        limx_w = max(limx_w, __shfl_xor(limx_w, o, 64));
+        limn_w = min(limn_w, __shfl_xor(limn_w, o, 64));
     }
-    h8_t qh[RT][KN], ql[RT][KN];
-    float qs[RT];
-    PagedAcc<HD, _Float16> acc[RT];
+    limx_w = __builtin_amdgcn_readfirstlane(limx_w);
+    limn_w = __builtin_amdgcn_readfirstlane(limn_w);
+    // the query: elements 16n + 8h .. of column c
+    h8_t qh[KS], ql[KS];
+    float qs;
+    {
+        const float* q = co.q(cc) + 8 * h;
+        float x[KS][8], mx = 0.0f;
 #pragma unroll
-    for (uint32_t u = 0; u < RT; ++u) {
-        qs[u] = paged_query<HD>(co.q(min(16 * (RT * w + u) + c, co.ncl - 1)), scale2, qh[u], ql[u]);
-        acc[u].start();
+        for (uint32_t n = 0; n < KS; ++n)
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e += 4) {
+                const f32x4 y = *(const f32x4*)(q + 16 * n + e);
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    x[n][e + k] = y[k];
+                    mx = fmaxf(mx, fabsf(y[k]));
+                }
+            }
+        qs = split_query<KS>(x, fmaxf(mx, __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, mx)))), scale2, qh, ql);
     }
+    f16v o[NB];
+#pragma unroll
+    for (uint32_t n = 0; n < NB; ++n) o[n] = f16v{};
+    float m = NEG, l = 0.0f;
     for (uint32_t i = 0; i < turns; ++i) {
-        const uint32_t t = t0 + i * step, p0 = (v.tb + t) * RT_PAGED_TILE;
-        const bool there[2] = {(here & 1) != 0, (here & 2) != 0};
+        const uint32_t p0 = (v.tb + t0 + i * step) * RT_PAGED_TILE;
+        const uint32_t there = here & 3;
         h8_t* st = lds + i % Stage::N * Stage::LEN;
         stages_left<Stage::LOADS>(turns - 1 - i);
         __builtin_amdgcn_s_barrier();  // (this stage is there, the one before is read)
@@ -972,82 +1000,103 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
         if (i + Stage::N - 1 < turns) {
             const uint32_t in = i + Stage::N - 1;
             if (in % 64 == 0) ids_from(in);
-            const uint32_t q0 = id(in, 0), q1 = id(in, 1);
-            here |= (q0 < v.num_pages ? 1u : 0u) << 4 | (q1 < v.num_pages ? 2u : 0u) << 4;
-            bring(in, q0, q1);
+            here |= bring(in) << 4;
         }
-        if (p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limx || !there[0] || !there[1]) {
+        if (p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limx || there != 3) {
             // positions that no column sees may hold anything: zeros
-            for (uint32_t n = tid; n < 32 * Stage::VROW; n += 64 * NW) {
-                const uint32_t r = n / Stage::VROW;
-                if (p0 + r < v.lo || p0 + r >= limx || !(r < 16 ? there[0] : there[1])) st[Stage::KOPS + n] = h8_t{};
+            for (uint32_t n = tid; n < 32 * Stage::ROW; n += 64 * NW) {
+                const uint32_t r = n / Stage::ROW;
+                if (p0 + r < v.lo || p0 + r >= limx || !(there >> r / 16 & 1)) st[32 * Stage::ROW + n] = h8_t{};
             }
             __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (LDS)
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
         }
         if (!idle && p0 < limx_w) {
-            const h8_t* op = st + lane;
-            f32x4 s[RT][2];
+            f16v s = {};
 #pragma unroll
-            for (uint32_t u = 0; u < RT; ++u) s[u][0] = s[u][1] = f32x4{0, 0, 0, 0};
+            for (uint32_t n = 0; n < KS; ++n) {
+                const h8_t k = st[Stage::piece(c, 2 * n + h)];
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[n], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[n], s, 0, 0, 0);
+            }
+            float p[16];  // of the positions 8(r / 4) + 4h + r % 4
 #pragma unroll
-            for (uint32_t n = 0; n < KN; ++n)
+            for (uint32_t r = 0; r < 16; ++r) p[r] = s[r];
+            if (p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn_w || there != 3) {
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    const h8_t k = op[(h * KN + n) * 64];
-#pragma unroll
-                    for (uint32_t u = 0; u < RT; ++u) s[u][h] = mfma32(k, qh[u][n], s[u][h]);
-#pragma unroll
-                    for (uint32_t u = 0; u < RT; ++u) s[u][h] = mfma32(k, ql[u][n], s[u][h]);
+                for (uint32_t r = 0; r < 16; ++r) {
+                    const uint32_t pos = p0 + 8 * (r / 4) + 4 * h + r % 4;
+                    if (pos < v.lo || pos >= lim || !(there >> r / 8 & 1)) p[r] = NEG;
                 }
-            h8_t ph[RT], pl[RT];
+            }
+            float tmax = p[0];
 #pragma unroll
-            for (uint32_t u = 0; u < RT; ++u) {
-                float p[8];
+            for (uint32_t r = 1; r < 16; ++r) tmax = fmaxf(tmax, p[r]);
+            tmax = fmaxf(tmax, __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, tmax)))) * qs;
+            if (__ballot(tmax > m + Acc::GROW)) {
+                const float mn = fmaxf(m, tmax), f = __builtin_amdgcn_exp2f(m - (mn == NEG ? 0.0f : mn));
+                m = mn;
+                l *= f;
 #pragma unroll
-                for (uint32_t r = 0; r < 8; ++r) p[r] = s[u][r / 4][r % 4];
-                if (p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn_w || !there[0] || !there[1]) {
+                for (uint32_t n = 0; n < NB; ++n) o[n] *= f;
+            }
+            const float md = (m == NEG ? 0.0f : m) - Acc::BIAS;
 #pragma unroll
-                    for (uint32_t r = 0; r < 8; ++r) {
-                        const uint32_t pos = p0 + 16 * (r / 4) + 4 * g + r % 4;
-                        if (pos < v.lo || pos >= lim[u] || !there[r / 4]) p[r] = NEG;
+            for (uint32_t r = 0; r < 16; ++r) {
+                p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], qs, -md));
+                l += p[r];
+            }
+            h8_t ph[2], pl[2];
+            split_weights(p, ph[0], pl[0]);
+            split_weights(p + 8, ph[1], pl[1]);
+#pragma unroll
+            for (uint32_t n = 0; n < NB; ++n)
+#pragma unroll
+                for (uint32_t x = 0; x < 2; ++x) {
+                    s4_t y[2];  // element 32n + c of the positions 16x + 4h .., and eight on
+#pragma unroll
+                    for (uint32_t k = 0; k < 2; ++k) {
+                        const uint32_t r = 32 + 16 * x + 8 * k + 4 * h + (lane >> 2 & 3);
+                        const h8_t* at = st + Stage::piece(r, 4 * n + (lane >> 3 & 2) + (lane >> 1 & 1));
+                        y[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr_t)((const s4_t*)at + (lane & 1)));
                     }
+                    const h8_t vv = __builtin_bit_cast(h8_t, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, ph[x], o[n], 0, 0, 0);
+                    o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, pl[x], o[n], 0, 0, 0);
                 }
-                acc[u].weigh(p, qs[u]);
-                split_weights(p, ph[u], pl[u]);
-            }
-#pragma unroll
-            for (uint32_t n = 0; n < HD / 16; ++n) {
-                s4_t y[2];  // element 16n + c of the positions 4g .. 4g + 3 of either tile
-#pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    const uint32_t r = 16 * h + 4 * g + (c >> 2);
-                    const h8_t* row = st + Stage::KOPS + Stage::piece(r, 2 * n + ((c & 3) >> 1));
-                    y[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr_t)((const s4_t*)row + (c & 1)));
-                }
-                const h8_t vv = __builtin_bit_cast(h8_t, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                for (uint32_t u = 0; u < RT; ++u) acc[u].o[n / VW][n % VW] = mfma32(vv, ph[u], acc[u].o[n / VW][n % VW]);
-#pragma unroll
-                for (uint32_t u = 0; u < RT; ++u) acc[u].o[n / VW][n % VW] = mfma32(vv, pl[u], acc[u].o[n / VW][n % VW]);
-            }
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (its reads are done before the next barrier)
     }
     if (idle) return;
     const bool alone = j.chunks == 1 && !a.shared_len;
+    l += __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, l)));
+    bool bad = !(l < __builtin_huge_valf());
 #pragma unroll
-    for (uint32_t u = 0; u < RT; ++u) {
-        const uint32_t cc = 16 * (RT * w + u) + c;
-        acc[u].join();
-        if (acc[u].finite()) {
-            co.template put<SR, true>(acc[u], j, job, cc, alone);
-        } else {
-            paged_f32<HD, _Float16, 2>(acc[u], v, co.q(min(cc, co.ncl - 1)), scale2, t0, step, lim[u], limn_w, limx_w);
-            co.template put<SR, false>(acc[u], j, job, cc, alone);
+    for (uint32_t n = 0; n < NB; ++n)
+#pragma unroll
+        for (uint32_t r = 0; r < 16; ++r) bad |= !(fabsf(o[n][r]) < __builtin_huge_valf());
+    if (!__ballot(bad)) {
+        if (32 * w + c < co.ncl) {
+            float* to = co.template place<SR>(job, cc, alone) + 4 * h;
+            const float f = !alone ? 1.0f : m == NEG ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (uint32_t n = 0; n < NB; ++n)
+#pragma unroll
+                for (uint32_t x = 0; x < 4; ++x)
+                    *(f32x4*)(to + 32 * n + 8 * x) = f32x4{o[n][4 * x], o[n][4 * x + 1], o[n][4 * x + 2], o[n][4 * x + 3]} * f;
+            if (h == 0) co.template state<SR>(j, job, cc, m, l, alone);
         }
+        return;
+    }
+#pragma unroll 1
+    for (uint32_t u = 0; u < 2; ++u) {  // 16 columns at a time
+        const uint32_t c1 = 32 * w + 16 * u + (lane & 15), c2 = min(c1, co.ncl - 1);
+        if (32 * w + 16 * u >= co.ncl) break;
+        Acc acc;
+        paged_f32<HD, _Float16, 2>(acc, v, co.q(c2), scale2, t0, step, co.lim(c2), limn_w, limx_w);
+        co.template put<SR>(acc, j, job, c1, alone);
     }
 }
 
@@ -1064,7 +1113,7 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
     const bool pre = j.seq == b.n_seqs;
     const uint32_t rows = j.rows, lo = pre ? 0 : a.shared_len, hi = min(j.kv, cap);
     const uint32_t* table = pre ? a.shared_table : b.table + (size_t)j.seq * b.table_stride;
-    const uint32_t bc = paged_block<HD, WIDE>(rows * G), col0 = j.rb * bc;
+    const uint32_t bc = paged_block<WIDE>(rows * G), col0 = j.rb * bc;
     const size_t head = ((size_t)kvh << b.ps_shift) * HD;
     const uint32_t tb = lo / RT_PAGED_TILE, tend = hi > lo ? (hi + RT_PAGED_TILE - 1) / RT_PAGED_TILE - tb : 0;
     const PagedView<T> v{(const T*)b.k + head, (const T*)b.v + head, table, b.page_stride, b.num_pages, b.ps_shift,
@@ -1083,7 +1132,7 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
 // the prefix's after the sequence's own
 template <int HD, bool WIDE>
 RT_DEV void paged_merge(const PagedAttnArgs& a) {
-    constexpr uint32_t TH = HD / 4, SR = paged_slot_rows<HD, WIDE>();
+    constexpr uint32_t TH = HD / 4, SR = paged_slot_rows<WIDE>();
     const PagedBatch& b = a.b;
     const uint32_t i = blockIdx.x * 256 + threadIdx.x, rh = i / TH, d = i % TH * 4;
     const uint32_t rows = b.row_start ? min(b.row_start[b.n_seqs], b.rows) : min(b.n_seqs, b.rows);

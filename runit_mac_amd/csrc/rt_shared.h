@@ -51,6 +51,7 @@ constexpr uint32_t RT_STEP_STATUS_OFF = 1280;  // its status word
 constexpr uint32_t RT_PAGED_ROWS = 16;
 constexpr uint32_t RT_PAGED_TILE = 16;
 constexpr uint32_t RT_PAGED_WAVES = 4;
+constexpr uint32_t RT_PAGED_WIDE_ROWS = 128;  // columns of a wide block, 32 a wave
 
 // One batch over a paged cache, as rt_paged_batch describes it.
 struct PagedBatch {

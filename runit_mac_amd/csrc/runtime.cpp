@@ -4238,7 +4238,7 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     // where one sequence's rows, or all over the prefix, may fill one
     const uint64_t cols = (uint64_t)rows * G, n = a.b.n_seqs;
     const bool wide = batch->f16 && cols > 32 && (shared_len || (rows >= n && (rows - n + 1) * G > 32));
-    const uint64_t SR = wide ? (hd == 256 ? 64 : 128) : RT_PAGED_ROWS;
+    const uint64_t SR = wide ? RT_PAGED_WIDE_ROWS : RT_PAGED_ROWS;
     uint64_t blocks = a.b.row_start ? cols / RT_PAGED_ROWS + n : n * ((G + RT_PAGED_ROWS - 1) / RT_PAGED_ROWS);
     if (wide) blocks = std::min(blocks, 2 * n + cols / SR);
     if (shared_len) blocks += (cols + SR - 1) / SR + 1;
@@ -4252,7 +4252,6 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     a.target = (uint32_t)(blocks >= 8 * slots ? 0 : blocks < slots / 2 ? slots - blocks : slots);
     const bool noted = wide || shared_len;  // (chunks meet in a launch of their own)
     if (!noted && 2 * (blocks + a.target) * a.b.KVH > kAttnCounters) a.target = 0;
-    if (getenv("XM")) a.min_chunk = atoi(getenv("XM"));
     a.jobs = (uint32_t)(blocks + a.target);
     a.slots = (uint32_t)std::min<uint64_t>(slots, a.jobs);
     if (noted || a.target) {
