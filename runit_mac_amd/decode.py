@@ -597,6 +597,45 @@ class DecodeModel:
     VERIFY_ROWS_MAX = 5
     VERIFY_ROWS_MAX_HIDDEN = 1024
 
+    def row_form(self, M: int) -> str:
+        """The form of a pass over M rows, "rows" or "gemm"."""
+        return "rows" if M <= self.VERIFY_ROWS_MAX and self.cfg.hidden <= self.VERIFY_ROWS_MAX_HIDDEN else "gemm"
+
+    def qkv_rows(self, L, F, B, M: int) -> None:
+        """Q/K/V (+ bias) of the normalised rows B["x"] by the multi-row
+        GEMVs, one call per format."""
+        c = self.cfg
+        for fmt in dict.fromkeys((F["q"], F["k"], F["v"])):
+            sel = lambda role, key: L[key] if F[role] == fmt else None
+            d.qkv_bias_rows_f32(self.ctx, fmt, sel("q", "wq"), sel("k", "wk"), sel("v", "wv"), B["x"],
+                                B["q"] if F["q"] == fmt else None,
+                                B["k"] if F["k"] == fmt else None,
+                                B["v"] if F["v"] == fmt else None,
+                                sel("q", "bq"), sel("k", "bk"), sel("v", "bv"), M, c.q_dim, c.kv_dim,
+                                c.hidden, gamma=L["attn_norm"], eps=c.eps)
+
+    def out_ffn_rows(self, L, F, B, M: int) -> None:
+        """O (+ residual), gate+up+SiLU of the normalised rows and down (+
+        residual) by the multi-row GEMVs, B["att"] and B["x"] into B["x"]."""
+        ctx, c = self.ctx, self.cfg
+        X = B["x"]
+        d.gemv_rows_add_f32(ctx, F["o"], L["wo"], B["att"], X, X, M, c.hidden, c.q_dim)
+        if F["gate"] != F["up"]:
+            raise ValueError(f"gate {F['gate']} / up {F['up']}: no fused gate+up+SiLU")
+        d.fused_ffn_rows_f32(ctx, F["gate"], L["wg"], L["wu"], X, B["g"], M, c.ff, c.hidden,
+                             gamma=L["ffn_norm"], eps=c.eps)
+        d.gemv_rows_add_f32(ctx, F["down"], L["wd"], B["g"], X, X, M, c.hidden, c.ff)
+
+    def head_rows(self, form: str, x, logits, xn, M: int) -> None:
+        """The final norm and the LM head of M rows x."""
+        ctx, c = self.ctx, self.cfg
+        if form == "rows":
+            d.gemv_rows_f32(ctx, self.lm_fmt, self.lm_head, x, logits, M, c.vocab, c.hidden,
+                            gamma=self.final_norm, eps=c.eps)
+        else:
+            d.gemm_set_f32(ctx, [self.lm_fmt], [self.lm_head], [logits], [c.vocab], x, M, c.hidden,
+                           gamma=self.final_norm, eps=c.eps, xn=xn)
+
     def verify_pass(self, M: int, start_pos: int, form: str | None = None,
                     last_only: bool = False) -> dict:
         """The launches of verify_forward for the M token ids already in the
@@ -608,23 +647,14 @@ class DecodeModel:
         B = self._verify_arena(M, logits=not last_only)
         h, qd, kvd, hd, ff = c.hidden, c.q_dim, c.kv_dim, c.head_dim, c.ff
         X, XN, Xo = B["x"], B["xn"], B["p"]
-        form = form or ("rows" if M <= self.VERIFY_ROWS_MAX and h <= self.VERIFY_ROWS_MAX_HIDDEN
-                        else "gemm")
+        form = form or self.row_form(M)
         if form not in ("rows", "gemm"):
             raise ValueError("form must be 'rows' or 'gemm'")
         d.embed_rows_f32(ctx, self.embd_fmt, self.embd, B["tok"], X, h, M)
 
         for L, F in zip(self.layers, self.fmts):
             if form == "rows":
-                # Q/K/V (+ bias) of the normalised rows, one call per format
-                for fmt in dict.fromkeys((F["q"], F["k"], F["v"])):
-                    sel = lambda role, key: L[key] if F[role] == fmt else None
-                    d.qkv_bias_rows_f32(ctx, fmt, sel("q", "wq"), sel("k", "wk"), sel("v", "wv"), X,
-                                        B["q"] if F["q"] == fmt else None,
-                                        B["k"] if F["k"] == fmt else None,
-                                        B["v"] if F["v"] == fmt else None,
-                                        sel("q", "bq"), sel("k", "bk"), sel("v", "bv"), M, qd, kvd, h,
-                                        gamma=L["attn_norm"], eps=c.eps)
+                self.qkv_rows(L, F, B, M)
                 d.rope_kv_write_batch_f32(ctx, B["q"], B["k"], B["v"], L["kc"], L["vc"], hd, c.heads,
                                           c.kv_heads, start_pos, c.theta, M, c.max_seq)
             else:
@@ -638,12 +668,7 @@ class DecodeModel:
             if form == "rows":
                 d.flash_attention_f32(ctx, B["q"], L["kc"], L["vc"], B["att"], 1, M, start_pos + M,
                                       c.heads, c.kv_heads, hd, c.max_seq, q_start=start_pos)
-                d.gemv_rows_add_f32(ctx, F["o"], L["wo"], B["att"], X, X, M, h, qd)
-                if F["gate"] != F["up"]:
-                    raise ValueError(f"gate {F['gate']} / up {F['up']}: no fused gate+up+SiLU")
-                d.fused_ffn_rows_f32(ctx, F["gate"], L["wg"], L["wu"], X, B["g"], M, ff, h,
-                                     gamma=L["ffn_norm"], eps=c.eps)
-                d.gemv_rows_add_f32(ctx, F["down"], L["wd"], B["g"], X, X, M, h, ff)
+                self.out_ffn_rows(L, F, B, M)
             else:
                 # the attention, O + residual (into Xo), norm, gate/up + SiLU,
                 # down + residual (back into X): the attention's key-range
@@ -660,12 +685,8 @@ class DecodeModel:
             # continues at position start_pos + M
             self._lm_head(X + 4 * (M - 1) * h)
             d.argmax_f32(ctx, self.logits, self.token, c.vocab)
-        elif form == "rows":
-            d.gemv_rows_f32(ctx, self.lm_fmt, self.lm_head, X, B["logits"], M, c.vocab, h,
-                            gamma=self.final_norm, eps=c.eps)
         else:
-            d.gemm_set_f32(ctx, [self.lm_fmt], [self.lm_head], [B["logits"]], [c.vocab], X, M, h,
-                           gamma=self.final_norm, eps=c.eps, xn=XN)
+            self.head_rows(form, X, B["logits"], XN, M)
         if not last_only:
             d.argmax_rows_first_f32(ctx, B["logits"], B["idx"], M, c.vocab)
         return B
