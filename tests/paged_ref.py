@@ -67,12 +67,13 @@ class Batch:
                             self.hd, self.bt, self.stride, len(self.seqs), self.bl, rows=self.rows,
                             row_start=self.bs, page_stride=self.page if self.gap else 0)
 
-    def attention(self, keys=None, vals=None):
+    def attention(self, keys=None, vals=None, only=None):
         """The outputs in 64 bits, and a bound of an f32 computation's error:
         scores of hd + 16 roundings of Σ|qk|, a weight and their sum e^ of that
         each, sums of L terms and 64 more roundings, all of Σ w|v|.  f16 pages:
         weights as pairs of f16, the largest scaled to 2^12 or more, the smaller half's last place
-        2^-24: an absolute 2^-37 of the largest weight, and that of the values."""
+        2^-24: an absolute 2^-37 of the largest weight, and that of the values.
+        `only`: of these rows (the others' are zeros)."""
         H, KVH, hd, G = self.H, self.KVH, self.hd, self.H // self.KVH
         out, tol = np.zeros((self.R, H, hd)), np.zeros((self.R, H, hd))
         for s in range(len(self.seqs)):
@@ -81,7 +82,7 @@ class Batch:
             for i in range(int(self.new[s])):
                 r, p = int(self.start[s]) + i, int(self.kv[s] - self.new[s]) + i
                 seen = np.flatnonzero(~np.isnan(K[:p + 1, 0, 0])) if p >= 0 else np.zeros(0, int)
-                if not len(seen):
+                if not len(seen) or only is not None and r not in only:
                     continue
                 for h in range(H):
                     k, v = K[seen, h // G], V[seen, h // G]

@@ -132,6 +132,36 @@ def test_later_values_stay_with_the_rows_that_see_them(ctx, bad, f16):
     check(got[~sees], ref[~sees], tol[~sees])
 
 
+@pytest.mark.parametrize("H,KVH,hd", [(14, 2, 64), (14, 2, 128), (10, 1, 256)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_later_values_in_wide_blocks(ctx, H, KVH, hd, bad):
+    """The same where many rows' columns share the tiles."""
+    G = H // KVH
+    b = Batch([(20, 60), (3, 1)], H, KVH, hd, 16, True, seed=31)
+    at = (b.table[0, 61 // 16], KVH - 1, 61 % 16, 5)
+    b.cells(b.v)[at] = bad
+    got = attend(ctx, b)
+    b.cells(b.v)[at] = 0
+    ref, tol = b.attention()
+    sees = np.zeros(got.shape, bool)
+    sees[41:60, (KVH - 1) * G:, 5] = True  # rows at positions 61 .. 79
+    assert np.all(np.isnan(got[sees]) if bad != bad else got[sees] == bad)
+    check(got[~sees], ref[~sees], tol[~sees])
+
+
+@pytest.mark.parametrize("hd,rows", [(64, 376), (128, 256), (256, 128)])
+def test_wide_blocks_of_long_chunks(ctx, hd, rows):
+    """As many blocks as fit at once: each takes its whole sequence, of 140
+    tiles, in one chunk."""
+    b = Batch([(2240 - rows, rows)], 256, 16, hd, 64, True, seed=hd)
+    b.table[0, 33] = NONE
+    keys, vals = [b.get(b.k, 0)], [b.get(b.v, 0)]
+    keys[0][33 * 64:34 * 64] = np.nan
+    only = [0, 1, rows // 2, rows - 1]
+    ref, tol = b.attention(keys, vals, only)
+    check(attend(ctx, b)[only], ref[only], tol[only])
+
+
 @pytest.mark.parametrize("f16", [False, True])
 def test_values_far_apart(ctx, f16):
     """A heavy weight on tiny values, a light one on the largest, large and
@@ -340,6 +370,15 @@ def test_append_then_attention(ctx, f16):
             got = b.get(b.k, s)[-1]
             assert np.max(np.abs(got - rope64(k[s:s + 1], pos[s:s + 1], theta)[0])) <= (2.0 ** -10 if f16 else 2.0 ** -18) * 8
         check(bo.read(np.float32).reshape(q.shape), *b.attention(), what=step)
+
+
+def test_a_context_leaves_no_error():
+    """What a context's start looks for and does not find is not reported to
+    the next user of the device."""
+    hip = d.load_library()  # (its dependency's symbols too)
+    hip.hipGetLastError()
+    with d.HipContext():
+        assert hip.hipPeekAtLastError() == 0
 
 
 def test_refusals(ctx):
