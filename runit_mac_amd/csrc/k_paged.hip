@@ -27,7 +27,9 @@ RT_DEV SeqRows seq_rows(const PagedBatch& b, uint32_t s) {
 // One workgroup a row and group of heads: its first HD/2 threads make the
 // row's cosines and sines while the heads' loads are on their way.  The angle's
 // turns are reduced in 64 bits: position · θ^(-2d/HD) in 32 would be off by
-// 2^-24 of itself, half a percent of a radian at position 100,000.
+// 2^-24 of itself, half a percent of a radian at position 100,000.  Bound by
+// the rows' bytes: 2,068 rows of 28 + 2·4 heads of 128 into f16 pages
+// (72 MB) 15 µs = 4.8 TB/s; few rows, by the launch (2.3 µs).
 template <int HD, class T>
 RT_DEV void store4(T* p, f32x4 v) {
     if constexpr (sizeof(T) == 4) {
@@ -106,21 +108,30 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 //
 // Narrow blocks (16 columns; decoding rows): the four waves take the chunk's
 // tiles in turn, keys and values straight from the pages into registers, each
-// with a softmax of its own, and meet in LDS.  Bound by the pages' bytes.
+// with a softmax of its own, and meet in LDS.  Bound by the pages' bytes: 24
+// sequences of up to 8,000 positions, 4 KV heads of 128, f16 (182 MB) 41.7 µs
+// = 4.4 TB/s; one of 100,003, f32 (410 MB) 79 µs = 5.2 TB/s; a large copy
+// makes 5.1.  A few hundred positions: 8.5 µs, of which the launch and the
+// planning are 4, two trips to memory and the meeting the rest.
 // Wide blocks (f16 pages; prompt chunks, a shared prefix): each of four waves has
 // 32 columns of its own and all take every tile, from LDS, on the 32x32x16 f16
-// matrix cores.  Bound by the instructions that go beside the matrix cores' —
-// they overlap up to about three vector operations a 16 cycles of matrix product
-// (measured) —, so that the 16x16x32 form, with twice the products to issue and
-// a second column's statistics a lane, was slower.
+// matrix cores.  Bound by these and the vector operations beside them (32 and
+// some 200 a turn of 32 positions): 1.88 µs a turn of all workgroups, two a CU,
+// = 1.14 PFLOP/s of products (a large f16 product makes 1.10), and before and
+// behind a job's turns by its planning, first tiles and parts (some 14 µs).
+// Prompt chunks of 644 rows of 28 heads over 245 .. 4,005 positions 58 µs, 40
+// rows over a shared prefix of 8,192 36 µs, with the parts' launch of 8 and 6 µs;
+// the 16x16x32 form, with twice the products to issue and two columns' statistics
+// a lane, took 3 % longer, blocks of 16 columns alone 280 and 118.
 //
 // f32 pages use the f32 matrix cores.  f16 pages use the f16 ones, keys and
 // values as they are, queries and weights as pairs of f16 (x = hi + lo: 22
 // bits): queries scaled by a power of two to [2^14, 2^15) a column, weights so
 // that the largest is between 2^12 and 2^15: those down to 2^-14 of it keep
-// their 22 bits, smaller ones are off by at most 2^-37 of it.  A job whose sums come out not
-// finite (a value that is not, in places that only some of its columns see; the
-// pairs make NaN of ∞ too) is computed again on the f32 matrix cores.
+// their 22 bits, smaller ones are off by at most 2^-37 of it.  A job whose sums
+// come out not finite (a value that is not, in places that only some of its
+// columns see; the pairs make NaN of ∞ too) is computed again on the f32 matrix
+// cores.
 
 template <bool WIDE>
 constexpr uint32_t paged_slot_rows() { return WIDE ? RT_PAGED_WIDE_ROWS : RT_PAGED_ROWS; }
@@ -1138,39 +1149,45 @@ RT_DEV void paged_merge(const PagedAttnArgs& a) {
     const uint32_t rows = b.row_start ? min(b.row_start[b.n_seqs], b.rows) : min(b.n_seqs, b.rows);
     if (rh >= rows * a.H) return;
     const uint32_t kvh = rh % a.H / (a.H / b.KVH);
-    const uint32_t* in = a.info + (size_t)rh * 4;
-    const uint32_t parts = a.shared_len ? 2 : 1;
-    if (parts == 1 && in[1] / SR == 1) return;  // (written whole)
+    typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+    const u4_t in = *(const u4_t*)(a.info + (size_t)rh * 4);
+    const uint32_t n0 = in[1] / SR, n = n0 + (a.shared_len ? in[3] / SR : 0);
+    if (!a.shared_len && n0 == 1) return;  // (written whole)
+    if (in[0] >= a.jobs || n0 > a.jobs - in[0] || n > n0 && (in[2] >= a.jobs || n - n0 > a.jobs - in[2])) return;
     const float NEG = -__builtin_huge_valf();
     float M = NEG, L = 0.0f;
     f32x4 o = {0, 0, 0, 0};
-    for (uint32_t p = 0; p < parts; ++p) {
-        const uint32_t first = in[2 * p], n = in[2 * p + 1] / SR, k = in[2 * p + 1] % SR;
-        if (first >= a.jobs || n > a.jobs - first) return;
-        for (uint32_t x0 = 0; x0 < n; x0 += 4) {
-            float mc[4], lc[4], mx = M;
-            f32x4 oc[4];
+    // BATCH chunks from x0 on, all on their way together
+    auto take = [&]<uint32_t BATCH>(uint32_t x0) {
+        float mc[BATCH], lc[BATCH], mx = M;
+        f32x4 oc[BATCH];
 #pragma unroll
-            for (uint32_t u = 0; u < 4; ++u) {
-                const size_t slot = ((size_t)(first + min(x0 + u, n - 1)) * b.KVH + kvh) * SR + k;
-                mc[u] = a.ml[2 * slot], lc[u] = a.ml[2 * slot + 1];
-                oc[u] = *(const f32x4*)(a.part + slot * HD + d);
-            }
-#pragma unroll
-            for (uint32_t u = 0; u < 4; ++u) mx = fmaxf(mx, mc[u]);
-            const float md = mx == NEG ? 0.0f : mx, f0 = __builtin_amdgcn_exp2f(M - md);
-            M = mx;
-            L *= f0;
-            o *= f0;
-#pragma unroll
-            for (uint32_t u = 0; u < 4; ++u) {
-                if (x0 + u >= n || mc[u] == NEG) continue;
-                const float f = __builtin_amdgcn_exp2f(mc[u] - md);
-                L = fmaf(f, lc[u], L);
-                o += f * oc[u];
-            }
+        for (uint32_t u = 0; u < BATCH; ++u) {
+            const uint32_t x = min(x0 + u, n - 1), job = x < n0 ? in[0] + x : in[2] + x - n0;
+            const size_t slot = ((size_t)job * b.KVH + kvh) * SR + (x < n0 ? in[1] : in[3]) % SR;
+            mc[u] = a.ml[2 * slot], lc[u] = a.ml[2 * slot + 1];
+            oc[u] = *(const f32x4*)(a.part + slot * HD + d);
         }
-    }
+#pragma unroll
+        for (uint32_t u = 0; u < BATCH; ++u) mx = fmaxf(mx, mc[u]);
+        const float md = mx == NEG ? 0.0f : mx, f0 = __builtin_amdgcn_exp2f(M - md);
+        M = mx;
+        L *= f0;
+        o *= f0;
+#pragma unroll
+        for (uint32_t u = 0; u < BATCH; ++u) {
+            if (x0 + u >= n || mc[u] == NEG) continue;
+            const float f = __builtin_amdgcn_exp2f(mc[u] - md);
+            L = fmaf(f, lc[u], L);
+            o += f * oc[u];
+        }
+    };
+    // (a prefix has tens of chunks: 40 rows over 8,192 positions 6.5 µs eight at a time, 8.0 four; a sequence's few
+    // 9.4 and 7.8)
+    if (a.shared_len)
+        for (uint32_t x0 = 0; x0 < n; x0 += 8) take.template operator()<8>(x0);
+    else
+        for (uint32_t x0 = 0; x0 < n; x0 += 4) take.template operator()<4>(x0);
     *(f32x4*)(a.out + (size_t)rh * HD + d) = M == NEG ? f32x4{0, 0, 0, 0} : o / L;
 }
 
