@@ -115,12 +115,13 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 // planning are 4, two trips to memory and the meeting the rest.
 // Wide blocks (f16 pages; prompt chunks, a shared prefix): each of four waves has
 // 32 columns of its own and all take every tile, from LDS, on the 32x32x16 f16
-// matrix cores.  Bound by these and the vector operations beside them (32 and
-// some 200 a turn of 32 positions): 1.88 µs a turn of all workgroups, two a CU,
-// = 1.14 PFLOP/s of products (a large f16 product makes 1.10), and before and
-// behind a job's turns by its planning, first tiles and parts (some 14 µs).
-// Prompt chunks of 644 rows of 28 heads over 245 .. 4,005 positions 58 µs, 40
-// rows over a shared prefix of 8,192 36 µs, with the parts' launch of 8 and 6 µs;
+// matrix cores.  Bound by these and the vector operations beside them, 32 and
+// some 200 a turn of 32 positions: 1.88 µs a turn of all workgroups, two a CU,
+// = 1.14 PFLOP/s of products (a large f16 product makes 1.10).  Of its 4,500
+// cycles the same products and operations alone take 3,300 (measured), the
+// products 2,050.  Planning, queries and parts: 10 µs a launch.
+// Prompt chunks of 644 rows of 28 heads over 245 .. 4,005 positions 55 µs, 40
+// rows over a shared prefix of 8,192 35 µs, with the parts' launch of 8 and 6 µs;
 // the 16x16x32 form, with twice the products to issue and two columns' statistics
 // a lane, took 3 % longer, blocks of 16 columns alone 280 and 118.
 //
@@ -964,7 +965,7 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
         return there;
     };
     // the block's queries into all stages, a wave's 32 KB·HD / 256 in its own quarter, each instruction whole rows of
-    // them: lanes that read their columns' pieces side by side took 6 µs more of the prompt chunks' 57
+    // them: lanes that read and wrote their columns' pieces themselves took 3 µs more of the prompt chunks' 57
     constexpr uint32_t PC = HD / 4, QL = HD / 8;  // 16-byte pieces a column, instructions a wave
     h8_t* own = lds + w * 32 * PC;
     const uint32_t cc = min(32 * w + c, co.ncl - 1), rh = co.row(cc) * a.H + co.head(cc);
