@@ -753,7 +753,8 @@ int rt_rope_kv_append_paged_f32(rt_ctx* ctx, const rt_paged_batch* batch, const 
                                 float theta);
 /* Causal attention of the batch's rows, q and out [rows][num_heads][head_dim],
  * scale 1/sqrt(head_dim), f32 sums: a row at position p sees the positions ≤ p
- * of its sequence.  A row that sees none gives zeros.  What is behind a
+ * of its sequence.  A row that sees none gives zeros (so do scores of −∞
+ * alone), one with a score that is NaN or +∞ NaN.  What is behind a
  * sequence's length in its pages, and what a row does not see, may hold
  * anything.  Workspace as rt_flash_attention_f32's: sized by the first call of
  * a size, before it is captured. */

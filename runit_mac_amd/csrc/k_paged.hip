@@ -370,7 +370,8 @@ struct PagedAcc {
         m = -__builtin_huge_valf();
         l = 0.0f;
     }
-    // products (NEG: unseen), scores times 1 / scale, to weights
+    // products (NEG: unseen), scores times 1 / scale, to weights.  A column that has seen nothing has the sum 0;
+    // the maximum does not tell: it passes NaN over.
     template <uint32_t N>
     RT_DEV void weigh(float (&p)[N], float scale) {
         const float NEG = -__builtin_huge_valf();
@@ -690,7 +691,7 @@ struct PagedCols {
         if (cc >= ncl) return;
         const uint32_t g = (threadIdx.x & 63) >> 4;
         float* o = place<SR>(job, cc, alone);
-        const float f = !alone ? 1.0f : acc.m == -__builtin_huge_valf() ? 0.0f : 1.0f / acc.l;
+        const float f = !alone ? 1.0f : acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
 #pragma unroll
         for (uint32_t i = 0; i < VN; ++i)
 #pragma unroll
@@ -770,7 +771,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
         }
         const size_t slot = ((size_t)job * b.KVH + co.kvh) * SR + k, rh = (size_t)co.row(k) * a.H + co.head(k);
         if (alone) {
-            *(f32x4*)(a.out + rh * HD + d) = M == NEG ? f32x4{0, 0, 0, 0} : o / L;
+            *(f32x4*)(a.out + rh * HD + d) = L == 0.0f ? f32x4{0, 0, 0, 0} : o / L;
         } else if (noted) {
             *(f32x4*)(a.part + slot * HD + d) = o;
             if (d == 0) {
@@ -853,8 +854,8 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
             if (i >= items) break;
             if (out) {
                 float* op = a.out + ((size_t)co.row(k) * a.H + co.head(k)) * HD + d;
-                op[0] = M[u] == NEG ? 0.0f : o[u][0] / L[u];
-                op[1] = M[u] == NEG ? 0.0f : o[u][1] / L[u];
+                op[0] = L[u] == 0.0f ? 0.0f : o[u][0] / L[u];
+                op[1] = L[u] == 0.0f ? 0.0f : o[u][1] / L[u];
             } else {
                 const size_t slot = slot_of(at) + k;
                 dev_store((uint64_t*)(a.part + slot * HD + d), pair_of(o[u][0], o[u][1]));
@@ -1108,7 +1109,7 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
         for (uint32_t r = 0; r < 16; ++r) bad |= !(fabsf(o[n][r]) < __builtin_huge_valf());
     if (!__ballot(bad)) {
         // through the wave's quarter, so that a row leaves whole
-        const float f = !alone ? 1.0f : m == NEG ? 0.0f : 1.0f / l;
+        const float f = !alone ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (uint32_t n = 0; n < NB; ++n)
 #pragma unroll
@@ -1145,7 +1146,8 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
     const PagedBatch& b = a.b;
     const uint32_t kvh = blockIdx.x % b.KVH, job = blockIdx.x / b.KVH;
     const PagedJob j = paged_job<HD, T, WIDE>(a, job);
-    if (!j.any) return;
+    // (row starts that are not in order may plan more jobs than the launch has)
+    if (!j.any || j.chunks > a.jobs - j.first) return;
     const uint32_t G = a.H / b.KVH, cap = b.table_stride << b.ps_shift;
     const bool pre = j.seq == b.n_seqs;
     const uint32_t rows = j.rows, lo = pre ? 0 : a.shared_len, hi = min(j.kv, cap);
@@ -1202,7 +1204,7 @@ RT_DEV void paged_merge(const PagedAttnArgs& a) {
         o *= f0;
 #pragma unroll
         for (uint32_t u = 0; u < BATCH; ++u) {
-            if (x0 + u >= n || mc[u] == NEG) continue;
+            if (x0 + u >= n) continue;
             const float f = __builtin_amdgcn_exp2f(mc[u] - md);
             L = fmaf(f, lc[u], L);
             o += f * oc[u];
@@ -1214,7 +1216,7 @@ RT_DEV void paged_merge(const PagedAttnArgs& a) {
         for (uint32_t x0 = 0; x0 < n; x0 += 8) take.template operator()<8>(x0);
     else
         for (uint32_t x0 = 0; x0 < n; x0 += 4) take.template operator()<4>(x0);
-    *(f32x4*)(a.out + (size_t)rh * HD + d) = M == NEG ? f32x4{0, 0, 0, 0} : o / L;
+    *(f32x4*)(a.out + (size_t)rh * HD + d) = L == 0.0f ? f32x4{0, 0, 0, 0} : o / L;
 }
 
 #define RT_PAGED_KERNELS(HD)                                                                              \

@@ -149,6 +149,27 @@ def test_later_values_in_wide_blocks(ctx, H, KVH, hd, bad):
     check(got[~sees], ref[~sees], tol[~sees])
 
 
+@pytest.mark.parametrize("f16,new", [(False, 1), (False, 40), (True, 1), (True, 40)])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("kept,P", [(50, 0), (3000, 0), (0, 300)])
+def test_queries_that_are_not_finite(ctx, bad, f16, new, kept, P):
+    """They cost their own row and head its outputs, and no other's: in one
+    chunk, in several, over a shared prefix."""
+    seqs, args = [(kept, new), (9, 2)], (14, 2, 64, 16, f16)
+    if P:
+        b, table, *kv = shared_batch(seqs, P, *args, seed=33)
+    else:
+        b, table, kv = Batch(seqs, *args, seed=33), None, []
+    b.q[new - 1, 3, 7] = bad
+    got = attend(ctx, b, shared=(table, P) if P else None)
+    assert not np.any(np.isfinite(got[new - 1, 3]))
+    b.q[new - 1, 3, 7] = 0.0
+    ref, tol = b.attention(*kv)
+    rest = np.ones(got.shape, bool)
+    rest[new - 1, 3] = False
+    check(got[rest], ref[rest], tol[rest])
+
+
 @pytest.mark.parametrize("hd,rows", [(64, 376), (128, 256), (256, 128)])
 def test_wide_blocks_of_long_chunks(ctx, hd, rows):
     """As many blocks as fit at once: each takes its whole sequence, of 140
