@@ -95,6 +95,25 @@ def test_strides(ctx, half):
 
 
 @pytest.mark.parametrize("half", [False, True])
+def test_rows_four_billion_apart(ctx, half):
+    """A row behind 2^32 elements is the same row as one beside it."""
+    n, far, dt = 5003, 2 ** 32 + 5, np.float16 if half else np.float32
+    x = np.random.default_rng(40).standard_normal((2, n)).astype(dt)
+    tok, outs = ctx.buffer_from(np.array([7, 4000], np.uint32)), []
+    for stride in (n, far):
+        buf = ctx.new_buffer((stride + n) * x.itemsize)
+        buf.write(x[0])
+        buf.write(x[1], stride * x.itemsize)
+        lp, ids, tops = ctx.new_buffer(8), ctx.new_buffer(24), ctx.new_buffer(24)
+        (d.token_logprobs_f16 if half else d.token_logprobs_f32)(ctx, buf, tok, 2, n, lp, top=3, top_ids=ids,
+                                                                  top_logprobs=tops, row_stride=stride)
+        ctx.flush()
+        outs.append([lp.read(np.float32), ids.read(np.uint32), tops.read(np.float32)])
+        buf.free()
+    assert all(np.array_equal(*p) for p in zip(*outs)) and np.all(np.isfinite(outs[0][0]))
+
+
+@pytest.mark.parametrize("half", [False, True])
 @pytest.mark.parametrize("n", [700, 20001])
 def test_ties(ctx, n, half):
     """Few different values, both zeros among them: equal logits go by the lower id."""

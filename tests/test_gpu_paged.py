@@ -82,6 +82,36 @@ def test_page_stride(ctx, f16):
     check(attend(ctx, b), *b.attention())
 
 
+@pytest.mark.parametrize("f16,new", [(False, 3), (True, 3), (True, 40)])
+def test_pages_behind_four_billion_elements(ctx, f16, new):
+    """The same bytes as from a small pool, appended and read."""
+    H, KVH, hd, ps, far = 14, 2, 64, 16, 2 ** 32 + 64
+    b = Batch([(50, new)], H, KVH, hd, ps, f16, seed=34)
+    rng = np.random.default_rng(35)
+    kv = [ctx.buffer_from(rng.standard_normal((new, KVH, hd)).astype(np.float32)) for _ in range(2)]
+    size, outs = b.k.dtype.itemsize, []
+    end = (50 + new - 1) // ps
+    first, last = b.table[0, 0], b.table[0, end]
+    table = np.full(b.table.size, NONE, np.uint32)
+    table[0], table[end] = 0, 1  # the sequence's other pages are none
+    for stride in (b.page, far):
+        pools = [ctx.new_buffer((stride + b.page) * size) for _ in range(2)]
+        for pool, data in zip(pools, (b.k, b.v)):
+            pool.write(data[first])
+            pool.write(data[last], stride * size)
+        batch = d.PagedBatch(*pools, "f16" if f16 else "f32", 2, ps, KVH, hd, ctx.buffer_from(table), table.size, 1,
+                             ctx.buffer_from(b.kv.astype(np.uint32)), rows=new,
+                             row_start=ctx.buffer_from(b.start.astype(np.uint32)), page_stride=stride)
+        q, o = ctx.buffer_from(b.q[:new]), ctx.new_buffer(4 * new * H * hd)
+        d.rope_kv_append_paged_f32(ctx, batch, q, *kv, q, H, 1e6)
+        d.paged_attention_f32(ctx, batch, q, o, H)
+        ctx.flush()
+        outs.append(o.read(np.float32))
+        for x in pools:
+            x.free()
+    assert np.all(np.isfinite(outs[0])) and np.array_equal(*outs)
+
+
 @pytest.mark.parametrize("f16", [False, True])
 def test_missing_pages(ctx, f16):
     """Ids that are no page: their positions are not seen; a row that sees
