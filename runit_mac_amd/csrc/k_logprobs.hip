@@ -17,7 +17,7 @@
 //
 // Bound by the logits' bytes, with many alternatives by the vector operations that
 // look for them, with few rows by trips to memory: 500 rows of 152,064 f32 with
-// 20 alternatives 75 µs, with 5 67, without 59 (304 MB, 5.2 TB/s; a large copy
+// 20 alternatives 74 µs, with 5 66, without 59 (304 MB, 5.2 TB/s; a large copy
 // makes 5.1); 93 of 50,001 f16 without 8.4 (9.3 MB); 4 of 151,936 f32 with 5
 // 11.6.  One workgroup of 16 waves a row instead of segments that meet was no
 // faster from 93 rows on, and slower below.
@@ -190,7 +190,7 @@ RT_DEV void logprobs(const LogprobsArgs& a) {
         queued = 0;
     };
     for (uint32_t b = e0; b < e1; b += STEP) {
-        float v[U][N], mx = NEG;
+        float v[U][N], mu[U], mx = NEG;
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
             const uint32_t i = b + 256 * N * u + N * tid;
@@ -200,8 +200,10 @@ RT_DEV void logprobs(const LogprobsArgs& a) {
 #pragma unroll
                 for (uint32_t k = 0; k < N; ++k) v[u][k] = i + k < e1 ? (float)x[i + k] : NEG;
             }
+            mu[u] = v[u][0];
 #pragma unroll
-            for (uint32_t k = 0; k < N; ++k) mx = fmaxf(mx, v[u][k]);
+            for (uint32_t k = 1; k < N; ++k) mu[u] = fmaxf(mu[u], v[u][k]);
+            mx = fmaxf(mx, mu[u]);
         }
         if (b + STEP < e1) load(b + STEP);
         if (mx > t.m) t.to(mx);
@@ -225,7 +227,8 @@ RT_DEV void logprobs(const LogprobsArgs& a) {
                 // what reaches it into the wave's queue, from there into its list when
                 // they are as many as it holds
 #pragma unroll
-                for (uint32_t u = 0; u < U; ++u)
+                for (uint32_t u = 0; u < U; ++u) {
+                    if (!__ballot(!(mu[u] < thr))) continue;
 #pragma unroll
                     for (uint32_t k = 0; k < N; ++k) {
                         const uint32_t id = b + 256 * N * u + N * tid + k;
@@ -238,6 +241,7 @@ RT_DEV void logprobs(const LogprobsArgs& a) {
                             queued += __popcll(hit);
                         }
                     }
+                }
                 if (queued >= min(64u, a.top) || b == e0) empty();
             }
         }
