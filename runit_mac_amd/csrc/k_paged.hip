@@ -240,6 +240,15 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
             if (own + pb * ceil_div(pt, c1, inv1) <= a.slots) j.len = c1;
         }
     }
+    if (!WIDE && !a.shared_len && a.target && n <= 64) {
+        // no more than sixteen chunks, which meet in one trip, where that takes chunks twice as long at most
+        // (nine sequences of up to 4,000 positions with drafts 17.8 -> 15.8 µs, sixteen decoding 13.8 -> 12.5)
+        uint32_t most = mt;
+        most = max(most, lane_xor<1>(most)), most = max(most, lane_xor<2>(most)), most = max(most, lane_xor<4>(most));
+        most = max(most, lane_xor<8>(most)), most = max(most, lane_xor<16>(most)), most = max(most, lane_xor<32>(most));
+        const uint32_t len = ((uint32_t)__builtin_amdgcn_readfirstlane(most) / 16 + STEP) / STEP * STEP;
+        if (j.len < len && len <= 2 * j.len) j.len = len;
+    }
     const float inv = 1.0f / (float)j.len;
     auto found = [&](uint32_t seq, uint32_t base, uint32_t nc) {
         const uint32_t k = job - base;
