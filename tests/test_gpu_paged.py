@@ -311,6 +311,40 @@ def test_attention_repeats_and_replays(ctx):
         check(oo.read(np.float32).reshape(3, 14, 64), *other.attention(), what=n)
 
 
+@pytest.mark.parametrize("P", [0, 133])
+def test_wide_blocks_replay(ctx, P):
+    """A captured call of wide blocks follows the lengths too, with an eager
+    call of another batch over the same workspace between the replays."""
+    seqs, args = [(700, 40), (10, 1)], (14, 2, 64, 16, True)
+    if P:
+        b, table, keys, vals = shared_batch(seqs, P, *args, seed=36)
+        bt = ctx.buffer_from(table.astype(np.uint32))
+        call = lambda *x: d.shared_prefix_attention_f32(ctx, *x, 14, bt, P)
+    else:
+        b = Batch(seqs, *args, seed=36)
+        keys, vals = [b.get(b.k, s) for s in range(2)], [b.get(b.v, s) for s in range(2)]
+        call = lambda *x: d.paged_attention_f32(ctx, *x, 14)
+    other = Batch([(300, 30), (5, 9)], *args, seed=37)
+    batch, bq, bo = b.upload(ctx), ctx.buffer_from(b.q), ctx.new_buffer(4 * b.q.size)
+    call(batch, bq, bo)
+    ctx.flush()
+    first, most = bo.read(np.float32), int(b.kv[0])
+    ctx.capture_begin()
+    call(batch, bq, bo)
+    graph = ctx.capture_end()
+    for n in (most, 300, 190, most):
+        b.kv[0] = n
+        b.bl.write(b.kv.astype(np.uint32))
+        check(attend(ctx, other), *other.attention(), what="eager")
+        graph.launch()
+        ctx.flush()
+        got = bo.read(np.float32)
+        if n == most:
+            assert np.array_equal(got, first)
+        ref = b.attention([keys[0][:n], keys[1]], [vals[0][:n], vals[1]])
+        check(got.reshape(b.q.shape)[:b.R], *ref, what=n)
+
+
 # ───────────────────────────── append ─────────────────────────────
 
 @pytest.mark.parametrize("f16", [False, True])
