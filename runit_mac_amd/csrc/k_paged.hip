@@ -116,10 +116,11 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 // Wide blocks (f16 pages; prompt chunks, a shared prefix): each of four waves has
 // 32 columns of its own and all take every tile, from LDS, on the 32x32x16 f16
 // matrix cores.  Bound by these and the vector operations beside them, 32 and
-// some 200 a turn of 32 positions: 1.88 µs a turn of all workgroups, two a CU,
+// some 140 a turn of 32 positions: 1.88 µs a turn of all workgroups, two a CU,
 // = 1.14 PFLOP/s of products (a large f16 product makes 1.10).  Of its 4,500
-// cycles the same products and operations alone take 3,300 (measured), the
-// products 2,050.  Planning, queries and parts: 10 µs a launch.
+// cycles 32 products with 100 and 200 such operations alone take 2,800 and 3,300,
+// the products 2,500 (measured); the rest waits, for reads of LDS and at
+// barriers.  Planning, queries and parts: 10 µs a launch.
 // Prompt chunks of 644 rows of 28 heads over 245 .. 4,005 positions 55 µs, 40
 // rows over a shared prefix of 8,192 35 µs, with the parts' launch of 8 and 6 µs;
 // the 16x16x32 form, with twice the products to issue and two columns' statistics
@@ -1023,6 +1024,12 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
 #pragma unroll
     for (uint32_t i = 0; i < Stage::N - 1; ++i)
         if (i < turns) here |= bring(i) << 2 * i;
+    // where in a stage the lane's values of elements 32n .. are (of positions 16x + 8k .., as many rows on: the
+    // permutation goes by the row's last bits)
+    uint32_t vat[NB];
+#pragma unroll
+    for (uint32_t n = 0; n < NB; ++n)
+        vat[n] = Stage::piece(32 + 4 * h + (lane >> 2 & 3), 4 * n + (lane >> 3 & 2) + (lane >> 1 & 1)) * 16 + (lane & 1) * 8;
     f16v o[NB];
 #pragma unroll
     for (uint32_t n = 0; n < NB; ++n) o[n] = f16v{};
@@ -1088,17 +1095,16 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
             h8_t ph[2], pl[2];
             split_weights(p, ph[0], pl[0]);
             split_weights(p + 8, ph[1], pl[1]);
+            const uint32_t vst = lds0 + i % Stage::N * Stage::LEN * 16;
 #pragma unroll
             for (uint32_t n = 0; n < NB; ++n)
 #pragma unroll
                 for (uint32_t x = 0; x < 2; ++x) {
                     s4_t y[2];  // element 32n + c of the positions 16x + 4h .., and eight on
 #pragma unroll
-                    for (uint32_t k = 0; k < 2; ++k) {
-                        const uint32_t r = 32 + 16 * x + 8 * k + 4 * h + (lane >> 2 & 3);
-                        const h8_t* at = st + Stage::piece(r, 4 * n + (lane >> 3 & 2) + (lane >> 1 & 1));
-                        y[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr_t)((const s4_t*)at + (lane & 1)));
-                    }
+                    for (uint32_t k = 0; k < 2; ++k)
+                        y[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (tptr_t)(uintptr_t)(vst + vat[n] + (16 * x + 8 * k) * Stage::ROW * 16));
                     const h8_t vv = __builtin_bit_cast(h8_t, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
                     o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, ph[x], o[n], 0, 0, 0);
                     o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, pl[x], o[n], 0, 0, 0);
