@@ -119,8 +119,9 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 // some 140 a turn of 32 positions: 1.88 µs a turn of all workgroups, two a CU,
 // = 1.14 PFLOP/s of products (a large f16 product makes 1.10).  Of its 4,500
 // cycles 32 products with 100 and 200 such operations alone take 2,800 and 3,300,
-// the products 2,500 (measured); the rest waits, for reads of LDS and at
-// barriers.  Planning, queries and parts: 10 µs a launch.
+// the products 2,500 (measured).  What the rest goes to was not found: half as
+// many barriers, fewer vector operations, other orders and priorities change
+// nothing.  Planning, queries and parts: 10 µs a launch.
 // Prompt chunks of 644 rows of 28 heads over 245 .. 4,005 positions 55 µs, 40
 // rows over a shared prefix of 8,192 35 µs, with the parts' launch of 8 and 6 µs;
 // the 16x16x32 form, with twice the products to issue and two columns' statistics
