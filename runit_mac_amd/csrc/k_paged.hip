@@ -135,6 +135,14 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 // come out not finite (a value that is not, in places that only some of its
 // columns see; the pairs make NaN of ∞ too) is computed again on the f32 matrix
 // cores.
+//
+// The scale (1 / (√HD·ln 2)) comes before the maximum, one rounding: f32 scores
+// take it as they leave the first product, f16 queries before they are split, and
+// scores are in units of log 2 times a power of two.  So the reference is one of
+// them, and a weight's exponent the difference of two rounded scores.  Scaled in
+// the exponent's fma, the reference would be rounded apart from the scores: a factor of
+// 2^16 at scores of 2^28, more than f32 holds from 2^32 on.  (f32 queries scaled
+// instead hold up the first tile: 8.7 µs for 8.4 at a few hundred positions.)
 
 template <bool WIDE>
 constexpr uint32_t paged_slot_rows() { return WIDE ? RT_PAGED_WIDE_ROWS : RT_PAGED_ROWS; }
@@ -381,8 +389,8 @@ struct PagedAcc {
         m = -__builtin_huge_valf();
         l = 0.0f;
     }
-    // products (NEG: unseen), scores times 1 / scale, to weights.  A column that has seen nothing has the sum 0;
-    // the maximum does not tell: it passes NaN over.
+    // products (NEG: unseen), scores in units of log 2 divided by scale, a power of two, to weights.  A column that
+    // has seen nothing has the sum 0; the maximum does not tell: it passes NaN over.
     template <uint32_t N>
     RT_DEV void weigh(float (&p)[N], float scale) {
         const float NEG = -__builtin_huge_valf();
@@ -421,6 +429,12 @@ struct PagedAcc {
         return !__ballot(bad);
     }
 };
+
+// (a product that no later sum takes in unrounded)
+RT_DEV float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
 
 // The tiles t0, t0 + step, ... of a chunk (RUN 2: pairs of tiles there) for 16
 // columns on the f32 matrix cores: q is the lane's column, [0, lim) what it sees, limn / limx the
@@ -470,9 +484,9 @@ RT_DEV void paged_f32(PagedAcc<HD, T>& acc, const PagedView<T>& v, const float* 
 #pragma unroll
         for (uint32_t r = 0; r < 4; ++r) {
             const uint32_t pos = p0 + 4 * g + r;
-            p[r] = edge && (pos < v.lo || pos >= lim) ? -__builtin_huge_valf() : sa[r] + sb[r];
+            p[r] = edge && (pos < v.lo || pos >= lim) ? -__builtin_huge_valf() : rounded_product(sa[r] + sb[r], scale2);
         }
-        acc.weigh(p, scale2);
+        acc.weigh(p, 1.0f);
         bool bad = false;
         if (edge) {
             // what only later columns see must not reach the earlier ones as 0·∞
@@ -515,10 +529,10 @@ RT_DEV void paged_f32(PagedAcc<HD, T>& acc, const PagedView<T>& v, const float* 
     acc.join();
 }
 
-// A column's query as pairs of f16, x·2^e = hi + lo, from the lane's part of it
-// and the column's largest; returns scale2·2^-e.
+// A column's scaled query as pairs of f16, x·2^e = hi + lo, from the lane's part of it
+// and the column's largest; returns 2^-e.
 template <uint32_t N>
-RT_DEV float split_query(const float (&x)[N][8], float mx, float scale2, h8_t (&qh)[N], h8_t (&ql)[N]) {
+RT_DEV float split_query(const float (&x)[N][8], float mx, h8_t (&qh)[N], h8_t (&ql)[N]) {
     // (at most 126: 2^-e stays a normal number)
     const int e = mx > 0.0f ? min(126, 15 - __builtin_amdgcn_frexp_expf(mx)) : 0;
     const float f = ldexpf(1.0f, e);
@@ -530,7 +544,7 @@ RT_DEV float split_query(const float (&x)[N][8], float mx, float scale2, h8_t (&
             qh[i][k] = (_Float16)y;
             ql[i][k] = (_Float16)(y - (float)qh[i][k]);
         }
-    return scale2 * ldexpf(1.0f, -e);
+    return ldexpf(1.0f, -e);
 }
 template <int HD>
 RT_DEV float paged_query(const float* q, float scale2, h8_t (&qh)[HD / 32], h8_t (&ql)[HD / 32]) {
@@ -540,7 +554,7 @@ RT_DEV float paged_query(const float* q, float scale2, h8_t (&qh)[HD / 32], h8_t
     for (uint32_t i = 0; i < HD / 32; ++i)
 #pragma unroll
         for (uint32_t k = 0; k < 8; k += 4) {
-            const f32x4 v = *(const f32x4*)(q + 32 * i + 8 * g + k);
+            const f32x4 v = *(const f32x4*)(q + 32 * i + 8 * g + k) * scale2;
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) {
                 x[i][k + e] = v[e];
@@ -549,7 +563,7 @@ RT_DEV float paged_query(const float* q, float scale2, h8_t (&qh)[HD / 32], h8_t
         }
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    return split_query<HD / 32>(x, mx, scale2, qh, ql);
+    return split_query<HD / 32>(x, mx, qh, ql);
 }
 // (hi towards zero, two at a time; what is left has at most 14 bits, lo the
 // nearest of it)
@@ -1009,14 +1023,14 @@ RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, _Float16>& co
         for (uint32_t n = 0; n < KS; ++n)
 #pragma unroll
             for (uint32_t e = 0; e < 8; e += 4) {
-                const f32x4 y = *(const f32x4*)(own + piece(c, 4 * n + 2 * h + e / 4));
+                const f32x4 y = *(const f32x4*)(own + piece(c, 4 * n + 2 * h + e / 4)) * scale2;
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k) {
                     x[n][e + k] = y[k];
                     mx = fmaxf(mx, fabsf(y[k]));
                 }
             }
-        qs = split_query<KS>(x, fmaxf(mx, __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, mx)))), scale2, qh, ql);
+        qs = split_query<KS>(x, fmaxf(mx, __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, mx)))), qh, ql);
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (the queries are read before tiles come)

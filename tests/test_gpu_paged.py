@@ -264,6 +264,49 @@ def test_shared_prefix_wide_batch(ctx, f16):
     check(attend(ctx, b, shared=(table, 2048)), *b.attention(keys, vals))
 
 
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("mag", [26, 28, 31, 34])
+@pytest.mark.parametrize("seqs,P,H,KVH,hd", [
+    ([(0, 1), (16, 1), (129, 1), (3000, 1)], 0, 14, 2, 64),
+    ([(300, 60), (3, 1)], 0, 14, 2, 64),
+    ([(300, 60), (3, 1)], 0, 10, 1, 256),
+    ([(5, 1), (40, 12), (0, 60)], 300, 28, 4, 128),
+])
+def test_large_scores(ctx, seqs, P, H, KVH, hd, mag, f16):
+    """Scores of about 2^mag log 2, each row's largest far above the others: its
+    value is the output, however the maximum itself is rounded.  A weight as a
+    pair of f16 is off by at most 2^-21 of it, product, sums over waves and
+    chunks and the division are less than eight roundings, 2^-21; the other
+    weights are e^ of minus thousands."""
+    ps, rng = 16, np.random.default_rng(mag)
+    if P:
+        b, table, *_ = shared_batch(seqs, P, H, KVH, hd, ps, f16, seed=mag)
+    else:
+        b, table = Batch(seqs, H, KVH, hd, ps, f16, seed=mag), np.zeros(0, np.uint32)
+    sign = rng.choice([-1.0, 1.0], hd)
+    page = lambda s, p: table[p // ps] if p < P else b.table[s, p // ps]
+    shared = {0, *rng.integers(0, P, 8).tolist()} if P else set()
+    best = []  # of each sequence: up to each position, the one with the largest score
+    for s in range(len(seqs)):
+        n, up, last = int(b.kv[s]), 0, -1
+        larger = shared | {P, *rng.integers(P, n, 8).tolist()}  # than all before them
+        best.append([])
+        for i in range(n):
+            up, last = (up + 1, i) if i in larger else (up, last)
+            best[s].append(last)
+            t = 0.5 + up / 64 if last == i else 0.25 * rng.random()
+            if i >= P or not s:
+                b.cells(b.k)[page(s, i), :, i % ps] = (256 * t * sign * rng.uniform(1, 1.01, (KVH, hd))).astype(b.k.dtype)
+    a = 2.0 ** (mag - 8) / (1.4427 * np.sqrt(hd))
+    b.q[:] = a * sign * rng.uniform(1, 1.01, b.q.shape)
+    got = attend(ctx, b, shared=(table, P) if P else None)
+    for s in range(len(seqs)):
+        for i in range(int(b.new[s])):
+            at = best[s][int(b.kv[s] - b.new[s]) + i]
+            v = np.repeat(b.cells(b.v)[page(s, at), :, at % ps].astype(np.float64), H // KVH, 0)
+            check(got[int(b.start[s]) + i], v, np.abs(v) * 2.0 ** -20, what=(s, i))
+
+
 def test_shared_prefix_rows_inside_it(ctx):
     """Rows whose position is inside the shared positions see their part."""
     b, table, keys, vals = shared_batch([(0, 4), (5, 2)], 50, 4, 2, 64, 16, False, seed=13)
