@@ -177,6 +177,7 @@ RT_DEV void logprobs(const LogprobsArgs& a) {
     if (e0 < e1) load(e0);
     const uint32_t tok = a.tokens[row];
     const float xt = tok < a.n ? (float)x[tok] : NEG;
+    const float xr = xt != xt ? NEG : xt;  // (NaN ranks as −∞)
     if (TOP && tid == 0) floor_s = 0;
     if constexpr (TOP) __syncthreads();
     LogSum t;
@@ -216,7 +217,7 @@ RT_DEV void logprobs(const LogprobsArgs& a) {
                 const float d = (v[u][k] - mm) * 1.44269504f, e = __builtin_amdgcn_exp2f(d);
                 t.s += e;
                 t.u = fmaf(e, fmaxf(d, -1e30f), t.u);  // (−∞: 0)
-                more += v[u][k] > xt;
+                more += v[u][k] > xr;
             }
         if constexpr (TOP) {
             uint32_t fl = *(volatile uint32_t*)&floor_s;

@@ -175,6 +175,22 @@ def test_rows_without_a_distribution(ctx, n, half):
     check(x[3:], tokens[3:], 4, (lp[3:], en[3:], rk[3:], ids[3:], tl[3:]))
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("n,top", [(500, 0), (500, 4), (20001, 0), (20001, 4)])
+def test_tokens_that_are_nan(ctx, n, top, half):
+    """A given token whose own logit is NaN ranks as one at -inf does: below
+    every logit above -inf, in one segment and in several."""
+    rng = np.random.default_rng(41)
+    x = logits(rng, 3, n, half)
+    x[0, 7] = np.nan
+    x[1, n - 1], x[1, : n // 2] = np.nan, -np.inf
+    x[2, [3, n // 2]] = np.nan, np.inf
+    tokens = [7, n - 1, 3]
+    lp, en, rk, _, tl = run(ctx, x, tokens, top)
+    assert np.array_equal(rk, (x > -np.inf).sum(1))
+    assert np.all(np.isnan(lp)) and np.all(np.isnan(en)) and np.all(np.isnan(tl))
+
+
 def test_tokens_out_of_range(ctx):
     rng = np.random.default_rng(7)
     x = logits(rng, 3, 5000, False)
