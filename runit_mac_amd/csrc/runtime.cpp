@@ -492,7 +492,10 @@ Plan plan_gemv(const rt_ctx* c, const Fmt& f, uint32_t nvrows, uint32_t K, bool 
     return p;
 }
 
-// Grows a context buffer to `need` bytes (not during graph capture).
+// Grows a context buffer to `need` bytes or more (not during graph capture).
+// From the second size on to twice the size before at least, where that much
+// memory is there: the buffers kept below are then together no larger than the
+// one in use, however many sizes the calls come in.
 int ensure_buf(rt_ctx* c, void*& buf, size_t& bytes, size_t need, const char* who) {
     if (need <= bytes) return RT_OK;
     if (c->noalloc)
@@ -503,17 +506,21 @@ int ensure_buf(rt_ctx* c, void*& buf, size_t& bytes, size_t need, const char* wh
     if (c->capturing)
         return fail(c, RT_ERR_DISPATCH,
                     "kernel dispatch error: %s: workspace must be sized before graph capture", who);
-    if (buf) {
-        // the old buffer stays allocated until the context is destroyed: a
-        // graph captured before this growth holds its address in its kernel
-        // arguments and may still be replayed
-        c->retired.push_back(buf);
-        buf = nullptr;
-        bytes = 0;
+    void* grown = nullptr;
+    size_t n = std::max(need, 2 * bytes);
+    hipError_t e = hipMalloc(&grown, n);
+    if (e != hipSuccess && n > need) {
+        (void)hipGetLastError();
+        n = need;
+        e = hipMalloc(&grown, n);
     }
-    hipError_t e = hipMalloc(&buf, need);
     if (e != hipSuccess) return hip_fail(c, e, "workspace hipMalloc");
-    bytes = need;
+    // the old buffer stays allocated until the context is destroyed: a
+    // graph captured before this growth holds its address in its kernel
+    // arguments and may still be replayed
+    if (buf) c->retired.push_back(buf);
+    buf = grown;
+    bytes = n;
     return RT_OK;
 }
 // The activation workspace (pre-pass records, normalised x, GEMM operands,

@@ -3,6 +3,8 @@ rt_paged_attention_f32, rt_shared_prefix_attention_f32) against 64 bits.
 What no row may see — places behind a sequence's length, pages that no table
 names, later rows' positions — holds NaN or infinities; rows behind the last
 sequence keep what they held."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -498,6 +500,31 @@ def test_append_then_attention(ctx, f16):
             got = b.get(b.k, s)[-1]
             assert np.max(np.abs(got - rope64(k[s:s + 1], pos[s:s + 1], theta)[0])) <= (2.0 ** -10 if f16 else 2.0 ** -18) * 8
         check(bo.read(np.float32).reshape(q.shape), *b.attention(), what=step)
+
+
+def test_workspace_of_growing_calls():
+    """Calls that each need a little more than the one before keep memory in
+    proportion to the largest, not to the number of sizes."""
+    hip = d.load_library()
+
+    def free():
+        hip.hipDeviceSynchronize()
+        n, total = ctypes.c_size_t(), ctypes.c_size_t()
+        assert hip.hipMemGetInfo(ctypes.byref(n), ctypes.byref(total)) == 0
+        return n.value
+
+    def taken(sizes):
+        with d.HipContext() as ctx:
+            b = Batch([(60, 1)] * 40, 28, 4, 128, 16, True, seed=38, one=True)
+            batch, q, o = b.upload(ctx), ctx.buffer_from(b.q), ctx.new_buffer(4 * b.q.size)
+            before = free()
+            for n in sizes:
+                batch.n_seqs = batch.rows = n
+                d.shared_prefix_attention_f32(ctx, batch, q, o, 28, b.bt, 48)
+            return before - free()
+
+    once = taken([40])
+    assert 0 < once and taken(range(1, 41)) <= 4 * once + (8 << 20)
 
 
 def test_a_context_leaves_no_error():
