@@ -228,9 +228,19 @@ class BatchDecoder:
 
     def _run(self, work: dict, keep: dict | None, top: int | None = None, given: bool = False) -> dict:
         """The passes over `work`; of the tokens in `keep`'s ranges the argmax,
-        or (`given`) the token that follows, and with `top` its scores."""
+        or (`given`) the token that follows, and with `top` its scores.  If one
+        fails, the sequences are as they were before all of them."""
         if top is not None and not 0 <= top <= self.max_top:
             raise ValueError(f"top {top} is not within 0 .. {self.max_top}")
+        before = {s: self._seqs[s].len for s in work}
+        try:
+            return self._passes(work, keep, top, given)
+        except BaseException:
+            for s, n in before.items():
+                self.trim(s, n)
+            raise
+
+    def _passes(self, work: dict, keep: dict | None, top: int | None, given: bool) -> dict:
         parts = {s: [] for s in work}
         left = [(s, 0) for s, t in work.items() if t.size]
         while left:

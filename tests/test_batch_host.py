@@ -122,6 +122,41 @@ def test_verify_keeps_the_accepted():
     assert b.length(s) == 3 and b.length(t) == 1
 
 
+class Failing(Recorder):
+    """The launches of a pass fail when `left` others have run."""
+    left = 1 << 30
+
+    def _launch(self, *args):
+        if self.left == 0:
+            raise d.Dispatch("kernel dispatch error: none")
+        self.left -= 1
+        return super()._launch(*args)
+
+
+@pytest.mark.parametrize("left", [0, 1, 2])
+@pytest.mark.parametrize("prefix", [0, 21])
+def test_a_call_that_fails_changes_no_sequence(left, prefix):
+    """Lengths and pages as before it, in whichever pass it fails; the next
+    call begins there."""
+    b = decoder(Failing, num_pages=16)
+    b.share_prefix(np.arange(prefix))
+    s, t = b.open(), b.open()
+    b.step({s: np.arange(10), t: [1]})
+    free, lens = b.pool.free, [b.length(s), b.length(t)]
+    for call in (lambda: b.step({s: np.arange(15), t: np.arange(9)}), lambda: b.score({t: np.arange(20), s: [1]}),
+                 lambda: b.verify({s: (1, np.arange(18)), t: (2, [3])})):
+        b.left = left
+        with pytest.raises(d.Dispatch):
+            call()
+        assert b.pool.free == free and [b.length(s), b.length(t)] == lens
+    b.left = 1 << 30
+    b.step({s: [7]})
+    assert b.passes[-1]["kv_len"][0] == lens[0] + 1 and b.length(s) == lens[0] + 1
+    b.close(s), b.close(t)
+    b.share_prefix([])
+    assert b.pool.free == 16
+
+
 def test_refusals():
     for kw in (dict(max_seqs=0), dict(num_pages=0), dict(page_size=8), dict(page_size=48), dict(kv="bf16"),
                dict(max_rows=0), dict(max_logits=0), dict(max_top=-1), dict(max_len=0)):
