@@ -141,12 +141,16 @@ class BatchDecoder:
 
     def share_prefix(self, tokens) -> None:
         """Runs `tokens` as the beginning of every sequence to come, in pages
-        of their own.  While no sequence is open; no tokens: none any more."""
+        of their own.  While no sequence is open; no tokens: none any more.
+        Refused, it leaves the former ones; if a pass fails, there are none."""
         if self._seqs:
             raise ValueError("share_prefix: sequences are open")
         toks = self._tokens(tokens)
         if toks.size > self.max_len:
             raise ValueError(f"share_prefix: {toks.size} tokens exceed max_len {self.max_len}")
+        need, there = -(-toks.size // self.page_size), self.pool.free + len(self._prefix_pages)
+        if need > there:
+            raise d.BufferSize(f"buffer size mismatch: expected {need} free pages, got {there}")
         self.pool.give(self._prefix_pages)
         self._prefix_pages, self.prefix_len = [], 0
         if toks.size == 0:

@@ -157,6 +157,25 @@ def test_a_call_that_fails_changes_no_sequence(left, prefix):
     assert b.pool.free == 16
 
 
+def test_a_prompt_that_does_not_fit_leaves_the_shared_one():
+    """Refused before anything of it has run; one whose passes fail is gone,
+    as is the old one, whose pages it may have taken."""
+    b = decoder(Failing, num_pages=4)
+    b.share_prefix(np.arange(20))
+    n = len(b.passes)
+    with pytest.raises(d.BufferSize):
+        b.share_prefix(np.arange(65))
+    assert b.prefix_len == 20 and b.pool.free == 2 and len(b.passes) == n
+    b.share_prefix(np.arange(64))  # (with the old one's pages)
+    assert b.prefix_len == 64 and b.pool.free == 0
+    b.left = 1
+    with pytest.raises(d.Dispatch):
+        b.share_prefix(np.arange(20))
+    assert b.prefix_len == 0 and b.pool.free == 4
+    with pytest.raises(ValueError):
+        b.length(b._next)
+
+
 def test_refusals():
     for kw in (dict(max_seqs=0), dict(num_pages=0), dict(page_size=8), dict(page_size=48), dict(kv="bf16"),
                dict(max_rows=0), dict(max_logits=0), dict(max_top=-1), dict(max_len=0)):
