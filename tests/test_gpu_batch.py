@@ -95,6 +95,35 @@ def test_steps_and_a_shared_prompt(ctx, kv):
     b.free(), m.free()
 
 
+def test_few_rows_of_a_large_model(ctx):
+    """Passes of one to five rows where the hidden size takes them to the
+    batched GEMMs: steps of one sequence and of three, a draft to verify."""
+    cfg = DecodeConfig(layers=2, hidden=1280, heads=10, kv_heads=2, head_dim=128, ff=1536, vocab=1000, max_seq=64)
+    m = DecodeModel(ctx, cfg, seed=11, quant=Q4K_M)
+    assert m.row_form(1) == m.row_form(5) == "gemm"
+    host = ora.HostStepModel.from_recipe(m)
+    rng = np.random.default_rng(12)
+    b = BatchDecoder(m, 3, 12, 16, kv="f32", max_rows=8, max_top=4)
+    seqs = [b.open() for _ in range(3)]
+    history = {s: [] for s in seqs}
+    for sizes in ((1,), (1, 1, 1), (2, 1, 2), (4,), (1, 1, 1)):
+        work = {s: rng.integers(cfg.vocab, size=n) for s, n in zip(seqs, sizes)}
+        got = b.step(work, top=4)
+        for s, t in work.items():
+            history[s] += list(t)
+            token, scores = got[s]
+            assert token == scores.top_ids[0, 0] and scores.rank[0] == 0
+            check_scores(scores, host_logits(host, history[s])[-1:], np.array([token]), "f32")
+    s = seqs[0]
+    before = b.length(s)
+    kept, following = b.verify({s: (3, [4, 5])})[s]
+    logits = host_logits(host, history[s] + [3, 4, 5])[-3:]
+    fits = [np.flatnonzero(x >= x.max() - 2 * tolerance(x, "f32")) for x in logits]
+    assert all([4, 5][i] in fits[i] for i in range(kept)) and following in fits[kept]
+    assert b.length(s) == before + 1 + kept
+    b.free(), m.free()
+
+
 def test_verify_of_several_sequences(ctx):
     """Drafts that the reference model would have decoded are kept up to the
     first that no logits within the tolerance allow, and the sequence goes on

@@ -77,6 +77,76 @@ def test_many_sequences(ctx):
     check(attend(ctx, b), *b.attention())
 
 
+def spread(n, rows, seed):
+    """n sequences of up to 60 positions, but for long ones before, at and
+    behind every 64th; rows(i) new ones each."""
+    rng = np.random.default_rng(seed)
+    kept = rng.integers(0, 60, n)
+    for i, k in ((0, 1100), (62, 1500), (63, 900), (64, 2300), (n - 3, 3900), (n - 1, 1700)):
+        kept[i] = k
+    return [(int(kept[i]), rows(i)) for i in range(n)], [0, 1, 62, 63, 64, n - 3, n - 2, n - 1]
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("one", [False, True])
+@pytest.mark.parametrize("n", [67, 130, 200])
+def test_many_sequences_in_chunks(ctx, n, one, f16):
+    """Long sequences on both sides of the 64th: their chunks' jobs, parts and
+    arrivals follow those of all sequences before them."""
+    seqs, _ = spread(n, (lambda i: 1) if one else (lambda i: i % 3), n)
+    b = Batch(seqs, 4, 2, 64, 16, f16, seed=n, one=one, spare_rows=1)
+    check(attend(ctx, b), *b.attention())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_sequences_in_wide_blocks(ctx, hd):
+    """The same among prompt chunks of f16 pages."""
+    seqs, at = spread(130, lambda i: (0, 1, 5, 1)[i % 4] if i not in (1, 63, 64, 128) else 40, 51)
+    b = Batch(seqs, 14, 2, hd, 16, True, seed=52)
+    only = [int(b.start[i]) + j for i in at for j in range(int(b.new[i]))]
+    ref, tol = b.attention(only=only)
+    got = attend(ctx, b)
+    assert np.all(np.isfinite(got))
+    check(got[only], ref[only], tol[only])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_many_sequences_unsplit(ctx, f16):
+    """So many KV heads and sequences that no block is split."""
+    seqs, at = spread(140, lambda i: 1, 53)
+    b = Batch(seqs, 32, 32, 64, 16, f16, seed=54, one=True)
+    ref, tol = b.attention(only=at)
+    got = attend(ctx, b)
+    assert np.all(np.isfinite(got))
+    check(got[at], ref[at], tol[at])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,KVH,hd", [(71, 1, 64), (80, 2, 128), (130, 1, 64)])
+@pytest.mark.parametrize("P", [0, 70])
+def test_many_heads_of_a_group(ctx, H, KVH, hd, P, f16):
+    """One row a sequence fills a wide block, or more than one."""
+    seqs = [(0, 1), (16, 1), (200, 1), (1900, 1)]
+    if P:
+        b, table, *kv = shared_batch(seqs, P, H, KVH, hd, 16, f16, seed=H, one=True)
+    else:
+        b, table, kv = Batch(seqs, H, KVH, hd, 16, f16, seed=H, one=True), None, []
+    check(attend(ctx, b, shared=(table, P) if P else None), *b.attention(*kv))
+
+
+@pytest.mark.parametrize("f16,new", [(False, 3), (True, 3), (True, 40)])
+def test_tables_without_a_place(ctx, f16, new):
+    """No table: nothing is seen or stored."""
+    b = Batch([(20, new), (0, 1)], 14, 2, 64, 16, f16, seed=55)
+    batch = b.upload(ctx)
+    batch.table, batch.table_stride = None, 0
+    assert np.all(attend(ctx, b, batch) == 0.0)
+    ones = ctx.buffer_from(np.ones((b.R, 2, 64), np.float32))
+    d.rope_kv_append_paged_f32(ctx, batch, ctx.buffer_from(b.q), ones, ones, ctx.new_buffer(4 * b.q.size), 14, 1e4)
+    ctx.flush()
+    assert np.array_equal(b.bk.read(b.k.dtype), b.k.ravel(), equal_nan=True)
+
+
 @pytest.mark.parametrize("f16", [False, True])
 def test_page_stride(ctx, f16):
     """Pools with other things between the pages."""
@@ -264,6 +334,16 @@ def test_shared_prefix_wide_batch(ctx, f16):
     b, table, keys, vals = shared_batch([(int(k), 1) for k in rng.integers(0, 90, 70)], 2048, 14, 2, 64, 64, f16,
                                         seed=12, one=True)
     check(attend(ctx, b, shared=(table, 2048)), *b.attention(keys, vals))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_shared_prefix_ragged_batch(ctx, f16):
+    """Rows of more than 64 sequences, some without any, over a prefix that
+    ends inside a page."""
+    rng = np.random.default_rng(56)
+    seqs = [(int(k), i % 4 if i < 131 else 0) for i, k in enumerate(rng.integers(0, 60, 140))]
+    b, table, keys, vals = shared_batch(seqs, 1003, 4, 2, 64, 16, f16, seed=57, spare_rows=2)
+    check(attend(ctx, b, shared=(table, 1003)), *b.attention(keys, vals))
 
 
 @pytest.mark.parametrize("f16", [False, True])
