@@ -4317,7 +4317,10 @@ static int token_logprobs(rt_ctx* c, const char* type, uint32_t el, const void* 
     const uint32_t segs = std::max(1u, std::min({want, RT_LOGPROBS_SEG_MAX, (n + 4095) / 4096}));
     a.seg_len = ((n + segs - 1) / segs + 4095) / 4096 * 4096;
     a.segs = (n + a.seg_len - 1) / a.seg_len;
-    if (a.segs > 1) {  // (then rows ≤ the CUs)
+    if (a.segs > 1) {  // (then rows ≤ twice the CUs)
+        if (rows > kAttnCounters)
+            return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: token_logprobs: rows=%u exceed %u counters", rows,
+                        kAttnCounters);
         const size_t nk = (size_t)rows * a.segs;
         const int st = ensure_ws(c, nk * (16 + 8 * top), "token_logprobs");
         if (st != RT_OK) return st;
