@@ -377,8 +377,9 @@ template <int HD, class T>
 struct PagedAcc {
     typedef PagedTile<HD, T> Tile;
     static constexpr uint32_t VW = Tile::VW, VN = Tile::VN;
-    // weights are 2^BIAS·e^(s − m); m follows the maximum when that has grown by 2^GROW
-    static constexpr float GROW = 3.0f, BIAS = sizeof(T) == 2 ? 15.0f - GROW : 0.0f;
+    // weights are 2^BIAS·e^(s − m); m follows the maximum when that has grown by 2^GROW.  f32 pages: so that the
+    // largest weight is 1, and a product with the type's largest value finite
+    static constexpr float GROW = 3.0f, BIAS = sizeof(T) == 2 ? 15.0f - GROW : -GROW;
     f32x4 o[VN][VW];
     float m, l;
     RT_DEV void start() {

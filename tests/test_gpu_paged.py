@@ -300,6 +300,25 @@ def test_values_far_apart(ctx, f16):
     check(attend(ctx, b), *b.attention())
 
 
+@pytest.mark.parametrize("f16,new", [(False, 1), (False, 5), (True, 1), (True, 40)])
+@pytest.mark.parametrize("at", [70, 100])
+def test_the_largest_values(ctx, at, f16, new):
+    """A value of almost the type's largest where the scores have risen a
+    little, in a later tile: its share of the output is no more than it."""
+    b = Batch([(120 - new, new), (9, 1)], 4, 2, 64, 16, f16, seed=58)
+    for s in range(2):
+        n, dt = int(b.kv[s]), b.k.dtype
+        K, V = np.zeros((n, 2, 64), dt), np.zeros((n, 2, 64), dt)
+        if s == 0:
+            K[at, :, 0] = 2.5 * np.log(2) * 8
+            V[at] = 0.97 * np.finfo(dt).max * b.rng.choice([-1, 1], (2, 64))
+        b.put(b.k, s, 0, K)
+        b.put(b.v, s, 0, V)
+    b.q[:] = 0
+    b.q[:, :, 0] = 1.0
+    check(attend(ctx, b), *b.attention())
+
+
 def shared_batch(seqs, P, H, KVH, hd, ps, f16, seed, **kw):
     """Sequences (P + kept, new) whose first P positions are the same; the
     shared table, and own tables that hold nothing there but their last page."""
