@@ -81,6 +81,8 @@ class BatchDecoder:
         if any(F["gate"] != F["up"] for F in model.fmts):
             raise ValueError("gate and up in different formats: no fused gate+up+SiLU")
         self.model, self.ctx, self.kv, self.page_size = model, model.ctx, kv, page_size
+        # (the embedding takes 65,535 rows, the argmax of rows 14,336)
+        max_rows, max_logits = min(max_rows, 65535), min(max_logits, 14336)
         self.max_seqs, self.max_len, self.max_rows = max_seqs, max_len, max_rows
         self.max_logits, self.max_top = min(max_logits, max_rows), min(max_top, c.vocab, 64)
         self.stride = -(-max_len // page_size)

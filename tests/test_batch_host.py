@@ -77,6 +77,12 @@ def test_step_in_passes():
     assert b.pool.free == 12
 
 
+def test_passes_stay_within_what_their_calls_take():
+    """65,535 rows of the embedding, 14,336 of the argmax."""
+    b = decoder(max_rows=100_000, max_logits=100_000)
+    assert b.max_rows == 65535 and b.max_logits == 14336
+
+
 def test_score_keeps_all_but_the_last():
     b = decoder()
     s, t = b.open(), b.open()
