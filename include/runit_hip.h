@@ -762,14 +762,16 @@ int rt_paged_attention_f32(rt_ctx* ctx, const rt_paged_batch* batch, const float
                            uint32_t num_heads);
 /* rt_paged_attention_f32 where the first shared_len positions of every
  * sequence are the same: they are read through shared_table (device,
- * ceil(shared_len / page_size) page ids), once for all rows of the batch, and
- * the sequences' own tables from position shared_len on.  kv_len counts them. */
+ * ceil(shared_len / page_size) page ids), by the rows of all sequences together
+ * (once for each 16 (row, head) pairs of a KV head, with many over f16 pages each
+ * 128; not once a sequence), and the sequences' own tables from position
+ * shared_len on.  kv_len counts them. */
 int rt_shared_prefix_attention_f32(rt_ctx* ctx, const rt_paged_batch* batch, const float* q,
                                    float* out, uint32_t num_heads, const uint32_t* shared_table,
                                    uint32_t shared_len);
 /* Log probabilities of given tokens (new; the reference samples on the CPU and
- * reports none).  logits [rows] of n values, row r at logits + r·row_stride;
- * tokens [rows]:
+ * reports none).  logits [rows] of n values, row r at logits + r·row_stride, at
+ * most 65,535 of them; tokens [rows]:
  *   logprob[r] = x_t − ln Σ e^x     (−inf for a token id ≥ n)
  *   entropy[r] = −Σ p·ln p          (nats; may be NULL)
  *   rank[r]    = logits above x_t   (may be NULL)

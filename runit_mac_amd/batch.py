@@ -4,7 +4,7 @@ reference, whose engine holds one sequence in one KvCache).
 A BatchDecoder takes a DecodeModel's weights and gives its sequences pages of
 one pool as they grow.  Each pass runs any number of rows of any of them
 together: prompts, single tokens, drafts to verify.  All sequences may begin
-with the same prompt, held and read once.
+with the same prompt, held once and read for all together.
 """
 from __future__ import annotations
 

@@ -111,7 +111,7 @@ RT_DEV void paged_append(const PagedAppendArgs& a) {
 // with a softmax of its own, and meet in LDS.  Bound by the pages' bytes: 24
 // sequences of up to 8,000 positions, 4 KV heads of 128, f16 (182 MB) 41.7 µs
 // = 4.4 TB/s; one of 100,003, f32 (410 MB) 79 µs = 5.2 TB/s; a large copy
-// makes 5.1.  A few hundred positions: 8.5 µs, of which the launch and the
+// makes 5.1.  A few hundred positions: 8.3 µs, of which the launch and the
 // planning are 4, two trips to memory and the meeting the rest.
 // Wide blocks (f16 pages; prompt chunks, a shared prefix): each of four waves has
 // 32 columns of its own and all take every tile, from LDS, on the 32x32x16 f16

@@ -923,7 +923,7 @@ def paged_attention_f32(ctx, batch, q, out, num_heads):
 
 def shared_prefix_attention_f32(ctx, batch, q, out, num_heads, shared_table, shared_len):
     """paged_attention_f32 where all sequences begin with the same shared_len
-    positions, in the pages of shared_table, read once for all (new)."""
+    positions, in the pages of shared_table, read for all together (new)."""
     ctx._check(ctx.lib.rt_shared_prefix_attention_f32(ctx.handle, batch.ref, _ptr(q), _ptr(out), num_heads,
                                                       _ptr(shared_table), shared_len))
 
