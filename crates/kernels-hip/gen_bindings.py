@@ -27,7 +27,7 @@ POINTEE = {"void": "c_void", "float": "f32", "uint16_t": "u16", "uint32_t": "u32
            "char": "c_char", "int64_t": "i64", "double": "f64", "uint8_t": "u8"}
 OPAQUE = {"rt_ctx": "RtCtx", "rt_event": "RtEvent", "rt_graph": "RtGraph", "rt_gguf": "RtGguf",
           "rt_step": "RtStep", "rt_step_model": "RtStepModel", "rt_step_layer": "RtStepLayer",
-          "rt_paged_batch": "RtPagedBatch"}
+          "rt_paged_batch": "RtPagedBatch", "rt_logit_rules": "RtLogitRules"}
 MANUAL_PREFIXES = ("rt_ctx_", "rt_flush", "rt_last_error", "rt_global_last_error", "rt_malloc",
                    "rt_free", "rt_upload", "rt_download", "rt_memset", "rt_copy_d2d", "rt_event_",
                    "rt_capture_", "rt_graph_", "rt_gguf_", "rt_decode_step_", "rt_has_kernel",
@@ -119,6 +119,16 @@ def ffi_rs(funcs) -> str:
            "    pub head_dim: u32, pub table_stride: u32, pub n_seqs: u32, pub rows: u32,",
            "    pub page_stride: u64,",
            "    pub table: *const u32, pub row_start: *const u32, pub kv_len: *const u32,",
+           "}",
+           "/// rt_logit_rules (include/runit_hip.h)",
+           "#[repr(C)] #[derive(Clone, Copy)]",
+           "pub struct RtLogitRules {",
+           "    pub tokens: *const u32, pub token_start: *const u32, pub token_len: *const u32,",
+           "    pub prompt_len: *const u32, pub n_tokens: u64,",
+           "    pub repetition: *const f32, pub frequency: *const f32, pub presence: *const f32,",
+           "    pub bias_ids: *const u32, pub bias_start: *const u32, pub bias_len: *const u32,",
+           "    pub bias: *const f32, pub n_bias: u64,",
+           "    pub mask: *const u32, pub mask_row: *const u32, pub mask_stride: u64, pub mask_rows: u32,",
            "}", "", "extern \"C\" {"]
     for ret, name, params in funcs:
         args = ", ".join(f"{ident(n)}: {rust_type(c, b, s)}" for c, b, s, n in params)
@@ -154,8 +164,13 @@ def dispatch_rs(funcs) -> str:
                 sig.append(f"{ident(pn)}: &Buffer")
                 cast = rust_type(c, b, 1)
                 call.append(f"{ident(pn)}.as_ptr() as {cast}")
-            elif s == 1 and b == "rt_paged_batch":
-                sig.append(f"{ident(pn)}: &ffi::RtPagedBatch")
+            elif s == 1 and pn == "batches":  # (with its length)
+                sig.append(f"{pn}: &[ffi::{OPAQUE[b]}]")
+                call.append(f"{pn}.as_ptr(), {pn}.len() as u32")
+            elif pn == "n_batches":
+                continue
+            elif s == 1 and b in ("rt_paged_batch", "rt_logit_rules"):
+                sig.append(f"{ident(pn)}: &ffi::{OPAQUE[b]}")
                 call.append(ident(pn))
             elif s == 0 and b in SCALARS:
                 sig.append(f"{ident(pn)}: {SCALARS[b]}")

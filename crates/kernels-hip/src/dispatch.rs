@@ -458,6 +458,21 @@ pub fn paged_attention_f32(ctx: &HipContext, batch: &ffi::RtPagedBatch, q: &Buff
 pub fn shared_prefix_attention_f32(ctx: &HipContext, batch: &ffi::RtPagedBatch, q: &Buffer, out: &Buffer, num_heads: u32, shared_table: &Buffer, shared_len: u32) -> Result<()> {
     status(ctx.raw(), unsafe { ffi::rt_shared_prefix_attention_f32(ctx.raw(), batch, q.as_ptr() as *const f32, out.as_ptr() as *mut f32, num_heads, shared_table.as_ptr() as *const u32, shared_len) })
 }
+pub fn paged_gather_f32(ctx: &HipContext, batch: &ffi::RtPagedBatch, k: &Buffer, v: &Buffer) -> Result<()> {
+    status(ctx.raw(), unsafe { ffi::rt_paged_gather_f32(ctx.raw(), batch, k.as_ptr() as *mut f32, v.as_ptr() as *mut f32) })
+}
+pub fn paged_gather_f16(ctx: &HipContext, batch: &ffi::RtPagedBatch, k: &Buffer, v: &Buffer) -> Result<()> {
+    status(ctx.raw(), unsafe { ffi::rt_paged_gather_f16(ctx.raw(), batch, k.as_ptr() as *mut u16, v.as_ptr() as *mut u16) })
+}
+pub fn paged_copy(ctx: &HipContext, batches: &[ffi::RtPagedBatch], src: &Buffer, dst: &Buffer, n: u32) -> Result<()> {
+    status(ctx.raw(), unsafe { ffi::rt_paged_copy(ctx.raw(), batches.as_ptr(), batches.len() as u32, src.as_ptr() as *const u32, dst.as_ptr() as *const u32, n) })
+}
+pub fn adjust_logits_f32(ctx: &HipContext, logits: &Buffer, out: &Buffer, rows: u32, n: u32, row_stride: u64, rules: &ffi::RtLogitRules) -> Result<()> {
+    status(ctx.raw(), unsafe { ffi::rt_adjust_logits_f32(ctx.raw(), logits.as_ptr() as *const f32, out.as_ptr() as *mut f32, rows, n, row_stride, rules) })
+}
+pub fn adjust_logits_f16(ctx: &HipContext, logits: &Buffer, out: &Buffer, rows: u32, n: u32, row_stride: u64, rules: &ffi::RtLogitRules) -> Result<()> {
+    status(ctx.raw(), unsafe { ffi::rt_adjust_logits_f16(ctx.raw(), logits.as_ptr() as *const u16, out.as_ptr() as *mut u16, rows, n, row_stride, rules) })
+}
 pub fn token_logprobs_f32(ctx: &HipContext, logits: &Buffer, tokens: &Buffer, rows: u32, n: u32, row_stride: u64, logprob: &Buffer, entropy: &Buffer, rank: &Buffer, top: u32, top_ids: &Buffer, top_logprobs: &Buffer) -> Result<()> {
     status(ctx.raw(), unsafe { ffi::rt_token_logprobs_f32(ctx.raw(), logits.as_ptr() as *const f32, tokens.as_ptr() as *const u32, rows, n, row_stride, logprob.as_ptr() as *mut f32, entropy.as_ptr() as *mut f32, rank.as_ptr() as *mut u32, top, top_ids.as_ptr() as *mut u32, top_logprobs.as_ptr() as *mut f32) })
 }

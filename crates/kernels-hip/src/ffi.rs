@@ -37,6 +37,16 @@ pub struct RtPagedBatch {
     pub page_stride: u64,
     pub table: *const u32, pub row_start: *const u32, pub kv_len: *const u32,
 }
+/// rt_logit_rules (include/runit_hip.h)
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct RtLogitRules {
+    pub tokens: *const u32, pub token_start: *const u32, pub token_len: *const u32,
+    pub prompt_len: *const u32, pub n_tokens: u64,
+    pub repetition: *const f32, pub frequency: *const f32, pub presence: *const f32,
+    pub bias_ids: *const u32, pub bias_start: *const u32, pub bias_len: *const u32,
+    pub bias: *const f32, pub n_bias: u64,
+    pub mask: *const u32, pub mask_row: *const u32, pub mask_stride: u64, pub mask_rows: u32,
+}
 
 extern "C" {
     pub fn rt_ctx_create(out: *mut *mut RtCtx, code_object_path: *const c_char) -> c_int;
@@ -214,6 +224,11 @@ extern "C" {
     pub fn rt_rope_kv_append_paged_f32(ctx: *mut RtCtx, batch: *const RtPagedBatch, q: *const f32, k: *const f32, v: *const f32, q_out: *mut f32, num_heads: u32, theta: f32) -> c_int;
     pub fn rt_paged_attention_f32(ctx: *mut RtCtx, batch: *const RtPagedBatch, q: *const f32, out: *mut f32, num_heads: u32) -> c_int;
     pub fn rt_shared_prefix_attention_f32(ctx: *mut RtCtx, batch: *const RtPagedBatch, q: *const f32, out: *mut f32, num_heads: u32, shared_table: *const u32, shared_len: u32) -> c_int;
+    pub fn rt_paged_gather_f32(ctx: *mut RtCtx, batch: *const RtPagedBatch, k: *mut f32, v: *mut f32) -> c_int;
+    pub fn rt_paged_gather_f16(ctx: *mut RtCtx, batch: *const RtPagedBatch, k: *mut u16, v: *mut u16) -> c_int;
+    pub fn rt_paged_copy(ctx: *mut RtCtx, batches: *const RtPagedBatch, n_batches: u32, src: *const u32, dst: *const u32, n: u32) -> c_int;
+    pub fn rt_adjust_logits_f32(ctx: *mut RtCtx, logits: *const f32, out: *mut f32, rows: u32, n: u32, row_stride: u64, rules: *const RtLogitRules) -> c_int;
+    pub fn rt_adjust_logits_f16(ctx: *mut RtCtx, logits: *const u16, out: *mut u16, rows: u32, n: u32, row_stride: u64, rules: *const RtLogitRules) -> c_int;
     pub fn rt_token_logprobs_f32(ctx: *mut RtCtx, logits: *const f32, tokens: *const u32, rows: u32, n: u32, row_stride: u64, logprob: *mut f32, entropy: *mut f32, rank: *mut u32, top: u32, top_ids: *mut u32, top_logprobs: *mut f32) -> c_int;
     pub fn rt_token_logprobs_f16(ctx: *mut RtCtx, logits: *const u16, tokens: *const u32, rows: u32, n: u32, row_stride: u64, logprob: *mut f32, entropy: *mut f32, rank: *mut u32, top: u32, top_ids: *mut u32, top_logprobs: *mut f32) -> c_int;
     pub fn rt_embed_q8_0_f32(ctx: *mut RtCtx, table: *const c_void, token: *const u32, out: *mut f32, k: u32) -> c_int;

@@ -731,14 +731,29 @@ int rt_argmax_rows_first_f32(rt_ctx* ctx, const float* in, uint32_t* result, uin
  * them.  Rows behind the last sequence's are left as they are, here and in the
  * outputs.  Positions from table_stride·page_size on are neither stored nor
  * seen, nor are rows at positions below 0 (kv_len[s] < n). */
+/* Pages of 4 bits hold a code n of 0 .. 15 an element and, for each 32 elements of
+ * a head, a scale word: an f16 step d in its upper twelve bits, a zero point z in the
+ * lower four.  The element is d·(n − z), an f16 exactly.  From a group's smallest
+ * and largest elements, and 0, d is a fifteenth of their distance, up to seven
+ * significant bits and to 2^-20, z = −smallest / d, n = x / d + z, each to the nearest
+ * (even): an element is off by d / 2 at most.  A group with an
+ * element beyond 32,768 or not finite is held as NaN.  head_dim · 9/16 bytes a
+ * position and KV head; a KV head's part of a page is [page_size · head_dim / 2] bytes of
+ * codes and [page_size · head_dim / 32] scale words:
+ *   keys    codes as 32-bit words of 8 elements in a row, from the lowest bits
+ *           0, 2, 4, 6, 1, 3, 5, 7; scales [page_size][head_dim / 32];
+ *   values  by 16 positions: words [head_dim / 16w][4][16][2][w / 4] (w = 4 at head_dim 64,
+ *           else 8); word (i, g, c, p, h) has the elements 16w·i + w·c + 4h .. + 3 of
+ *           position 4g + 2p, then those of the next; scales [head_dim / 32][16]. */
+#define RT_PAGES_Q4 4
 typedef struct {
     void *k_pages, *v_pages;     /* device, 16-byte aligned */
-    uint32_t f16;                /* elements of a page: 0 f32, 1 f16 */
+    uint32_t f16;                /* elements of a page: 0 f32, 1 f16, 4 (RT_PAGES_Q4) 4 bits */
     uint32_t num_pages, page_size;    /* page_size: a power of two, 16 or more */
     uint32_t num_kv_heads, head_dim;  /* head_dim 64, 128 or 256 */
     uint32_t table_stride, n_seqs;
     uint32_t rows;               /* rows of the activations (at least row_start[n_seqs]) */
-    uint64_t page_stride;        /* elements, a multiple of 8; 0: pages one after another */
+    uint64_t page_stride;        /* elements, a multiple of 8 (4 bits: bytes, of 16); 0: pages one after another */
     const uint32_t* table;       /* device [n_seqs][table_stride] */
     const uint32_t* row_start;   /* device [n_seqs + 1]; NULL: one row a sequence */
     const uint32_t* kv_len;      /* device [n_seqs] */
@@ -746,7 +761,7 @@ typedef struct {
 /* RoPE of q [rows][num_heads][head_dim] into q_out (may alias q) and of k
  * [rows][num_kv_heads][head_dim] at the rows' positions (pairs (d, d +
  * head_dim/2), the angles reduced in 64 bits), k and v (as k) stored into the
- * pages (f16: rounded to nearest even).  Rows that several sequences store in one place
+ * pages (f16: rounded to nearest even; 4 bits: as above).  Rows that several sequences store in one place
  * leave either's elements there: a shared page is copied before it is written. */
 int rt_rope_kv_append_paged_f32(rt_ctx* ctx, const rt_paged_batch* batch, const float* q,
                                 const float* k, const float* v, float* q_out, uint32_t num_heads,
@@ -769,6 +784,46 @@ int rt_paged_attention_f32(rt_ctx* ctx, const rt_paged_batch* batch, const float
 int rt_shared_prefix_attention_f32(rt_ctx* ctx, const rt_paged_batch* batch, const float* q,
                                    float* out, uint32_t num_heads, const uint32_t* shared_table,
                                    uint32_t shared_len);
+/* The keys and values of the batch's rows as the pages hold them, k and v [rows][num_kv_heads]
+ * [head_dim] (either may be NULL): the inverse of the append, so a sequence whole where
+ * it brings kv_len[s] rows.  Rows without a place give zeros, those behind the last
+ * sequence's are left as they are.  f16 outputs are rounded to nearest even (exact but for f32 pages). */
+int rt_paged_gather_f32(rt_ctx* ctx, const rt_paged_batch* batch, float* k, float* v);
+int rt_paged_gather_f16(rt_ctx* ctx, const rt_paged_batch* batch, uint16_t* k, uint16_t* v);
+/* Copies pages: in the key and value pools of each of n_batches batches (a model's
+ * layers; pages of one type, size, number and stride, sequences and tables not looked
+ * at), page dst[i] becomes what page src[i] is, i < n ≤ 65,535, as if one after another:
+ * chains, cycles and pages written twice included.  src and dst are device arrays; an
+ * entry with an id ≥ num_pages copies nothing.  No two pools may overlap. */
+int rt_paged_copy(rt_ctx* ctx, const rt_paged_batch* batches, uint32_t n_batches,
+                  const uint32_t* src, const uint32_t* dst, uint32_t n);
+/* Rules on logits (new; the reference's sampler has none).  Row r's list of tokens is
+ * tokens[token_start[r]] .. token_len[r] of them, the first prompt_len[r] (NULL: 0) of
+ * its prompt; its biases likewise.  Lists may overlap and are cut at n_tokens and n_bias;
+ * ids ≥ n are passed over.  A token that is c times in the list, c' times behind the prompt:
+ *   x → (c > 0: x > 0 ? x / repetition : x · repetition) − frequency · c'
+ *         − (c' > 0 ? presence : 0) + Σ bias,
+ * in f32, rounded once; then −inf if the row has a mask without the token's bit (bit t % 32 of
+ * word t / 32).  mask_row[r] (NULL: r) is the row's mask; none if ≥ mask_rows.  All pointers
+ * are device arrays, NULL with n_tokens, n_bias or mask_rows 0. */
+typedef struct {
+    const uint32_t *tokens, *token_start, *token_len, *prompt_len;
+    uint64_t n_tokens;                               /* elements of tokens */
+    const float *repetition, *frequency, *presence;  /* [rows]; NULL: 1, 0, 0 */
+    const uint32_t *bias_ids, *bias_start, *bias_len;
+    const float* bias;
+    uint64_t n_bias;                                 /* elements of bias_ids and bias */
+    const uint32_t *mask, *mask_row;                 /* [mask_rows][mask_stride], [rows] */
+    uint64_t mask_stride;                            /* words; 0: ceil(n / 32) */
+    uint32_t mask_rows;
+} rt_logit_rules;
+/* Applies them to logits [rows] of n values, row r at logits + r·row_stride (at most
+ * 65,535 of them), into out (the same stride): the same buffer, of which only what
+ * changes is written, or one apart.  Logits that no rule names keep their bits. */
+int rt_adjust_logits_f32(rt_ctx* ctx, const float* logits, float* out, uint32_t rows, uint32_t n,
+                         uint64_t row_stride, const rt_logit_rules* rules);
+int rt_adjust_logits_f16(rt_ctx* ctx, const uint16_t* logits, uint16_t* out, uint32_t rows,
+                         uint32_t n, uint64_t row_stride, const rt_logit_rules* rules);
 /* Log probabilities of given tokens (new; the reference samples on the CPU and
  * reports none).  logits [rows] of n values, row r at logits + r·row_stride, at
  * most 65,535 of them; tokens [rows]:

@@ -1,0 +1,392 @@
+// k_paged_q4.hip — batches over paged caches of 4 bits: the rotary embedding
+// with the append of new rows, their way back, and the causal attention.
+//
+// A group of 32 elements of a head's key or value has one scale word: the step d,
+// an f16 of seven significant bits, whose lowest four bits hold the zero point z; a code n in
+// 0 .. 15 stands for d·(n − z).  Seven bits times the four of n − z are the eleven
+// of an f16: what the codes stand for is one exactly, and the f16 matrix
+// cores take it as they take f16 pages.  4.5 bits an element.
+//
+// A KV head's part of a page of ps positions: ps·HD/2 bytes of codes, then
+// ps·HD/32 scale words, so laid out that a lane's operands of the matrix
+// cores are one load:
+//   keys    codes [ps][HD/8] words of 8 elements, the even ones in the lower half;
+//           scales [ps][HD/32];
+//   values  per tile of 16 positions: codes [HD/(16·W)][4][16][2][W/4] words, W =
+//           4 at head size 64, else 8: word (i, g, c, p, h) has the elements 16·W·i + W·c
+//           + 4h .. + 3 of the positions 4g + 2p (lower half) and 4g + 2p + 1; scales
+//           [HD/32][16].
+// So no byte is two positions', and rows are stored without a look at others.
+#include "rt_paged.h"
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// (the type of these pages' elements in rt_paged.h's templates: a byte)
+struct Q4 {
+    uint8_t b;
+};
+template <int HD>
+struct Q4Layout {
+    static constexpr uint32_t W = HD == 64 ? 4 : 8, VN = HD / (16 * W);
+    static constexpr uint32_t TILE = RT_PAGED_TILE * HD / 2;    // bytes of a tile's codes
+    static constexpr uint32_t SCALES = RT_PAGED_TILE * HD / 16;  // of its scales
+    static constexpr uint32_t ROW = HD / 2 + HD / 16;            // of a position
+};
+
+// The eight values of a word of codes as four pairs (code k of the lower half, k of the upper).  z: 1024 +
+// the zero points, d: the steps of the two halves; z16 = 1024 + 16·z, d16 = d / 16.
+// (1024 + n as an f16 has n in its lowest bits, 1024 + 16n four above.)
+struct Q4Scale {
+    h2_t z, z16, d, d16;
+    RT_DEV explicit Q4Scale(uint32_t w) {  // the halves' scale words
+        z = __builtin_bit_cast(h2_t, (w & 0x000F000Fu) | 0x64006400u);
+        z16 = __builtin_bit_cast(h2_t, (w & 0x000F000Fu) << 4 | 0x64006400u);
+        d = __builtin_bit_cast(h2_t, w & 0xFFF0FFF0u);
+        d16 = d * (h2_t){(_Float16)0.0625f, (_Float16)0.0625f};
+    }
+};
+RT_DEV void q4_values(uint32_t w, const Q4Scale& s, h2_t (&o)[4]) {
+    const uint32_t v = w >> 8;
+    o[0] = (__builtin_bit_cast(h2_t, (w & 0x000F000Fu) | 0x64006400u) - s.z) * s.d;
+    o[1] = (__builtin_bit_cast(h2_t, (w & 0x00F000F0u) | 0x64006400u) - s.z16) * s.d16;
+    o[2] = (__builtin_bit_cast(h2_t, (v & 0x000F000Fu) | 0x64006400u) - s.z) * s.d;
+    o[3] = (__builtin_bit_cast(h2_t, (v & 0x00F000F0u) | 0x64006400u) - s.z16) * s.d16;
+}
+RT_DEV h8_t q4_row(uint32_t w, const Q4Scale& s) {  // a word of a key's codes, in order
+    h2_t o[4];
+    q4_values(w, s, o);
+    return (h8_t){o[0][0], o[0][1], o[1][0], o[1][1], o[2][0], o[2][1], o[3][0], o[3][1]};
+}
+
+template <>
+struct PagedView<Q4> {
+    const Q4 *k, *v;         // the KV head's part of page 0
+    const uint32_t* table;
+    uint64_t page_stride;    // bytes
+    uint32_t num_pages, ps_shift;
+    uint32_t tb, t1;
+    uint32_t lo;
+    RT_DEV uint32_t page(uint32_t t) const {
+        typedef const __attribute__((address_space(4))) uint32_t* sptr_t;  // (a scalar load)
+        return t < t1 ? ((sptr_t)table)[(tb + t) * RT_PAGED_TILE >> ps_shift] : num_pages;
+    }
+    RT_DEV uint32_t slot(uint32_t t) const { return (tb + t) * RT_PAGED_TILE & ((1u << ps_shift) - 1); }
+    // byte of a tile's codes; its scales'
+    RT_DEV size_t place(uint32_t t, uint32_t page, uint32_t hd) const {
+        return page * page_stride + (size_t)slot(t) * (hd / 2);
+    }
+    RT_DEV size_t scales(size_t off, uint32_t t, uint32_t hd) const {
+        return off + ((size_t)(hd / 2) << ps_shift) - (size_t)slot(t) * (hd / 2 - hd / 16);
+    }
+    template <int HD>
+    RT_DEV float value(size_t off, uint32_t t, uint32_t r, uint32_t d) const {
+        constexpr uint32_t W = Q4Layout<HD>::W;
+        const uint32_t n = (((d / (16 * W) * 4 + r / 4) * 16 + d / W % 16) * 2 + r % 4 / 2) * (W / 4) + d % W / 4;
+        const uint32_t s = ((const uint16_t*)(v + scales(off, t, HD)))[d / 32 * 16 + r];
+        h2_t o[4];
+        q4_values(((const uint32_t*)(v + off))[n], Q4Scale(s | s << 16), o);
+        float x = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) x = d % 4 == k ? (float)(r & 1 ? o[k][1] : o[k][0]) : x;
+        return x;
+    }
+    template <int HD>
+    static RT_DEV size_t part(uint32_t kvh, uint32_t ps_shift) { return ((size_t)kvh << ps_shift) * Q4Layout<HD>::ROW; }
+};
+
+// A tile's operands for the f32 matrix cores (jobs whose sums are not finite), as an f16 page's.
+template <int HD>
+struct PagedTile<HD, Q4> {
+    static constexpr uint32_t KW = 8, KN = HD / 32, VW = Q4Layout<HD>::W, VN = Q4Layout<HD>::VN;
+    typedef _Float16 vvec __attribute__((ext_vector_type(VW)));
+    h8_t k[KN];
+    vvec v[4][VN];
+    RT_DEV void load_k(const PagedView<Q4>& w, size_t off, uint32_t t, uint32_t lane) {
+        const uint32_t r = lane & 15, g = lane >> 4;
+        const uint32_t* c = (const uint32_t*)(w.k + off) + r * (HD / 8) + g;
+        const uint16_t* s = (const uint16_t*)(w.k + w.scales(off, t, HD)) + r * (HD / 32);
+#pragma unroll
+        for (uint32_t i = 0; i < KN; ++i) k[i] = q4_row(c[4 * i], Q4Scale(s[i] * 0x10001u));
+    }
+    RT_DEV void load_v(const PagedView<Q4>& w, size_t off, uint32_t t, uint32_t lane) {
+        const uint32_t c = lane & 15, g = lane >> 4;
+        const uint16_t* s = (const uint16_t*)(w.v + w.scales(off, t, HD));
+#pragma unroll
+        for (uint32_t i = 0; i < VN; ++i)
+#pragma unroll
+            for (uint32_t p = 0; p < 2; ++p)
+#pragma unroll
+                for (uint32_t h = 0; h < VW / 4; ++h) {
+                    const uint32_t* ss = (const uint32_t*)(s + (16 * VW * i + VW * c) / 32 * 16 + 4 * g + 2 * p);
+                    h2_t o[4];
+                    q4_values(((const uint32_t*)(w.v + off))[(((i * 4 + g) * 16 + c) * 2 + p) * (VW / 4) + h], Q4Scale(*ss), o);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        v[2 * p][i][4 * h + e] = o[e][0];
+                        v[2 * p + 1][i][4 * h + e] = o[e][1];
+                    }
+                }
+    }
+    RT_DEV void clear(uint32_t pos0, uint32_t lo, uint32_t limx) {
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r)
+#pragma unroll
+            for (uint32_t i = 0; i < VN; ++i) v[r][i] = pos0 + r < lo || pos0 + r >= limx ? vvec{} : v[r][i];
+    }
+};
+
+// ───────────────────────────── append, and back ─────────────────────────────
+//
+// As k_paged_append's: a workgroup a row and group of heads, a thread four elements of a head's
+// lower half and the four behind them of its upper.  Eight threads have a group:
+// its limits are three steps across lanes.
+//
+// lo = min(0, x), hi = max(0, x); d = (hi − lo) / 15 up to seven bits, 2^-20 at
+// least apart; z = −lo/d and n = x/d + z, each to the nearest, n kept within 0 .. 15.
+struct Q4Group {
+    uint32_t word;    // the scale word
+    uint32_t n[4];
+};
+RT_DEV Q4Group q4_code(f32x4 x) {
+    float lo = 0.0f, hi = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]);
+        bad |= !(fabsf(x[i]) <= 32768.0f);
+    }
+    lo = -max8(-lo), hi = max8(hi);
+    bad = max8(bad ? 1.0f : 0.0f) > 0.0f;
+    const float step = (hi - lo) / 15.0f;
+    // up to six bits behind the leading one; below 2^-14 to multiples of 2^-20
+    const float d = step < 6.103515625e-5f ? ceilf(step * 1048576.0f) * 9.5367431640625e-7f
+                                            : __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, step) + 0x1FFFFu) & ~0x1FFFFu);
+    const float inv = d > 0.0f ? 1.0f / d : 0.0f, z = rintf(-lo * inv);
+    Q4Group g;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) g.n[i] = bad ? 0u : (uint32_t)fminf(fmaxf(rintf(x[i] * inv) + z, 0.0f), 15.0f);
+    g.word = bad ? 0x7E00u : (uint32_t)f2h(d) | (uint32_t)z;
+    return g;
+}
+template <int HD>
+RT_DEV void q4_store(const PagedBatch& b, uint32_t page, uint32_t kvh, uint32_t slot, bool isv, uint32_t d, const Q4Group& g) {
+    constexpr uint32_t W = Q4Layout<HD>::W;
+    uint8_t* part = (uint8_t*)(isv ? b.v : b.k) + page * b.page_stride + PagedView<Q4>::part<HD>(kvh, b.ps_shift);
+    uint16_t* scales = (uint16_t*)(part + ((size_t)(HD / 2) << b.ps_shift));
+    if (isv) {
+        const uint32_t r = slot % 16;
+        uint16_t* tile = (uint16_t*)(part + (slot / 16) * Q4Layout<HD>::TILE);
+        const uint32_t n = (((d / (16 * W) * 4 + r / 4) * 16 + d / W % 16) * 2 + r % 4 / 2) * (W / 4) + d % W / 4;
+        tile[2 * n + r % 2] = (uint16_t)(g.n[0] | g.n[1] << 4 | g.n[2] << 8 | g.n[3] << 12);
+        if (d % 32 == 0) scales[slot / 16 * (HD / 2) + d / 32 * 16 + r] = (uint16_t)g.word;
+    } else {
+        // (eight elements are two threads')
+        const uint32_t mine = g.n[0] | g.n[2] << 4 | g.n[1] << 16 | g.n[3] << 20, next = lane_xor<1>(mine);
+        if (d % 8 == 0) ((uint32_t*)part)[slot * (HD / 8) + d / 8] = mine | next << 8;
+        if (d % 32 == 0) scales[slot * (HD / 32) + d / 32] = (uint16_t)g.word;
+    }
+}
+template <int HD>
+RT_DEV void paged_append_q4(const PagedAppendArgs& a) {
+    constexpr uint32_t half = HD / 2, TH = half / 4, HW = 256 / TH;  // threads a head, heads a pass
+    __shared__ float cs[half], sn[half];
+    const PagedBatch& b = a.b;
+    const uint32_t row = blockIdx.x, tid = threadIdx.x, ht = tid / TH, d = tid % TH * 4;
+    const uint32_t s = paged_seq(b, row);
+    if (s >= b.n_seqs) return;  // behind the last sequence
+    const auto [pos, page] = paged_place(b, s, row);
+    paged_turns<HD>(pos, a.log2_theta, cs, sn);
+    __syncthreads();
+    const uint32_t slot = pos & ((1u << b.ps_shift) - 1);
+    f32x4 c4, s4;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) c4[i] = cs[d + i], s4[i] = sn[d + i];
+    const uint32_t heads = a.H + 2 * b.KVH;
+    for (uint32_t h = blockIdx.y * HW + ht; h < heads; h += gridDim.y * HW) {
+        const bool isq = h < a.H, isv = h >= a.H + b.KVH;
+        const uint32_t kh = isq ? h : isv ? h - a.H - b.KVH : h - a.H;
+        const float* src = (isq ? a.q + ((size_t)row * a.H + kh) * HD : (isv ? a.v : a.k) + ((size_t)row * b.KVH + kh) * HD) + d;
+        const f32x4 lo = *(const f32x4*)src, hi = *(const f32x4*)(src + half);
+        f32x4 x = lo, y = hi;
+        if (!isv) {
+            x = lo * c4 - hi * s4;
+            y = lo * s4 + hi * c4;
+        }
+        if (isq) {
+            float* o = a.q_out + ((size_t)row * a.H + kh) * HD + d;
+            *(f32x4*)o = x;
+            *(f32x4*)(o + half) = y;
+        } else if (page < b.num_pages) {
+            q4_store<HD>(b, page, kh, slot, isv, d, q4_code(x));
+            q4_store<HD>(b, page, kh, slot, isv, d + half, q4_code(y));
+        }
+    }
+}
+
+// Four elements of a row's key or value, from d on.
+template <int HD>
+RT_DEV f32x4 q4_load(const PagedBatch& b, uint32_t page, uint32_t kvh, uint32_t slot, bool isv, uint32_t d) {
+    constexpr uint32_t W = Q4Layout<HD>::W;
+    const uint8_t* part = (const uint8_t*)(isv ? b.v : b.k) + page * b.page_stride + PagedView<Q4>::part<HD>(kvh, b.ps_shift);
+    const uint16_t* scales = (const uint16_t*)(part + ((size_t)(HD / 2) << b.ps_shift));
+    f32x4 x;
+    h2_t o[4];
+    if (isv) {
+        const uint32_t r = slot % 16;
+        const uint32_t n = (((d / (16 * W) * 4 + r / 4) * 16 + d / W % 16) * 2 + r % 4 / 2) * (W / 4) + d % W / 4;
+        const uint32_t w = ((const uint16_t*)(part + (slot / 16) * Q4Layout<HD>::TILE))[2 * n + r % 2];
+        q4_values(w, Q4Scale(scales[slot / 16 * (HD / 2) + d / 32 * 16 + r]), o);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) x[i] = (float)o[i][0];
+    } else {
+        const uint32_t w = ((const uint32_t*)part)[slot * (HD / 8) + d / 8] >> (d % 8 ? 8 : 0);
+        q4_values(w, Q4Scale(scales[slot * (HD / 32) + d / 32] * 0x10001u), o);
+        x = (f32x4){(float)o[0][0], (float)o[0][1], (float)o[1][0], (float)o[1][1]};
+    }
+    return x;
+}
+template <class O>
+RT_DEV void paged_gather_q4(const PagedGatherArgs& a) {
+    paged_gather<O>(a, [&](uint32_t page, uint32_t kvh, uint32_t slot, bool isv, uint32_t d) {
+        return a.head_dim == 64    ? q4_load<64>(a.b, page, kvh, slot, isv, d)
+               : a.head_dim == 128 ? q4_load<128>(a.b, page, kvh, slot, isv, d)
+                                   : q4_load<256>(a.b, page, kvh, slot, isv, d);
+    });
+}
+
+// ───────────────────────────── attention ─────────────────────────────
+
+// What a lane loads of a tile: keys, of position l % 16 the elements HD/4·(l / 16)
+// ..; values, of positions 4·(l / 16) .. + 3, W of every 16·W elements from W·(l % 16) on.
+template <int HD>
+struct Q4Raw {
+    static constexpr uint32_t W = Q4Layout<HD>::W, VN = Q4Layout<HD>::VN, KN = HD / 32;
+    static constexpr uint32_t CW = HD == 64 ? 2 : 4;  // words of a load of codes
+    typedef uint32_t cvec __attribute__((ext_vector_type(CW)));
+    cvec k[KN / CW], v[KN / CW];
+    uint32_t ks;        // at head size 256 two words
+    u32x2 vs[VN];
+    RT_DEV void load(const PagedView<Q4>& w, uint32_t t, uint32_t page, uint32_t lane) {
+        const uint32_t c = lane & 15, g = lane >> 4;
+        const size_t off = w.place(t, page, HD), so = w.scales(off, t, HD);
+#pragma unroll
+        for (uint32_t i = 0; i < KN / CW; ++i) k[i] = *(const cvec*)(w.k + off + c * (HD / 2) + g * (HD / 8) + i * CW * 4);
+        const uint16_t* s = (const uint16_t*)(w.k + so) + c * (HD / 32);
+        if constexpr (HD == 256) ks = ((const uint32_t*)s)[g];
+        else ks = s[HD == 128 ? g : g / 2];
+#pragma unroll
+        for (uint32_t i = 0; i < KN / CW; ++i) v[i] = *(const cvec*)(w.v + off + ((i * 4 + g) * 16 + c) * CW * 4);
+#pragma unroll
+        for (uint32_t i = 0; i < VN; ++i)
+            vs[i] = *(const u32x2*)((const uint16_t*)(w.v + so) + (16 * W * i + W * c) / 32 * 16 + 4 * g);
+    }
+    RT_DEV void none() {
+#pragma unroll
+        for (uint32_t i = 0; i < KN / CW; ++i) k[i] = cvec{}, v[i] = cvec{};
+        ks = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < VN; ++i) vs[i] = u32x2{};
+    }
+    // positions that no column sees may hold anything: steps of zero (a code is always finite)
+    RT_DEV void clear(uint32_t pos0, uint32_t lo, uint32_t limx) {
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r)
+            if (pos0 + r < lo || pos0 + r >= limx)
+#pragma unroll
+                for (uint32_t i = 0; i < VN; ++i) vs[i][r / 2] &= r % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+    }
+    RT_DEV uint32_t kscale(uint32_t i) const {  // of the key's words i, twice
+        if constexpr (HD == 256) return i < KN / 2 ? (ks & 0xFFFFu) * 0x10001u : (ks >> 16) * 0x10001u;
+        return ks * 0x10001u;
+    }
+};
+
+// The tiles t0, t0 + 1, t0 + step, ... for 16 columns, as f16 pages': queries and
+// weights as pairs of f16, two tiles at a time.
+template <int HD>
+RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float* q, float scale2, uint32_t t0,
+                      uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx) {
+    typedef Q4Raw<HD> Raw;
+    constexpr uint32_t KN = Raw::KN, VW = Raw::W, VN = Raw::VN, CW = Raw::CW;
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
+    Raw raw[2];
+    bool there[2];
+    auto load = [&](uint32_t t) {
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            const uint32_t page = v.page(t + u);
+            there[u] = page < v.num_pages;
+            if (there[u]) raw[u].load(v, t + u, page, lane);
+            else raw[u].none();
+        }
+    };
+    load(t0);
+    h8_t qh[KN], ql[KN];
+    const float qs = paged_query<HD, true>(q, scale2, qh, ql);
+    acc.start();
+    for (uint32_t t = t0; t < v.t1; t += step) {
+        const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE;
+        Raw now[2] = {raw[0], raw[1]};
+        const bool here[2] = {there[0], there[1]};
+        if (t + step < v.t1) load(t + step);
+        float p[8];
+        const bool edge = p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn || !here[0] || !here[1];
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            f32x4 sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t i = 0; i < KN; ++i) {
+                const h8_t k = q4_row(now[u].k[i / CW][i % CW], Q4Scale(now[u].kscale(i)));
+                sa = mfma32(k, qh[i], sa);
+                sb = mfma32(k, ql[i], sb);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) p[4 * u + r] = sa[r] + sb[r];
+        }
+        if (edge) {
+#pragma unroll
+            for (uint32_t r = 0; r < 8; ++r) {
+                const uint32_t pos = p0 + 16 * (r / 4) + 4 * g + r % 4;
+                if (pos < v.lo || pos >= lim || !here[r / 4]) p[r] = -__builtin_huge_valf();
+            }
+            now[0].clear(p0 + 4 * g, v.lo, limx);
+            now[1].clear(p0 + 16 + 4 * g, v.lo, limx);
+        }
+        acc.weigh(p, qs);
+        h8_t ph, pl;
+        split_weights(p, ph, pl);
+#pragma unroll
+        for (uint32_t i = 0; i < VN; ++i)
+#pragma unroll
+            for (uint32_t h = 0; h < VW / 4; ++h) {
+                h2_t o[4][4];  // of the pairs of positions, the elements 4h ..
+#pragma unroll
+                for (uint32_t x = 0; x < 4; ++x) {
+                    const uint32_t n = (i * 2 + x % 2) * (VW / 4) + h;
+                    q4_values(now[x / 2].v[n / CW][n % CW], Q4Scale(now[x / 2].vs[i][x % 2]), o[x]);
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const h8_t a = {o[0][e][0], o[0][e][1], o[1][e][0], o[1][e][1],
+                                    o[2][e][0], o[2][e][1], o[3][e][0], o[3][e][1]};
+                    acc.o[i][4 * h + e] = mfma32(a, ph, acc.o[i][4 * h + e]);
+                    acc.o[i][4 * h + e] = mfma32(a, pl, acc.o[i][4 * h + e]);
+                }
+            }
+    }
+    acc.join();
+}
+
+#define RT_PAGED_Q4_KERNELS(HD)                                                                           \
+    extern "C" __global__ void __launch_bounds__(256) k_paged_append_q4_hd##HD(PagedAppendArgs a) {      \
+        paged_append_q4<HD>(a);                                                                           \
+    }                                                                                                     \
+    extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_paged_attn_q4_hd##HD(PagedAttnArgs a) { \
+        paged_attn<HD, Q4, false>(a);                                                                     \
+    }
+RT_PAGED_Q4_KERNELS(64)
+RT_PAGED_Q4_KERNELS(128)
+RT_PAGED_Q4_KERNELS(256)
+extern "C" __global__ void __launch_bounds__(256) k_paged_gather_q4_f32(PagedGatherArgs a) { paged_gather_q4<float>(a); }
+extern "C" __global__ void __launch_bounds__(256) k_paged_gather_q4_f16(PagedGatherArgs a) { paged_gather_q4<_Float16>(a); }

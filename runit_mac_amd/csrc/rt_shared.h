@@ -55,7 +55,7 @@ constexpr uint32_t RT_PAGED_WIDE_ROWS = 128;  // columns of a wide block, 32 a w
 
 // One batch over a paged cache, as rt_paged_batch describes it.
 struct PagedBatch {
-    void* k;                    // page p at p·page_stride elements: [KVH][page size][head size]
+    void* k;                    // page p at p·page_stride elements (4 bits: bytes): [KVH][page size][head size]
     void* v;
     const uint32_t* table;      // [n_seqs][table_stride] page ids
     const uint32_t* row_start;  // [n_seqs + 1], or null: one row a sequence
@@ -71,6 +71,21 @@ struct PagedAppendArgs {
     float* q_out;
     double log2_theta;
     uint32_t H;
+};
+struct PagedGatherArgs {
+    PagedBatch b;
+    void* k_out;  // [rows][KVH][head size], or null
+    void* v_out;
+    uint32_t head_dim;
+};
+constexpr uint32_t RT_COPY_MAX = 65535;    // pages of a call (at most)
+constexpr uint32_t RT_COPY_SLICE = 16384;  // bytes of a workgroup (at most)
+constexpr uint32_t RT_COPY_POOLS = 256;  // pools of a launch (at most; 2 KB of its arguments)
+struct PagedCopyArgs {
+    const uint32_t *src, *dst;
+    uint64_t page_stride;  // bytes
+    uint32_t page_bytes, slice_bytes, slices, num_pages, n;
+    void* pools[RT_COPY_POOLS];
 };
 struct PagedAttnArgs {
     PagedBatch b;
@@ -89,6 +104,24 @@ struct PagedAttnArgs {
     uint32_t slots;      // workgroups of a KV head that are resident together, ≤ jobs
     uint32_t min_chunk;  // tiles of a chunk (at least)
     float scale;
+};
+
+// Rules on logits (k_rules.hip).
+constexpr uint32_t RT_RULES_SEG = 4096;  // tokens of a workgroup
+struct RulesArgs {
+    const void* x;  // [rows][row_stride]
+    void* out;
+    uint64_t row_stride;
+    uint32_t n, inplace;
+    // lists: row r's is at start[r], len[r] long, cut to the n_* that are there
+    const uint32_t *tokens, *token_start, *token_len, *prompt_len;
+    uint64_t n_tokens, n_bias;
+    const float *repetition, *frequency, *presence;
+    const uint32_t *bias_ids, *bias_start, *bias_len;
+    const float* bias;
+    const uint32_t *mask, *mask_row;
+    uint64_t mask_stride;
+    uint32_t mask_rows;
 };
 
 // Token log probabilities (k_logprobs.hip).

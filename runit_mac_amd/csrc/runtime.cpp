@@ -190,6 +190,11 @@ const char* const kKernelNames[] = {
     "k_paged_attn_f16w_hd64", "k_paged_attn_f16w_hd128", "k_paged_attn_f16w_hd256",
     "k_paged_merge_hd64", "k_paged_merge_hd128", "k_paged_merge_hd256",
     "k_paged_mergew_hd64", "k_paged_mergew_hd128", "k_paged_mergew_hd256",
+    "k_paged_append_q4_hd64", "k_paged_append_q4_hd128", "k_paged_append_q4_hd256",
+    "k_paged_attn_q4_hd64", "k_paged_attn_q4_hd128", "k_paged_attn_q4_hd256",
+    "k_paged_gather_f32_f32", "k_paged_gather_f32_f16", "k_paged_gather_f16_f32", "k_paged_gather_f16_f16",
+    "k_paged_gather_q4_f32", "k_paged_gather_q4_f16", "k_paged_copy",
+    "k_adjust_logits_f32", "k_adjust_logits_f16",
     "k_logprobs_f32", "k_logprobs_f16", "k_logprobs_top_f32", "k_logprobs_top_f16",
 };
 
@@ -4153,27 +4158,43 @@ int rt_flash_attention_f32(rt_ctx* c, const float* q, const float* k, const floa
 
 // ───────────────────────── batches over a paged cache ─────────────────────────
 
-static int paged_check(rt_ctx* c, const rt_paged_batch* b, uint32_t num_heads, const char* who, PagedBatch& d) {
-    if (!b) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: null batch", who);
-    const int st = attn_check(c, num_heads, b->num_kv_heads, b->head_dim);
-    if (st != RT_OK) return st;
-    if (num_heads == 0) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: num_heads=0", who);
-    if (b->f16 > 1)
-        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: f16=%u is neither 0 nor 1", who, b->f16);
+// The pages' type as kernels are named by it.
+static const char* paged_type(const rt_paged_batch* b) { return b->f16 == RT_PAGES_Q4 ? "q4" : b->f16 ? "f16" : "f32"; }
+
+// What a pool's pages are; `page` and `stride` in elements (4 bits: bytes).
+static int paged_pool_check(rt_ctx* c, const rt_paged_batch* b, const char* who, uint64_t& page, uint64_t& stride) {
+    if (b->f16 > 1 && b->f16 != RT_PAGES_Q4)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: f16=%u is none of 0, 1 and %d", who, b->f16,
+                    RT_PAGES_Q4);
     if (b->page_size < RT_PAGED_TILE || (b->page_size & (b->page_size - 1)))
         return fail(c, RT_ERR_DISPATCH,
                     "kernel dispatch error: %s: page_size=%u must be a power of two, %u or more", who,
                     b->page_size, RT_PAGED_TILE);
     if (b->num_pages == 0 || b->num_pages > 0x7fffffffu)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: num_pages=%u", who, b->num_pages);
-    const uint64_t page = (uint64_t)b->num_kv_heads * b->page_size * b->head_dim;
-    const uint64_t stride = b->page_stride ? b->page_stride : page;
-    if (stride < page || stride % 8)
+    const uint32_t unit = b->f16 == RT_PAGES_Q4 ? 16 : 8;
+    page = (uint64_t)b->num_kv_heads * b->page_size * b->head_dim;
+    if (b->f16 == RT_PAGES_Q4) page = page / 16 * 9;
+    stride = b->page_stride ? b->page_stride : page;
+    if (stride < page || stride % unit)
         return fail(c, RT_ERR_DISPATCH,
-                    "kernel dispatch error: %s: page_stride=%llu must be a multiple of 8, at least %llu", who,
-                    (unsigned long long)stride, (unsigned long long)page);
+                    "kernel dispatch error: %s: page_stride=%llu must be a multiple of %u, at least %llu", who,
+                    (unsigned long long)stride, unit, (unsigned long long)page);
     if (stride > (1ull << 60) / b->num_pages)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: the pool exceeds the address space", who);
+    if (!aligned(b->k_pages, 16) || !aligned(b->v_pages, 16))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: pages must be 16-byte aligned", who);
+    return RT_OK;
+}
+
+static int paged_check(rt_ctx* c, const rt_paged_batch* b, uint32_t num_heads, const char* who, PagedBatch& d) {
+    if (!b) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: null batch", who);
+    int st = attn_check(c, num_heads, b->num_kv_heads, b->head_dim);
+    if (st != RT_OK) return st;
+    if (num_heads == 0) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: num_heads=0", who);
+    uint64_t page, stride;
+    st = paged_pool_check(c, b, who, page, stride);
+    if (st != RT_OK) return st;
     if ((uint64_t)b->table_stride * b->page_size > 0x10000000u)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: %u pages of %u positions exceed 2^28", who,
                     b->table_stride, b->page_size);
@@ -4183,8 +4204,6 @@ static int paged_check(rt_ctx* c, const rt_paged_batch* b, uint32_t num_heads, c
     if (b->n_seqs && b->rows &&
         (!b->k_pages || !b->v_pages || !b->kv_len || (!b->table && b->table_stride)))
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: null buffer", who);
-    if (!aligned(b->k_pages, 16) || !aligned(b->v_pages, 16))
-        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: pages must be 16-byte aligned", who);
     if (!b->row_start && b->rows < b->n_seqs)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: %u rows for %u sequences of one", who,
                     b->rows, b->n_seqs);
@@ -4212,7 +4231,7 @@ int rt_rope_kv_append_paged_f32(rt_ctx* c, const rt_paged_batch* batch, const fl
     a.log2_theta = log2((double)theta);
     a.H = num_heads;
     char name[48];
-    snprintf(name, sizeof name, "k_paged_append_%s_hd%u", batch->f16 ? "f16" : "f32", batch->head_dim);
+    snprintf(name, sizeof name, "k_paged_append_%s_hd%u", paged_type(batch), batch->head_dim);
     const uint32_t rows = a.b.row_start ? a.b.rows : a.b.n_seqs;
     const uint32_t per = 2048 / batch->head_dim;  // heads of a pass
     const uint32_t passes = (num_heads + 2 * a.b.KVH + per - 1) / per;
@@ -4244,13 +4263,13 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     // workgroups leaves beyond one a block; the kernel with wide blocks
     // where one sequence's rows, or all over the prefix, may fill one
     const uint64_t cols = (uint64_t)rows * G, n = a.b.n_seqs;
-    const bool wide = batch->f16 && cols > 32 && (shared_len || (rows >= n && (rows - n + 1) * G > 32));
+    const bool wide = batch->f16 == 1 && cols > 32 && (shared_len || (rows >= n && (rows - n + 1) * G > 32));
     const uint64_t SR = wide ? RT_PAGED_WIDE_ROWS : RT_PAGED_ROWS;
     uint64_t blocks = a.b.row_start ? cols / RT_PAGED_ROWS + n : n * ((G + RT_PAGED_ROWS - 1) / RT_PAGED_ROWS);
     if (wide) blocks = std::min(blocks, 2 * n + cols / SR);
     if (shared_len) blocks += (cols + SR - 1) / SR + 1;
     char name[48];
-    snprintf(name, sizeof name, "k_paged_attn_%s_hd%u", wide ? "f16w" : batch->f16 ? "f16" : "f32", hd);
+    snprintf(name, sizeof name, "k_paged_attn_%s%s_hd%u", paged_type(batch), wide ? "w" : "", hd);
     // (narrow blocks: half of what may be resident; they wait for memory, and more jobs only split it up: 100,003
     // positions of 128-sized heads in f16 pages 82 -> 80 µs, of 64-sized heads in f32 pages 30 -> 27.  Wide
     // blocks wait for instructions, of which two workgroups have more: prompt chunks 66 -> 59 µs)
@@ -4287,6 +4306,139 @@ int rt_paged_attention_f32(rt_ctx* c, const rt_paged_batch* batch, const float* 
 int rt_shared_prefix_attention_f32(rt_ctx* c, const rt_paged_batch* batch, const float* q, float* out,
                                    uint32_t num_heads, const uint32_t* shared_table, uint32_t shared_len) {
     return paged_attention(c, batch, q, out, num_heads, shared_table, shared_len, "shared_prefix_attention");
+}
+
+static int paged_gather(rt_ctx* c, const rt_paged_batch* batch, void* k, void* v, const char* type) {
+    if (!c) return fail(nullptr, RT_ERR_DISPATCH, "kernel dispatch error: null context");
+    PagedGatherArgs a{};
+    const int st = paged_check(c, batch, batch ? batch->num_kv_heads : 1, "paged_gather", a.b);
+    if (st != RT_OK) return st;
+    if (a.b.n_seqs == 0 || a.b.rows == 0) return RT_OK;
+    if (!k && !v) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_gather: null buffer");
+    if (!aligned(k, 16) || !aligned(v, 16))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_gather: outputs must be 16-byte aligned");
+    a.k_out = k, a.v_out = v, a.head_dim = batch->head_dim;
+    char name[48];
+    snprintf(name, sizeof name, "k_paged_gather_%s_%s", paged_type(batch), type);
+    const uint32_t rows = a.b.row_start ? a.b.rows : a.b.n_seqs;
+    void* params[] = {&a};
+    return launch(c, name, dim3(rows, (2 * a.b.KVH * (a.head_dim / 4) + 255) / 256), dim3(256), 0, params);
+}
+int rt_paged_gather_f32(rt_ctx* c, const rt_paged_batch* batch, float* k, float* v) {
+    return paged_gather(c, batch, k, v, "f32");
+}
+int rt_paged_gather_f16(rt_ctx* c, const rt_paged_batch* batch, uint16_t* k, uint16_t* v) {
+    return paged_gather(c, batch, k, v, "f16");
+}
+
+int rt_paged_copy(rt_ctx* c, const rt_paged_batch* batches, uint32_t n_batches, const uint32_t* src,
+                  const uint32_t* dst, uint32_t n) {
+    if (!c) return fail(nullptr, RT_ERR_DISPATCH, "kernel dispatch error: null context");
+    if (n_batches == 0 || n == 0) return RT_OK;
+    if (!batches) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: null batch");
+    if (!src || !dst) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: null buffer");
+    if (n > RT_COPY_MAX)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: %u pages exceed %u", n, RT_COPY_MAX);
+    const rt_paged_batch& b = batches[0];
+    PagedCopyArgs a{};
+    uint64_t page, stride;
+    for (uint32_t i = 0; i < n_batches; ++i) {
+        const rt_paged_batch& o = batches[i];
+        int st = attn_check(c, o.num_kv_heads, o.num_kv_heads, o.head_dim);
+        if (st == RT_OK) st = paged_pool_check(c, &o, "paged_copy", page, stride);
+        if (st != RT_OK) return st;
+        if (!o.k_pages || !o.v_pages)
+            return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: null buffer");
+        if (o.f16 != b.f16 || o.num_pages != b.num_pages || o.page_size != b.page_size ||
+            o.num_kv_heads != b.num_kv_heads || o.head_dim != b.head_dim || o.page_stride != b.page_stride)
+            return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: the pages of batch %u differ from those of batch 0", i);
+    }
+    std::vector<const void*> pools;
+    for (uint32_t i = 0; i < n_batches; ++i) pools.insert(pools.end(), {batches[i].k_pages, batches[i].v_pages});
+    std::sort(pools.begin(), pools.end());
+    if (std::adjacent_find(pools.begin(), pools.end()) != pools.end())
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: a pool is there twice");
+    const uint32_t el = b.f16 == RT_PAGES_Q4 ? 1 : b.f16 ? 2 : 4;
+    if (page * el > 0x7fffffffu)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: pages of %llu bytes",
+                    (unsigned long long)(page * el));
+    a.src = src, a.dst = dst, a.n = n, a.num_pages = b.num_pages;
+    a.page_stride = stride * el;
+    a.page_bytes = (uint32_t)(page * el);
+    a.slices = (a.page_bytes + RT_COPY_SLICE - 1) / RT_COPY_SLICE;
+    a.slice_bytes = ((a.page_bytes + a.slices - 1) / a.slices + 15) / 16 * 16;
+    // (2^32 threads a launch; its pools are arguments)
+    const uint64_t wgs = (uint64_t)n * a.slices;
+    if (wgs > 0xffffffu)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: %u pages of %u bytes are too many", n,
+                    a.page_bytes);
+    const uint32_t most = (uint32_t)std::min<uint64_t>(RT_COPY_POOLS, 0xffffffu / wgs);
+    for (uint64_t p = 0; p < 2ull * n_batches; p += most) {
+        const uint32_t k = (uint32_t)std::min<uint64_t>(most, 2ull * n_batches - p);
+        for (uint32_t i = 0; i < k; ++i) {
+            const rt_paged_batch& o = batches[(p + i) / 2];
+            a.pools[i] = (p + i) % 2 ? o.v_pages : o.k_pages;
+        }
+        void* params[] = {&a};
+        const int st = launch(c, "k_paged_copy", dim3((uint32_t)wgs, k), dim3(256), 0, params);
+        if (st != RT_OK) return st;
+    }
+    return RT_OK;
+}
+
+// ───────────────────────── rules on logits ─────────────────────────
+
+static int adjust_logits(rt_ctx* c, const char* type, uint32_t el, const void* x, void* out, uint32_t rows, uint32_t n,
+                         uint64_t row_stride, const rt_logit_rules* r) {
+    if (!c) return fail(nullptr, RT_ERR_DISPATCH, "kernel dispatch error: null context");
+    if (rows == 0) return RT_OK;
+    if (!r) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: null rules");
+    if (n == 0 || n > 0x7fffffffu || row_stride < n || row_stride > 1ull << 40)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: rows of n=%u, row_stride=%llu", n,
+                    (unsigned long long)row_stride);
+    if (rows > 65535)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: rows=%u exceeds 65535", rows);
+    if (!x || !out) return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: null buffer");
+    if (!aligned(x, el) || !aligned(out, el))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: misaligned logits");
+    const uint64_t bytes = ((rows - 1) * row_stride + n) * el;
+    if (x != out && (uintptr_t)x < (uintptr_t)out + bytes && (uintptr_t)out < (uintptr_t)x + bytes)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: out overlaps logits");
+    if (r->n_tokens && (!r->tokens || !r->token_start || !r->token_len))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: %llu tokens in no list",
+                    (unsigned long long)r->n_tokens);
+    if (r->n_bias && (!r->bias_ids || !r->bias || !r->bias_start || !r->bias_len))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: %llu biases in no list",
+                    (unsigned long long)r->n_bias);
+    const uint64_t words = ((uint64_t)n + 31) / 32, stride = r->mask_stride ? r->mask_stride : words;
+    if (r->mask_rows && (!r->mask || stride < words))
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: %u masks, %llu of %llu words each",
+                    r->mask_rows, (unsigned long long)(r->mask ? stride : 0), (unsigned long long)words);
+    if (x == out && !r->n_tokens && !r->n_bias && !r->mask_rows) return RT_OK;
+    RulesArgs a{};
+    a.x = x, a.out = out, a.row_stride = row_stride, a.n = n, a.inplace = x == out;
+    if (r->n_tokens) {
+        a.tokens = r->tokens, a.n_tokens = r->n_tokens, a.token_start = r->token_start, a.token_len = r->token_len;
+        a.prompt_len = r->prompt_len, a.repetition = r->repetition, a.frequency = r->frequency;
+        a.presence = r->presence;
+    }
+    if (r->n_bias) {
+        a.bias_ids = r->bias_ids, a.bias = r->bias, a.n_bias = r->n_bias;
+        a.bias_start = r->bias_start, a.bias_len = r->bias_len;
+    }
+    if (r->mask_rows) a.mask = r->mask, a.mask_row = r->mask_row, a.mask_stride = stride, a.mask_rows = r->mask_rows;
+    char name[48];
+    snprintf(name, sizeof name, "k_adjust_logits_%s", type);
+    void* params[] = {&a};
+    return launch(c, name, dim3((n + RT_RULES_SEG - 1) / RT_RULES_SEG, rows), dim3(256), 0, params);
+}
+int rt_adjust_logits_f32(rt_ctx* c, const float* logits, float* out, uint32_t rows, uint32_t n, uint64_t row_stride,
+                         const rt_logit_rules* rules) {
+    return adjust_logits(c, "f32", 4, logits, out, rows, n, row_stride, rules);
+}
+int rt_adjust_logits_f16(rt_ctx* c, const uint16_t* logits, uint16_t* out, uint32_t rows, uint32_t n,
+                         uint64_t row_stride, const rt_logit_rules* rules) {
+    return adjust_logits(c, "f16", 2, logits, out, rows, n, row_stride, rules);
 }
 
 // ───────────────────────── token log probabilities ─────────────────────────

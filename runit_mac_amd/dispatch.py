@@ -170,6 +170,9 @@ _SIGS = {
     "rt_rope_kv_append_paged_f32": [_P] + [_P] * 5 + [_U32, _F],
     "rt_paged_attention_f32": [_P, _P, _P, _P, _U32],
     "rt_shared_prefix_attention_f32": [_P, _P, _P, _P, _U32, _P, _U32],
+    **{f"rt_paged_gather_{_t}": [_P, _P, _P, _P] for _t in ("f32", "f16")},
+    "rt_paged_copy": [_P, _P, _U32, _P, _P, _U32],
+    **{f"rt_adjust_logits_{_t}": [_P, _P, _P, _U32, _U32, _U64, _P] for _t in ("f32", "f16")},
     **{f"rt_token_logprobs_{_t}": [_P, _P, _P, _U32, _U32, _U64, _P, _P, _P, _U32, _P, _P]
        for _t in ("f32", "f16")},
     "rt_stream_read": [_P, _P, c_size_t, _P, c_size_t],
@@ -299,8 +302,9 @@ def _ptr(b) -> int | None:
 
 class PagedBatch(ctypes.Structure):
     """rt_paged_batch (include/runit_hip.h): a batch of sequences over a pool
-    of key / value pages, dtype "f32" or "f16".  Buffers are Buffer objects or
-    device pointers; keep the object for as long as pool and tables stay."""
+    of key / value pages, dtype "f32", "f16" or "q4" (4 bits).  Buffers are Buffer
+    objects or device pointers; keep the object for as long as pool and tables stay."""
+    TYPES = {"f32": 0, "f16": 1, "q4": 4}
     _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p)] + \
                [(n, c_uint32) for n in ("f16", "num_pages", "page_size", "num_kv_heads", "head_dim",
                                         "table_stride", "n_seqs", "rows")] + \
@@ -309,12 +313,46 @@ class PagedBatch(ctypes.Structure):
 
     def __init__(self, k_pages, v_pages, dtype, num_pages, page_size, num_kv_heads, head_dim, table,
                  table_stride, n_seqs, kv_len, rows=None, row_start=None, page_stride=0):
-        if dtype not in ("f32", "f16"):
-            raise ValueError(f"pages of dtype {dtype!r}: 'f32' or 'f16' expected")
-        super().__init__(_ptr(k_pages), _ptr(v_pages), int(dtype == "f16"), num_pages, page_size,
+        if dtype not in self.TYPES:
+            raise ValueError(f"pages of dtype {dtype!r}: 'f32', 'f16' or 'q4' expected")
+        super().__init__(_ptr(k_pages), _ptr(v_pages), self.TYPES[dtype], num_pages, page_size,
                          num_kv_heads, head_dim, table_stride, n_seqs, n_seqs if rows is None else rows,
                          page_stride, _ptr(table), _ptr(row_start), _ptr(kv_len))
         self._held = (k_pages, v_pages, table, row_start, kv_len)  # (a Buffer is freed with its object)
+        self.ref = ctypes.addressof(self)
+
+    @staticmethod
+    def page_bytes(dtype, num_kv_heads, page_size, head_dim) -> int:
+        """Bytes of a page's keys (as many of its values)."""
+        return num_kv_heads * page_size * head_dim * {"f32": 64, "f16": 32, "q4": 9}[dtype] // 16
+
+    @classmethod
+    def array(cls, batches):
+        """Several of them (a model's layers) as paged_copy takes them."""
+        batches = list(batches)
+        a = (cls * len(batches))(*batches)
+        a._held = batches
+        return a
+
+
+class LogitRules(ctypes.Structure):
+    """rt_logit_rules (include/runit_hip.h): penalties for the tokens of lists,
+    biases, grammar masks.  Buffers are Buffer objects or device pointers of u32
+    (f32: the penalties and `bias`); keep the object for as long as they stay."""
+    _fields_ = [(n, c_void_p) for n in ("tokens", "token_start", "token_len", "prompt_len")] + \
+               [("n_tokens", c_uint64)] + \
+               [(n, c_void_p) for n in ("repetition", "frequency", "presence", "bias_ids", "bias_start",
+                                        "bias_len", "bias")] + \
+               [("n_bias", c_uint64), ("mask", c_void_p), ("mask_row", c_void_p), ("mask_stride", c_uint64),
+                ("mask_rows", c_uint32)]
+
+    def __init__(self, tokens=None, n_tokens=0, token_start=None, token_len=None, prompt_len=None, repetition=None,
+                 frequency=None, presence=None, bias_ids=None, bias=None, n_bias=0, bias_start=None, bias_len=None,
+                 mask=None, mask_rows=0, mask_row=None, mask_stride=0):
+        p = (tokens, token_start, token_len, prompt_len), (repetition, frequency, presence, bias_ids, bias_start,
+                                                           bias_len, bias), (mask, mask_row)
+        super().__init__(*map(_ptr, p[0]), n_tokens, *map(_ptr, p[1]), n_bias, *map(_ptr, p[2]), mask_stride, mask_rows)
+        self._held = p
         self.ref = ctypes.addressof(self)
 
 
@@ -926,6 +964,42 @@ def shared_prefix_attention_f32(ctx, batch, q, out, num_heads, shared_table, sha
     positions, in the pages of shared_table, read for all together (new)."""
     ctx._check(ctx.lib.rt_shared_prefix_attention_f32(ctx.handle, batch.ref, _ptr(q), _ptr(out), num_heads,
                                                       _ptr(shared_table), shared_len))
+
+
+def paged_gather_f32(ctx, batch, k, v):
+    """The batch's rows' keys and values as the pages hold them, in f32 (new)."""
+    ctx._check(ctx.lib.rt_paged_gather_f32(ctx.handle, batch.ref, _ptr(k), _ptr(v)))
+
+
+def paged_gather_f16(ctx, batch, k, v):
+    """The batch's rows' keys and values as the pages hold them, in f16 (new)."""
+    ctx._check(ctx.lib.rt_paged_gather_f16(ctx.handle, batch.ref, _ptr(k), _ptr(v)))
+
+
+def paged_copy(ctx, batches, src, dst, n):
+    """Pages dst[i] of all batches' pools made copies of pages src[i] (device
+    u32), as if one after another; batches: a PagedBatch, a list of them, or
+    PagedBatch.array's (new)."""
+    if isinstance(batches, PagedBatch):
+        batches = (batches,)
+    if not isinstance(batches, ctypes.Array):
+        batches = PagedBatch.array(batches)
+    ctx._check(ctx.lib.rt_paged_copy(ctx.handle, ctypes.addressof(batches), len(batches), _ptr(src), _ptr(dst), n))
+
+
+def _adjust_logits(name):
+    symbol = "rt_" + name
+
+    def fn(ctx, logits, out, rows, n, rules, row_stride=None):
+        ctx._check(getattr(ctx.lib, symbol)(ctx.handle, _ptr(logits), _ptr(out), rows, n,
+                                            n if row_stride is None else row_stride, rules.ref))
+    fn.__name__ = name
+    fn.__doc__ = (f"LogitRules applied to {name[-3:]} logits, in place or into a buffer apart (new).")
+    return fn
+
+
+adjust_logits_f32 = _adjust_logits("adjust_logits_f32")
+adjust_logits_f16 = _adjust_logits("adjust_logits_f16")
 
 
 def _token_logprobs(name):

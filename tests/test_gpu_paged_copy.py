@@ -1,0 +1,142 @@
+"""Pages copied through pools (rt_paged_copy) against the same on the host, one after
+another: forks, chains, cycles, pages written twice, ids that are none."""
+import numpy as np
+import pytest
+
+from runit_mac_amd import dispatch as d
+
+pytestmark = pytest.mark.gpu
+
+#       type   KVH, page size, head size
+SHAPES = [("q4", 1, 16, 64), ("q4", 4, 64, 128), ("f16", 2, 64, 64), ("f32", 3, 32, 256), ("f32", 8, 128, 128)]
+
+
+class Pools:
+    def __init__(self, ctx, kind, KVH, ps, hd, pages, layers, gap=0, seed=0):
+        rng = np.random.default_rng(seed)
+        self.ctx, self.pages = ctx, pages
+        self.page = d.PagedBatch.page_bytes(kind, KVH, ps, hd)
+        el = {"f32": 4, "f16": 2, "q4": 1}[kind]
+        self.host = rng.integers(0, 256, (2 * layers, pages, self.page + gap), np.uint8)
+        self.bufs = [ctx.buffer_from(h) for h in self.host]
+        self.batches = [d.PagedBatch(k, v, kind, pages, ps, KVH, hd, None, 0, 0, None,
+                                     page_stride=(self.page + gap) // el if gap else 0)
+                        for k, v in zip(self.bufs[::2], self.bufs[1::2])]
+
+    def copy(self, src, dst):
+        src, dst = np.asarray(src, np.uint32), np.asarray(dst, np.uint32)
+        for s, t in zip(src, dst):
+            if s < self.pages and t < self.pages:
+                self.host[:, t, :self.page] = self.host[:, s, :self.page]
+        d.paged_copy(self.ctx, self.batches, self.ctx.buffer_from(src), self.ctx.buffer_from(dst), len(src))
+        self.ctx.flush()
+
+    def check(self):
+        for h, b in zip(self.host, self.bufs):
+            assert np.array_equal(b.read(np.uint8).reshape(h.shape), h)
+
+
+LISTS = {
+    "fork": ([3, 3, 5, 3], [7, 8, 9, 10]),
+    "one": ([0], [11]),
+    "itself": ([4, 4], [4, 6]),
+    "chain": ([0, 1, 2, 3], [1, 2, 3, 4]),
+    "chain back": ([1, 2, 3, 4], [0, 1, 2, 3]),
+    "swap": ([0, 1, 9, 5], [9, 0, 1, 6]),
+    "twice": ([0, 1, 2], [5, 5, 6]),
+    "late": ([0, 1, 2, 7, 8], [3, 4, 5, 8, 9]),
+    "none": ([0xFFFFFFFF, 2, 12, 1], [5, 12, 6, 7]),
+    "none in a chain": ([0, 0xFFFFFFFF, 6], [6, 6, 0x80000000]),
+}
+
+
+@pytest.mark.parametrize("kind,KVH,ps,hd", SHAPES)
+@pytest.mark.parametrize("name", LISTS)
+def test_lists(ctx, name, kind, KVH, ps, hd):
+    p = Pools(ctx, kind, KVH, ps, hd, 12, 2, gap=32 if name in ("fork", "chain") else 0, seed=hd)
+    p.copy(*LISTS[name])
+    p.check()
+    if name == "fork":
+        p.copy(*LISTS["chain"])
+        p.check()
+
+
+@pytest.mark.parametrize("pages,n", [(40, 700), (3000, 900), (5000, 1100)])
+def test_long_lists(ctx, pages, n):
+    """More entries than threads, some of them meeting others, or almost all."""
+    rng = np.random.default_rng(n)
+    p = Pools(ctx, "q4", 1, 16, 64, pages, 2, seed=n)
+    p.copy(rng.integers(0, pages + 2, n), rng.integers(0, pages + 2, n))
+    p.check()
+
+
+def test_more_pools_than_a_launch_takes(ctx):
+    p = Pools(ctx, "q4", 1, 16, 64, 9, 150, seed=3)
+    n = d.launch_count(ctx)
+    p.copy([0, 1, 1], [1, 2, 5])
+    assert d.launch_count(ctx) == n + 2
+    p.check()
+
+
+def test_pages_behind_four_billion_bytes(ctx):
+    stride, page = 2 ** 32 + 256, d.PagedBatch.page_bytes("f16", 1, 16, 64)
+    bufs = [ctx.new_buffer(stride + page) for _ in range(2)]
+    rows = [np.random.default_rng(i).integers(0, 256, page, np.uint8) for i in range(2)]
+    for b, r in zip(bufs, rows):
+        b.write(r)
+    batch = d.PagedBatch(*bufs, "f16", 2, 16, 1, 64, None, 0, 0, None, page_stride=stride // 2)
+    d.paged_copy(ctx, batch, ctx.buffer_from(np.zeros(1, np.uint32)), ctx.buffer_from(np.ones(1, np.uint32)), 1)
+    ctx.flush()
+    for b, r in zip(bufs, rows):
+        assert np.array_equal(b.read(np.uint8, page, stride), r)
+        b.free()
+
+
+def test_replays_follow_the_lists(ctx):
+    p = Pools(ctx, "f16", 2, 16, 64, 20, 3, seed=5)
+    src, dst = ctx.buffer_from(np.zeros(3, np.uint32)), ctx.buffer_from(np.zeros(3, np.uint32))
+    ctx.capture_begin()
+    d.paged_copy(ctx, d.PagedBatch.array(p.batches), src, dst, 3)
+    graph = ctx.capture_end()
+    for s, t in (([1, 2, 3], [4, 5, 6]), ([4, 5, 9], [9, 4, 5]), ([0, 0, 0], [7, 8, 19])):
+        src.write(np.array(s, np.uint32)), dst.write(np.array(t, np.uint32))
+        graph.launch()
+        ctx.flush()
+        for a, b in zip(s, t):
+            p.host[:, b] = p.host[:, a]
+        p.check()
+        p.copy([10], [11])
+
+
+def test_refusals(ctx):
+    p = Pools(ctx, "q4", 1, 16, 64, 4, 2)
+    ids = ctx.buffer_from(np.zeros(4, np.uint32))
+
+    def refused(what, src=ids, n=1, first=True, **kw):
+        batches = d.PagedBatch.array(p.batches)
+        for k, v in kw.items():
+            setattr(batches[0 if first else 1], k, v)
+        before = d.launch_count(ctx)
+        with pytest.raises(d.Dispatch, match=what):
+            d.paged_copy(ctx, batches, src, ids, n)
+        assert d.launch_count(ctx) == before
+
+    refused("null buffer", src=None)
+    refused("exceed 65535", n=65536)
+    refused("null buffer", k_pages=None)
+    refused("16-byte aligned", v_pages=p.bufs[1].ptr + 8)
+    refused("page_size=8", page_size=8)
+    refused("num_pages=0", num_pages=0)
+    refused("f16=2", f16=2)
+    refused("head_dim=80", head_dim=80)
+    refused("num_kv_heads=0", num_kv_heads=0)
+    refused("page_stride=100", page_stride=100)
+    refused("differ from", first=False, num_pages=3)
+    refused("differ from", first=False, f16=1)
+    refused("pool is there twice", first=False, k_pages=p.bufs[0].ptr)
+    refused("too many|pages of", n=65535, page_size=1 << 25, num_pages=1, k_pages=p.bufs[0].ptr)
+    n = d.launch_count(ctx)
+    d.paged_copy(ctx, [], ids, ids, 1)
+    d.paged_copy(ctx, p.batches, None, None, 0)
+    assert d.launch_count(ctx) == n
+    p.check()
