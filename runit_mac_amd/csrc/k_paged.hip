@@ -414,19 +414,35 @@ RT_DEV void paged_copy(const PagedCopyArgs& a) {
     // whether entry j (pages s, d) meets another; the whole workgroup's answer
     auto meets = [&](uint32_t j, uint32_t s, uint32_t d) {
         bool hit = false;
+#pragma unroll 4
         for (uint32_t k = tid; k < a.n; k += 256) {
             uint32_t s2, d2;
             hit |= entry(k, s2, d2) && k != j && (d2 == d || d2 == s || s2 == d);
         }
         return __syncthreads_or(hit);
     };
-    auto copy = [&](uint32_t s, uint32_t d) {
+    // (the slice is on its way while the lists are looked through)
+    constexpr uint32_t V = RT_COPY_SLICE / (256 * 16);
+    u32x4 v[V];
+    auto load = [&](uint32_t s) {
         const uint8_t* from = pool + s * a.page_stride;
-        uint8_t* to = pool + d * a.page_stride;
-        for (uint32_t o = b0 + tid * 16; o < b1; o += 256 * 16) *(u32x4*)(to + o) = *(const u32x4*)(from + o);
+#pragma unroll
+        for (uint32_t u = 0; u < V; ++u) {
+            const uint32_t o = b0 + (256 * u + tid) * 16;
+            if (o < b1) v[u] = *(const u32x4*)(from + o);
+        }
     };
+    auto store = [&](uint32_t d) {
+        uint8_t* to = pool + d * a.page_stride;
+#pragma unroll
+        for (uint32_t u = 0; u < V; ++u) {
+            const uint32_t o = b0 + (256 * u + tid) * 16;
+            if (o < b1) *(u32x4*)(to + o) = v[u];
+        }
+    };
+    load(s);
     if (!meets(i, s, d)) {
-        if (s != d) copy(s, d);
+        if (s != d) store(d);
         return;
     }
     for (uint32_t j = 0; j < i; ++j) {
@@ -435,7 +451,7 @@ RT_DEV void paged_copy(const PagedCopyArgs& a) {
     }
     for (uint32_t j = i; j < a.n; ++j) {
         uint32_t s2, d2;
-        if (entry(j, s2, d2) && s2 != d2 && meets(j, s2, d2)) copy(s2, d2);
+        if (entry(j, s2, d2) && s2 != d2 && meets(j, s2, d2)) load(s2), store(d2);
     }
 }
 extern "C" __global__ void __launch_bounds__(256) k_paged_copy(PagedCopyArgs a) { paged_copy(a); }

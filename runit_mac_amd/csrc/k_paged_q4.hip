@@ -19,6 +19,13 @@
 // So no byte is two positions', and rows are stored without a look at others.
 #include "rt_paged.h"
 
+#ifndef Q4_STAGES
+#define Q4_STAGES 4
+#endif
+#ifndef Q4_WAVES
+#define Q4_WAVES 2
+#endif
+
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
@@ -47,11 +54,14 @@ struct Q4Scale {
     }
 };
 RT_DEV void q4_values(uint32_t w, const Q4Scale& s, h2_t (&o)[4]) {
+    // (constants known to the compiler would be literals, of which an instruction takes one: two for each of these)
+    uint32_t low = 0x000F000Fu, high = 0x00F000F0u, one = 0x64006400u;
+    asm("" : "+s"(low), "+s"(high), "+v"(one));
     const uint32_t v = w >> 8;
-    o[0] = (__builtin_bit_cast(h2_t, (w & 0x000F000Fu) | 0x64006400u) - s.z) * s.d;
-    o[1] = (__builtin_bit_cast(h2_t, (w & 0x00F000F0u) | 0x64006400u) - s.z16) * s.d16;
-    o[2] = (__builtin_bit_cast(h2_t, (v & 0x000F000Fu) | 0x64006400u) - s.z) * s.d;
-    o[3] = (__builtin_bit_cast(h2_t, (v & 0x00F000F0u) | 0x64006400u) - s.z16) * s.d16;
+    o[0] = (__builtin_bit_cast(h2_t, (w & low) | one) - s.z) * s.d;
+    o[1] = (__builtin_bit_cast(h2_t, (w & high) | one) - s.z16) * s.d16;
+    o[2] = (__builtin_bit_cast(h2_t, (v & low) | one) - s.z) * s.d;
+    o[3] = (__builtin_bit_cast(h2_t, (v & high) | one) - s.z16) * s.d16;
 }
 RT_DEV h8_t q4_row(uint32_t w, const Q4Scale& s) {  // a word of a key's codes, in order
     h2_t o[4];
@@ -257,36 +267,70 @@ RT_DEV void paged_gather_q4(const PagedGatherArgs& a) {
 
 // ───────────────────────────── attention ─────────────────────────────
 
-// What a lane loads of a tile: keys, of position l % 16 the elements HD/4·(l / 16)
-// ..; values, of positions 4·(l / 16) .. + 3, W of every 16·W elements from W·(l % 16) on.
+// A wave's own ring of stages in LDS, a turn's two tiles each: codes of keys and values as their
+// lanes' operands, scale words as they are.  A lane reads what it, or its wave, brought: no
+// barriers; and any number of turns may be on their way, waited for by their number of loads (loads
+// into registers, two turns ahead, are waited for one too early at the loop's end).
+template <int HD>
+struct Q4Stage {
+    static constexpr uint32_t W = Q4Layout<HD>::W, VN = Q4Layout<HD>::VN, KN = HD / 32;
+    static constexpr uint32_t CW = HD == 64 ? 2 : 4;      // words of a read of codes
+    static constexpr uint32_t CODES = HD * 8, SCALES = HD;  // bytes of a tile's keys, values
+    static constexpr uint32_t LEN = 4 * (CODES + SCALES), N = HD == 256 ? 3 : Q4_STAGES;
+    static constexpr uint32_t LOADS = HD == 64 ? 3 : HD == 128 ? 6 : 12;
+};
+template <int HD>
+struct PagedWave<HD, Q4> {
+    static constexpr uint32_t LDS = Q4Stage<HD>::N * Q4Stage<HD>::LEN / 4, BATCH = 8;
+    static_assert(LDS >= 16 * (HD + 4), "the outputs fit");
+};
+// 16 or 4 bytes a lane from p (the lane's own) to LDS, lane 0's at byte `at`, each next behind it.
+template <uint32_t BYTES>
+RT_DEV void q4_bring(const void* p, uint32_t at) {
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(at) : "memory", "m0");
+}
+// waits until at most n of the wave's last `most` stages are on their way
+template <uint32_t LOADS, uint32_t MOST>
+RT_DEV void q4_stages_left(uint32_t n) {
+    constexpr auto wait = [](uint32_t c) constexpr { return (c & 15) | (c >> 4) << 14 | 7 << 4 | 15 << 8; };
+    if constexpr (MOST > 0) {
+        if (n >= MOST) __builtin_amdgcn_s_waitcnt(wait(MOST * LOADS));
+        else q4_stages_left<LOADS, MOST - 1>(n);
+    } else {
+        __builtin_amdgcn_s_waitcnt(wait(0));
+    }
+}
+
+// A turn's operands, as a lane reads them from its stage: keys, of position l % 16 the elements
+// HD/4·(l / 16) ..; values, of positions 4·(l / 16) .. + 3, W of every 16·W elements from W·(l % 16) on.
 template <int HD>
 struct Q4Raw {
-    static constexpr uint32_t W = Q4Layout<HD>::W, VN = Q4Layout<HD>::VN, KN = HD / 32;
-    static constexpr uint32_t CW = HD == 64 ? 2 : 4;  // words of a load of codes
+    typedef Q4Stage<HD> S;
+    static constexpr uint32_t W = S::W, VN = S::VN, KN = S::KN, CW = S::CW;
     typedef uint32_t cvec __attribute__((ext_vector_type(CW)));
     cvec k[KN / CW], v[KN / CW];
     uint32_t ks;        // at head size 256 two words
     u32x2 vs[VN];
-    RT_DEV void load(const PagedView<Q4>& w, uint32_t t, uint32_t page, uint32_t lane) {
+    RT_DEV void keys(const uint8_t* st, uint32_t u, uint32_t lane) {
         const uint32_t c = lane & 15, g = lane >> 4;
-        const size_t off = w.place(t, page, HD), so = w.scales(off, t, HD);
+        const uint8_t* p = st + u * 2 * S::CODES + (HD == 64 ? c * 32 + g * 8 : lane * 16);
 #pragma unroll
-        for (uint32_t i = 0; i < KN / CW; ++i) k[i] = *(const cvec*)(w.k + off + c * (HD / 2) + g * (HD / 8) + i * CW * 4);
-        const uint16_t* s = (const uint16_t*)(w.k + so) + c * (HD / 32);
-        if constexpr (HD == 256) ks = ((const uint32_t*)s)[g];
-        else ks = s[HD == 128 ? g : g / 2];
-#pragma unroll
-        for (uint32_t i = 0; i < KN / CW; ++i) v[i] = *(const cvec*)(w.v + off + ((i * 4 + g) * 16 + c) * CW * 4);
-#pragma unroll
-        for (uint32_t i = 0; i < VN; ++i)
-            vs[i] = *(const u32x2*)((const uint16_t*)(w.v + so) + (16 * W * i + W * c) / 32 * 16 + 4 * g);
+        for (uint32_t i = 0; i < KN / CW; ++i) k[i] = *(const cvec*)(p + i * 1024);
+        const uint8_t* s = st + 4 * S::CODES + u * 2 * S::SCALES + c * (HD / 16) + (HD == 256 ? 4 * g : HD == 128 ? 2 * g : g / 2 * 2);
+        if constexpr (HD == 256) ks = *(const uint32_t*)s;
+        else ks = *(const uint16_t*)s;
     }
-    RT_DEV void none() {
+    RT_DEV void values(const uint8_t* st, uint32_t u, uint32_t lane) {
+        const uint32_t c = lane & 15, g = lane >> 4;
+        const uint8_t* p = st + (u * 2 + 1) * S::CODES + lane * CW * 4;
+        const uint8_t* s = st + 4 * S::CODES + (u * 2 + 1) * S::SCALES + W * c / 32 * 32 + 8 * g;
 #pragma unroll
-        for (uint32_t i = 0; i < KN / CW; ++i) k[i] = cvec{}, v[i] = cvec{};
-        ks = 0;
+        for (uint32_t i = 0; i < KN / CW; ++i) v[i] = *(const cvec*)(p + i * 1024);
 #pragma unroll
-        for (uint32_t i = 0; i < VN; ++i) vs[i] = u32x2{};
+        for (uint32_t i = 0; i < VN; ++i) vs[i] = *(const u32x2*)(s + i * 16 * W);
     }
     // positions that no column sees may hold anything: steps of zero (a code is always finite)
     RT_DEV void clear(uint32_t pos0, uint32_t lo, uint32_t limx) {
@@ -297,49 +341,121 @@ struct Q4Raw {
                 for (uint32_t i = 0; i < VN; ++i) vs[i][r / 2] &= r % 2 ? 0x0000FFFFu : 0xFFFF0000u;
     }
     RT_DEV uint32_t kscale(uint32_t i) const {  // of the key's words i, twice
-        if constexpr (HD == 256) return i < KN / 2 ? (ks & 0xFFFFu) * 0x10001u : (ks >> 16) * 0x10001u;
-        return ks * 0x10001u;
+        if constexpr (HD == 256) return i < KN / 2 ? (ks & 0xFFFFu) | ks << 16 : ks >> 16 | (ks & 0xFFFF0000u);
+        return ks | ks << 16;
     }
 };
 
 // The tiles t0, t0 + 1, t0 + step, ... for 16 columns, as f16 pages': queries and
-// weights as pairs of f16, two tiles at a time.
+// weights as pairs of f16, two tiles a turn.  A tile without a page is read from the
+// pool's first and seen by none.
 template <int HD>
 RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float* q, float scale2, uint32_t t0,
-                      uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx) {
+                      uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx, float* lds) {
+    typedef Q4Stage<HD> S;
     typedef Q4Raw<HD> Raw;
-    constexpr uint32_t KN = Raw::KN, VW = Raw::W, VN = Raw::VN, CW = Raw::CW;
-    const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
-    Raw raw[2];
-    bool there[2];
-    auto load = [&](uint32_t t) {
+    constexpr uint32_t KN = S::KN, VW = S::W, VN = S::VN, CW = S::CW, N = S::N;
+    const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const uint32_t turns = t0 < v.t1 ? (v.t1 - t0 + step - 1) / step : 0;
+    // the pages of 64 turns' tiles, a turn a lane
+    uint32_t ids[2];
+    auto ids_from = [&](uint32_t i0) {
+        const uint32_t t = t0 + (i0 + lane) * step;
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u)
+            ids[u] = i0 + lane < turns && t + u < v.t1 ? v.table[(v.tb + t + u) * RT_PAGED_TILE >> v.ps_shift] : v.num_pages;
+    };
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const float*)lds);
+    // what a lane brings, from a tile's codes (scale words) on
+    const uint8_t *kc, *vc, *sc;
+    if constexpr (HD == 64) {  // keys by the lower half of the lanes; both tiles' scales at once
+        kc = vc = (const uint8_t*)(lane < 32 ? v.k : v.v) + lane % 32 * 16;
+        sc = (const uint8_t*)(lane & 16 ? v.v : v.k) + c * 4;
+    } else {
+        kc = (const uint8_t*)v.k + (HD == 128 ? c * 64 + g * 16 : c * 128 + g * 32);
+        vc = (const uint8_t*)v.v + lane * 16;
+        sc = (const uint8_t*)(HD == 128 && lane >= 32 ? v.v : v.k) + (HD == 128 ? lane % 32 * 4 : lane * 4);
+    }
+    const size_t s0 = (size_t)(HD / 2) << v.ps_shift;  // of a page's scale words
+    // turn i's tiles into stage i % N; whether they have a page, a bit each
+    auto bring = [&](uint32_t i) {
+        const uint32_t t = t0 + i * step, st = lds0 + i % N * S::LEN;
+        size_t off[2], so[2];
+        uint32_t there = 0;
 #pragma unroll
         for (uint32_t u = 0; u < 2; ++u) {
-            const uint32_t page = v.page(t + u);
-            there[u] = page < v.num_pages;
-            if (there[u]) raw[u].load(v, t + u, page, lane);
-            else raw[u].none();
+            const uint32_t page = __builtin_amdgcn_readlane(ids[u], i & 63);
+            there |= page < v.num_pages ? 1u << u : 0u;
+            const size_t at = (page < v.num_pages ? page : 0) * v.page_stride;
+            off[u] = at + v.slot(t + u) * (HD / 2);
+            so[u] = at + s0 + v.slot(t + u) * (HD / 16);
         }
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            const uint32_t to = st + u * 2 * S::CODES;
+            if constexpr (HD == 64) {
+                q4_bring<16>(kc + off[u], to);
+            } else {
+#pragma unroll
+                for (uint32_t x = 0; x < HD / 128; ++x) {
+                    q4_bring<16>(kc + off[u] + x * 16, to + x * 1024);
+                    q4_bring<16>(vc + off[u] + x * 1024, to + S::CODES + x * 1024);
+                }
+            }
+        }
+        const uint32_t to = st + 4 * S::CODES;
+        if constexpr (HD == 64) {
+            q4_bring<4>(sc + (lane < 32 ? so[0] : so[1]), to);
+        } else {
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u) {
+                q4_bring<4>(sc + so[u], to + u * 2 * S::SCALES);
+                if constexpr (HD == 256) q4_bring<4>((const uint8_t*)v.v + lane * 4 + so[u], to + (u * 2 + 1) * S::SCALES);
+            }
+        }
+        return there;
     };
-    load(t0);
+    uint32_t here = 0;  // bring()'s bits of turns i .. i + N - 1
+    if (turns) {
+        ids_from(0);
+#pragma unroll
+        for (uint32_t i = 0; i < N - 1; ++i)
+            if (i < turns) here |= bring(i) << 2 * i;
+    }
     h8_t qh[KN], ql[KN];
     const float qs = paged_query<HD, true>(q, scale2, qh, ql);
     acc.start();
-    for (uint32_t t = t0; t < v.t1; t += step) {
-        const uint32_t p0 = (v.tb + t) * RT_PAGED_TILE;
-        Raw now[2] = {raw[0], raw[1]};
-        const bool here[2] = {there[0], there[1]};
-        if (t + step < v.t1) load(t + step);
+    // turn i's operands out of its stage, on their way while the turn before is computed
+    auto take = [&](uint32_t i, Raw (&raw)[2]) {
+        q4_stages_left<S::LOADS, N - 2>(turns - 1 - i);
+        asm volatile("" ::: "memory");
+        const uint8_t* st = (const uint8_t*)lds + i % N * S::LEN;
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) raw[u].keys(st, u, lane);
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) raw[u].values(st, u, lane);
+    };
+    auto turn = [&](uint32_t i, Raw (&raw)[2], Raw (&next)[2]) {
+        const uint32_t p0 = (v.tb + t0 + i * step) * RT_PAGED_TILE;
+        const bool there[2] = {(here & 1) != 0, (here & 2) != 0};
+        here >>= 2;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (LDS: this turn's stage is read)
+        if (i + 1 < turns) take(i + 1, next);
+        if (i + N - 1 < turns) {  // (into the stage before this one)
+            if ((i + N - 1) % 64 == 0) ids_from(i + N - 1);
+            here |= bring(i + N - 1) << 2 * (N - 2);
+        }
         float p[8];
-        const bool edge = p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn || !here[0] || !here[1];
+        const bool edge = p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn || !there[0] || !there[1];
 #pragma unroll
         for (uint32_t u = 0; u < 2; ++u) {
             f32x4 sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
 #pragma unroll
-            for (uint32_t i = 0; i < KN; ++i) {
-                const h8_t k = q4_row(now[u].k[i / CW][i % CW], Q4Scale(now[u].kscale(i)));
-                sa = mfma32(k, qh[i], sa);
-                sb = mfma32(k, ql[i], sb);
+            for (uint32_t n = 0; n < KN; ++n) {
+                const h8_t k = q4_row(raw[u].k[n / CW][n % CW], Q4Scale(raw[u].kscale(n)));
+                sa = mfma32(k, qh[n], sa);
+                sb = mfma32(k, ql[n], sb);
             }
 #pragma unroll
             for (uint32_t r = 0; r < 4; ++r) p[4 * u + r] = sa[r] + sb[r];
@@ -348,32 +464,38 @@ RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float
 #pragma unroll
             for (uint32_t r = 0; r < 8; ++r) {
                 const uint32_t pos = p0 + 16 * (r / 4) + 4 * g + r % 4;
-                if (pos < v.lo || pos >= lim || !here[r / 4]) p[r] = -__builtin_huge_valf();
+                if (pos < v.lo || pos >= lim || !there[r / 4]) p[r] = -__builtin_huge_valf();
             }
-            now[0].clear(p0 + 4 * g, v.lo, limx);
-            now[1].clear(p0 + 16 + 4 * g, v.lo, limx);
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u) raw[u].clear(p0 + 16 * u + 4 * g, v.lo, there[u] ? limx : 0);
         }
         acc.weigh(p, qs);
         h8_t ph, pl;
         split_weights(p, ph, pl);
 #pragma unroll
-        for (uint32_t i = 0; i < VN; ++i)
+        for (uint32_t n = 0; n < VN; ++n)
 #pragma unroll
             for (uint32_t h = 0; h < VW / 4; ++h) {
                 h2_t o[4][4];  // of the pairs of positions, the elements 4h ..
 #pragma unroll
                 for (uint32_t x = 0; x < 4; ++x) {
-                    const uint32_t n = (i * 2 + x % 2) * (VW / 4) + h;
-                    q4_values(now[x / 2].v[n / CW][n % CW], Q4Scale(now[x / 2].vs[i][x % 2]), o[x]);
+                    const uint32_t m = (n * 2 + x % 2) * (VW / 4) + h;
+                    q4_values(raw[x / 2].v[m / CW][m % CW], Q4Scale(raw[x / 2].vs[n][x % 2]), o[x]);
                 }
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) {
                     const h8_t a = {o[0][e][0], o[0][e][1], o[1][e][0], o[1][e][1],
                                     o[2][e][0], o[2][e][1], o[3][e][0], o[3][e][1]};
-                    acc.o[i][4 * h + e] = mfma32(a, ph, acc.o[i][4 * h + e]);
-                    acc.o[i][4 * h + e] = mfma32(a, pl, acc.o[i][4 * h + e]);
+                    acc.o[n][4 * h + e] = mfma32(a, ph, acc.o[n][4 * h + e]);
+                    acc.o[n][4 * h + e] = mfma32(a, pl, acc.o[n][4 * h + e]);
                 }
             }
+    };
+    Raw even[2], odd[2];
+    if (turns) take(0, even);
+    for (uint32_t i = 0; i < turns; i += 2) {
+        turn(i, even, odd);
+        if (i + 1 < turns) turn(i + 1, odd, even);
     }
     acc.join();
 }
@@ -382,7 +504,7 @@ RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float
     extern "C" __global__ void __launch_bounds__(256) k_paged_append_q4_hd##HD(PagedAppendArgs a) {      \
         paged_append_q4<HD>(a);                                                                           \
     }                                                                                                     \
-    extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_paged_attn_q4_hd##HD(PagedAttnArgs a) { \
+    extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : Q4_WAVES) k_paged_attn_q4_hd##HD(PagedAttnArgs a) { \
         paged_attn<HD, Q4, false>(a);                                                                     \
     }
 RT_PAGED_Q4_KERNELS(64)

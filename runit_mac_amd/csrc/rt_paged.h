@@ -577,7 +577,7 @@ RT_DEV void split_weights(const float* p, h8_t& hi, h8_t& lo) {
 // 1, t0 + step, ...
 template <int HD>
 RT_DEV void paged_f16(PagedAcc<HD, _Float16>& acc, const PagedView<_Float16>& v, const float* q, float scale2,
-                      uint32_t t0, uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx) {
+                      uint32_t t0, uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx, float*) {
     typedef PagedTile<HD, _Float16> Tile;
     constexpr uint32_t KN = Tile::KN, VW = Tile::VW, VN = Tile::VN;
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
@@ -730,13 +730,20 @@ struct PagedCols {
     }
 };
 
+// A wave of a narrow block: its LDS (its columns' outputs, before them what it likes), in floats; chunks
+// that meet at a time.
+template <int HD, class T>
+struct PagedWave {
+    static constexpr uint32_t LDS = 16 * (HD + 4), BATCH = 16;
+};
+
 template <int HD, class T, bool WIDE>
 RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, const PagedJob& j, uint32_t job,
                          float* lds) {
     constexpr uint32_t NW = RT_PAGED_WAVES, SR = paged_slot_rows<WIDE>();
     constexpr uint32_t VW = PagedTile<HD, T>::VW, VN = PagedTile<HD, T>::VN;
-    float (*olds)[16][HD + 4] = (float (*)[16][HD + 4])lds;
-    float (*mlds)[16] = (float (*)[16])(lds + NW * 16 * (HD + 4)), (*llds)[16] = mlds + NW;
+    auto olds = [&](uint32_t u, uint32_t k) { return lds + u * PagedWave<HD, T>::LDS + k * (HD + 4); };
+    float (*mlds)[16] = (float (*)[16])(lds + NW * PagedWave<HD, T>::LDS), (*llds)[16] = mlds + NW;
     const PagedBatch& b = a.b;
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t c = lane & 15, g = lane >> 4, ncl = co.ncl, cc = min(c, ncl - 1), lim = co.lim(cc);
@@ -753,7 +760,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
     const uint32_t t0 = j.chunk * NW + w, stride = j.chunks * NW;
     PagedAcc<HD, T> acc;
     if constexpr (sizeof(T) < 4) {
-        paged_f16<HD>(acc, v, co.q(cc), scale2, 2 * t0, 2 * stride, lim, limn, limx);
+        paged_f16<HD>(acc, v, co.q(cc), scale2, 2 * t0, 2 * stride, lim, limn, limx, lds + w * PagedWave<HD, T>::LDS);
         if (!acc.finite()) paged_f32<HD, T, 2>(acc, v, co.q(cc), scale2, 2 * t0, 2 * stride, lim, limn, limx);
     } else {
         paged_f32<HD, T>(acc, v, co.q(cc), scale2, t0, stride, lim, limn, limx);
@@ -763,7 +770,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
 #pragma unroll
         for (uint32_t x = 0; x < 4; ++x)
 #pragma unroll
-            for (uint32_t e = 0; e < VW; ++e) olds[w][c][i * 16 * VW + (4 * g + x) * VW + e] = acc.o[i][e][x];
+            for (uint32_t e = 0; e < VW; ++e) olds(w, c)[i * 16 * VW + (4 * g + x) * VW + e] = acc.o[i][e][x];
     if (g == 0) {
         mlds[w][c] = acc.m;
         llds[w][c] = acc.l;
@@ -784,7 +791,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
             // (one that the others outweigh keeps its NaN, one that saw nothing adds nothing)
             const float f = mlds[u][k] == NEG ? 0.0f : __builtin_amdgcn_exp2f(mlds[u][k] - md);
             L += f * llds[u][k];
-            o += f * *(const f32x4*)&olds[u][k][d];
+            o += f * *(const f32x4*)(olds(u, k) + d);
         }
         const size_t slot = ((size_t)job * b.KVH + co.kvh) * SR + k, rh = (size_t)co.row(k) * a.H + co.head(k);
         if (alone) {
@@ -807,7 +814,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
     // than 24, the last of each group of about √chunks those of the group first.
     // All loads of sixteen chunks are in flight at once.
     __shared__ uint32_t turn;
-    constexpr uint32_t PW = HD / 2, PT = 16 * PW / (64 * NW), BATCH = 16;  // pairs a row, a thread; chunks at a time
+    constexpr uint32_t PW = HD / 2, PT = 16 * PW / (64 * NW), BATCH = PagedWave<HD, T>::BATCH;  // pairs a row, a thread; chunks at a time
     __shared__ float mc[BATCH][16], lc[BATCH][16];
     auto last_of = [&](uint32_t* counter, uint32_t n) {
         dev_stores_done();
@@ -830,7 +837,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
             uint64_t x[PT][BATCH];
             const uint32_t mk = tid & 15, my = tid >> 4;
             uint64_t ml = pair_of(NEG, 0.0f);
-            if (x0 + my < n && mk < ncl) ml = dev_load((const uint64_t*)a.ml + slot_of(at + (x0 + my) * step) + mk);
+            if (my < BATCH && x0 + my < n && mk < ncl) ml = dev_load((const uint64_t*)a.ml + slot_of(at + (x0 + my) * step) + mk);
 #pragma unroll
             for (uint32_t u = 0; u < PT; ++u)
                 if (256 * u < items) {
@@ -840,8 +847,10 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
                         if (x0 + y < n) x[u][y] = dev_load((const uint64_t*)(a.part + slot_of(at + (x0 + y) * step) * HD) + i);
                 }
             if (x0) __syncthreads();
-            mc[my][mk] = pair_lo(ml);
-            lc[my][mk] = pair_hi(ml);
+            if (my < BATCH) {
+                mc[my][mk] = pair_lo(ml);
+                lc[my][mk] = pair_hi(ml);
+            }
             __syncthreads();
 #pragma unroll
             for (uint32_t u = 0; u < PT; ++u)
@@ -930,7 +939,7 @@ RT_DEV void paged_wide();
 
 template <int HD, class T, bool WIDE>
 RT_DEV void paged_attn(const PagedAttnArgs& a) {
-    constexpr uint32_t NARROW = RT_PAGED_WAVES * 16 * (HD + 4 + 2) / 4;  // in 16 bytes
+    constexpr uint32_t NARROW = RT_PAGED_WAVES * (PagedWave<HD, T>::LDS + 32) / 4;  // in 16 bytes
     constexpr uint32_t STAGES = WIDE ? PagedStage<HD>::N * PagedStage<HD>::LEN : 0;
     __shared__ f32x4 lds[NARROW > STAGES ? NARROW : STAGES];
     const PagedBatch& b = a.b;

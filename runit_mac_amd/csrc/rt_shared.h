@@ -107,12 +107,14 @@ struct PagedAttnArgs {
 };
 
 // Rules on logits (k_rules.hip).
-constexpr uint32_t RT_RULES_SEG = 4096;  // tokens of a workgroup
+constexpr uint32_t RT_RULES_SEG = 4096;     // tokens of a workgroup
+constexpr uint32_t RT_RULES_THREADS = 512;  // its threads
 struct RulesArgs {
     const void* x;  // [rows][row_stride]
     void* out;
     uint64_t row_stride;
-    uint32_t n, inplace;
+    uint32_t n, rows, segs, inplace;
+    float inv_more;  // 1 / (segs − 1)
     // lists: row r's is at start[r], len[r] long, cut to the n_* that are there
     const uint32_t *tokens, *token_start, *token_len, *prompt_len;
     uint64_t n_tokens, n_bias;

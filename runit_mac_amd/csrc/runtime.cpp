@@ -4272,9 +4272,10 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     snprintf(name, sizeof name, "k_paged_attn_%s%s_hd%u", paged_type(batch), wide ? "w" : "", hd);
     // (narrow blocks: half of what may be resident; they wait for memory, and more jobs only split it up: 100,003
     // positions of 128-sized heads in f16 pages 82 -> 80 µs, of 64-sized heads in f32 pages 30 -> 27.  Wide
-    // blocks wait for instructions, of which two workgroups have more: prompt chunks 66 -> 59 µs)
+    // blocks, and all of pages of 4 bits, wait for instructions, of which two workgroups have more: prompt chunks 66
+    // -> 59 µs, 32 decoding sequences of 4 bits 55 -> 40)
     const uint32_t per_cu = (uint32_t)occupancy(c, name, 64 * RT_PAGED_WAVES, 0);
-    const uint64_t slots = std::max<uint64_t>(1, (uint64_t)(wide ? per_cu : (per_cu + 1) / 2) * c->cu_count / a.b.KVH);
+    const uint64_t slots = std::max<uint64_t>(1, (uint64_t)(wide || batch->f16 == RT_PAGES_Q4 ? per_cu : (per_cu + 1) / 2) * c->cu_count / a.b.KVH);
     if ((blocks + slots) * a.b.KVH > 0xffffffu)  // (2^32 threads a launch)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: too many rows (%u of %u heads)", who, rows,
                     num_heads);
@@ -4417,6 +4418,9 @@ static int adjust_logits(rt_ctx* c, const char* type, uint32_t el, const void* x
     if (x == out && !r->n_tokens && !r->n_bias && !r->mask_rows) return RT_OK;
     RulesArgs a{};
     a.x = x, a.out = out, a.row_stride = row_stride, a.n = n, a.inplace = x == out;
+    a.rows = rows, a.segs = (n - 1) / RT_RULES_SEG + 1, a.inv_more = a.segs > 1 ? 1.0f / (float)(a.segs - 1) : 0.0f;
+    if ((uint64_t)rows * a.segs > 0xffffffffu / RT_RULES_THREADS)  // (2^32 threads a launch)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: %u rows of n=%u are too many", rows, n);
     if (r->n_tokens) {
         a.tokens = r->tokens, a.n_tokens = r->n_tokens, a.token_start = r->token_start, a.token_len = r->token_len;
         a.prompt_len = r->prompt_len, a.repetition = r->repetition, a.frequency = r->frequency;
@@ -4430,7 +4434,7 @@ static int adjust_logits(rt_ctx* c, const char* type, uint32_t el, const void* x
     char name[48];
     snprintf(name, sizeof name, "k_adjust_logits_%s", type);
     void* params[] = {&a};
-    return launch(c, name, dim3((n + RT_RULES_SEG - 1) / RT_RULES_SEG, rows), dim3(256), 0, params);
+    return launch(c, name, dim3(rows * a.segs), dim3(RT_RULES_THREADS), 0, params);
 }
 int rt_adjust_logits_f32(rt_ctx* c, const float* logits, float* out, uint32_t rows, uint32_t n, uint64_t row_stride,
                          const rt_logit_rules* rules) {

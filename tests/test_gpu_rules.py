@@ -311,6 +311,7 @@ def test_refusals(ctx):
     refused("row_stride=63", stride=63)
     refused("row_stride", stride=1 << 41)
     refused("rows=65536", rows=65536)
+    refused("too many", out=a, rows=65535, n=600_000, mask_rows=0)
     refused("overlaps", out=a.ptr + 4)
     refused("overlaps", out=a.ptr + 4 * 127)
     refused("tokens in no list", tokens=None)
