@@ -19,13 +19,6 @@
 // So no byte is two positions', and rows are stored without a look at others.
 #include "rt_paged.h"
 
-#ifndef Q4_STAGES
-#define Q4_STAGES 4
-#endif
-#ifndef Q4_WAVES
-#define Q4_WAVES 2
-#endif
-
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
@@ -276,21 +269,26 @@ struct Q4Stage {
     static constexpr uint32_t W = Q4Layout<HD>::W, VN = Q4Layout<HD>::VN, KN = HD / 32;
     static constexpr uint32_t CW = HD == 64 ? 2 : 4;      // words of a read of codes
     static constexpr uint32_t CODES = HD * 8, SCALES = HD;  // bytes of a tile's keys, values
-    static constexpr uint32_t LEN = 4 * (CODES + SCALES), N = HD == 256 ? 3 : Q4_STAGES;
+    static constexpr uint32_t LEN = 4 * (CODES + SCALES), N = HD == 256 ? 3 : 4;
     static constexpr uint32_t LOADS = HD == 64 ? 3 : HD == 128 ? 6 : 12;
 };
 template <int HD>
 struct PagedWave<HD, Q4> {
-    static constexpr uint32_t LDS = Q4Stage<HD>::N * Q4Stage<HD>::LEN / 4, BATCH = 8;
+    static constexpr uint32_t LDS = Q4Stage<HD>::N * Q4Stage<HD>::LEN / 4, BATCH = 16;
+    static constexpr bool HALF = true, MAY_NOTE = true;
     static_assert(LDS >= 16 * (HD + 4), "the outputs fit");
 };
-// 16 or 4 bytes a lane from p (the lane's own) to LDS, lane 0's at byte `at`, each next behind it.
+// 16 or 4 bytes a lane to LDS, lane 0's at byte `at`, each next behind it: from p (the lane's own), and
+// from off (the lane's own) behind p.
 template <uint32_t BYTES>
 RT_DEV void q4_bring(const void* p, uint32_t at) {
     if constexpr (BYTES == 16)
         asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory", "m0");
     else
         asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(at) : "memory", "m0");
+}
+RT_DEV void q4_bring16(const void* p, uint32_t off, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p), "s"(at) : "memory", "m0");
 }
 // waits until at most n of the wave's last `most` stages are on their way
 template <uint32_t LOADS, uint32_t MOST>
@@ -348,10 +346,12 @@ struct Q4Raw {
 
 // The tiles t0, t0 + 1, t0 + step, ... for 16 columns, as f16 pages': queries and
 // weights as pairs of f16, two tiles a turn.  A tile without a page is read from the
-// pool's first and seen by none.
-template <int HD>
-RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float* q, float scale2, uint32_t t0,
-                      uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx, float* lds) {
+// pool's first and seen by none.  HALF: eight columns, the upper parts of queries and weights in
+// the lanes of columns 0 .. 7, the lower ones in those of 8 .. 15: one product instead of two.
+template <int HD, bool HALF>
+RT_DEV void q4_chunk(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float* q, float scale2, uint32_t t0,
+                     uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx, float* lds) {
+    constexpr int ROW_ROR8 = 0x128;  // the lane of the column eight away
     typedef Q4Stage<HD> S;
     typedef Q4Raw<HD> Raw;
     constexpr uint32_t KN = S::KN, VW = S::W, VN = S::VN, CW = S::CW, N = S::N;
@@ -367,13 +367,12 @@ RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float
     };
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const float*)lds);
     // what a lane brings, from a tile's codes (scale words) on
-    const uint8_t *kc, *vc, *sc;
+    const uint8_t *kc, *sc;
+    const uint32_t ko = HD == 128 ? c * 64 + g * 16 : c * 128 + g * 32, vo = lane * 16;
     if constexpr (HD == 64) {  // keys by the lower half of the lanes; both tiles' scales at once
-        kc = vc = (const uint8_t*)(lane < 32 ? v.k : v.v) + lane % 32 * 16;
+        kc = (const uint8_t*)(lane < 32 ? v.k : v.v) + lane % 32 * 16;
         sc = (const uint8_t*)(lane & 16 ? v.v : v.k) + c * 4;
     } else {
-        kc = (const uint8_t*)v.k + (HD == 128 ? c * 64 + g * 16 : c * 128 + g * 32);
-        vc = (const uint8_t*)v.v + lane * 16;
         sc = (const uint8_t*)(HD == 128 && lane >= 32 ? v.v : v.k) + (HD == 128 ? lane % 32 * 4 : lane * 4);
     }
     const size_t s0 = (size_t)(HD / 2) << v.ps_shift;  // of a page's scale words
@@ -389,6 +388,7 @@ RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float
             const size_t at = (page < v.num_pages ? page : 0) * v.page_stride;
             off[u] = at + v.slot(t + u) * (HD / 2);
             so[u] = at + s0 + v.slot(t + u) * (HD / 16);
+            asm("" : "+s"(off[u]), "+s"(so[u]));  // (sums of all lanes', not of each)
         }
 #pragma unroll
         for (uint32_t u = 0; u < 2; ++u) {
@@ -398,8 +398,8 @@ RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float
             } else {
 #pragma unroll
                 for (uint32_t x = 0; x < HD / 128; ++x) {
-                    q4_bring<16>(kc + off[u] + x * 16, to + x * 1024);
-                    q4_bring<16>(vc + off[u] + x * 1024, to + S::CODES + x * 1024);
+                    q4_bring16((const uint8_t*)v.k + off[u], ko + x * 16, to + x * 1024);
+                    q4_bring16((const uint8_t*)v.v + off[u], vo + x * 1024, to + S::CODES + x * 1024);
                 }
             }
         }
@@ -424,6 +424,9 @@ RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float
     }
     h8_t qh[KN], ql[KN];
     const float qs = paged_query<HD, true>(q, scale2, qh, ql);
+    if constexpr (HALF)
+#pragma unroll
+        for (uint32_t n = 0; n < KN; ++n) qh[n] = c < 8 ? qh[n] : ql[n];
     acc.start();
     // turn i's operands out of its stage, on their way while the turn before is computed
     auto take = [&](uint32_t i, Raw (&raw)[2]) {
@@ -455,10 +458,10 @@ RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float
             for (uint32_t n = 0; n < KN; ++n) {
                 const h8_t k = q4_row(raw[u].k[n / CW][n % CW], Q4Scale(raw[u].kscale(n)));
                 sa = mfma32(k, qh[n], sa);
-                sb = mfma32(k, ql[n], sb);
+                if constexpr (!HALF) sb = mfma32(k, ql[n], sb);
             }
 #pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) p[4 * u + r] = sa[r] + sb[r];
+            for (uint32_t r = 0; r < 4; ++r) p[4 * u + r] = sa[r] + (HALF ? dpp_f<ROW_ROR8>(sa[r]) : sb[r]);
         }
         if (edge) {
 #pragma unroll
@@ -472,6 +475,7 @@ RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float
         acc.weigh(p, qs);
         h8_t ph, pl;
         split_weights(p, ph, pl);
+        if constexpr (HALF) ph = c < 8 ? ph : pl;
 #pragma unroll
         for (uint32_t n = 0; n < VN; ++n)
 #pragma unroll
@@ -487,7 +491,7 @@ RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float
                     const h8_t a = {o[0][e][0], o[0][e][1], o[1][e][0], o[1][e][1],
                                     o[2][e][0], o[2][e][1], o[3][e][0], o[3][e][1]};
                     acc.o[n][4 * h + e] = mfma32(a, ph, acc.o[n][4 * h + e]);
-                    acc.o[n][4 * h + e] = mfma32(a, pl, acc.o[n][4 * h + e]);
+                    if constexpr (!HALF) acc.o[n][4 * h + e] = mfma32(a, pl, acc.o[n][4 * h + e]);
                 }
             }
     };
@@ -497,15 +501,211 @@ RT_DEV void paged_f16(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float
         turn(i, even, odd);
         if (i + 1 < turns) turn(i + 1, odd, even);
     }
+    if constexpr (HALF)
+#pragma unroll
+        for (uint32_t n = 0; n < VN; ++n)
+#pragma unroll
+            for (uint32_t e = 0; e < VW; ++e)
+#pragma unroll
+                for (uint32_t x = 0; x < 4; ++x) acc.o[n][e][x] += dpp_f<ROW_ROR8>(acc.o[n][e][x]);
     acc.join();
+}
+template <int HD>
+RT_DEV void paged_pairs(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float* q, float scale2, uint32_t t0,
+                      uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx, float* lds, bool half) {
+    if (half) q4_chunk<HD, true>(acc, v, q, scale2, t0, step, lim, limn, limx, lds);
+    else q4_chunk<HD, false>(acc, v, q, scale2, t0, step, lim, limn, limx, lds);
+}
+
+// Wide blocks: the codes become f16 on their way to LDS, once for the block's 128 columns; from
+// there on they are f16 pages.  Two waves have the keys of a turn's two tiles, two the values, from
+// registers that hold the turn after; a stage is written while the one before is computed.
+template <int HD>
+struct PagedFeed<HD, Q4> {
+    typedef PagedStage<HD> Stage;
+    static constexpr uint32_t N = 2, W = Q4Layout<HD>::W, VN = Q4Layout<HD>::VN, KN = HD / 32, CW = HD == 64 ? 2 : 4;
+    typedef uint32_t cvec __attribute__((ext_vector_type(CW)));
+    const PagedView<Q4>& v;
+    h8_t* lds;
+    uint32_t t0, step, turns, limx, here = 0;  // here: fetch()'s bits of turns i, i + 1
+    uint32_t ids[2];  // the pages of 64 turns' tiles, a turn a lane
+    cvec codes[KN / CW];
+    uint32_t ks;
+    u32x2 vs[VN];
+    RT_DEV PagedFeed(const PagedView<Q4>& v, h8_t* lds, uint32_t t0, uint32_t step, uint32_t turns, uint32_t limx)
+        : v(v), lds(lds), t0(t0), step(step), turns(turns), limx(limx) {}
+    RT_DEV uint32_t wave() const { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+    RT_DEV void ids_from(uint32_t i0) {
+        const uint32_t lane = threadIdx.x & 63, t = t0 + (i0 + lane) * step;
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u)
+            ids[u] = i0 + lane < turns && t + u < v.t1 ? v.table[(v.tb + t + u) * RT_PAGED_TILE >> v.ps_shift] : v.num_pages;
+    }
+    // the wave's part of turn i into registers; whether its tiles have a page
+    RT_DEV uint32_t fetch(uint32_t i) {
+        const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, u = wave() & 1, t = t0 + i * step + u;
+        const uint32_t id0 = __builtin_amdgcn_readlane(ids[0], i & 63), id1 = __builtin_amdgcn_readlane(ids[1], i & 63);
+        const uint32_t page = u ? id1 : id0;
+        const size_t off = v.place(t, page < v.num_pages ? page : 0, HD), so = v.scales(off, t, HD);
+        if (wave() < 2) {
+            const uint8_t* p = (const uint8_t*)v.k;
+#pragma unroll
+            for (uint32_t n = 0; n < KN / CW; ++n) codes[n] = *(const cvec*)(p + off + c * (HD / 2) + g * (HD / 8) + n * CW * 4);
+            p += so + c * (HD / 16);
+            ks = HD == 256 ? *(const uint32_t*)(p + 4 * g) : *(const uint16_t*)(p + (HD == 128 ? 2 * g : g / 2 * 2));
+        } else {
+            const uint8_t* p = (const uint8_t*)v.v;
+#pragma unroll
+            for (uint32_t n = 0; n < KN / CW; ++n) codes[n] = *(const cvec*)(p + off + ((n * 4 + g) * 16 + c) * CW * 4);
+#pragma unroll
+            for (uint32_t n = 0; n < VN; ++n) vs[n] = *(const u32x2*)(p + so + W * c / 32 * 32 + 8 * g + n * 16 * W);
+        }
+        return (id0 < v.num_pages ? 1u : 0u) | (id1 < v.num_pages ? 2u : 0u);
+    }
+    // and from there as f16 into stage i % N; positions that no column sees may hold anything: steps of zero
+    RT_DEV void put(uint32_t i, uint32_t there) {
+        const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, u = wave() & 1;
+        h8_t* st = lds + i % N * Stage::LEN;
+        if (wave() < 2) {
+#pragma unroll
+            for (uint32_t n = 0; n < KN; ++n) {
+                const uint32_t w = HD < 256 ? ks | ks << 16 : n < KN / 2 ? (ks & 0xFFFFu) | ks << 16 : ks >> 16 | (ks & 0xFFFF0000u);
+                st[Stage::piece(16 * u + c, KN * g + n)] = q4_row(codes[n / CW][n % CW], Q4Scale(w));
+            }
+            return;
+        }
+        const uint32_t p0 = (v.tb + t0 + i * step + u) * RT_PAGED_TILE;
+        if (p0 < v.lo || p0 + RT_PAGED_TILE > limx || !(there >> u & 1)) {
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                const uint32_t pos = p0 + 4 * g + r;
+                if (pos < v.lo || pos >= limx || !(there >> u & 1))
+#pragma unroll
+                    for (uint32_t n = 0; n < VN; ++n) vs[n][r / 2] &= r % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+            }
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < VN; ++n)
+#pragma unroll
+            for (uint32_t p = 0; p < 2; ++p) {  // two positions
+                h2_t o[W / 4][4];
+                const Q4Scale s(vs[n][p]);
+#pragma unroll
+                for (uint32_t h = 0; h < W / 4; ++h) {
+                    const uint32_t m = (n * 2 + p) * (W / 4) + h;
+                    q4_values(codes[m / CW][m % CW], s, o[h]);
+                }
+#pragma unroll
+                for (uint32_t x = 0; x < 2; ++x) {
+                    const uint32_t row = 32 + 16 * u + 4 * g + 2 * p + x;
+                    if constexpr (W == 8) {
+                        st[Stage::piece(row, 16 * n + c)] =
+                            (h8_t){o[0][0][x], o[0][1][x], o[0][2][x], o[0][3][x], o[1][0][x], o[1][1][x], o[1][2][x], o[1][3][x]};
+                    } else {
+                        ((h4_t*)(st + Stage::piece(row, c / 2)))[c & 1] = (h4_t){o[0][0][x], o[0][1][x], o[0][2][x], o[0][3][x]};
+                    }
+                }
+            }
+    }
+    RT_DEV void start() {
+        if (!turns) return;
+        here = fetch(0);
+        put(0, here & 3);
+        if (turns > 1) here |= fetch(1) << 2;
+    }
+    RT_DEV uint32_t turn(uint32_t i) {
+        const uint32_t there = here & 3;
+        here >>= 2;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (LDS)
+        __builtin_amdgcn_s_barrier();  // (this stage is there, the one before is read)
+        asm volatile("" ::: "memory");
+        if (i + 1 < turns) put(i + 1, here & 3);
+        if (i + 2 < turns) {
+            if ((i + 2) % 64 == 0) ids_from(i + 2);
+            here |= fetch(i + 2) << 2;
+        }
+        return there;
+    }
+};
+
+// As paged_merge, of many chunks: a workgroup a (row, head), HD / 4 threads a group, each group every
+// G-th chunk; the groups meet in LDS.  (40 rows over a prefix of 8,192 positions in 30 chunks: 7.2 µs as
+// paged_merge, with a thread's chunks one batch after another.)
+template <int HD, bool WIDE>
+RT_DEV void paged_meet(const PagedAttnArgs& a) {
+    constexpr uint32_t TH = HD / 4, G = 256 / TH, SR = paged_slot_rows<WIDE>(), BATCH = 4;
+    __shared__ f32x4 os[G][TH];
+    __shared__ float ms[G], ls[G];
+    const PagedBatch& b = a.b;
+    const uint32_t rh = blockIdx.x, grp = threadIdx.x / TH, t = threadIdx.x % TH;
+    const uint32_t rows = b.row_start ? min(b.row_start[b.n_seqs], b.rows) : min(b.n_seqs, b.rows);
+    if (rh >= rows * a.H) return;
+    const uint32_t kvh = rh % a.H / (a.H / b.KVH);
+    const u32x4 in = *(const u32x4*)(a.info + (size_t)rh * 4);
+    const uint32_t n0 = in[1] / SR, n = n0 + (a.shared_len ? in[3] / SR : 0);
+    if (!a.shared_len && n0 == 1) return;  // (written whole)
+    if (in[0] >= a.jobs || n0 > a.jobs - in[0] || (n > n0 && (in[2] >= a.jobs || n - n0 > a.jobs - in[2]))) return;
+    const float NEG = -__builtin_huge_valf();
+    float M = NEG, L = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    for (uint32_t x0 = grp; x0 < n; x0 += BATCH * G) {
+        float mc[BATCH], lc[BATCH], mx = M;
+        f32x4 oc[BATCH];
+#pragma unroll
+        for (uint32_t u = 0; u < BATCH; ++u) {
+            const uint32_t x = min(x0 + u * G, n - 1), job = x < n0 ? in[0] + x : in[2] + x - n0;
+            const size_t slot = ((size_t)job * b.KVH + kvh) * SR + (x < n0 ? in[1] : in[3]) % SR;
+            mc[u] = a.ml[2 * slot], lc[u] = a.ml[2 * slot + 1];
+            oc[u] = *(const f32x4*)(a.part + slot * HD + 4 * t);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < BATCH; ++u) mx = fmaxf(mx, mc[u]);
+        const float md = mx == NEG ? 0.0f : mx, f0 = __builtin_amdgcn_exp2f(M - md);
+        M = mx;
+        L *= f0;
+        o *= f0;
+#pragma unroll
+        for (uint32_t u = 0; u < BATCH; ++u) {
+            if (x0 + u * G >= n) continue;
+            const float f = __builtin_amdgcn_exp2f(mc[u] - md);
+            L = fmaf(f, lc[u], L);
+            o += f * oc[u];
+        }
+    }
+    os[grp][t] = o;
+    if (t == 0) ms[grp] = M, ls[grp] = L;
+    __syncthreads();
+    if (grp) return;
+#pragma unroll
+    for (uint32_t g = 1; g < G; ++g) M = fmaxf(M, ms[g]);
+    const float md = M == NEG ? 0.0f : M;
+    L = 0.0f;
+    o = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t g = 0; g < G; ++g) {
+        const float f = __builtin_amdgcn_exp2f(ms[g] - md);
+        L = fmaf(f, ls[g], L);
+        o += f * os[g][t];
+    }
+    *(f32x4*)(a.out + (size_t)rh * HD + 4 * t) = L == 0.0f ? f32x4{0, 0, 0, 0} : o / L;
 }
 
 #define RT_PAGED_Q4_KERNELS(HD)                                                                           \
     extern "C" __global__ void __launch_bounds__(256) k_paged_append_q4_hd##HD(PagedAppendArgs a) {      \
         paged_append_q4<HD>(a);                                                                           \
     }                                                                                                     \
-    extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : Q4_WAVES) k_paged_attn_q4_hd##HD(PagedAttnArgs a) { \
+    extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_paged_attn_q4_hd##HD(PagedAttnArgs a) { \
         paged_attn<HD, Q4, false>(a);                                                                     \
+    }                                                                                                     \
+    extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_paged_attn_q4w_hd##HD(PagedAttnArgs a) { \
+        paged_attn<HD, Q4, true>(a);                                                                      \
+    }                                                                                                     \
+    extern "C" __global__ void __launch_bounds__(256) k_paged_meet_hd##HD(PagedAttnArgs a) {             \
+        paged_meet<HD, false>(a);                                                                         \
+    }                                                                                                     \
+    extern "C" __global__ void __launch_bounds__(256) k_paged_meetw_hd##HD(PagedAttnArgs a) {            \
+        paged_meet<HD, true>(a);                                                                          \
     }
 RT_PAGED_Q4_KERNELS(64)
 RT_PAGED_Q4_KERNELS(128)

@@ -129,6 +129,16 @@ RT_DEV void paged_gather(const PagedGatherArgs& a, const Load& load) {
 template <bool WIDE>
 constexpr uint32_t paged_slot_rows() { return WIDE ? RT_PAGED_WIDE_ROWS : RT_PAGED_ROWS; }
 
+// A wave of a narrow block: its LDS (its columns' outputs, before them what it likes), in floats; chunks
+// that meet at a time.
+// (HALF: blocks of eight columns or less are computed as eight, in lanes c and c + 8; MAY_NOTE: whether
+// chunks meet in a launch of their own is the host's choice)
+template <int HD, class T>
+struct PagedWave {
+    static constexpr uint32_t LDS = 16 * (HD + 4), BATCH = 16;
+    static constexpr bool HALF = false, MAY_NOTE = false;
+};
+
 // The jobs of one KV head: blocks × chunks of every sequence in turn (and, with
 // a shared prefix, before them those of all rows over it).  The chunk length
 // comes from the work that the device finds, so that the jobs are alike
@@ -232,7 +242,7 @@ RT_DEV PagedJob paged_job(const PagedAttnArgs& a, uint32_t job) {
             if (own + pb * ceil_div(pt, c1, inv1) <= a.slots) j.len = c1;
         }
     }
-    if (!WIDE && !a.shared_len && a.target && n <= 64) {
+    if (!WIDE && !a.shared_len && a.target && n <= 64 && !(PagedWave<HD, T>::MAY_NOTE && a.noted)) {
         // no more than sixteen chunks, which meet in one trip, where that takes chunks twice as long at most
         // (nine sequences of up to 4,000 positions with drafts 17.8 -> 15.8 µs, sixteen decoding 13.8 -> 12.5)
         uint32_t most = mt;
@@ -388,8 +398,9 @@ struct PagedAcc {
         float tmax = p[0];
 #pragma unroll
         for (uint32_t r = 1; r < N; ++r) tmax = fmaxf(tmax, p[r]);
-        tmax = column_max(tmax) * scale;
+        tmax *= scale;
         if (__ballot(tmax > m + GROW)) {
+            tmax = column_max(tmax);
             const float mn = fmaxf(m, tmax), md = mn == NEG ? 0.0f : mn, f = __builtin_amdgcn_exp2f(m - md);
             m = mn;
             l *= f;
@@ -576,8 +587,8 @@ RT_DEV void split_weights(const float* p, h8_t& hi, h8_t& lo) {
 // The same for f16 pages on the f16 matrix cores, two tiles at a time: t0, t0 +
 // 1, t0 + step, ...
 template <int HD>
-RT_DEV void paged_f16(PagedAcc<HD, _Float16>& acc, const PagedView<_Float16>& v, const float* q, float scale2,
-                      uint32_t t0, uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx, float*) {
+RT_DEV void paged_pairs(PagedAcc<HD, _Float16>& acc, const PagedView<_Float16>& v, const float* q, float scale2,
+                      uint32_t t0, uint32_t step, uint32_t lim, uint32_t limn, uint32_t limx, float*, bool) {
     typedef PagedTile<HD, _Float16> Tile;
     constexpr uint32_t KN = Tile::KN, VW = Tile::VW, VN = Tile::VN;
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
@@ -730,13 +741,6 @@ struct PagedCols {
     }
 };
 
-// A wave of a narrow block: its LDS (its columns' outputs, before them what it likes), in floats; chunks
-// that meet at a time.
-template <int HD, class T>
-struct PagedWave {
-    static constexpr uint32_t LDS = 16 * (HD + 4), BATCH = 16;
-};
-
 template <int HD, class T, bool WIDE>
 RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, const PagedJob& j, uint32_t job,
                          float* lds) {
@@ -746,7 +750,9 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
     float (*mlds)[16] = (float (*)[16])(lds + NW * PagedWave<HD, T>::LDS), (*llds)[16] = mlds + NW;
     const PagedBatch& b = a.b;
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t c = lane & 15, g = lane >> 4, ncl = co.ncl, cc = min(c, ncl - 1), lim = co.lim(cc);
+    const uint32_t c = lane & 15, g = lane >> 4, ncl = co.ncl;
+    const bool half = PagedWave<HD, T>::HALF && ncl <= 8;
+    const uint32_t cc = min(half ? c & 7 : c, ncl - 1), lim = co.lim(cc);
     uint32_t limx = lim, limn = lim;  // of the block's columns: the largest, the smallest
     for (uint32_t o = 1; o < 16; o *= 2) {
         limx = max(limx, __shfl_xor(limx, o, 64));
@@ -760,7 +766,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
     const uint32_t t0 = j.chunk * NW + w, stride = j.chunks * NW;
     PagedAcc<HD, T> acc;
     if constexpr (sizeof(T) < 4) {
-        paged_f16<HD>(acc, v, co.q(cc), scale2, 2 * t0, 2 * stride, lim, limn, limx, lds + w * PagedWave<HD, T>::LDS);
+        paged_pairs<HD>(acc, v, co.q(cc), scale2, 2 * t0, 2 * stride, lim, limn, limx, lds + w * PagedWave<HD, T>::LDS, half);
         if (!acc.finite()) paged_f32<HD, T, 2>(acc, v, co.q(cc), scale2, 2 * t0, 2 * stride, lim, limn, limx);
     } else {
         paged_f32<HD, T>(acc, v, co.q(cc), scale2, t0, stride, lim, limn, limx);
@@ -776,7 +782,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
         llds[w][c] = acc.l;
     }
     __syncthreads();
-    const bool noted = WIDE || a.shared_len, alone = j.chunks == 1 && !a.shared_len;
+    const bool noted = PagedWave<HD, T>::MAY_NOTE ? a.noted : WIDE || a.shared_len, alone = j.chunks == 1 && !a.shared_len;
     for (uint32_t i = tid; i < 16 * HD / 4; i += 64 * NW) {
         const uint32_t k = i / (HD / 4), d = i % (HD / 4) * 4;
         if (k >= ncl) break;
@@ -933,9 +939,269 @@ RT_DEV void stages_left(uint32_t n) {
     else __builtin_amdgcn_s_waitcnt(wait(0));
 }
 
-// (of the pages' type; where there are wide blocks)
+// What brings a wide block's turns to LDS: turn(i) has turn i's two tiles in stage i % N, for all waves,
+// and returns whether they have a page, a bit each.
+template <int HD, class T>
+struct PagedFeed;
 template <int HD>
-RT_DEV void paged_wide();
+struct PagedFeed<HD, _Float16> {
+    typedef PagedStage<HD> Stage;
+    static constexpr uint32_t N = Stage::N, NW = RT_PAGED_WAVES;
+    const PagedView<_Float16>& v;
+    h8_t* lds;
+    uint32_t t0, step, turns, limx, lds0, here = 0;  // here: bring()'s bits of turns i .. i + 3
+    // where the two tiles of 64 turns are, one turn a lane, from the KV head's part of the pool on (~0:
+    // nowhere).  Scalar loads in the loop would hold up its LDS reads, which share their counter.
+    uint64_t at[2];
+    // a wave's parts of a stage, 64 pieces each: what its lanes read from a tile's place on
+    const uint8_t* src[Stage::LOADS];
+    RT_DEV PagedFeed(const PagedView<_Float16>& v, h8_t* lds, uint32_t t0, uint32_t step, uint32_t turns, uint32_t limx)
+        : v(v), lds(lds), t0(t0), step(step), turns(turns), limx(limx) {
+        const uint32_t lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const h8_t*)lds);
+#pragma unroll
+        for (uint32_t x = 0; x < Stage::LOADS; ++x) {
+            const uint32_t n = (x * NW + w) * 64 + lane, r = n / Stage::ROW, p = n % Stage::ROW;
+            // (the permutation undoes itself)
+            src[x] = (const uint8_t*)((r < 32 ? v.k : v.v) + (size_t)(r & 15) * HD + (Stage::piece(r, p) - r * Stage::ROW) * 8);
+        }
+    }
+    RT_DEV void ids_from(uint32_t i0) {
+        const uint32_t lane = threadIdx.x & 63, t = t0 + (i0 + lane) * step;
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            const uint32_t page =
+                i0 + lane < turns && t + u < v.t1 ? v.table[(v.tb + t + u) * RT_PAGED_TILE >> v.ps_shift] : v.num_pages;
+            at[u] = page < v.num_pages ? v.place(t + u, page, HD) * 2 : ~0ull;
+        }
+    }
+    // turn i's tiles into stage i % N; whether they have a page
+    RT_DEV uint32_t bring(uint32_t i) {
+        const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        uint64_t off[2];
+        uint32_t there = 0;
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at[u], i & 63);
+            const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(at[u] >> 32), i & 63);
+            there |= hi != 0xffffffffu ? 1u << u : 0u;
+            off[u] = hi != 0xffffffffu ? (uint64_t)hi << 32 | lo : 0;  // (nowhere: the pool's first page)
+        }
+        const uint32_t st = lds0 + i % N * Stage::LEN * 16;
+#pragma unroll
+        for (uint32_t x = 0; x < Stage::LOADS; ++x) {
+            const uint32_t n = (x * NW + w) * 64;
+            bring16(src[x] + (n / Stage::ROW & 16 ? off[1] : off[0]), st + n * 16);
+        }
+        return there;
+    }
+    RT_DEV void start() {
+#pragma unroll
+        for (uint32_t i = 0; i < N - 1; ++i)
+            if (i < turns) here |= bring(i) << 2 * i;
+    }
+    RT_DEV uint32_t turn(uint32_t i) {
+        const uint32_t p0 = (v.tb + t0 + i * step) * RT_PAGED_TILE;
+        const uint32_t there = here & 3;
+        h8_t* st = lds + i % N * Stage::LEN;
+        stages_left<Stage::LOADS>(turns - 1 - i);
+        __builtin_amdgcn_s_barrier();  // (this stage is there, the one before is read)
+        asm volatile("" ::: "memory");
+        here >>= 2;
+        if (i + N - 1 < turns) {
+            const uint32_t in = i + N - 1;
+            if (in % 64 == 0) ids_from(in);
+            here |= bring(in) << 4;
+        }
+        if (p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limx || there != 3) {
+            // positions that no column sees may hold anything: zeros
+            for (uint32_t n = threadIdx.x; n < 32 * Stage::ROW; n += 64 * NW) {
+                const uint32_t r = n / Stage::ROW;
+                if (p0 + r < v.lo || p0 + r >= limx || !(there >> r / 16 & 1)) st[32 * Stage::ROW + n] = h8_t{};
+            }
+            __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (LDS)
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        }
+        return there;
+    }
+};
+
+template <int HD, class T>
+RT_DEV void paged_wide(const PagedAttnArgs& a, const PagedCols<HD, T>& co, const PagedJob& j, uint32_t job, h8_t* lds) {
+    typedef PagedStage<HD> Stage;
+    typedef PagedAcc<HD, T> Acc;
+    typedef short s4_t __attribute__((ext_vector_type(4)));
+    typedef float f16v __attribute__((ext_vector_type(16)));
+    typedef __attribute__((address_space(3))) s4_t* tptr_t;
+    constexpr uint32_t NW = RT_PAGED_WAVES, SR = RT_PAGED_WIDE_ROWS, KS = HD / 16, NB = HD / 32;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t c = lane & 31, h = lane >> 5;  // column; of its positions and elements 4h .. of every 8
+    const float NEG = -__builtin_huge_valf(), scale2 = a.scale * 1.44269504f;
+    PagedView<T> v = co.v;
+    const bool idle = 32 * w >= co.ncl;  // (brings tiles, computes none)
+    const uint32_t limx = co.pre ? co.hi : __builtin_amdgcn_readfirstlane(co.lim(co.ncl - 1));
+    v.t1 = min(v.t1, limx > v.lo ? (limx + RT_PAGED_TILE - 1) / RT_PAGED_TILE - v.tb : 0u);
+    const uint32_t t0 = 2 * j.chunk, step = 2 * j.chunks;
+    const uint32_t turns = t0 < v.t1 ? (v.t1 - t0 + step - 1) / step : 0;
+    typedef PagedFeed<HD, T> Feed;
+    Feed feed(v, lds, t0, step, turns, limx);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const h8_t*)lds);
+    // the block's queries into all stages, a wave's 32 KB·HD / 256 in its own quarter, each instruction whole rows of
+    // them: lanes that read and wrote their columns' pieces themselves took 3 µs more of the prompt chunks' 57
+    constexpr uint32_t PC = HD / 4, QL = HD / 8;  // 16-byte pieces a column, instructions a wave
+    h8_t* own = lds + w * 32 * PC;
+    const uint32_t cc = min(32 * w + c, co.ncl - 1), rh = co.row(cc) * a.H + co.head(cc);
+    auto piece = [&](uint32_t col, uint32_t p) { return col * PC + (p ^ (col & 15)); };  // (16 columns' same one: all banks)
+    feed.ids_from(0);
+#pragma unroll 2
+    for (uint32_t x = 0; x < QL; ++x) {
+        const uint32_t col = (64 * x + lane) / PC, p = lane % PC;
+        bring16(a.q + (size_t)__shfl(rh, col, 64) * HD + 4 * (piece(col, p) - col * PC),
+                lds0 + (w * 32 * PC + 64 * x) * 16);
+    }
+    // the column's limit, and what the last (the most) and the first of the wave's see
+    const uint32_t lim = co.lim(cc);
+    uint32_t limx_w = lim, limn_w = lim;
+    for (uint32_t o = 1; o < 32; o *= 2) {
+        limx_w = max(limx_w, __shfl_xor(limx_w, o, 64));
+        limn_w = min(limn_w, __shfl_xor(limn_w, o, 64));
+    }
+    limx_w = __builtin_amdgcn_readfirstlane(limx_w);
+    limn_w = __builtin_amdgcn_readfirstlane(limn_w);
+    // the query: elements 16n + 8h .. of column c
+    h8_t qh[KS], ql[KS];
+    float qs;
+    {
+        stages_left<Stage::LOADS>(0);
+        asm volatile("" ::: "memory");
+        float x[KS][8], mx = 0.0f;
+#pragma unroll
+        for (uint32_t n = 0; n < KS; ++n)
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e += 4) {
+                const f32x4 y = *(const f32x4*)(own + piece(c, 4 * n + 2 * h + e / 4)) * scale2;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    x[n][e + k] = y[k];
+                    mx = fmaxf(mx, fabsf(y[k]));
+                }
+            }
+        qs = split_query<KS>(x, fmaxf(mx, __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, mx)))), qh, ql);
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (the queries are read before tiles come)
+    __builtin_amdgcn_s_barrier();
+    feed.start();
+    // where in a stage the lane's values of elements 32n .. are (of positions 16x + 8k .., as many rows on: the
+    // permutation goes by the row's last bits)
+    uint32_t vat[NB];
+#pragma unroll
+    for (uint32_t n = 0; n < NB; ++n)
+        vat[n] = Stage::piece(32 + 4 * h + (lane >> 2 & 3), 4 * n + (lane >> 3 & 2) + (lane >> 1 & 1)) * 16 + (lane & 1) * 8;
+    f16v o[NB];
+#pragma unroll
+    for (uint32_t n = 0; n < NB; ++n) o[n] = f16v{};
+    float m = NEG, l = 0.0f;
+    for (uint32_t i = 0; i < turns; ++i) {
+        const uint32_t p0 = (v.tb + t0 + i * step) * RT_PAGED_TILE;
+        const uint32_t there = feed.turn(i);
+        h8_t* st = lds + i % Feed::N * Stage::LEN;
+        if (!idle && p0 < limx_w) {
+            f16v s = {};
+#pragma unroll
+            for (uint32_t n = 0; n < KS; ++n) {
+                const h8_t k = st[Stage::piece(c, 2 * n + h)];
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[n], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[n], s, 0, 0, 0);
+            }
+            float p[16];  // of the positions 8(r / 4) + 4h + r % 4
+#pragma unroll
+            for (uint32_t r = 0; r < 16; ++r) p[r] = s[r];
+            if (p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn_w || there != 3) {
+#pragma unroll
+                for (uint32_t r = 0; r < 16; ++r) {
+                    const uint32_t pos = p0 + 8 * (r / 4) + 4 * h + r % 4;
+                    if (pos < v.lo || pos >= lim || !(there >> r / 8 & 1)) p[r] = NEG;
+                }
+            }
+            float tmax = p[0];
+#pragma unroll
+            for (uint32_t r = 1; r < 16; ++r) tmax = fmaxf(tmax, p[r]);
+            tmax = fmaxf(tmax, __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, tmax)))) * qs;
+            if (__ballot(tmax > m + Acc::GROW)) {
+                const float mn = fmaxf(m, tmax), f = __builtin_amdgcn_exp2f(m - (mn == NEG ? 0.0f : mn));
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (uint32_t n = 0; n < NB; ++n) o[n] *= f;
+            }
+            const float md = (m == NEG ? 0.0f : m) - Acc::BIAS;
+#pragma unroll
+            for (uint32_t r = 0; r < 16; ++r) {
+                p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], qs, -md));
+                l += p[r];
+            }
+            h8_t ph[2], pl[2];
+            split_weights(p, ph[0], pl[0]);
+            split_weights(p + 8, ph[1], pl[1]);
+            const uint32_t vst = lds0 + i % Feed::N * Stage::LEN * 16;
+#pragma unroll
+            for (uint32_t n = 0; n < NB; ++n)
+#pragma unroll
+                for (uint32_t x = 0; x < 2; ++x) {
+                    s4_t y[2];  // element 32n + c of the positions 16x + 4h .., and eight on
+#pragma unroll
+                    for (uint32_t k = 0; k < 2; ++k)
+                        y[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (tptr_t)(uintptr_t)(vst + vat[n] + (16 * x + 8 * k) * Stage::ROW * 16));
+                    const h8_t vv = __builtin_bit_cast(h8_t, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, ph[x], o[n], 0, 0, 0);
+                    o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, pl[x], o[n], 0, 0, 0);
+                }
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (its reads are done before the next barrier)
+    }
+    __builtin_amdgcn_s_barrier();  // (all stages are read)
+    if (idle) return;
+    const bool alone = j.chunks == 1 && !a.shared_len;
+    l += __builtin_bit_cast(float, lane_xor<32>(__builtin_bit_cast(uint32_t, l)));
+    bool bad = !(l < __builtin_huge_valf());
+#pragma unroll
+    for (uint32_t n = 0; n < NB; ++n)
+#pragma unroll
+        for (uint32_t r = 0; r < 16; ++r) bad |= !(fabsf(o[n][r]) < __builtin_huge_valf());
+    if (!__ballot(bad)) {
+        // through the wave's quarter, so that a row leaves whole
+        const float f = !alone ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (uint32_t n = 0; n < NB; ++n)
+#pragma unroll
+            for (uint32_t x = 0; x < 4; ++x)
+                *(f32x4*)(own + piece(c, 8 * n + 2 * x + h)) =
+                    f32x4{o[n][4 * x], o[n][4 * x + 1], o[n][4 * x + 2], o[n][4 * x + 3]} * f;
+        asm volatile("" ::: "memory");
+        float* part = co.template place<SR>(job, 32 * w, false);
+#pragma unroll 2
+        for (uint32_t x = 0; x < QL; ++x) {
+            const uint32_t col = (64 * x + lane) / PC, p = lane % PC;
+            const f32x4 y = *(const f32x4*)(own + piece(col, p));
+            float* to = alone ? a.out + (size_t)__shfl(rh, col, 64) * HD : part + col * HD;
+            if (32 * w + col < co.ncl) *(f32x4*)(to + 4 * p) = y;
+        }
+        if (32 * w + c < co.ncl && h == 0) co.template state<SR>(j, job, cc, m, l, alone);
+        return;
+    }
+#pragma unroll 1
+    for (uint32_t u = 0; u < 2; ++u) {  // 16 columns at a time
+        const uint32_t c1 = 32 * w + 16 * u + (lane & 15), c2 = min(c1, co.ncl - 1);
+        if (32 * w + 16 * u >= co.ncl) break;
+        Acc acc;
+        paged_f32<HD, T, 2>(acc, v, co.q(c2), scale2, t0, step, co.lim(c2), limn_w, limx_w);
+        co.template put<SR>(acc, j, job, c1, alone);
+    }
+}
 
 template <int HD, class T, bool WIDE>
 RT_DEV void paged_attn(const PagedAttnArgs& a) {
@@ -959,7 +1225,7 @@ RT_DEV void paged_attn(const PagedAttnArgs& a) {
     const PagedCols<HD, T> co{a, v, kvh, G, j.row0, col0, min(bc, rows * G - col0), hi, pre, rows, j.kv};
     if constexpr (WIDE) {
         if (bc > RT_PAGED_ROWS) {
-            paged_wide<HD>(a, co, j, job, (h8_t*)lds);
+            paged_wide<HD, T>(a, co, j, job, (h8_t*)lds);
             return;
         }
     }

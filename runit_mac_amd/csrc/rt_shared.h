@@ -103,6 +103,7 @@ struct PagedAttnArgs {
     uint32_t target;  // its chunks beyond one a block (at most; 0: blocks are not split)
     uint32_t slots;      // workgroups of a KV head that are resident together, ≤ jobs
     uint32_t min_chunk;  // tiles of a chunk (at least)
+    uint32_t noted;      // chunks meet in a launch of their own (pages of 4 bits)
     float scale;
 };
 

@@ -192,6 +192,9 @@ const char* const kKernelNames[] = {
     "k_paged_mergew_hd64", "k_paged_mergew_hd128", "k_paged_mergew_hd256",
     "k_paged_append_q4_hd64", "k_paged_append_q4_hd128", "k_paged_append_q4_hd256",
     "k_paged_attn_q4_hd64", "k_paged_attn_q4_hd128", "k_paged_attn_q4_hd256",
+    "k_paged_attn_q4w_hd64", "k_paged_attn_q4w_hd128", "k_paged_attn_q4w_hd256",
+    "k_paged_meet_hd64", "k_paged_meet_hd128", "k_paged_meet_hd256",
+    "k_paged_meetw_hd64", "k_paged_meetw_hd128", "k_paged_meetw_hd256",
     "k_paged_gather_f32_f32", "k_paged_gather_f32_f16", "k_paged_gather_f16_f32", "k_paged_gather_f16_f16",
     "k_paged_gather_q4_f32", "k_paged_gather_q4_f16", "k_paged_copy",
     "k_adjust_logits_f32", "k_adjust_logits_f16",
@@ -4263,7 +4266,7 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     // workgroups leaves beyond one a block; the kernel with wide blocks
     // where one sequence's rows, or all over the prefix, may fill one
     const uint64_t cols = (uint64_t)rows * G, n = a.b.n_seqs;
-    const bool wide = batch->f16 == 1 && cols > 32 && (shared_len || (rows >= n && (rows - n + 1) * G > 32));
+    const bool wide = batch->f16 && cols > 32 && (shared_len || (rows >= n && (rows - n + 1) * G > 32));
     const uint64_t SR = wide ? RT_PAGED_WIDE_ROWS : RT_PAGED_ROWS;
     uint64_t blocks = a.b.row_start ? cols / RT_PAGED_ROWS + n : n * ((G + RT_PAGED_ROWS - 1) / RT_PAGED_ROWS);
     if (wide) blocks = std::min(blocks, 2 * n + cols / SR);
@@ -4280,7 +4283,12 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: too many rows (%u of %u heads)", who, rows,
                     num_heads);
     a.target = (uint32_t)(blocks >= 8 * slots ? 0 : blocks < slots / 2 ? slots - blocks : slots);
-    const bool noted = wide || shared_len;  // (chunks meet in a launch of their own)
+    // narrow blocks of pages of 4 bits: in the launch's last workgroups only where heads and tables are small (heads of
+    // 128, one sequence of 600 positions 10.6 against 10.3 µs, 8,000 14.2 and 11.7, 200,003 46 and 39; heads of 64: 600
+    // 8.0 and 9.0, 40 sequences of up to 2,000 9.8 and 11.0, 16 of up to 8,000 13.2 and 12.0)
+    const bool many = batch->f16 == RT_PAGES_Q4 && (hd > 64 || (uint64_t)a.b.table_stride * batch->page_size > 4096);
+    const bool noted = wide || shared_len || many;  // (chunks meet in a launch of their own)
+    a.noted = noted;
     if (!noted && 2 * (blocks + a.target) * a.b.KVH > kAttnCounters) a.target = 0;
     a.jobs = (uint32_t)(blocks + a.target);
     a.slots = (uint32_t)std::min<uint64_t>(slots, a.jobs);
@@ -4296,6 +4304,10 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     void* params[] = {&a};
     st = launch(c, name, dim3(a.jobs * a.b.KVH), dim3(64 * RT_PAGED_WAVES), 0, params);
     if (st != RT_OK || !noted) return st;
+    if (batch->f16 == RT_PAGES_Q4 && (!wide || shared_len)) {
+        snprintf(name, sizeof name, "k_paged_meet%s_hd%u", wide ? "w" : "", hd);
+        return launch(c, name, dim3(rows * num_heads), dim3(256), 0, params);
+    }
     snprintf(name, sizeof name, "k_paged_merge%s_hd%u", wide ? "w" : "", hd);
     return launch(c, name, dim3((uint32_t)(((size_t)rows * num_heads * (hd / 4) + 255) / 256)), dim3(256), 0, params);
 }
