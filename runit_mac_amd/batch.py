@@ -4,7 +4,10 @@ reference, whose engine holds one sequence in one KvCache).
 A BatchDecoder takes a DecodeModel's weights and gives its sequences pages of
 one pool as they grow.  Each pass runs any number of rows of any of them
 together: prompts, single tokens, drafts to verify.  All sequences may begin
-with the same prompt, held once and read for all together.
+with the same prompt, held once and read for all together; a sequence may go on
+as several, which share its pages until they write to them.  Rules on a
+sequence's next token (penalties, biases, a grammar's mask) come before the
+choice.
 """
 from __future__ import annotations
 
@@ -19,11 +22,13 @@ NO_PAGE = 0xFFFFFFFF
 
 
 class PagePool:
-    """The page ids 0 .. num_pages - 1, given out and taken back."""
+    """The page ids 0 .. num_pages - 1, given out and taken back; a page that
+    several hold is free when each has given it."""
 
     def __init__(self, num_pages: int):
         self.num_pages = num_pages
         self._free = list(range(num_pages - 1, -1, -1))
+        self._holders: dict[int, int] = {}
 
     @property
     def free(self) -> int:
@@ -32,10 +37,34 @@ class PagePool:
     def take(self, n: int) -> list[int]:
         if n > len(self._free):
             raise d.BufferSize(f"buffer size mismatch: expected {n} free pages, got {len(self._free)}")
-        return [self._free.pop() for _ in range(n)]
+        pages = [self._free.pop() for _ in range(n)]
+        self._holders.update(dict.fromkeys(pages, 1))
+        return pages
 
     def give(self, pages) -> None:
-        self._free.extend(reversed(pages))
+        for p in reversed(pages):
+            self._holders[p] -= 1
+            if not self._holders[p]:
+                del self._holders[p]
+                self._free.append(p)
+
+    def share(self, pages) -> None:
+        """Another holder of pages that are held."""
+        for p in pages:
+            self._holders[p] += 1
+
+    def holders(self, page: int) -> int:
+        return self._holders.get(page, 0)
+
+    def compaction(self) -> dict[int, int]:
+        """Where the held pages would go ({from: to}) to be the first ones."""
+        n = len(self._holders)
+        return dict(zip(sorted(p for p in self._holders if p >= n), sorted(p for p in self._free if p < n)))
+
+    def move(self, moves: dict[int, int]) -> None:
+        """Held pages have moved to free ones."""
+        self._holders = {moves.get(p, p): k for p, k in self._holders.items()}
+        self._free = sorted(set(range(self.num_pages)) - set(self._holders), reverse=True)
 
 
 @dataclass
@@ -51,15 +80,52 @@ class TokenScores:
     top_logprobs: np.ndarray
 
 
+@dataclass
+class Rules:
+    """What holds for a sequence's next token, in this order: penalties for the
+    tokens that it has (rt_logit_rules: `repetition` for all of them, `frequency`
+    a time and `presence` once for those behind the first `prompt_len`), biases
+    ({token: value}), the tokens that a grammar allows ([vocab] truth values, or
+    bits in ceil(vocab / 32) u32 words)."""
+    repetition: float = 1.0
+    frequency: float = 0.0
+    presence: float = 0.0
+    prompt_len: int = 0
+    bias: dict | None = None
+    allowed: np.ndarray | None = None
+
+    def checked(self, vocab: int) -> "Rules":
+        if not 0 < self.repetition < np.inf or not np.isfinite([self.frequency, self.presence]).all():
+            raise ValueError(f"rules: penalties {self.repetition}, {self.frequency}, {self.presence}")
+        if self.prompt_len < 0:
+            raise ValueError(f"rules: prompt_len {self.prompt_len}")
+        if any(not 0 <= t < vocab for t in self.bias or ()):
+            raise ValueError(f"rules: a bias's token is out of range [0, {vocab})")
+        if self.allowed is not None:
+            self.mask(vocab)
+        return self
+
+    def mask(self, vocab: int) -> np.ndarray:
+        a, words = np.asarray(self.allowed), -(-vocab // 32)
+        if a.dtype == np.uint32 and a.shape == (words,):
+            return a
+        if a.dtype != bool or a.shape != (vocab,):
+            raise ValueError(f"rules: allowed is neither {vocab} truth values nor {words} u32 words")
+        bits = np.zeros(32 * words, bool)
+        bits[:vocab] = a
+        return np.packbits(bits, bitorder="little").view(np.uint32)
+
+
 class _Sequence:
-    def __init__(self, length: int):
-        self.len = length
+    def __init__(self, tokens):
+        self.tokens = list(tokens)
+        self.len = len(self.tokens)
         self.pages: list[int] = []  # from the prefix's last whole page on
 
 
 class BatchDecoder:
     """`max_seqs` sequences of up to `max_len` positions over `num_pages` pages
-    of `page_size` positions (f16 or f32) a layer; passes of up to `max_rows`
+    of `page_size` positions (f16, f32 or, q4, 4 bits) a layer; passes of up to `max_rows`
     rows, the logits of up to `max_logits` of them at once, up to `max_top`
     alternatives.  Longer prompts run in several passes."""
 
@@ -72,8 +138,8 @@ class BatchDecoder:
             raise ValueError("batch decoder: sizes must be positive")
         if page_size < 16 or page_size & (page_size - 1):
             raise ValueError(f"batch decoder: page_size {page_size} is not a power of two from 16 on")
-        if kv not in ("f16", "f32"):
-            raise ValueError(f"batch decoder: kv {kv!r}: 'f16' or 'f32' expected")
+        if kv not in ("f16", "f32", "q4"):
+            raise ValueError(f"batch decoder: kv {kv!r}: 'f16', 'f32' or 'q4' expected")
         if c.head_dim not in (64, 128, 256):
             raise ValueError(f"batch decoder: head size {c.head_dim}: 64, 128 or 256 expected")
         if model.lm_fmt in ("f16", "f32"):
@@ -90,14 +156,19 @@ class BatchDecoder:
         self._seqs: dict[int, _Sequence] = {}
         self._next = 0
         self._prefix_pages: list[int] = []
+        self._prefix_tokens: list[int] = []
         self.prefix_len = 0
-        page = c.kv_heads * page_size * c.head_dim * (2 if kv == "f16" else 4)
+        self._copied: list = []  # of the call that runs: (sequence, place, the page before)
+        self._pick_rules: list | None = None  # of the pass's kept rows: rules and tokens
+        self._rules_buf: dict = {}
+        page = d.PagedBatch.page_bytes(kv, c.kv_heads, page_size, c.head_dim)
         # what a pass reads of its sequences, written in one piece: tokens, kept rows, targets, lengths, row
-        # starts, tables
+        # starts, tables; and the pages that are copied
         R, words = max_rows, 0
         self._meta = {}
         for name, n in (("tok", R), ("keep", R), ("target", R), ("kv_len", max_seqs), ("start", max_seqs + 1),
-                        ("shared", self.stride), ("table", max_seqs * self.stride)):
+                        ("shared", self.stride), ("table", max_seqs * self.stride),
+                        ("src", max(max_seqs, num_pages)), ("dst", max(max_seqs, num_pages))):
             self._meta[name] = words
             words += -(-n // 64) * 64
         self._host = np.zeros(words, np.uint32)
@@ -113,6 +184,7 @@ class BatchDecoder:
         self._pages = [d.PagedBatch(a.take(page * num_pages), a.take(page * num_pages), kv, num_pages, page_size,
                                     c.kv_heads, c.head_dim, self._at["table"], self.stride, 0, self._at["kv_len"])
                        for _ in range(c.layers)]
+        self._all_pages = d.PagedBatch.array(self._pages)
 
     # ───────────────────────────── sequences ─────────────────────────────
 
@@ -121,8 +193,29 @@ class BatchDecoder:
         if len(self._seqs) >= self.max_seqs:
             raise d.BufferSize(f"buffer size mismatch: expected room for another sequence, got {self.max_seqs}")
         self._next += 1
-        self._seqs[self._next] = _Sequence(self.prefix_len)
+        self._seqs[self._next] = _Sequence(self._prefix_tokens)
         return self._next
+
+    def fork(self, seq: int) -> int:
+        """A new sequence that goes on from where `seq` is.  Their pages are the
+        same ones until either writes to one, which is copied first."""
+        s = self._seq(seq)
+        new = self.open()
+        f = self._seqs[new]
+        f.tokens, f.len, f.pages = list(s.tokens), s.len, list(s.pages)
+        self.pool.share(f.pages)
+        return new
+
+    def compact(self) -> int:
+        """Moves the pages in use to the pools' beginning; how many they are."""
+        moves = self.pool.compaction()
+        if moves:
+            self._copy_pages(list(moves), list(moves.values()))
+            for s in self._seqs.values():
+                s.pages = [moves.get(p, p) for p in s.pages]
+            self._prefix_pages = [moves.get(p, p) for p in self._prefix_pages]
+            self.pool.move(moves)
+        return self.pool.num_pages - self.pool.free
 
     def close(self, seq: int) -> None:
         self.pool.give(self._seq(seq).pages)
@@ -137,6 +230,7 @@ class BatchDecoder:
         if not self.prefix_len <= length <= s.len:
             raise ValueError(f"trim: {length} is not within {self.prefix_len} .. {s.len}")
         s.len = length
+        del s.tokens[length:]
         keep = -(-length // self.page_size) - self.prefix_len // self.page_size if length > self.prefix_len else 0
         self.pool.give(s.pages[keep:])
         del s.pages[keep:]
@@ -154,7 +248,7 @@ class BatchDecoder:
         if need > there:
             raise d.BufferSize(f"buffer size mismatch: expected {need} free pages, got {there}")
         self.pool.give(self._prefix_pages)
-        self._prefix_pages, self.prefix_len = [], 0
+        self._prefix_pages, self._prefix_tokens, self.prefix_len = [], [], 0
         if toks.size == 0:
             return
         seq = self.open()
@@ -164,7 +258,7 @@ class BatchDecoder:
             self.close(seq)
             raise
         s = self._seqs.pop(seq)
-        self._prefix_pages, self.prefix_len = s.pages, s.len
+        self._prefix_pages, self._prefix_tokens, self.prefix_len = s.pages, s.tokens, s.len
 
     def _seq(self, seq: int) -> _Sequence:
         if seq not in self._seqs:
@@ -181,14 +275,19 @@ class BatchDecoder:
 
     # ────────────────────────────── passes ──────────────────────────────
 
-    def step(self, work: dict, top: int | None = None) -> dict:
+    def step(self, work: dict, top: int | None = None, rules: dict | None = None) -> dict:
         """Appends tokens to sequences ({sequence: tokens}) and returns the
-        likeliest next token of each; with `top`, pairs of it and its
-        TokenScores with that many alternatives."""
+        likeliest next token of each that its `rules` ({sequence: Rules}) leave;
+        with `top`, pairs of it and its TokenScores with that many alternatives,
+        the model's own: without the rules."""
         work = self._checked(work)
         if any(t.size == 0 for t in work.values()):
             raise ValueError("step: empty sequence of tokens")
-        got = self._run(work, {s: range(t.size - 1, t.size) for s, t in work.items()}, top)
+        for s, r in (rules or {}).items():
+            if s not in work:
+                raise ValueError(f"rules: sequence {s!r} is not in the step")
+            r.checked(self.model.cfg.vocab)
+        got = self._run(work, {s: range(t.size - 1, t.size) for s, t in work.items()}, top, rules=rules)
         if top is None:
             return {s: int(g.tokens[0]) for s, g in got.items()}
         return {s: (int(g.tokens[0]), g) for s, g in got.items()}
@@ -217,36 +316,54 @@ class BatchDecoder:
 
     def _checked(self, work: dict) -> dict:
         work = {s: self._tokens(t) for s, t in work.items()}
-        need = 0
+        need, writers = 0, {}
         for s, t in work.items():
             q = self._seq(s)
             if q.len + t.size > self.max_len:
                 raise ValueError(f"sequence {s}: {q.len} + {t.size} tokens exceed max_len {self.max_len}")
             need += self._more_pages(q, t.size)
+            if t.size and self._shared_end(q) is not None:
+                writers[q.pages[-1]] = writers.get(q.pages[-1], 0) + 1
+        # (the last holder of a page keeps it)
+        need += sum(min(n, self.pool.holders(p) - 1) for p, n in writers.items())
         if need > self.pool.free:
             raise d.BufferSize(f"buffer size mismatch: expected {need} free pages, got {self.pool.free}")
         return work
+
+    def _shared_end(self, q: _Sequence) -> int | None:
+        """The page that the sequence's next position is in, if others hold it too."""
+        begun = q.pages and q.len % self.page_size
+        return q.pages[-1] if begun and self.pool.holders(q.pages[-1]) > 1 else None
 
     def _more_pages(self, q: _Sequence, n: int) -> int:
         if n == 0:
             return 0
         return -(-(q.len + n) // self.page_size) - self.prefix_len // self.page_size - len(q.pages)
 
-    def _run(self, work: dict, keep: dict | None, top: int | None = None, given: bool = False) -> dict:
+    def _run(self, work: dict, keep: dict | None, top: int | None = None, given: bool = False,
+             rules: dict | None = None) -> dict:
         """The passes over `work`; of the tokens in `keep`'s ranges the argmax,
         or (`given`) the token that follows, and with `top` its scores.  If one
         fails, the sequences are as they were before all of them."""
         if top is not None and not 0 <= top <= self.max_top:
             raise ValueError(f"top {top} is not within 0 .. {self.max_top}")
         before = {s: self._seqs[s].len for s in work}
+        self._copied = []
         try:
-            return self._passes(work, keep, top, given)
+            return self._passes(work, keep, top, given, rules or {})
         except BaseException:
             for s, n in before.items():
                 self.trim(s, n)
+            # (what others hold of a page that was copied is as it was)
+            for q, at, page in reversed(self._copied):
+                self.pool.share([page])
+                self.pool.give([q.pages[at]])
+                q.pages[at] = page
             raise
+        finally:
+            self._copied = []
 
-    def _passes(self, work: dict, keep: dict | None, top: int | None, given: bool) -> dict:
+    def _passes(self, work: dict, keep: dict | None, top: int | None, given: bool, rules: dict) -> dict:
         parts = {s: [] for s in work}
         left = [(s, 0) for s, t in work.items() if t.size]
         while left:
@@ -267,9 +384,13 @@ class BatchDecoder:
                 targets += [work[s][i + 1] for i in kept] if given else ()
                 row += n
             self._place(batch, work, picks, targets)
+            upto = {s: at + n for s, at, n in batch}
+            self._pick_rules = [(rules[s], self._seqs[s].tokens + work[s][upto[s] - n:upto[s]].tolist()) if s in rules
+                                else None for s, _, n in batch if s in owner] if any(s in rules for s in owner) else None
             got = self._launch(batch, row, picks, targets if given else None, top)
-            for s, _, n in batch:
+            for s, at, n in batch:
                 self._seqs[s].len += n
+                self._seqs[s].tokens += work[s][at:at + n].tolist()
             owner = np.array(owner)
             for s, _, _ in batch:
                 if np.any(owner == s):
@@ -288,6 +409,7 @@ class BatchDecoder:
         table[:] = NO_PAGE
         put = lambda name, at, v: host.__setitem__(slice(meta[name] + at, meta[name] + at + len(v)), v)
         row = 0
+        self._own_ends([self._seqs[s] for s, _, _ in batch])
         for i, (s, at, n) in enumerate(batch):
             q = self._seqs[s]
             q.pages += self.pool.take(self._more_pages(q, n))
@@ -299,6 +421,65 @@ class BatchDecoder:
         put("keep", 0, picks)
         put("target", 0, targets)
         put("shared", 0, self._prefix_pages)
+
+    def _own_ends(self, seqs) -> None:
+        """Copies the pages that these sequences write to next and others hold."""
+        writers, left = [], {}
+        for q in seqs:
+            page = self._shared_end(q)
+            if page is not None and left.setdefault(page, self.pool.holders(page)) > 1:
+                left[page] -= 1
+                writers.append((q, page))
+        if not writers:
+            return
+        fresh = self.pool.take(len(writers))
+        try:
+            self._copy_pages([page for _, page in writers], fresh)
+        except BaseException:
+            self.pool.give(fresh)
+            raise
+        for (q, page), new in zip(writers, fresh):
+            self._copied.append((q, len(q.pages) - 1, page))
+            q.pages[-1] = new
+            self.pool.give([page])
+
+    def _copy_pages(self, src, dst) -> None:
+        """Pages of every layer, of the same lengths, none both read and written."""
+        ctx = self.ctx
+        for name, ids in (("src", src), ("dst", dst)):
+            at, n = self._meta[name], len(ids)
+            self._host[at:at + n] = ids
+            ctx._check(ctx.lib.rt_upload(ctx.handle, self._at[name], self._host[at:].ctypes.data, 4 * n))
+        d.paged_copy(ctx, self._all_pages, self._at["src"], self._at["dst"], len(src))
+
+    def _rules(self, rows):
+        """LogitRules of rows of (rules, tokens) or None, their arrays on the device."""
+        vocab, n = self.model.cfg.vocab, len(rows)
+        rules = [r[0] if r else Rules() for r in rows]
+        lists = [r[1] if r else [] for r in rows]
+        biases = [list((r.bias or {}).items()) for r in rules]
+        masks = [r.mask(vocab) for r in rules if r.allowed is not None]
+        starts = lambda x: np.concatenate([[0], np.cumsum([len(v) for v in x])[:-1]])
+        u32, f32 = (lambda v: np.asarray(v, np.int64).astype(np.uint32)), (lambda v: np.asarray(v, np.float32).view(np.uint32))
+        parts = dict(
+            tokens=u32([t for v in lists for t in v]), token_start=u32(starts(lists)), token_len=u32([len(v) for v in lists]),
+            prompt_len=u32([min(r.prompt_len, 0xFFFFFFFF) for r in rules]), repetition=f32([r.repetition for r in rules]),
+            frequency=f32([r.frequency for r in rules]), presence=f32([r.presence for r in rules]),
+            bias_ids=u32([t for v in biases for t, _ in v]), bias=f32([b for v in biases for _, b in v]),
+            bias_start=u32(starts(biases)), bias_len=u32([len(v) for v in biases]),
+            mask=np.concatenate(masks) if masks else u32([]),
+            mask_row=u32(np.where([r.allowed is not None for r in rules],
+                                  np.cumsum([r.allowed is not None for r in rules]) - 1, NO_PAGE)))
+        host, at = np.concatenate(list(parts.values())), {}
+        for k, v in parts.items():
+            at[k] = sum(x.size for x in list(parts.values())[:len(at)])
+        buf = self._rules_buf.get("lists")
+        if buf is None or buf.nbytes < host.nbytes:
+            self.ctx.flush()  # (calls before may read the old one)
+            buf = self._rules_buf["lists"] = self.ctx.new_buffer(2 * host.nbytes)
+        buf.write(host)
+        p = {k: buf.ptr + 4 * v for k, v in at.items()}
+        return d.LogitRules(n_tokens=parts["tokens"].size, n_bias=parts["bias"].size, mask_rows=len(masks), **p)
 
     def _launch(self, batch, rows, picks, targets, top):
         m, c, ctx, B, at = self.model, self.model.cfg, self.ctx, self._b, self._at
@@ -338,7 +519,14 @@ class BatchDecoder:
             n = min(nk - r, self.max_logits)
             m.head_rows(m.row_form(n), x + 4 * r * h, B["logits"], B["xn"], n)
             if targets is None:
-                d.argmax_rows_first_f32(ctx, B["logits"], B["idx"] + 4 * r, n, c.vocab)
+                logits, rules = B["logits"], self._pick_rules
+                if rules is not None and any(rules[r:r + n]):
+                    if top is not None:  # (the scores are of the logits as they are)
+                        if "logits" not in self._rules_buf:
+                            self._rules_buf["logits"] = ctx.new_buffer(4 * self.max_logits * c.vocab)
+                        logits = self._rules_buf["logits"].ptr
+                    d.adjust_logits_f32(ctx, B["logits"], logits, n, c.vocab, self._rules(rules[r:r + n]))
+                d.argmax_rows_first_f32(ctx, logits, B["idx"] + 4 * r, n, c.vocab)
             if top is not None:
                 d.token_logprobs_f32(ctx, B["logits"], wanted + 4 * r, n, c.vocab, B["logprob"] + 4 * r,
                                      entropy=B["entropy"] + 4 * r, rank=B["rank"] + 4 * r, top=top,
@@ -358,3 +546,6 @@ class BatchDecoder:
 
     def free(self) -> None:
         self.arena.buf.free()
+        for b in self._rules_buf.values():
+            b.free()
+        self._rules_buf = {}
