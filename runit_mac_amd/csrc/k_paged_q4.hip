@@ -290,6 +290,9 @@ RT_DEV void q4_bring(const void* p, uint32_t at) {
 RT_DEV void q4_bring16(const void* p, uint32_t off, uint32_t at) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p), "s"(at) : "memory", "m0");
 }
+RT_DEV void q4_bring4(const void* p, uint32_t off, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(p), "s"(at) : "memory", "m0");
+}
 // waits until at most n of the wave's last `most` stages are on their way
 template <uint32_t LOADS, uint32_t MOST>
 RT_DEV void q4_stages_left(uint32_t n) {
@@ -312,19 +315,19 @@ struct Q4Raw {
     cvec k[KN / CW], v[KN / CW];
     uint32_t ks;        // at head size 256 two words
     u32x2 vs[VN];
-    RT_DEV void keys(const uint8_t* st, uint32_t u, uint32_t lane) {
+    RT_DEV void keys(const uint8_t* p, const uint8_t* s, uint32_t lane) {
         const uint32_t c = lane & 15, g = lane >> 4;
-        const uint8_t* p = st + u * 2 * S::CODES + (HD == 64 ? c * 32 + g * 8 : lane * 16);
+        p += HD == 64 ? c * 32 + g * 8 : lane * 16;
 #pragma unroll
         for (uint32_t i = 0; i < KN / CW; ++i) k[i] = *(const cvec*)(p + i * 1024);
-        const uint8_t* s = st + 4 * S::CODES + u * 2 * S::SCALES + c * (HD / 16) + (HD == 256 ? 4 * g : HD == 128 ? 2 * g : g / 2 * 2);
+        s += c * (HD / 16) + (HD == 256 ? 4 * g : HD == 128 ? 2 * g : g / 2 * 2);
         if constexpr (HD == 256) ks = *(const uint32_t*)s;
         else ks = *(const uint16_t*)s;
     }
-    RT_DEV void values(const uint8_t* st, uint32_t u, uint32_t lane) {
+    RT_DEV void values(const uint8_t* p, const uint8_t* s, uint32_t lane) {
         const uint32_t c = lane & 15, g = lane >> 4;
-        const uint8_t* p = st + (u * 2 + 1) * S::CODES + lane * CW * 4;
-        const uint8_t* s = st + 4 * S::CODES + (u * 2 + 1) * S::SCALES + W * c / 32 * 32 + 8 * g;
+        p += lane * CW * 4;
+        s += W * c / 32 * 32 + 8 * g;
 #pragma unroll
         for (uint32_t i = 0; i < KN / CW; ++i) v[i] = *(const cvec*)(p + i * 1024);
 #pragma unroll
@@ -434,9 +437,10 @@ RT_DEV void q4_chunk(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float*
         asm volatile("" ::: "memory");
         const uint8_t* st = (const uint8_t*)lds + i % N * S::LEN;
 #pragma unroll
-        for (uint32_t u = 0; u < 2; ++u) raw[u].keys(st, u, lane);
+        for (uint32_t u = 0; u < 2; ++u) raw[u].keys(st + u * 2 * S::CODES, st + 4 * S::CODES + u * 2 * S::SCALES, lane);
 #pragma unroll
-        for (uint32_t u = 0; u < 2; ++u) raw[u].values(st, u, lane);
+        for (uint32_t u = 0; u < 2; ++u)
+            raw[u].values(st + (u * 2 + 1) * S::CODES, st + 4 * S::CODES + (u * 2 + 1) * S::SCALES, lane);
     };
     auto turn = [&](uint32_t i, Raw (&raw)[2], Raw (&next)[2]) {
         const uint32_t p0 = (v.tb + t0 + i * step) * RT_PAGED_TILE;
@@ -449,33 +453,53 @@ RT_DEV void q4_chunk(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float*
             if ((i + N - 1) % 64 == 0) ids_from(i + N - 1);
             here |= bring(i + N - 1) << 2 * (N - 2);
         }
-        float p[8];
         const bool edge = p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn || !there[0] || !there[1];
+        f32x4 sa[2] = {}, sb[2] = {};
 #pragma unroll
-        for (uint32_t u = 0; u < 2; ++u) {
-            f32x4 sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
+        for (uint32_t u = 0; u < 2; ++u)
 #pragma unroll
             for (uint32_t n = 0; n < KN; ++n) {
                 const h8_t k = q4_row(raw[u].k[n / CW][n % CW], Q4Scale(raw[u].kscale(n)));
-                sa = mfma32(k, qh[n], sa);
-                if constexpr (!HALF) sb = mfma32(k, ql[n], sb);
+                sa[u] = mfma32(k, qh[n], sa[u]);
+                if constexpr (!HALF) sb[u] = mfma32(k, ql[n], sb[u]);
             }
+        // HALF: the scores of the first tile in the lanes of columns 0 .. 7, of the second in the others'
+        constexpr uint32_t P = HALF ? 4 : 8;
+        float p[P];
+        if constexpr (HALF) {
 #pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) p[4 * u + r] = sa[r] + (HALF ? dpp_f<ROW_ROR8>(sa[r]) : sb[r]);
+            for (uint32_t r = 0; r < 4; ++r) p[r] = (c < 8 ? sa[0][r] : sa[1][r]) + dpp_f<ROW_ROR8>(c < 8 ? sa[1][r] : sa[0][r]);
+        } else {
+#pragma unroll
+            for (uint32_t r = 0; r < 8; ++r) p[r] = sa[r / 4][r % 4] + sb[r / 4][r % 4];
         }
         if (edge) {
 #pragma unroll
-            for (uint32_t r = 0; r < 8; ++r) {
-                const uint32_t pos = p0 + 16 * (r / 4) + 4 * g + r % 4;
-                if (pos < v.lo || pos >= lim || !there[r / 4]) p[r] = -__builtin_huge_valf();
+            for (uint32_t r = 0; r < P; ++r) {
+                const uint32_t u = HALF ? c / 8 : r / 4, pos = p0 + 16 * u + 4 * g + r % 4;
+                if (pos < v.lo || pos >= lim || !(u ? there[1] : there[0])) p[r] = -__builtin_huge_valf();
             }
 #pragma unroll
             for (uint32_t u = 0; u < 2; ++u) raw[u].clear(p0 + 16 * u + 4 * g, v.lo, there[u] ? limx : 0);
         }
-        acc.weigh(p, qs);
+        acc.template weigh<P, HALF>(p, qs);
         h8_t ph, pl;
-        split_weights(p, ph, pl);
-        if constexpr (HALF) ph = c < 8 ? ph : pl;
+        if constexpr (HALF) {
+            // the upper parts of all eight to the lanes of columns 0 .. 7, the lower ones to the others
+            h4_t hi, lo;
+            split_weights_of<4>(p, hi, lo);
+            const u32x2 h2 = __builtin_bit_cast(u32x2, hi), l2 = __builtin_bit_cast(u32x2, lo);
+            u32x4 w;
+#pragma unroll
+            for (uint32_t x = 0; x < 2; ++x) {
+                const uint32_t own = c < 8 ? h2[x] : l2[x], other = (uint32_t)dpp_i<ROW_ROR8>((int)(c < 8 ? l2[x] : h2[x]));
+                w[x] = c < 8 ? own : other;
+                w[2 + x] = c < 8 ? other : own;
+            }
+            ph = __builtin_bit_cast(h8_t, w);
+        } else {
+            split_weights(p, ph, pl);
+        }
 #pragma unroll
         for (uint32_t n = 0; n < VN; ++n)
 #pragma unroll
@@ -508,6 +532,7 @@ RT_DEV void q4_chunk(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float*
             for (uint32_t e = 0; e < VW; ++e)
 #pragma unroll
                 for (uint32_t x = 0; x < 4; ++x) acc.o[n][e][x] += dpp_f<ROW_ROR8>(acc.o[n][e][x]);
+    if constexpr (HALF) acc.l += dpp_f<ROW_ROR8>(acc.l);
     acc.join();
 }
 template <int HD>
@@ -518,22 +543,28 @@ RT_DEV void paged_pairs(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const flo
 }
 
 // Wide blocks: the codes become f16 on their way to LDS, once for the block's 128 columns; from
-// there on they are f16 pages.  Two waves have the keys of a turn's two tiles, two the values, from
-// registers that hold the turn after; a stage is written while the one before is computed.
+// there on they are f16 pages.  Two waves have the keys of a turn's two tiles, two the values, each
+// from a ring of its own that is brought three turns ahead (one turn ahead into registers, the turns waited for
+// memory: prompt chunks 62 µs for WIDE_US); a stage is written while the one before is computed.
 template <int HD>
 struct PagedFeed<HD, Q4> {
     typedef PagedStage<HD> Stage;
-    static constexpr uint32_t N = 2, W = Q4Layout<HD>::W, VN = Q4Layout<HD>::VN, KN = HD / 32, CW = HD == 64 ? 2 : 4;
-    typedef uint32_t cvec __attribute__((ext_vector_type(CW)));
+    typedef Q4Raw<HD> Raw;
+    static constexpr uint32_t N = 2, W = Q4Layout<HD>::W, VN = Q4Layout<HD>::VN, KN = HD / 32, CW = Raw::CW;
+    static constexpr uint32_t CODES = HD * 8, SCALES = HD, RING = 4;  // bytes of a tile's; turns
+    static constexpr uint32_t LOADS = HD == 256 ? 3 : 2;
+    static_assert(N * Stage::LEN * 16 + RT_PAGED_WAVES * RING * (CODES + SCALES) <= Stage::N * Stage::LEN * 16, "LDS");
     const PagedView<Q4>& v;
     h8_t* lds;
-    uint32_t t0, step, turns, limx, here = 0;  // here: fetch()'s bits of turns i, i + 1
-    uint32_t ids[2];  // the pages of 64 turns' tiles, a turn a lane
-    cvec codes[KN / CW];
-    uint32_t ks;
-    u32x2 vs[VN];
+    uint32_t t0, step, turns, limx, here = 0;  // here: bring()'s bits of turns i .. i + 4
+    uint32_t ring;     // the wave's, in LDS
+    const uint8_t* mine;  // its keys, or values
+    uint32_t ids[2];   // the pages of 64 turns' tiles, a turn a lane
     RT_DEV PagedFeed(const PagedView<Q4>& v, h8_t* lds, uint32_t t0, uint32_t step, uint32_t turns, uint32_t limx)
-        : v(v), lds(lds), t0(t0), step(step), turns(turns), limx(limx) {}
+        : v(v), lds(lds), t0(t0), step(step), turns(turns), limx(limx) {
+        ring = N * Stage::LEN * 16 + wave() * RING * (CODES + SCALES);
+        mine = (const uint8_t*)(wave() < 2 ? v.k : v.v);
+    }
     RT_DEV uint32_t wave() const { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
     RT_DEV void ids_from(uint32_t i0) {
         const uint32_t lane = threadIdx.x & 63, t = t0 + (i0 + lane) * step;
@@ -541,59 +572,55 @@ struct PagedFeed<HD, Q4> {
         for (uint32_t u = 0; u < 2; ++u)
             ids[u] = i0 + lane < turns && t + u < v.t1 ? v.table[(v.tb + t + u) * RT_PAGED_TILE >> v.ps_shift] : v.num_pages;
     }
-    // the wave's part of turn i into registers; whether its tiles have a page
-    RT_DEV uint32_t fetch(uint32_t i) {
+    // the wave's part of turn i into its ring; whether the turn's tiles have a page
+    RT_DEV uint32_t bring(uint32_t i) {
         const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, u = wave() & 1, t = t0 + i * step + u;
         const uint32_t id0 = __builtin_amdgcn_readlane(ids[0], i & 63), id1 = __builtin_amdgcn_readlane(ids[1], i & 63);
         const uint32_t page = u ? id1 : id0;
-        const size_t off = v.place(t, page < v.num_pages ? page : 0, HD), so = v.scales(off, t, HD);
-        if (wave() < 2) {
-            const uint8_t* p = (const uint8_t*)v.k;
-#pragma unroll
-            for (uint32_t n = 0; n < KN / CW; ++n) codes[n] = *(const cvec*)(p + off + c * (HD / 2) + g * (HD / 8) + n * CW * 4);
-            p += so + c * (HD / 16);
-            ks = HD == 256 ? *(const uint32_t*)(p + 4 * g) : *(const uint16_t*)(p + (HD == 128 ? 2 * g : g / 2 * 2));
+        const size_t at = (page < v.num_pages ? page : 0) * v.page_stride;
+        const uint8_t* codes = mine + at + v.slot(t) * (HD / 2);
+        const uint8_t* scales = mine + at + ((size_t)(HD / 2) << v.ps_shift) + v.slot(t) * (HD / 16);
+        const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const h8_t*)lds);
+        const uint32_t to = lds0 + ring + i % RING * (CODES + SCALES);
+        // (of 128 and 256 the keys as their lanes' operands; of 64 both as they are, 32 lanes' worth)
+        const uint32_t off = wave() >= 2 || HD == 64 ? lane * 16 : HD == 128 ? c * 64 + g * 16 : c * 128 + g * 32;
+        if constexpr (HD == 64) {
+            if (lane < 32) q4_bring16(codes, off, to);
         } else {
-            const uint8_t* p = (const uint8_t*)v.v;
 #pragma unroll
-            for (uint32_t n = 0; n < KN / CW; ++n) codes[n] = *(const cvec*)(p + off + ((n * 4 + g) * 16 + c) * CW * 4);
-#pragma unroll
-            for (uint32_t n = 0; n < VN; ++n) vs[n] = *(const u32x2*)(p + so + W * c / 32 * 32 + 8 * g + n * 16 * W);
+            for (uint32_t x = 0; x < HD / 128; ++x) q4_bring16(codes, off + x * (wave() < 2 ? 16 : 1024), to + x * 1024);
         }
+        if (lane < HD / 4) q4_bring4(scales, lane * 4, to + CODES);
         return (id0 < v.num_pages ? 1u : 0u) | (id1 < v.num_pages ? 2u : 0u);
     }
     // and from there as f16 into stage i % N; positions that no column sees may hold anything: steps of zero
     RT_DEV void put(uint32_t i, uint32_t there) {
         const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, u = wave() & 1;
+        const uint8_t* from = (const uint8_t*)lds + ring + i % RING * (CODES + SCALES);
         h8_t* st = lds + i % N * Stage::LEN;
+        q4_stages_left<LOADS, RING - 1>(turns - 1 - i);
+        asm volatile("" ::: "memory");
+        Raw raw;
         if (wave() < 2) {
+            raw.keys(from, from + CODES, lane);
 #pragma unroll
-            for (uint32_t n = 0; n < KN; ++n) {
-                const uint32_t w = HD < 256 ? ks | ks << 16 : n < KN / 2 ? (ks & 0xFFFFu) | ks << 16 : ks >> 16 | (ks & 0xFFFF0000u);
-                st[Stage::piece(16 * u + c, KN * g + n)] = q4_row(codes[n / CW][n % CW], Q4Scale(w));
-            }
+            for (uint32_t n = 0; n < KN; ++n)
+                st[Stage::piece(16 * u + c, KN * g + n)] = q4_row(raw.k[n / CW][n % CW], Q4Scale(raw.kscale(n)));
             return;
         }
+        raw.values(from, from + CODES, lane);
         const uint32_t p0 = (v.tb + t0 + i * step + u) * RT_PAGED_TILE;
-        if (p0 < v.lo || p0 + RT_PAGED_TILE > limx || !(there >> u & 1)) {
-#pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) {
-                const uint32_t pos = p0 + 4 * g + r;
-                if (pos < v.lo || pos >= limx || !(there >> u & 1))
-#pragma unroll
-                    for (uint32_t n = 0; n < VN; ++n) vs[n][r / 2] &= r % 2 ? 0x0000FFFFu : 0xFFFF0000u;
-            }
-        }
+        if (p0 < v.lo || p0 + RT_PAGED_TILE > limx || !(there >> u & 1)) raw.clear(p0 + 4 * g, v.lo, there >> u & 1 ? limx : 0);
 #pragma unroll
         for (uint32_t n = 0; n < VN; ++n)
 #pragma unroll
             for (uint32_t p = 0; p < 2; ++p) {  // two positions
                 h2_t o[W / 4][4];
-                const Q4Scale s(vs[n][p]);
+                const Q4Scale s(raw.vs[n][p]);
 #pragma unroll
                 for (uint32_t h = 0; h < W / 4; ++h) {
                     const uint32_t m = (n * 2 + p) * (W / 4) + h;
-                    q4_values(codes[m / CW][m % CW], s, o[h]);
+                    q4_values(raw.v[m / CW][m % CW], s, o[h]);
                 }
 #pragma unroll
                 for (uint32_t x = 0; x < 2; ++x) {
@@ -609,22 +636,23 @@ struct PagedFeed<HD, Q4> {
     }
     RT_DEV void start() {
         if (!turns) return;
-        here = fetch(0);
+#pragma unroll
+        for (uint32_t i = 0; i < RING; ++i)
+            if (i < turns) here |= bring(i) << 2 * i;
         put(0, here & 3);
-        if (turns > 1) here |= fetch(1) << 2;
     }
     RT_DEV uint32_t turn(uint32_t i) {
         const uint32_t there = here & 3;
         here >>= 2;
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (LDS)
+        __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (LDS: its part of this stage is written, of the ring read)
         __builtin_amdgcn_s_barrier();  // (this stage is there, the one before is read)
         asm volatile("" ::: "memory");
-        if (i + 1 < turns) put(i + 1, here & 3);
-        if (i + 2 < turns) {
-            if ((i + 2) % 64 == 0) ids_from(i + 2);
-            here |= fetch(i + 2) << 2;
+        if (i + RING < turns) {
+            if ((i + RING) % 64 == 0) ids_from(i + RING);
+            here |= bring(i + RING) << 2 * (RING - 1);
         }
+        if (i + 1 < turns) put(i + 1, here & 3);
         return there;
     }
 };

@@ -392,7 +392,8 @@ struct PagedAcc {
     }
     // products (NEG: unseen), scores in units of log 2 divided by scale, a power of two, to weights.  A column that
     // has seen nothing has the sum 0; the maximum does not tell: it passes NaN over.
-    template <uint32_t N>
+    // HALF: a column's are in the lanes c and c + 8 of sixteen (and its sum: both).
+    template <uint32_t N, bool HALF = false>
     RT_DEV void weigh(float (&p)[N], float scale) {
         const float NEG = -__builtin_huge_valf();
         float tmax = p[0];
@@ -400,6 +401,7 @@ struct PagedAcc {
         for (uint32_t r = 1; r < N; ++r) tmax = fmaxf(tmax, p[r]);
         tmax *= scale;
         if (__ballot(tmax > m + GROW)) {
+            if constexpr (HALF) tmax = fmaxf(tmax, dpp_f<0x128>(tmax));  // (a row of sixteen lanes by eight)
             tmax = column_max(tmax);
             const float mn = fmaxf(m, tmax), md = mn == NEG ? 0.0f : mn, f = __builtin_amdgcn_exp2f(m - md);
             m = mn;
@@ -570,19 +572,21 @@ RT_DEV float paged_query(const float* q, float scale2, h8_t (&qh)[HD / 32], h8_t
 }
 // (hi towards zero, two at a time; what is left has at most 14 bits, lo the
 // nearest of it)
-RT_DEV void split_weights(const float* p, h8_t& hi, h8_t& lo) {
+template <uint32_t N, class H>
+RT_DEV void split_weights_of(const float* p, H& hi, H& lo) {
     float minus = -1.0f;  // (known, it would be two conversions and subtractions; so it is one mixed fma each)
     asm("" : "+s"(minus));
     typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
     typedef float f2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (uint32_t r = 0; r < 8; r += 2) {
+    for (uint32_t r = 0; r < N; r += 2) {
         const h2_t h = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(p[r], p[r + 1]));
         const h2_t l = __builtin_convertvector((f2_t{fmaf((float)h[0], minus, p[r]), fmaf((float)h[1], minus, p[r + 1])}), h2_t);
         hi[r] = h[0], hi[r + 1] = h[1];
         lo[r] = l[0], lo[r + 1] = l[1];
     }
 }
+RT_DEV void split_weights(const float* p, h8_t& hi, h8_t& lo) { split_weights_of<8>(p, hi, lo); }
 
 // The same for f16 pages on the f16 matrix cores, two tiles at a time: t0, t0 +
 // 1, t0 + step, ...
