@@ -56,6 +56,28 @@ RT_DEV void q4_values(uint32_t w, const Q4Scale& s, h2_t (&o)[4]) {
     o[2] = (__builtin_bit_cast(h2_t, (v & low) | one) - s.z) * s.d;
     o[3] = (__builtin_bit_cast(h2_t, (v & high) | one) - s.z16) * s.d16;
 }
+// A word of a key's codes in the order 0, 4, 1, 5, 2, 6, 3, 7, two instructions in thirteen fewer: a byte
+// of 0 .. 15 is n·2^-9 as an e4m3 (no exponent, then the first of its exponents: both in steps of 2^-9), and n·d −
+// z·d, z·d an f16 exactly, is one fma (34.6 -> 33.8 µs; values would have to change places first).
+struct Q4KScale {
+    h2_t d, zd;
+    RT_DEV explicit Q4KScale(uint32_t w) {  // the scale word, twice
+        const h2_t one = {(_Float16)1024.0f, (_Float16)1024.0f};
+        d = __builtin_bit_cast(h2_t, w & 0xFFF0FFF0u);
+        zd = (__builtin_bit_cast(h2_t, (w & 0x000F000Fu) | 0x64006400u) - one) * d;
+    }
+};
+RT_DEV h8_t q4_row_by_fours(uint32_t w, const Q4KScale& s) {
+    const uint32_t lo = w & 0x0F0F0F0Fu, hi = w >> 4 & 0x0F0F0F0Fu;
+    h2_t o[4];
+    o[0] = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false));
+    o[1] = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true));
+    o[2] = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false));
+    o[3] = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true));
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) o[i] = __builtin_elementwise_fma(o[i], s.d, -s.zd);
+    return (h8_t){o[0][0], o[0][1], o[1][0], o[1][1], o[2][0], o[2][1], o[3][0], o[3][1]};
+}
 RT_DEV h8_t q4_row(uint32_t w, const Q4Scale& s) {  // a word of a key's codes, in order
     h2_t o[4];
     q4_values(w, s, o);
@@ -427,11 +449,17 @@ RT_DEV void q4_chunk(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float*
     }
     h8_t qh[KN], ql[KN];
     const float qs = paged_query<HD, true>(q, scale2, qh, ql);
+#pragma unroll
+    for (uint32_t n = 0; n < KN; ++n) {  // (as the keys come)
+        qh[n] = __builtin_shufflevector(qh[n], qh[n], 0, 4, 1, 5, 2, 6, 3, 7);
+        ql[n] = __builtin_shufflevector(ql[n], ql[n], 0, 4, 1, 5, 2, 6, 3, 7);
+    }
     if constexpr (HALF)
 #pragma unroll
         for (uint32_t n = 0; n < KN; ++n) qh[n] = c < 8 ? qh[n] : ql[n];
     acc.start();
-    // turn i's operands out of its stage, on their way while the turn before is computed
+    // turn i's operands out of its stage, on their way while the turn before is computed; the N − 2 stages behind it
+    // may still be on theirs
     auto take = [&](uint32_t i, Raw (&raw)[2]) {
         q4_stages_left<S::LOADS, N - 2>(turns - 1 - i);
         asm volatile("" ::: "memory");
@@ -448,18 +476,18 @@ RT_DEV void q4_chunk(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float*
         here >>= 2;
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4 | 0 << 8);  // (LDS: this turn's stage is read)
-        if (i + 1 < turns) take(i + 1, next);
         if (i + N - 1 < turns) {  // (into the stage before this one)
             if ((i + N - 1) % 64 == 0) ids_from(i + N - 1);
             here |= bring(i + N - 1) << 2 * (N - 2);
         }
+        if (i + 1 < turns) take(i + 1, next);  // (N − 2 stages are brought behind it, or all there are)
         const bool edge = p0 < v.lo || p0 + 2 * RT_PAGED_TILE > limn || !there[0] || !there[1];
         f32x4 sa[2] = {}, sb[2] = {};
 #pragma unroll
         for (uint32_t u = 0; u < 2; ++u)
 #pragma unroll
             for (uint32_t n = 0; n < KN; ++n) {
-                const h8_t k = q4_row(raw[u].k[n / CW][n % CW], Q4Scale(raw[u].kscale(n)));
+                const h8_t k = q4_row_by_fours(raw[u].k[n / CW][n % CW], Q4KScale(raw[u].kscale(n)));
                 sa[u] = mfma32(k, qh[n], sa[u]);
                 if constexpr (!HALF) sb[u] = mfma32(k, ql[n], sb[u]);
             }

@@ -74,6 +74,58 @@ def test_many_sequences_among_prompt_chunks(ctx):
     check(got[only], ref[only], tol[only])
 
 
+@pytest.mark.parametrize("new", [1, 2, 40])
+@pytest.mark.parametrize("H,KVH,hd", [(14, 2, 64), (28, 4, 128), (14, 2, 256)])
+def test_a_full_device(ctx, H, KVH, hd, new):
+    """Long sequences, so many that every workgroup has tens of turns and memory
+    is busy: what is read is what has come.  Against what the pages hold, read
+    back row by row."""
+    rng, ps, n = np.random.default_rng(hd + new), 64, 24
+    kv = rng.integers(5000, 9000, n) + new
+    per = -(-kv // ps)
+    total, page = int(per.sum()), d.PagedBatch.page_bytes("q4", KVH, ps, hd)
+    table = np.full((n, per.max()), NONE, np.uint32)
+    at = 0
+    for s, k in enumerate(per):
+        table[s, :k] = np.arange(at, at + k)
+        at += k
+    pools = []
+    for _ in range(2):
+        raw = rng.integers(0, 256, (total * KVH, page // KVH), np.uint8)
+        words = raw[:, ps * hd // 2:].view(np.uint16)  # steps of 0.02 .. 0.4, zero points of 6 .. 9
+        words[:] = (np.exp(rng.uniform(np.log(0.02), np.log(0.4), words.shape)).astype(np.float16).view(np.uint16) & 0xFFF0) | \
+            rng.integers(6, 10, words.shape, np.uint16)
+        pools.append(ctx.buffer_from(raw))
+    u = lambda a: ctx.buffer_from(np.asarray(a, np.uint32))
+    start = np.arange(n + 1) * new
+    q = rng.standard_normal((n * new, H, hd)).astype(np.float32)
+    batch = d.PagedBatch(*pools, "q4", total, ps, KVH, hd, u(table), table.shape[1], n, u(kv), rows=n * new, row_start=u(start))
+    bq, bo = ctx.buffer_from(q), ctx.new_buffer(4 * q.size)
+    outs = []
+    for _ in range(3):
+        d.paged_attention_f32(ctx, batch, bq, bo, H)
+        ctx.flush()
+        outs.append(bo.read(np.float32).reshape(q.shape))
+    assert np.array_equal(outs[0], outs[1]) and np.array_equal(outs[0], outs[2])
+    for s in (0, 7, n - 1):
+        L = int(kv[s])
+        one = d.PagedBatch(*pools, "q4", total, ps, KVH, hd, u(table[s]), table.shape[1], 1, u([L]), rows=L, row_start=u([0, L]))
+        back = [ctx.new_buffer(4 * L * KVH * hd) for _ in range(2)]
+        d.paged_gather_f32(ctx, one, *back)
+        ctx.flush()
+        K, V = (b.read(np.float32).reshape(L, KVH, hd).astype(np.float64) for b in back)
+        for i in {0, new - 1}:
+            r, seen = s * new + i, L - new + i + 1
+            for h in range(0, H, 5):
+                k, v, x = K[:seen, h * KVH // H], V[:seen, h * KVH // H], q[r, h].astype(np.float64)
+                sc = k @ x / np.sqrt(hd)
+                w = np.exp(sc - sc.max())
+                mag = (np.abs(k) @ np.abs(x)).max() / np.sqrt(hd)
+                tol = w @ np.abs(v) / w.sum() * (2 * (hd + 16) * mag + seen + 64) * 2.0 ** -24
+                tol += seen * np.abs(v).max(0) * w.max() / w.sum() * 2.0 ** -37
+                assert np.all(np.abs(outs[0][r, h] - w @ v / w.sum()) <= tol), (s, i, h)
+
+
 @pytest.mark.parametrize("H,KVH,hd", [(71, 1, 64), (80, 2, 128), (130, 1, 64)])
 @pytest.mark.parametrize("P", [0, 70])
 def test_many_heads_of_a_group(ctx, H, KVH, hd, P):
