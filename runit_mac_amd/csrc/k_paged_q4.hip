@@ -169,29 +169,41 @@ struct PagedTile<HD, Q4> {
 //
 // lo = min(0, x), hi = max(0, x); d = (hi − lo) / 15 up to seven bits, 2^-20 at
 // least apart; z = −lo/d and n = x/d + z, each to the nearest, n kept within 0 .. 15.
+// In 64 bits, keys from their rotation on: in 32 an element in a million goes to the
+// code beside its own, and a group in a hundred thousand to another step.
+RT_DEV double max8_64(double v) {  // over aligned groups of 8 lanes
+    auto from = [&](auto dpp) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(double, (uint64_t)(uint32_t)dpp((int)(b >> 32)) << 32 | (uint32_t)dpp((int)b));
+    };
+    v = fmax(v, from([](int x) { return dpp_i<DPP_QUAD_PERM(1, 0, 3, 2)>(x); }));
+    v = fmax(v, from([](int x) { return dpp_i<DPP_QUAD_PERM(2, 3, 0, 1)>(x); }));
+    return fmax(v, from([](int x) { return dpp_i<DPP_ROW_HALF_MIRROR>(x); }));
+}
 struct Q4Group {
     uint32_t word;    // the scale word
     uint32_t n[4];
 };
-RT_DEV Q4Group q4_code(f32x4 x) {
-    float lo = 0.0f, hi = 0.0f;
+RT_DEV Q4Group q4_code(const double (&x)[4]) {
+    double lo = 0.0, hi = 0.0;
     bool bad = false;
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
-        lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]);
-        bad |= !(fabsf(x[i]) <= 32768.0f);
+        lo = fmin(lo, x[i]), hi = fmax(hi, x[i]);
+        bad |= !(fabs(x[i]) <= 32768.0);
     }
-    lo = -max8(-lo), hi = max8(hi);
+    lo = -max8_64(-lo), hi = max8_64(hi);
     bad = max8(bad ? 1.0f : 0.0f) > 0.0f;
-    const float step = (hi - lo) / 15.0f;
+    const double step = (hi - lo) / 15.0;
     // up to six bits behind the leading one; below 2^-14 to multiples of 2^-20
-    const float d = step < 6.103515625e-5f ? ceilf(step * 1048576.0f) * 9.5367431640625e-7f
-                                            : __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, step) + 0x1FFFFu) & ~0x1FFFFu);
-    const float inv = d > 0.0f ? 1.0f / d : 0.0f, z = rintf(-lo * inv);
+    const double d = step < 6.103515625e-5
+                         ? ceil(step * 1048576.0) * 9.5367431640625e-7
+                         : __builtin_bit_cast(double, (__builtin_bit_cast(uint64_t, step) + ((1ull << 46) - 1)) & ~((1ull << 46) - 1));
+    const double inv = d > 0.0 ? 1.0 / d : 0.0, z = rint(-lo * inv);
     Q4Group g;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) g.n[i] = bad ? 0u : (uint32_t)fminf(fmaxf(rintf(x[i] * inv) + z, 0.0f), 15.0f);
-    g.word = bad ? 0x7E00u : (uint32_t)f2h(d) | (uint32_t)z;
+    for (uint32_t i = 0; i < 4; ++i) g.n[i] = bad ? 0u : (uint32_t)(float)fmin(fmax(rint(x[i] * inv) + z, 0.0), 15.0);
+    g.word = bad ? 0x7E00u : (uint32_t)f2h((float)d) | (uint32_t)(float)z;
     return g;
 }
 template <int HD>
@@ -215,37 +227,49 @@ RT_DEV void q4_store(const PagedBatch& b, uint32_t page, uint32_t kvh, uint32_t 
 template <int HD>
 RT_DEV void paged_append_q4(const PagedAppendArgs& a) {
     constexpr uint32_t half = HD / 2, TH = half / 4, HW = 256 / TH;  // threads a head, heads a pass
-    __shared__ float cs[half], sn[half];
+    __shared__ double cs[half], sn[half];
     const PagedBatch& b = a.b;
     const uint32_t row = blockIdx.x, tid = threadIdx.x, ht = tid / TH, d = tid % TH * 4;
+    // (a head each group of threads; its elements are on their way while the row's place and angles are found, and
+    // heads of values alone need no angles)
+    const uint32_t h = blockIdx.y * HW + ht;
+    const bool some = h < a.H + 2 * b.KVH, isq = h < a.H, isv = h >= a.H + b.KVH;
+    const uint32_t kh = isq ? h : isv ? h - a.H - b.KVH : h - a.H;
+    f32x4 lo = {0, 0, 0, 0}, hi = lo;
+    if (some) {
+        const float* src = (isq ? a.q + ((size_t)row * a.H + kh) * HD : (isv ? a.v : a.k) + ((size_t)row * b.KVH + kh) * HD) + d;
+        lo = *(const f32x4*)src, hi = *(const f32x4*)(src + half);
+    }
     const uint32_t s = paged_seq(b, row);
     if (s >= b.n_seqs) return;  // behind the last sequence
     const auto [pos, page] = paged_place(b, s, row);
-    paged_turns<HD>(pos, a.log2_theta, cs, sn);
-    __syncthreads();
+    if (tid < half && blockIdx.y * HW < a.H + b.KVH) {
+        const double turns = (double)pos * exp2(-(double)(2 * tid) / HD * a.log2_theta) * 0.15915494309189535;
+        sincospi(2.0 * (turns - rint(turns)), &sn[tid], &cs[tid]);
+    }
+    lds_barrier();
     const uint32_t slot = pos & ((1u << b.ps_shift) - 1);
-    f32x4 c4, s4;
+    if (!some) return;
+    if (isq) {
+        f32x4 c4, s4;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) c4[i] = cs[d + i], s4[i] = sn[d + i];
-    const uint32_t heads = a.H + 2 * b.KVH;
-    for (uint32_t h = blockIdx.y * HW + ht; h < heads; h += gridDim.y * HW) {
-        const bool isq = h < a.H, isv = h >= a.H + b.KVH;
-        const uint32_t kh = isq ? h : isv ? h - a.H - b.KVH : h - a.H;
-        const float* src = (isq ? a.q + ((size_t)row * a.H + kh) * HD : (isv ? a.v : a.k) + ((size_t)row * b.KVH + kh) * HD) + d;
-        const f32x4 lo = *(const f32x4*)src, hi = *(const f32x4*)(src + half);
-        f32x4 x = lo, y = hi;
-        if (!isv) {
-            x = lo * c4 - hi * s4;
-            y = lo * s4 + hi * c4;
+        for (uint32_t i = 0; i < 4; ++i) c4[i] = (float)cs[d + i], s4[i] = (float)sn[d + i];
+        float* o = a.q_out + ((size_t)row * a.H + kh) * HD + d;
+        *(f32x4*)o = lo * c4 - hi * s4;
+        *(f32x4*)(o + half) = lo * s4 + hi * c4;
+    } else if (page < b.num_pages) {
+        double x[4], y[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            x[i] = (double)lo[i], y[i] = (double)hi[i];
+            if (!isv) {
+                const double c = cs[d + i], w = sn[d + i], z = x[i];
+                x[i] = z * c - y[i] * w;
+                y[i] = z * w + y[i] * c;
+            }
         }
-        if (isq) {
-            float* o = a.q_out + ((size_t)row * a.H + kh) * HD + d;
-            *(f32x4*)o = x;
-            *(f32x4*)(o + half) = y;
-        } else if (page < b.num_pages) {
-            q4_store<HD>(b, page, kh, slot, isv, d, q4_code(x));
-            q4_store<HD>(b, page, kh, slot, isv, d + half, q4_code(y));
-        }
+        q4_store<HD>(b, page, kh, slot, isv, d, q4_code(x));
+        q4_store<HD>(b, page, kh, slot, isv, d + half, q4_code(y));
     }
 }
 
