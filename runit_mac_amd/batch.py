@@ -450,7 +450,8 @@ class BatchDecoder:
             at, n = self._meta[name], len(ids)
             self._host[at:at + n] = ids
             ctx._check(ctx.lib.rt_upload(ctx.handle, self._at[name], self._host[at:].ctypes.data, 4 * n))
-        d.paged_copy(ctx, self._all_pages, self._at["src"], self._at["dst"], len(src))
+        for i in range(0, len(src), 65535):  # (of a call)
+            d.paged_copy(ctx, self._all_pages, self._at["src"] + 4 * i, self._at["dst"] + 4 * i, min(65535, len(src) - i))
 
     def _rules(self, rows):
         """LogitRules of rows of (rules, tokens) or None, their arrays on the device."""

@@ -164,7 +164,8 @@ RT_PAGED_GATHER(f16, _Float16, f16, _Float16)
 // of the lists goes on while the slice is on its way).  Entries that do, a chain or
 // a page written twice, are the first of them's: it copies its slice of all of
 // them in order, every byte by one thread, which sees its own stores.
-// Bound by the pages' bytes.
+// Bound by the pages' bytes: 277 pages of 18 KB in 56 pools 109 µs, 5.2 TB/s read and
+// written (a large copy makes 5.1); 8 pages of 16 KB in 48 pools 5.0 µs, a launch.
 RT_DEV void paged_copy(const PagedCopyArgs& a) {
     const uint32_t tid = threadIdx.x, i = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
     const uint32_t b0 = slice * a.slice_bytes, b1 = min(a.page_bytes, b0 + a.slice_bytes);

@@ -597,7 +597,7 @@ RT_DEV void paged_pairs(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const flo
 // Wide blocks: the codes become f16 on their way to LDS, once for the block's 128 columns; from
 // there on they are f16 pages.  Two waves have the keys of a turn's two tiles, two the values, each
 // from a ring of its own that is brought three turns ahead (one turn ahead into registers, the turns waited for
-// memory: prompt chunks 62 µs for WIDE_US); a stage is written while the one before is computed.
+// memory: prompt chunks 62 µs for 61); a stage is written while the one before is computed.
 template <int HD>
 struct PagedFeed<HD, Q4> {
     typedef PagedStage<HD> Stage;

@@ -78,9 +78,13 @@ struct PagedGatherArgs {
     void* v_out;
     uint32_t head_dim;
 };
-constexpr uint32_t RT_COPY_MAX = 65535;    // pages of a call (at most)
-constexpr uint32_t RT_COPY_SLICE = 16384;  // bytes of a workgroup (at most)
-constexpr uint32_t RT_COPY_POOLS = 256;  // pools of a launch (at most; 2 KB of its arguments)
+// Pages copied (k_paged.hip), at most: pages of a call; of a launch, as every workgroup looks through
+// its list (4,000 pages of 1 KB in 48 pools: 1,024 a launch 258 µs, 2,048 323, 4,000 443; 512 271);
+// bytes of a workgroup; pools of a launch (2 KB of its arguments).
+constexpr uint32_t RT_COPY_MAX = 65535;
+constexpr uint32_t RT_COPY_LIST = 1024;
+constexpr uint32_t RT_COPY_SLICE = 16384;
+constexpr uint32_t RT_COPY_POOLS = 256;
 struct PagedCopyArgs {
     const uint32_t *src, *dst;
     uint64_t page_stride;  // bytes

@@ -4278,7 +4278,8 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     // blocks, and all of pages of 4 bits, wait for instructions, of which two workgroups have more: prompt chunks 66
     // -> 59 µs, 32 decoding sequences of 4 bits 55 -> 40)
     const uint32_t per_cu = (uint32_t)occupancy(c, name, 64 * RT_PAGED_WAVES, 0);
-    const uint64_t slots = std::max<uint64_t>(1, (uint64_t)(wide || batch->f16 == RT_PAGES_Q4 ? per_cu : (per_cu + 1) / 2) * c->cu_count / a.b.KVH);
+    const uint64_t resident = wide || batch->f16 == RT_PAGES_Q4 ? per_cu : (per_cu + 1) / 2;
+    const uint64_t slots = std::max<uint64_t>(1, resident * c->cu_count / a.b.KVH);
     if ((blocks + slots) * a.b.KVH > 0xffffffu)  // (2^32 threads a launch)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: too many rows (%u of %u heads)", who, rows,
                     num_heads);
@@ -4286,7 +4287,7 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     // narrow blocks of pages of 4 bits: in the launch's last workgroups only where heads and tables are small (heads of
     // 128, one sequence of 600 positions 10.6 against 10.3 µs, 8,000 14.2 and 11.7, 200,003 46 and 39; heads of 64: 600
     // 8.0 and 9.0, 40 sequences of up to 2,000 9.8 and 11.0, 16 of up to 8,000 13.2 and 12.0)
-    const bool many = batch->f16 == RT_PAGES_Q4 && (hd > 64 || (uint64_t)a.b.table_stride * batch->page_size > 4096);
+    const bool many = batch->f16 == RT_PAGES_Q4 && a.target && (hd > 64 || (uint64_t)a.b.table_stride * batch->page_size > 4096);
     const bool noted = wide || shared_len || many;  // (chunks meet in a launch of their own)
     a.noted = noted;
     if (!noted && 2 * (blocks + a.target) * a.b.KVH > kAttnCounters) a.target = 0;
@@ -4304,7 +4305,7 @@ static int paged_attention(rt_ctx* c, const rt_paged_batch* batch, const float* 
     void* params[] = {&a};
     st = launch(c, name, dim3(a.jobs * a.b.KVH), dim3(64 * RT_PAGED_WAVES), 0, params);
     if (st != RT_OK || !noted) return st;
-    if (batch->f16 == RT_PAGES_Q4 && (!wide || shared_len)) {
+    if (batch->f16 == RT_PAGES_Q4 && a.target && (!wide || shared_len)) {  // (no more rows than blocks that are split have)
         snprintf(name, sizeof name, "k_paged_meet%s_hd%u", wide ? "w" : "", hd);
         return launch(c, name, dim3(rows * num_heads), dim3(256), 0, params);
     }
@@ -4381,20 +4382,22 @@ int rt_paged_copy(rt_ctx* c, const rt_paged_batch* batches, uint32_t n_batches, 
     a.slices = (a.page_bytes + RT_COPY_SLICE - 1) / RT_COPY_SLICE;
     a.slice_bytes = ((a.page_bytes + a.slices - 1) / a.slices + 15) / 16 * 16;
     // (2^32 threads a launch; its pools are arguments)
-    const uint64_t wgs = (uint64_t)n * a.slices;
-    if (wgs > 0xffffffu)
+    if ((uint64_t)n * a.slices > 0xffffffu)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: %u pages of %u bytes are too many", n,
                     a.page_bytes);
-    const uint32_t most = (uint32_t)std::min<uint64_t>(RT_COPY_POOLS, 0xffffffu / wgs);
+    const uint32_t most = std::min(RT_COPY_POOLS, 0xffffffu / (std::min(n, RT_COPY_LIST) * a.slices));
     for (uint64_t p = 0; p < 2ull * n_batches; p += most) {
         const uint32_t k = (uint32_t)std::min<uint64_t>(most, 2ull * n_batches - p);
         for (uint32_t i = 0; i < k; ++i) {
             const rt_paged_batch& o = batches[(p + i) / 2];
             a.pools[i] = (p + i) % 2 ? o.v_pages : o.k_pages;
         }
-        void* params[] = {&a};
-        const int st = launch(c, "k_paged_copy", dim3((uint32_t)wgs, k), dim3(256), 0, params);
-        if (st != RT_OK) return st;
+        for (uint32_t e = 0; e < n; e += RT_COPY_LIST) {
+            a.src = src + e, a.dst = dst + e, a.n = std::min(RT_COPY_LIST, n - e);
+            void* params[] = {&a};
+            const int st = launch(c, "k_paged_copy", dim3(a.n * a.slices, k), dim3(256), 0, params);
+            if (st != RT_OK) return st;
+        }
     }
     return RT_OK;
 }

@@ -153,6 +153,21 @@ def test_forks_are_their_sequences(ctx, kv):
     m.free()
 
 
+def test_more_pages_than_a_call_copies(ctx):
+    """A pool of 140,000 pages, half of them moved at once."""
+    m = DecodeModel(ctx, DecodeConfig(**TINY), seed=43)
+    b, n = BatchDecoder(m, 1, 140_000, 16, kv="q4", max_rows=16), 70_000
+    page, p = b._pages[0].page_bytes("q4", m.cfg.kv_heads, 16, m.cfg.head_dim), b._pages[-1]
+    for pool in (p.k_pages, p.v_pages):
+        raw = np.random.default_rng(pool % 1000).integers(0, 256, n * page, np.uint8)
+        ctx._check(ctx.lib.rt_upload(ctx.handle, pool, raw.ctypes.data, raw.nbytes))
+        b._copy_pages(range(n), range(2 * n - 1, n - 1, -1))
+        got = np.empty(n * page, np.uint8)
+        ctx._check(ctx.lib.rt_download(ctx.handle, got.ctypes.data, pool + n * page, got.nbytes))
+        assert np.array_equal(got.reshape(n, page)[::-1], raw.reshape(n, page))
+    b.free(), m.free()
+
+
 def test_rules_choose_the_token(ctx):
     """Penalties, biases and masks of some sequences of a step: the logits they
     leave, the token chosen from them, the scores of the logits as they are."""

@@ -70,6 +70,17 @@ def test_long_lists(ctx, pages, n):
     p.check()
 
 
+@pytest.mark.parametrize("shift", [0, 1])
+def test_lists_of_several_launches(ctx, shift):
+    """Thousands of entries: each page once, then every page one place on (a chain
+    through all of them)."""
+    n = 9001
+    p = Pools(ctx, "q4", 1, 16, 64, 2 * n, 1, seed=shift)
+    ids = np.random.default_rng(shift).permutation(2 * n)
+    p.copy(*((ids[:n], ids[n:]) if not shift else (np.arange(n), np.arange(n) + 1)))
+    p.check()
+
+
 def test_more_pools_than_a_launch_takes(ctx):
     p = Pools(ctx, "q4", 1, 16, 64, 9, 150, seed=3)
     n = d.launch_count(ctx)
