@@ -159,17 +159,19 @@ RT_PAGED_GATHER(f16, _Float16, f16, _Float16)
 // ───────────────────────────── pages copied ─────────────────────────────
 //
 // Entry i makes page dst[i] of every pool a copy of page src[i], as if one after
-// another.  A workgroup has a slice of one page of one pool, its entry alone where
+// another.  A workgroup has a slice of one page of one pool, or (SMALL) a page of several
+// pools (2,000 pages of 1,152 bytes in 48 pools 45 µs, of one pool each 120), its entry alone where
 // that shares no page with another entry but a source with sources (the scan
 // of the lists goes on while the slice is on its way).  Entries that do, a chain or
 // a page written twice, are the first of them's: it copies its slice of all of
 // them in order, every byte by one thread, which sees its own stores.
 // Bound by the pages' bytes: 277 pages of 18 KB in 56 pools 109 µs, 5.2 TB/s read and
 // written (a large copy makes 5.1); 8 pages of 16 KB in 48 pools 5.0 µs, a launch.
+template <bool SMALL>
 RT_DEV void paged_copy(const PagedCopyArgs& a) {
     const uint32_t tid = threadIdx.x, i = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
-    const uint32_t b0 = slice * a.slice_bytes, b1 = min(a.page_bytes, b0 + a.slice_bytes);
-    uint8_t* pool = (uint8_t*)a.pools[blockIdx.y];
+    const uint32_t b0 = slice * a.slice_bytes, bytes = min(a.page_bytes - b0, a.slice_bytes);
+    uint8_t* pool = (uint8_t*)a.pools[SMALL ? 0 : blockIdx.y] + b0;
     auto entry = [&](uint32_t j, uint32_t& s, uint32_t& d) {
         s = a.src[j], d = a.dst[j];
         return s < a.num_pages && d < a.num_pages;
@@ -189,20 +191,29 @@ RT_DEV void paged_copy(const PagedCopyArgs& a) {
     // (the slice is on its way while the lists are looked through)
     constexpr uint32_t V = RT_COPY_SLICE / (256 * 16);
     u32x4 v[V];
+    uint8_t* at[V];  // (small pages) in page 0; null: nothing
+    if constexpr (SMALL) {
+        const uint32_t p0 = blockIdx.y * a.group, pools = min(a.n_pools - p0, a.group);
+#pragma unroll
+        for (uint32_t u = 0; u < V; ++u) {
+            const uint32_t o = (256 * u + tid) * 16, p = o / bytes;
+            at[u] = p < pools ? (uint8_t*)a.pools[p0 + p] + (o - p * bytes) : nullptr;
+        }
+    }
     auto load = [&](uint32_t s) {
         const uint8_t* from = pool + s * a.page_stride;
 #pragma unroll
         for (uint32_t u = 0; u < V; ++u) {
-            const uint32_t o = b0 + (256 * u + tid) * 16;
-            if (o < b1) v[u] = *(const u32x4*)(from + o);
+            const uint32_t o = (256 * u + tid) * 16;
+            if (SMALL ? at[u] != nullptr : o < bytes) v[u] = *(const u32x4*)(SMALL ? at[u] + s * a.page_stride : from + o);
         }
     };
     auto store = [&](uint32_t d) {
         uint8_t* to = pool + d * a.page_stride;
 #pragma unroll
         for (uint32_t u = 0; u < V; ++u) {
-            const uint32_t o = b0 + (256 * u + tid) * 16;
-            if (o < b1) *(u32x4*)(to + o) = v[u];
+            const uint32_t o = (256 * u + tid) * 16;
+            if (SMALL ? at[u] != nullptr : o < bytes) *(u32x4*)(SMALL ? at[u] + d * a.page_stride : to + o) = v[u];
         }
     };
     load(s);
@@ -219,4 +230,5 @@ RT_DEV void paged_copy(const PagedCopyArgs& a) {
         if (entry(j, s2, d2) && s2 != d2 && meets(j, s2, d2)) load(s2), store(d2);
     }
 }
-extern "C" __global__ void __launch_bounds__(256) k_paged_copy(PagedCopyArgs a) { paged_copy(a); }
+extern "C" __global__ void __launch_bounds__(256) k_paged_copy(PagedCopyArgs a) { paged_copy<false>(a); }
+extern "C" __global__ void __launch_bounds__(256) k_paged_copy_small(PagedCopyArgs a) { paged_copy<true>(a); }

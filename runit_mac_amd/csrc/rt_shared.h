@@ -89,6 +89,7 @@ struct PagedCopyArgs {
     const uint32_t *src, *dst;
     uint64_t page_stride;  // bytes
     uint32_t page_bytes, slice_bytes, slices, num_pages, n;
+    uint32_t n_pools, group;  // small pages: pools, and those of a workgroup
     void* pools[RT_COPY_POOLS];
 };
 struct PagedAttnArgs {

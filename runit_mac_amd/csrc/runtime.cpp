@@ -196,7 +196,7 @@ const char* const kKernelNames[] = {
     "k_paged_meet_hd64", "k_paged_meet_hd128", "k_paged_meet_hd256",
     "k_paged_meetw_hd64", "k_paged_meetw_hd128", "k_paged_meetw_hd256",
     "k_paged_gather_f32_f32", "k_paged_gather_f32_f16", "k_paged_gather_f16_f32", "k_paged_gather_f16_f16",
-    "k_paged_gather_q4_f32", "k_paged_gather_q4_f16", "k_paged_copy",
+    "k_paged_gather_q4_f32", "k_paged_gather_q4_f16", "k_paged_copy", "k_paged_copy_small",
     "k_adjust_logits_f32", "k_adjust_logits_f16",
     "k_logprobs_f32", "k_logprobs_f16", "k_logprobs_top_f32", "k_logprobs_top_f16",
 };
@@ -4392,10 +4392,12 @@ int rt_paged_copy(rt_ctx* c, const rt_paged_batch* batches, uint32_t n_batches, 
             const rt_paged_batch& o = batches[(p + i) / 2];
             a.pools[i] = (p + i) % 2 ? o.v_pages : o.k_pages;
         }
+        a.n_pools = k;
+        a.group = a.slices > 1 ? 1 : std::min(k, RT_COPY_SLICE / a.slice_bytes);
         for (uint32_t e = 0; e < n; e += RT_COPY_LIST) {
             a.src = src + e, a.dst = dst + e, a.n = std::min(RT_COPY_LIST, n - e);
             void* params[] = {&a};
-            const int st = launch(c, "k_paged_copy", dim3(a.n * a.slices, k), dim3(256), 0, params);
+            const int st = launch(c, a.group > 1 ? "k_paged_copy_small" : "k_paged_copy", dim3(a.n * a.slices, (k + a.group - 1) / a.group), dim3(256), 0, params);
             if (st != RT_OK) return st;
         }
     }
