@@ -438,6 +438,37 @@ def test_append(ctx, H, KVH, hd, ps, one):
     assert np.array_equal(again[:b.R], got[:b.R]) and np.array_equal(again[b.R:], b.q[b.R:])
 
 
+@pytest.mark.parametrize("H,KVH,hd", HEADS)
+def test_append_of_many_rows(ctx, H, KVH, hd):
+    """Long chunks store and rotate what their rows do a few at a time."""
+    ps, seqs = 64, [(0, 900), (77, 0), (130, 1), (1000, 1200)]
+    kv, new = np.array([a + n for a, n in seqs]), np.array([n for _, n in seqs])
+    rng, R = np.random.default_rng(hd + H), int(new.sum())
+    per = -(-kv // ps)
+    table = np.full((len(seqs), per.max()), NONE, np.uint32)
+    for s, ids in enumerate(np.split(rng.permutation(per.sum()), np.cumsum(per)[:-1])):
+        table[s, :len(ids)] = ids
+    start = np.concatenate([[0], np.cumsum(new)])
+    q, k, v = (rng.standard_normal((R + 3, n, hd)).astype(np.float32) for n in (H, KVH, KVH))
+    size, got = int(per.sum()) * d.PagedBatch.page_bytes("q4", KVH, ps, hd), []
+    u = lambda a: ctx.buffer_from(np.asarray(a, np.uint32))
+    for most in (R, 200):
+        pools, out = [ctx.buffer_from(np.full(size, 0x5A, np.uint8)) for _ in range(2)], np.full_like(q, MARK)
+        for at in range(0, 1200, most):
+            n = np.clip(new - at, 0, most)
+            rows = np.concatenate([start[s] + at + np.arange(n[s]) for s in range(len(seqs))] + [np.arange(R, R + 3)]).astype(int)
+            bo = ctx.buffer_from(np.full((len(rows), H, hd), MARK, np.float32))
+            batch = d.PagedBatch(*pools, "q4", int(per.sum()), ps, KVH, hd, u(table), table.shape[1], len(seqs),
+                                 u(kv - new + at + n), rows=len(rows), row_start=u(np.concatenate([[0], np.cumsum(n)])))
+            d.rope_kv_append_paged_f32(ctx, batch, *(ctx.buffer_from(x[rows]) for x in (q, k, v)), bo, H, 1e6)
+            ctx.flush()
+            out[rows] = bo.read(np.float32).reshape(len(rows), H, hd)
+        got.append((out, *(p.read(np.uint8) for p in pools)))
+    for a, b in zip(*got):
+        assert np.array_equal(a, b)
+    assert np.all(got[0][0][R:] == MARK)
+
+
 def test_append_of_what_is_not_finite(ctx):
     """The group has NaN, the others their values."""
     b = Batch4([(0, 3)], 2, 1, 64, 16, seed=3)
