@@ -215,14 +215,14 @@ RT_DEV void q4_store(const PagedBatch& b, uint32_t page, uint32_t kvh, uint32_t 
     uint16_t* scales = (uint16_t*)(part + ((size_t)(HD / 2) << b.ps_shift));
     if (isv) {
         const uint32_t r = slot % 16;
-        uint16_t* tile = (uint16_t*)(part + (slot / 16) * Q4Layout<HD>::TILE);
+        uint16_t* tile = (uint16_t*)(part + (size_t)(slot / 16) * Q4Layout<HD>::TILE);
         const uint32_t n = (((d / (16 * W) * 4 + r / 4) * 16 + d / W % 16) * 2 + r % 4 / 2) * (W / 4) + d % W / 4;
         tile[2 * n + r % 2] = (uint16_t)(g.n[0] | g.n[1] << 4 | g.n[2] << 8 | g.n[3] << 12);
         if (d % 32 == 0) scales[slot / 16 * (HD / 2) + d / 32 * 16 + r] = (uint16_t)g.word;
     } else {
         // (eight elements are two threads')
         const uint32_t mine = g.n[0] | g.n[2] << 4 | g.n[1] << 16 | g.n[3] << 20, next = lane_xor<1>(mine);
-        if (d % 8 == 0) ((uint32_t*)part)[slot * (HD / 8) + d / 8] = mine | next << 8;
+        if (d % 8 == 0) ((uint32_t*)part)[(size_t)slot * (HD / 8) + d / 8] = mine | next << 8;
         if (d % 32 == 0) scales[slot * (HD / 32) + d / 32] = (uint16_t)g.word;
     }
 }
@@ -296,12 +296,12 @@ RT_DEV f32x4 q4_load(const PagedBatch& b, uint32_t page, uint32_t kvh, uint32_t 
     if (isv) {
         const uint32_t r = slot % 16;
         const uint32_t n = (((d / (16 * W) * 4 + r / 4) * 16 + d / W % 16) * 2 + r % 4 / 2) * (W / 4) + d % W / 4;
-        const uint32_t w = ((const uint16_t*)(part + (slot / 16) * Q4Layout<HD>::TILE))[2 * n + r % 2];
+        const uint32_t w = ((const uint16_t*)(part + (size_t)(slot / 16) * Q4Layout<HD>::TILE))[2 * n + r % 2];
         q4_values(w, Q4Scale(scales[slot / 16 * (HD / 2) + d / 32 * 16 + r]), o);
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) x[i] = (float)o[i][0];
     } else {
-        const uint32_t w = ((const uint32_t*)part)[slot * (HD / 8) + d / 8] >> (d % 8 ? 8 : 0);
+        const uint32_t w = ((const uint32_t*)part)[(size_t)slot * (HD / 8) + d / 8] >> (d % 8 ? 8 : 0);
         q4_values(w, Q4Scale(scales[slot * (HD / 32) + d / 32] * 0x10001u), o);
         x = (f32x4){(float)o[0][0], (float)o[0][1], (float)o[1][0], (float)o[1][1]};
     }
@@ -454,8 +454,8 @@ RT_DEV void q4_chunk(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float*
             const uint32_t page = __builtin_amdgcn_readlane(ids[u], i & 63);
             there |= page < v.num_pages ? 1u << u : 0u;
             const size_t at = (page < v.num_pages ? page : 0) * v.page_stride;
-            off[u] = at + v.slot(t + u) * (HD / 2);
-            so[u] = at + s0 + v.slot(t + u) * (HD / 16);
+            off[u] = at + (size_t)v.slot(t + u) * (HD / 2);
+            so[u] = at + s0 + (size_t)v.slot(t + u) * (HD / 16);
             asm("" : "+s"(off[u]), "+s"(so[u]));  // (sums of all lanes', not of each)
         }
 #pragma unroll
@@ -649,8 +649,8 @@ struct PagedFeed<HD, Q4> {
         const uint32_t id0 = __builtin_amdgcn_readlane(ids[0], i & 63), id1 = __builtin_amdgcn_readlane(ids[1], i & 63);
         const uint32_t page = u ? id1 : id0;
         const size_t at = (page < v.num_pages ? page : 0) * v.page_stride;
-        const uint8_t* codes = mine + at + v.slot(t) * (HD / 2);
-        const uint8_t* scales = mine + at + ((size_t)(HD / 2) << v.ps_shift) + v.slot(t) * (HD / 16);
+        const uint8_t* codes = mine + at + (size_t)v.slot(t) * (HD / 2);
+        const uint8_t* scales = mine + at + ((size_t)(HD / 2) << v.ps_shift) + (size_t)v.slot(t) * (HD / 16);
         const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const h8_t*)lds);
         const uint32_t to = lds0 + ring + i % RING * (CODES + SCALES);
         // (of 128 and 256 the keys as their lanes' operands; of 64 both as they are, 32 lanes' worth)

@@ -175,6 +175,75 @@ def test_pages_behind_four_billion_bytes(ctx, new):
     assert np.all(np.isfinite(outs[0])) and np.array_equal(*outs)
 
 
+@pytest.mark.parametrize("new", [2, 40])
+def test_a_page_of_more_than_four_billion_bytes(ctx, new):
+    """Rows behind a prefix that has no pages, at the end of a page of 2^26 positions
+    of 256 elements."""
+    H, KVH, hd, ps = 2, 1, 256, 2 ** 26
+    P, L = ps - 96, ps - 5
+    rng = np.random.default_rng(new)
+    u = lambda *a: ctx.buffer_from(np.array(a, np.uint32))
+    pools = [ctx.new_buffer(d.PagedBatch.page_bytes("q4", KVH, ps, hd)) for _ in range(2)]
+    q = rng.standard_normal((L - P, H, hd)).astype(np.float32)
+    k, v = (rng.standard_normal((L - P, KVH, hd)).astype(np.float32) for _ in range(2))
+    rows = L - P  # (all are stored, the last `new` attend)
+    batch = d.PagedBatch(*pools, "q4", 1, ps, KVH, hd, u(0), 1, 1, u(L), rows=rows, row_start=u(0, rows))
+    bo, back = ctx.new_buffer(q.nbytes), [ctx.new_buffer(k.nbytes) for _ in range(2)]
+    d.rope_kv_append_paged_f32(ctx, batch, ctx.buffer_from(q), ctx.buffer_from(k), ctx.buffer_from(v), bo, H, 1e6)
+    d.paged_gather_f32(ctx, batch, *back)
+    ctx.flush()
+    K, V = (b.read(np.float32).reshape(k.shape) for b in back)
+    pos = np.arange(P, L)
+    for got, x in ((K, rope64(k, pos, 1e6)), (V, v.astype(np.float64))):
+        g = x.reshape(rows, KVH, -1, 32)
+        half = up7(((np.maximum(g.max(-1), 0) - np.minimum(g.min(-1), 0)) / 15)) / 2
+        # (angles of 2^26 in 64 bits are off by 2^-27 at most)
+        assert np.all(np.abs(got - x) <= np.repeat(half, 32, -1) + 1e-6)
+    q = q[-new:]
+    batch = d.PagedBatch(*pools, "q4", 1, ps, KVH, hd, u(0), 1, 1, u(L), rows=new, row_start=u(0, new))
+    out = ctx.new_buffer(q.nbytes)
+    d.shared_prefix_attention_f32(ctx, batch, ctx.buffer_from(q), out, H, u(NONE), P)
+    ctx.flush()
+    got = out.read(np.float32).reshape(q.shape)
+    for i in range(new):
+        seen = rows - new + i + 1
+        for h in range(H):
+            x = K[:seen, 0].astype(np.float64) @ q[i, h] / np.sqrt(hd)
+            w = np.exp(x - x.max())
+            mag = (np.abs(K[:seen, 0]) @ np.abs(q[i, h])).max() / np.sqrt(hd)
+            tol = w @ np.abs(V[:seen, 0]) / w.sum() * (2 * (hd + 16) * mag + seen + 64) * 2.0 ** -24
+            tol += seen * np.abs(V[:seen, 0]).max(0) * w.max() / w.sum() * 2.0 ** -37
+            assert np.all(np.abs(got[i, h] - w @ V[:seen, 0].astype(np.float64) / w.sum()) <= tol), (i, h)
+    for x in pools:
+        x.free()
+
+
+@pytest.mark.parametrize("P", [0, 64])
+@pytest.mark.parametrize("new", [1, 40])
+def test_two_contexts_at_once(ctx, new, P):
+    """Calls of two contexts under way together give what each gives alone."""
+    other = d.HipContext()
+
+    def together():
+        sides, want = [], []
+        for c, seed in ((ctx, 1), (other, 2)):
+            b, table, *_ = shared4([(900, new), (P + 30, 1), (2000, new)], P, 28, 4, 128, 16, seed=seed)
+            want.append(attend(c, b, shared=(table, P) if P else None))
+            sides.append((c, b.upload(c), c.buffer_from(b.q), c.new_buffer(b.q.nbytes), c.buffer_from(table.astype(np.uint32)), b))
+        for _ in range(20):
+            for c, batch, q, out, table, b in sides:
+                if P:
+                    d.shared_prefix_attention_f32(c, batch, q, out, 28, table, P)
+                else:
+                    d.paged_attention_f32(c, batch, q, out, 28)
+        for (c, _, _, out, _, b), w in zip(sides, want):
+            c.flush()
+            assert np.array_equal(out.read(np.float32).reshape(b.q.shape)[:b.R], w)
+
+    together()
+    other.close()
+
+
 def test_missing_pages(ctx):
     """Ids that are no page: their positions are not seen; a row that sees
     nothing gives zeros."""
