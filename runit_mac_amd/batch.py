@@ -101,8 +101,11 @@ class Rules:
             raise ValueError(f"rules: prompt_len {self.prompt_len}")
         if any(not 0 <= t < vocab for t in self.bias or ()):
             raise ValueError(f"rules: a bias's token is out of range [0, {vocab})")
-        if self.allowed is not None:
-            self.mask(vocab)
+        if any(np.isnan(b) for b in (self.bias or {}).values()):
+            raise ValueError("rules: a bias is NaN")
+        if self.allowed is not None and not np.unpackbits(np.ascontiguousarray(self.mask(vocab)).view(np.uint8),
+                                                          bitorder="little")[:vocab].any():
+            raise ValueError("rules: no token is allowed")
         return self
 
     def mask(self, vocab: int) -> np.ndarray:

@@ -214,3 +214,14 @@ def test_rules_are_checked():
     with pytest.raises(ValueError):
         b.step({s: [1]}, rules={t: Rules()})
     assert not b.passes and b.length(s) == 0
+
+
+def test_rules_that_leave_no_choice():
+    n = CFG.vocab
+    b = decoder(Ruled)
+    s = b.open()
+    for bad in (dict(allowed=np.zeros(n, bool)), dict(allowed=np.zeros(-(-n // 32), np.uint32)), dict(bias={3: np.nan})):
+        with pytest.raises(ValueError):
+            b.step({s: [1]}, rules={s: Rules(**bad)})
+    assert not b.passes and b.length(s) == 0
+    b.step({s: [1]}, rules={s: Rules(allowed=np.arange(2 * n)[::2] == 2, bias={3: -np.inf})})
