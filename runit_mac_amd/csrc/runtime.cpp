@@ -4371,12 +4371,16 @@ int rt_paged_copy(rt_ctx* c, const rt_paged_batch* batches, uint32_t n_batches, 
             o.num_kv_heads != b.num_kv_heads || o.head_dim != b.head_dim || o.page_stride != b.page_stride)
             return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: the pages of batch %u differ from those of batch 0", i);
     }
-    std::vector<const void*> pools;
-    for (uint32_t i = 0; i < n_batches; ++i) pools.insert(pools.end(), {batches[i].k_pages, batches[i].v_pages});
-    std::sort(pools.begin(), pools.end());
-    if (std::adjacent_find(pools.begin(), pools.end()) != pools.end())
-        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: a pool is there twice");
     const uint32_t el = b.f16 == RT_PAGES_Q4 ? 1 : b.f16 ? 2 : 4;
+    std::vector<uintptr_t> pools;
+    for (uint32_t i = 0; i < n_batches; ++i)
+        pools.insert(pools.end(), {(uintptr_t)batches[i].k_pages, (uintptr_t)batches[i].v_pages});
+    std::sort(pools.begin(), pools.end());
+    for (size_t i = 1; i < pools.size(); ++i)  // (pools whose pages take turns are apart)
+        if (pools[i] - pools[i - 1] < page * el)
+            return fail(c, RT_ERR_DISPATCH, pools[i] == pools[i - 1]
+                                                ? "kernel dispatch error: paged_copy: a pool is there twice"
+                                                : "kernel dispatch error: paged_copy: pools overlap");
     if (page * el > 0x7fffffffu)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: pages of %llu bytes",
                     (unsigned long long)(page * el));

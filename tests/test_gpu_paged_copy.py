@@ -151,3 +151,20 @@ def test_refusals(ctx):
     d.paged_copy(ctx, p.batches, None, None, 0)
     assert d.launch_count(ctx) == n
     p.check()
+
+
+def test_pools_that_overlap(ctx):
+    """Refused where their pages do; pools whose pages take turns are apart."""
+    p = Pools(ctx, "q4", 1, 16, 64, 4, 1)
+    src, dst = ctx.buffer_from(np.array([1], np.uint32)), ctx.buffer_from(np.array([3], np.uint32))
+    page, raw = p.page, np.random.default_rng(7).integers(0, 256, (4, 2, p.page), np.uint8)
+    both = ctx.buffer_from(raw)
+    make = lambda at: d.PagedBatch(both.ptr, both.ptr + at, "q4", 4, 16, 1, 64, None, 0, 0, None, page_stride=2 * page)
+    n = d.launch_count(ctx)
+    with pytest.raises(d.Dispatch, match="overlap"):
+        d.paged_copy(ctx, make(page - 16), src, dst, 1)
+    assert d.launch_count(ctx) == n
+    d.paged_copy(ctx, make(page), src, dst, 1)
+    ctx.flush()
+    raw[3] = raw[1]
+    assert np.array_equal(both.read(np.uint8).reshape(raw.shape), raw)
