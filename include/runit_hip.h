@@ -737,7 +737,8 @@ int rt_argmax_rows_first_f32(rt_ctx* ctx, const float* in, uint32_t* result, uin
  * and largest elements, and 0, d is a fifteenth of their distance, up to seven
  * significant bits and to 2^-20, z = −smallest / d, n = x / d + z, each to the nearest
  * (even): an element is off by d / 2 at most.  A group with an
- * element beyond 32,768 or not finite is held as NaN.  head_dim · 9/16 bytes a
+ * element beyond 32,768 or not finite is held as NaN.  (Of pages written otherwise too d·z and
+ * d·(15 − z) must be within f16, d a multiple of 2^-20.)  head_dim · 9/16 bytes a
  * position and KV head; a KV head's part of a page is [page_size · head_dim / 2] bytes of
  * codes and [page_size · head_dim / 32] scale words:
  *   keys    codes as 32-bit words of 8 elements in a row, from the lowest bits

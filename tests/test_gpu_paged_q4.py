@@ -350,6 +350,18 @@ def test_the_largest_steps(ctx):
         check(attend(ctx, b), *b.attention())
 
 
+@pytest.mark.parametrize("new", [2, 44])
+@pytest.mark.parametrize("scale", [30000.0, 2.0 ** -18, 2.0 ** -15])
+def test_keys_of_the_largest_and_smallest_steps(ctx, scale, new):
+    """Keys below the normal numbers of f16, of almost 2^15, and queries as much the other way."""
+    b = Batch4([(120, 1), (90, new)], 14, 2, 128, 16, seed=59)
+    c = b.cells(b.k).astype(np.float64)
+    b.words["k"] = list(encode(np.clip(c / 3, -1, 1) * scale))
+    b.cells(b.k)[:] = decode(*b.words["k"])
+    b.q = (b.q / np.float32(scale)).astype(np.float32)
+    check(attend(ctx, b), *b.attention())
+
+
 @pytest.mark.parametrize("mag", [26, 31, 34])
 @pytest.mark.parametrize("new", [1, 60])
 def test_large_scores(ctx, mag, new):
