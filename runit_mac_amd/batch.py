@@ -119,10 +119,40 @@ class Rules:
         return np.packbits(bits, bitorder="little").view(np.uint32)
 
 
+class _Tokens:
+    """Token ids in an array that grows; equal to a list of the same."""
+
+    def __init__(self, ids=()):
+        self._room = np.array(ids, np.uint32)
+        self._n = self._room.size
+
+    @property
+    def ids(self) -> np.ndarray:
+        return self._room[:self._n]
+
+    def __len__(self) -> int:
+        return self._n
+
+    def __eq__(self, other) -> bool:
+        return np.array_equal(self.ids, other.ids if isinstance(other, _Tokens) else other)
+
+    def extend(self, ids) -> None:
+        n = self._n + len(ids)
+        if n > self._room.size:
+            room = np.empty(n + n // 2, np.uint32)
+            room[:self._n] = self.ids
+            self._room = room
+        self._room[self._n:n] = ids
+        self._n = n
+
+    def cut(self, n: int) -> None:
+        self._n = min(self._n, n)
+
+
 class _Sequence:
-    def __init__(self, tokens):
-        self.tokens = list(tokens)
-        self.len = len(self.tokens)
+    def __init__(self, tokens: _Tokens):
+        self.tokens = _Tokens(tokens.ids)
+        self.len = len(tokens)
         self.pages: list[int] = []  # from the prefix's last whole page on
 
 
@@ -159,7 +189,7 @@ class BatchDecoder:
         self._seqs: dict[int, _Sequence] = {}
         self._next = 0
         self._prefix_pages: list[int] = []
-        self._prefix_tokens: list[int] = []
+        self._prefix_tokens = _Tokens()
         self.prefix_len = 0
         self._copied: list = []  # of the call that runs: (sequence, place, the page before)
         self._pick_rules: list | None = None  # of the pass's kept rows: rules and tokens
@@ -205,7 +235,7 @@ class BatchDecoder:
         s = self._seq(seq)
         new = self.open()
         f = self._seqs[new]
-        f.tokens, f.len, f.pages = list(s.tokens), s.len, list(s.pages)
+        f.tokens, f.len, f.pages = _Tokens(s.tokens.ids), s.len, list(s.pages)
         self.pool.share(f.pages)
         return new
 
@@ -233,7 +263,7 @@ class BatchDecoder:
         if not self.prefix_len <= length <= s.len:
             raise ValueError(f"trim: {length} is not within {self.prefix_len} .. {s.len}")
         s.len = length
-        del s.tokens[length:]
+        s.tokens.cut(length)
         keep = -(-length // self.page_size) - self.prefix_len // self.page_size if length > self.prefix_len else 0
         self.pool.give(s.pages[keep:])
         del s.pages[keep:]
@@ -251,7 +281,7 @@ class BatchDecoder:
         if need > there:
             raise d.BufferSize(f"buffer size mismatch: expected {need} free pages, got {there}")
         self.pool.give(self._prefix_pages)
-        self._prefix_pages, self._prefix_tokens, self.prefix_len = [], [], 0
+        self._prefix_pages, self._prefix_tokens, self.prefix_len = [], _Tokens(), 0
         if toks.size == 0:
             return
         seq = self.open()
@@ -388,12 +418,13 @@ class BatchDecoder:
                 row += n
             self._place(batch, work, picks, targets)
             upto = {s: at + n for s, at, n in batch}
-            self._pick_rules = [(rules[s], self._seqs[s].tokens + work[s][upto[s] - n:upto[s]].tolist()) if s in rules
-                                else None for s, _, n in batch if s in owner] if any(s in rules for s in owner) else None
+            said = lambda s, n: _Tokens(np.concatenate([self._seqs[s].tokens.ids, work[s][upto[s] - n:upto[s]]]))
+            self._pick_rules = [(rules[s], said(s, n)) if s in rules else None
+                                for s, _, n in batch if s in owner] if any(s in rules for s in owner) else None
             got = self._launch(batch, row, picks, targets if given else None, top)
             for s, at, n in batch:
                 self._seqs[s].len += n
-                self._seqs[s].tokens += work[s][at:at + n].tolist()
+                self._seqs[s].tokens.extend(work[s][at:at + n])
             owner = np.array(owner)
             for s, _, _ in batch:
                 if np.any(owner == s):
@@ -460,13 +491,13 @@ class BatchDecoder:
         """LogitRules of rows of (rules, tokens) or None, their arrays on the device."""
         vocab, n = self.model.cfg.vocab, len(rows)
         rules = [r[0] if r else Rules() for r in rows]
-        lists = [r[1] if r else [] for r in rows]
+        lists = [(r[1] if r else _Tokens()).ids for r in rows]
         biases = [list((r.bias or {}).items()) for r in rules]
         masks = [r.mask(vocab) for r in rules if r.allowed is not None]
         starts = lambda x: np.concatenate([[0], np.cumsum([len(v) for v in x])[:-1]])
         u32, f32 = (lambda v: np.asarray(v, np.int64).astype(np.uint32)), (lambda v: np.asarray(v, np.float32).view(np.uint32))
         parts = dict(
-            tokens=u32([t for v in lists for t in v]), token_start=u32(starts(lists)), token_len=u32([len(v) for v in lists]),
+            tokens=np.concatenate(lists), token_start=u32(starts(lists)), token_len=u32([len(v) for v in lists]),
             prompt_len=u32([min(r.prompt_len, 0xFFFFFFFF) for r in rules]), repetition=f32([r.repetition for r in rules]),
             frequency=f32([r.frequency for r in rules]), presence=f32([r.presence for r in rules]),
             bias_ids=u32([t for v in biases for t, _ in v]), bias=f32([b for v in biases for _, b in v]),
