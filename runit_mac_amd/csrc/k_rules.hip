@@ -13,8 +13,8 @@
 // logits that change are written, and only those that no mask forbids read.
 //
 // Bound by the logits' bytes: 120 rows of 152,064 f32 with histories of up to 9,000
-// tokens, up to 300 biases and masks 34 µs for 147 MB (4.3 TB/s; a large copy makes
-// 5.1; without lists 29).  Few rows: by trips to memory, 5 rows 4.4 µs.  4,096
+// tokens, up to 300 biases and masks 33.7 µs for 147 MB (4.4 TB/s; a large copy makes
+// 5.1; without lists 29).  Few rows: by trips to memory, 5 rows 3.9 µs.  4,096
 // tokens and 512 threads: with 256 threads 39 µs, with 8,192 tokens 41, one thread
 // adding all biases of its token one after another 68.
 #include "rt_attn.h"
@@ -34,21 +34,26 @@ struct RuleVec<_Float16> {
     typedef _Float16 vec __attribute__((ext_vector_type(8), aligned(2)));
 };
 
-// The threads' entries of a list, UNROLL loads at a time: f(entry, its place).
-template <uint32_t UNROLL, class F>
-RT_DEV void each_entry(const uint32_t* ids, uint32_t n, const F& f) {
-    for (uint32_t j0 = 0; j0 < n; j0 += NT * UNROLL) {
-        uint32_t id[UNROLL];
+// A list's entries, UNROLL of a thread at a time: those from j0 on into id, and f(entry, its place) of them.
+template <uint32_t UNROLL>
+RT_DEV void load_entries(const uint32_t* ids, uint32_t n, uint32_t j0, uint32_t (&id)[UNROLL]) {
 #pragma unroll
-        for (uint32_t u = 0; u < UNROLL; ++u) {
-            const uint32_t j = j0 + NT * u + threadIdx.x;
-            id[u] = j < n ? ids[j] : 0xffffffffu;
-        }
+    for (uint32_t u = 0; u < UNROLL; ++u) {
+        const uint32_t j = j0 + NT * u + threadIdx.x;
+        id[u] = j < n ? ids[j] : 0xffffffffu;
+    }
+}
+template <uint32_t UNROLL, class F>
+RT_DEV void each_entry(const uint32_t* ids, uint32_t n, uint32_t (&id)[UNROLL], const F& f) {
+    for (uint32_t j0 = 0;;) {
 #pragma unroll
         for (uint32_t u = 0; u < UNROLL; ++u) {
             const uint32_t j = j0 + NT * u + threadIdx.x;
             if (j < n) f(id[u], j);
         }
+        if (n - j0 <= NT * UNROLL) break;
+        j0 += NT * UNROLL;
+        load_entries<UNROLL>(ids, n, j0, id);
     }
 }
 
@@ -101,19 +106,23 @@ RT_DEV void adjust_logits(const RulesArgs& a) {
         allowed[u] = mr < a.mask_rows && i < e1 ? a.mask[mr * a.mask_stride + i / 32] >> i % 32 : 0xffffffffu;
     }
     if (nt || nb) {
+        // (the lists' first entries are on their way while the counts are cleared)
+        uint32_t said[8], biased[2];
+        load_entries(a.tokens + ta, nt, 0, said);
+        load_entries(a.bias_ids + ba, nb, 0, biased);
         for (uint32_t i = tid; i < SEG / 4; i += NT) {
             count4[i] = cvec{0, 0, 0, 0};
             more4[i] = f32x4{0, 0, 0, 0};
         }
         if (tid == 0) twice = 0;
         lds_barrier();
-        each_entry<8>(a.tokens + ta, nt, [&](uint32_t id, uint32_t j) {
+        each_entry(a.tokens + ta, nt, said, [&](uint32_t id, uint32_t j) {
             if (id - e0 >= e1 - e0) return;
             if (j < np) atomicOr(&count[id - e0], PROMPT);
             else atomicAdd(&count[id - e0], 1u);
         });
         // a bias alone is its token's; where two meet they are summed again, in order
-        each_entry<2>(a.bias_ids + ba, nb, [&](uint32_t id, uint32_t j) {
+        each_entry(a.bias_ids + ba, nb, biased, [&](uint32_t id, uint32_t j) {
             if (id - e0 >= e1 - e0) return;
             const uint32_t b = __builtin_bit_cast(uint32_t, a.bias[ba + j] + 0.0f);
             if (b && atomicExch((uint32_t*)&more[id - e0], b)) twice = 1;
