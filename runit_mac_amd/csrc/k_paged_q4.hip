@@ -56,27 +56,37 @@ RT_DEV void q4_values(uint32_t w, const Q4Scale& s, h2_t (&o)[4]) {
     o[2] = (__builtin_bit_cast(h2_t, (v & low) | one) - s.z) * s.d;
     o[3] = (__builtin_bit_cast(h2_t, (v & high) | one) - s.z16) * s.d16;
 }
-// A word of a key's codes in the order 0, 4, 1, 5, 2, 6, 3, 7, two instructions in thirteen fewer: a byte
-// of 0 .. 15 is n·2^-9 as an e4m3 (no exponent, then the first of its exponents: both in steps of 2^-9), and n·d −
-// z·d, z·d an f16 exactly, is one fma (34.6 -> 33.8 µs; values would have to change places first).
-struct Q4KScale {
+// The same by way of bytes, for narrow blocks, an instruction or two in thirteen fewer: a byte of 0 .. 15 is
+// n·2^-9 as an e4m3 (no exponent, then the first of its exponents: both in steps of 2^-9), and n·d −
+// z·d, z·d an f16 exactly, is one fma (the 7B step 34.6 -> 33.8 µs with keys in the order 0, 4, 1, 5, 2, 6, 3, 7,
+// which queries take; 34.2 -> 33.6 with values, whose bytes change places first.  Wide blocks are slower for it,
+// prompt chunks 59.8 -> 61.2: there a wave waits for its own few words).
+struct Q4ByteScale {
     h2_t d, zd;
-    RT_DEV explicit Q4KScale(uint32_t w) {  // the scale word, twice
+    RT_DEV explicit Q4ByteScale(uint32_t w) {  // the halves' scale words
         const h2_t one = {(_Float16)1024.0f, (_Float16)1024.0f};
         d = __builtin_bit_cast(h2_t, w & 0xFFF0FFF0u);
         zd = (__builtin_bit_cast(h2_t, (w & 0x000F000Fu) | 0x64006400u) - one) * d;
     }
 };
-RT_DEV h8_t q4_row_by_fours(uint32_t w, const Q4KScale& s) {
+RT_DEV void q4_bytes(uint32_t w, const Q4ByteScale& s, h2_t (&o)[4]) {  // lower four bits, of the bytes 0, 1 and 2, 3; upper
     const uint32_t lo = w & 0x0F0F0F0Fu, hi = w >> 4 & 0x0F0F0F0Fu;
-    h2_t o[4];
     o[0] = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false));
     o[1] = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true));
     o[2] = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false));
     o[3] = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true));
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) o[i] = __builtin_elementwise_fma(o[i], s.d, -s.zd);
+}
+RT_DEV h8_t q4_row_by_fours(uint32_t w, const Q4ByteScale& s) {  // of a key's codes
+    h2_t o[4];
+    q4_bytes(w, s, o);
     return (h8_t){o[0][0], o[0][1], o[1][0], o[1][1], o[2][0], o[2][1], o[3][0], o[3][1]};
+}
+RT_DEV void q4_pairs(uint32_t w, const Q4ByteScale& s, h2_t (&o)[4]) {  // as q4_values
+    h2_t x[4];
+    q4_bytes(__builtin_amdgcn_perm(w, w, 0x03010200u), s, x);
+    o[0] = x[0], o[1] = x[2], o[2] = x[1], o[3] = x[3];
 }
 RT_DEV h8_t q4_row(uint32_t w, const Q4Scale& s) {  // a word of a key's codes, in order
     h2_t o[4];
@@ -530,7 +540,7 @@ RT_DEV void q4_chunk(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float*
         for (uint32_t u = 0; u < 2; ++u)
 #pragma unroll
             for (uint32_t n = 0; n < KN; ++n) {
-                const h8_t k = q4_row_by_fours(raw[u].k[n / CW][n % CW], Q4KScale(raw[u].kscale(n)));
+                const h8_t k = q4_row_by_fours(raw[u].k[n / CW][n % CW], Q4ByteScale(raw[u].kscale(n)));
                 sa[u] = mfma32(k, qh[n], sa[u]);
                 if constexpr (!HALF) sb[u] = mfma32(k, ql[n], sb[u]);
             }
@@ -579,7 +589,7 @@ RT_DEV void q4_chunk(PagedAcc<HD, Q4>& acc, const PagedView<Q4>& v, const float*
 #pragma unroll
                 for (uint32_t x = 0; x < 4; ++x) {
                     const uint32_t m = (n * 2 + x % 2) * (VW / 4) + h;
-                    q4_values(raw[x / 2].v[m / CW][m % CW], Q4Scale(raw[x / 2].vs[n][x % 2]), o[x]);
+                    q4_pairs(raw[x / 2].v[m / CW][m % CW], Q4ByteScale(raw[x / 2].vs[n][x % 2]), o[x]);
                 }
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) {
