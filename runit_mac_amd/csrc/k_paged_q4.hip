@@ -332,7 +332,7 @@ RT_DEV void paged_gather_q4(const PagedGatherArgs& a) {
 // weights as pairs of f16.  A code's f16 is exact, so that its step and zero point
 // need no sums of their own; but each code is made f16 once in every block that reads it,
 // which bounds narrow blocks beside memory: 32 sequences of up to 16,000 positions of 4 KV heads of
-// 128 with 7 query heads each 34 µs for 108 MB (3.2 TB/s), their loads and launches alone 26–28.
+// 128 with 7 query heads each 33 µs for 108 MB (3.3 TB/s), their loads and launches alone 26–28.
 // Of narrow blocks the parts meet in a launch of their own (paged_meet) where there may be many.
 
 // A wave's own ring of stages in LDS, a turn's two tiles each: codes of keys and values as their
