@@ -357,7 +357,7 @@ class BatchDecoder:
             need += self._more_pages(q, t.size)
             if t.size and self._shared_end(q) is not None:
                 writers[q.pages[-1]] = writers.get(q.pages[-1], 0) + 1
-        # (the last holder of a page keeps it)
+        # (one of a page's holders keeps it)
         need += sum(min(n, self.pool.holders(p) - 1) for p, n in writers.items())
         if need > self.pool.free:
             raise d.BufferSize(f"buffer size mismatch: expected {need} free pages, got {self.pool.free}")
@@ -387,7 +387,7 @@ class BatchDecoder:
         except BaseException:
             for s, n in before.items():
                 self.trim(s, n)
-            # (what others hold of a page that was copied is as it was)
+            # (of a page that was copied nobody has written to the positions of those that held it)
             for q, at, page in reversed(self._copied):
                 self.pool.share([page])
                 self.pool.give([q.pages[at]])
@@ -399,6 +399,7 @@ class BatchDecoder:
     def _passes(self, work: dict, keep: dict | None, top: int | None, given: bool, rules: dict) -> dict:
         parts = {s: [] for s in work}
         left = [(s, 0) for s, t in work.items() if t.size]
+        self._own_ends([self._seqs[s] for s, _ in left])
         while left:
             rows, batch = 0, []
             while left and rows < self.max_rows:
@@ -443,7 +444,6 @@ class BatchDecoder:
         table[:] = NO_PAGE
         put = lambda name, at, v: host.__setitem__(slice(meta[name] + at, meta[name] + at + len(v)), v)
         row = 0
-        self._own_ends([self._seqs[s] for s, _, _ in batch])
         for i, (s, at, n) in enumerate(batch):
             q = self._seqs[s]
             q.pages += self.pool.take(self._more_pages(q, n))
@@ -457,13 +457,18 @@ class BatchDecoder:
         put("shared", 0, self._prefix_pages)
 
     def _own_ends(self, seqs) -> None:
-        """Copies the pages that these sequences write to next and others hold."""
-        writers, left = [], {}
+        """Copies the pages that these sequences, all that a call appends to, write to
+        next and others hold.  A page that all of its holders write to is kept by the
+        longest: it stores nothing before the others' ends, so that they can have the
+        page back if the call fails."""
+        by_page, writers = {}, []
         for q in seqs:
             page = self._shared_end(q)
-            if page is not None and left.setdefault(page, self.pool.holders(page)) > 1:
-                left[page] -= 1
-                writers.append((q, page))
+            if page is not None:
+                by_page.setdefault(page, []).append(q)
+        for page, qs in by_page.items():
+            keeper = max(reversed(qs), key=lambda q: q.len) if len(qs) == self.pool.holders(page) else None
+            writers += [(q, page) for q in qs if q is not keeper]
         if not writers:
             return
         fresh = self.pool.take(len(writers))
