@@ -95,18 +95,34 @@ class Rules:
     allowed: np.ndarray | None = None
 
     def checked(self, vocab: int) -> "Rules":
-        if not 0 < self.repetition < np.inf or not np.isfinite([self.frequency, self.presence]).all():
+        rep, freq, pres = self.penalties()
+        if not 0 < rep < np.inf or not np.isfinite([freq, pres]).all():
             raise ValueError(f"rules: penalties {self.repetition}, {self.frequency}, {self.presence}")
         if self.prompt_len < 0:
             raise ValueError(f"rules: prompt_len {self.prompt_len}")
         if any(not 0 <= t < vocab for t in self.bias or ()):
             raise ValueError(f"rules: a bias's token is out of range [0, {vocab})")
-        if any(np.isnan(b) for b in (self.bias or {}).values()):
+        ids, bias = self.biases()
+        if np.isnan(bias).any():
             raise ValueError("rules: a bias is NaN")
-        if self.allowed is not None and not np.unpackbits(np.ascontiguousarray(self.mask(vocab)).view(np.uint8),
-                                                          bitorder="little")[:vocab].any():
+        left = np.ones(vocab, bool)
+        if self.allowed is not None:
+            left = np.unpackbits(np.ascontiguousarray(self.mask(vocab)).view(np.uint8), bitorder="little")[:vocab] > 0
+        left[ids[bias == -np.inf]] = False
+        if not left.any():
             raise ValueError("rules: no token is allowed")
         return self
+
+    def penalties(self) -> np.ndarray:
+        """Repetition, frequency and presence in the 32 bits that the device has."""
+        with np.errstate(over="ignore", under="ignore"):
+            return np.array([self.repetition, self.frequency, self.presence], np.float64).astype(np.float32)
+
+    def biases(self) -> tuple[np.ndarray, np.ndarray]:
+        """The biases' tokens and, in 32 bits, values."""
+        b = self.bias or {}
+        with np.errstate(over="ignore", under="ignore"):
+            return np.array(list(b), np.int64), np.array(list(b.values()), np.float64).astype(np.float32)
 
     def mask(self, vocab: int) -> np.ndarray:
         a, words = np.asarray(self.allowed), -(-vocab // 32)
@@ -497,16 +513,16 @@ class BatchDecoder:
         vocab, n = self.model.cfg.vocab, len(rows)
         rules = [r[0] if r else Rules() for r in rows]
         lists = [(r[1] if r else _Tokens()).ids for r in rows]
-        biases = [list((r.bias or {}).items()) for r in rules]
+        biases, penalties = [r.biases() for r in rules], np.stack([r.penalties() for r in rules]).view(np.uint32)
         masks = [r.mask(vocab) for r in rules if r.allowed is not None]
         starts = lambda x: np.concatenate([[0], np.cumsum([len(v) for v in x])[:-1]])
-        u32, f32 = (lambda v: np.asarray(v, np.int64).astype(np.uint32)), (lambda v: np.asarray(v, np.float32).view(np.uint32))
+        u32 = lambda v: np.asarray(v, np.int64).astype(np.uint32)
         parts = dict(
             tokens=np.concatenate(lists), token_start=u32(starts(lists)), token_len=u32([len(v) for v in lists]),
-            prompt_len=u32([min(r.prompt_len, 0xFFFFFFFF) for r in rules]), repetition=f32([r.repetition for r in rules]),
-            frequency=f32([r.frequency for r in rules]), presence=f32([r.presence for r in rules]),
-            bias_ids=u32([t for v in biases for t, _ in v]), bias=f32([b for v in biases for _, b in v]),
-            bias_start=u32(starts(biases)), bias_len=u32([len(v) for v in biases]),
+            prompt_len=u32([min(r.prompt_len, 0xFFFFFFFF) for r in rules]), repetition=penalties[:, 0],
+            frequency=penalties[:, 1], presence=penalties[:, 2],
+            bias_ids=u32(np.concatenate([t for t, _ in biases])), bias=np.concatenate([b for _, b in biases]).view(np.uint32),
+            bias_start=u32(starts([t for t, _ in biases])), bias_len=u32([len(t) for t, _ in biases]),
             mask=np.concatenate(masks) if masks else u32([]),
             mask_row=u32(np.where([r.allowed is not None for r in rules],
                                   np.cumsum([r.allowed is not None for r in rules]) - 1, NO_PAGE)))
