@@ -124,6 +124,13 @@ class Rules:
         with np.errstate(over="ignore", under="ignore"):
             return np.array(list(b), np.int64), np.array(list(b.values()), np.float64).astype(np.float32)
 
+    def forbids(self, token: int) -> bool:
+        """Whether the mask or a bias of -inf forbids a token."""
+        ids, bias = self.biases()
+        a = None if self.allowed is None else np.asarray(self.allowed)
+        off = a is not None and not (a[token] if a.dtype == bool else a[token // 32] >> token % 32 & 1)
+        return bool(off or np.any(bias[ids == token] == -np.inf))
+
     def mask(self, vocab: int) -> np.ndarray:
         a, words = np.asarray(self.allowed), -(-vocab // 32)
         if a.dtype == np.uint32 and a.shape == (words,):
@@ -326,8 +333,8 @@ class BatchDecoder:
 
     def step(self, work: dict, top: int | None = None, rules: dict | None = None) -> dict:
         """Appends tokens to sequences ({sequence: tokens}) and returns the
-        likeliest next token of each that its `rules` ({sequence: Rules}) leave;
-        with `top`, pairs of it and its TokenScores with that many alternatives,
+        likeliest next token of each that its `rules` ({sequence: Rules}) leave
+        (ValueError if they leave none with a logit above -inf); with `top`, pairs of it and its TokenScores with that many alternatives,
         the model's own: without the rules."""
         work = self._checked(work)
         if any(t.size == 0 for t in work.values()):
@@ -439,6 +446,10 @@ class BatchDecoder:
             self._pick_rules = [(rules[s], said(s, n)) if s in rules else None
                                 for s, _, n in batch if s in owner] if any(s in rules for s in owner) else None
             got = self._launch(batch, row, picks, targets if given else None, top)
+            # (a row of -inf and NaN has the first token for its likeliest)
+            for s, r, t in zip(owner, self._pick_rules or (), got[0] if got else ()):
+                if t == 0 and r is not None and r[0].forbids(0):
+                    raise ValueError(f"rules: they leave sequence {s} no token with a logit")
             for s, at, n in batch:
                 self._seqs[s].len += n
                 self._seqs[s].tokens.extend(work[s][at:at + n])

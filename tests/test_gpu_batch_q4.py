@@ -214,3 +214,22 @@ def test_rules_choose_the_token(ctx):
     assert np.all(np.abs(after - want) <= (np.abs(want) + np.abs(raw) + 10) * 6 * F32)
     assert tok == np.flatnonzero(after == after.max())[0]
     b.free(), m.free()
+
+
+def test_rules_leave_no_logit(ctx):
+    """Penalties that make the one token allowed -inf: an error, and the sequences
+    as they were."""
+    cfg = DecodeConfig(**TINY)
+    m = DecodeModel(ctx, cfg, seed=61)
+    b = BatchDecoder(m, 2, 20, 16, kv="q4", max_rows=8, max_logits=1)
+    s, t = b.open(), b.open()
+    b.step({s: [9, 9, 9], t: [3, 4]})
+    before, free = held(b, s, 1), b.pool.free
+    only = Rules(allowed=np.arange(cfg.vocab) == 9, frequency=3e38)
+    with pytest.raises(ValueError, match="no token"):
+        b.step({s: [9, 1], t: [5]}, rules={s: only})
+    assert b.length(s) == 3 and b.length(t) == 2 and b.pool.free == free
+    assert all(np.array_equal(x, y) for x, y in zip(held(b, s, 1), before))
+    only.frequency = 1.0
+    assert b.step({s: [9, 1], t: [5]}, rules={s: only})[s] == 9
+    b.free(), m.free()

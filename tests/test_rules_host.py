@@ -38,3 +38,18 @@ def test_something_is_left(rules):
     s = b.open()
     b.step({s: [1]}, rules={s: Rules(**rules)})
     assert b.length(s) == 1
+
+
+@pytest.mark.parametrize("rules", [dict(allowed=only(3, 4)), dict(allowed=words(only(3, 4))), dict(bias={0: -np.inf}),
+                                   dict(bias={0: -1e39}, allowed=only(0, 7))])
+def test_no_logit_is_left(rules):
+    """Of a row of -inf and NaN the first token is the likeliest: an error where the rules
+    forbid it, and the sequences of the call stay as they were."""
+    b = decoder(Ruled, num_pages=12)
+    s, t = b.open(), b.open()
+    b.step({s: [1], t: [2]})
+    with pytest.raises(ValueError, match="no token"):
+        b.step({s: [5], t: np.append(np.arange(20), N - 1)}, rules={t: Rules(**rules)})  # (N - 1: after it comes 0)
+    assert b.length(s) == b.length(t) == 1 and b.pool.free == 10
+    assert b.step({s: [N - 1], t: [5]}, rules={t: Rules(frequency=1.0)}) == {s: 0, t: 6}
+    assert b.step({t: [N - 1]}, rules={t: Rules(allowed=only(0, 7), bias={0: -3.0})}) == {t: 0}
