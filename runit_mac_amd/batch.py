@@ -98,10 +98,10 @@ class Rules:
         rep, freq, pres = self.penalties()
         if not 0 < rep < np.inf or not np.isfinite([freq, pres]).all():
             raise ValueError(f"rules: penalties {self.repetition}, {self.frequency}, {self.presence}")
-        if self.prompt_len < 0:
+        if not self.prompt_len >= 0 or self.prompt_len % 1:
             raise ValueError(f"rules: prompt_len {self.prompt_len}")
-        if any(not 0 <= t < vocab for t in self.bias or ()):
-            raise ValueError(f"rules: a bias's token is out of range [0, {vocab})")
+        if any(not 0 <= t < vocab or t % 1 for t in self.bias or ()):
+            raise ValueError(f"rules: a bias's token is none of [0, {vocab})")
         ids, bias = self.biases()
         if np.isnan(bias).any():
             raise ValueError("rules: a bias is NaN")

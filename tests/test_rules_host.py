@@ -53,3 +53,14 @@ def test_no_logit_is_left(rules):
     assert b.length(s) == b.length(t) == 1 and b.pool.free == 10
     assert b.step({s: [N - 1], t: [5]}, rules={t: Rules(frequency=1.0)}) == {s: 0, t: 6}
     assert b.step({t: [N - 1]}, rules={t: Rules(allowed=only(0, 7), bias={0: -3.0})}) == {t: 0}
+
+
+@pytest.mark.parametrize("rules", [dict(bias={1.5: 1.0}), dict(bias={np.nan: 1.0}), dict(bias={0.25: -np.inf}),
+                                   dict(prompt_len=1.5), dict(prompt_len=np.nan)])
+def test_numbers_that_are_not_whole(rules):
+    b = decoder(Ruled)
+    s = b.open()
+    with pytest.raises(ValueError):
+        b.step({s: [1]}, rules={s: Rules(**rules)})
+    assert not b.passes
+    b.step({s: [1]}, rules={s: Rules(bias={np.int64(3): 1.0, 4.0: 2.0}, prompt_len=np.uint32(2))})
