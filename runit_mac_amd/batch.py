@@ -118,6 +118,10 @@ class Rules:
         with np.errstate(over="ignore", under="ignore"):
             return np.array([self.repetition, self.frequency, self.presence], np.float64).astype(np.float32)
 
+    def penalises(self) -> bool:
+        """Whether the sequence's tokens change anything."""
+        return not np.array_equal(self.penalties(), [1, 0, 0])
+
     def biases(self) -> tuple[np.ndarray, np.ndarray]:
         """The biases' tokens and, in 32 bits, values."""
         b = self.bias or {}
@@ -443,7 +447,7 @@ class BatchDecoder:
             self._place(batch, work, picks, targets)
             upto = {s: at + n for s, at, n in batch}
             said = lambda s, n: _Tokens(np.concatenate([self._seqs[s].tokens.ids, work[s][upto[s] - n:upto[s]]]))
-            self._pick_rules = [(rules[s], said(s, n)) if s in rules else None
+            self._pick_rules = [(rules[s], said(s, n) if rules[s].penalises() else _Tokens()) if s in rules else None
                                 for s, _, n in batch if s in owner] if any(s in rules for s in owner) else None
             got = self._launch(batch, row, picks, targets if given else None, top)
             # (a row of -inf and NaN has the first token for its likeliest)

@@ -64,3 +64,15 @@ def test_numbers_that_are_not_whole(rules):
         b.step({s: [1]}, rules={s: Rules(**rules)})
     assert not b.passes
     b.step({s: [1]}, rules={s: Rules(bias={np.int64(3): 1.0, 4.0: 2.0}, prompt_len=np.uint32(2))})
+
+
+def test_masks_and_biases_need_no_tokens():
+    """A sequence's tokens are counted only where a penalty is for them."""
+    b = decoder(Ruled, max_rows=64)
+    s, t, u = b.open(), b.open(), b.open()
+    mask, bias, neutral = Rules(allowed=only(2, 6, 8)), Rules(bias={6: 1.0}, prompt_len=1), Rules(1.0, -0.0, 1e-50)
+    b.step({s: [5, 1], t: [5, 7], u: [9]}, rules={s: mask, t: bias, u: neutral})
+    assert b.seen[-1] == [(mask, []), (bias, []), (neutral, [])]
+    for r in (Rules(repetition=1.1), Rules(frequency=-0.1), Rules(presence=1e-30)):
+        b.step({s: [1], t: [7]}, rules={s: r, t: bias})
+        assert b.seen[-1] == [(r, b._seqs[s].tokens.ids), (bias, [])]
