@@ -4349,6 +4349,20 @@ int rt_paged_gather_f16(rt_ctx* c, const rt_paged_batch* batch, uint16_t* k, uin
     return paged_gather(c, batch, k, v, "f16");
 }
 
+// Whether no pools share a byte: n pages of `page` bytes each, `stride` from one to the next.  (Two whose pages take
+// turns are apart where the one's begin in the other's gaps.)  In order of their addresses.
+static bool pools_apart(const std::vector<uintptr_t>& pools, uint64_t page, uint64_t stride, uint32_t n) {
+    const uint64_t span = (n - 1) * stride + page;
+    std::vector<uint64_t> in(pools.size());  // from a page's beginning of the first pool on
+    for (size_t i = 0; i < pools.size(); ++i) in[i] = (pools[i] - pools[0]) % stride;
+    for (size_t i = 0; i < pools.size(); ++i)
+        for (size_t j = i + 1; j < pools.size() && pools[j] - pools[i] < span; ++j) {
+            const uint64_t gap = in[j] >= in[i] ? in[j] - in[i] : stride - in[i] + in[j];
+            if (gap < page || gap > stride - page) return false;
+        }
+    return true;
+}
+
 int rt_paged_copy(rt_ctx* c, const rt_paged_batch* batches, uint32_t n_batches, const uint32_t* src,
                   const uint32_t* dst, uint32_t n) {
     if (!c) return fail(nullptr, RT_ERR_DISPATCH, "kernel dispatch error: null context");
@@ -4376,11 +4390,11 @@ int rt_paged_copy(rt_ctx* c, const rt_paged_batch* batches, uint32_t n_batches, 
     for (uint32_t i = 0; i < n_batches; ++i)
         pools.insert(pools.end(), {(uintptr_t)batches[i].k_pages, (uintptr_t)batches[i].v_pages});
     std::sort(pools.begin(), pools.end());
-    for (size_t i = 1; i < pools.size(); ++i)  // (pools whose pages take turns are apart)
-        if (pools[i] - pools[i - 1] < page * el)
-            return fail(c, RT_ERR_DISPATCH, pools[i] == pools[i - 1]
-                                                ? "kernel dispatch error: paged_copy: a pool is there twice"
-                                                : "kernel dispatch error: paged_copy: pools overlap");
+    if (!pools_apart(pools, page * el, stride * el, b.num_pages))
+        return fail(c, RT_ERR_DISPATCH,
+                    std::adjacent_find(pools.begin(), pools.end()) != pools.end()
+                        ? "kernel dispatch error: paged_copy: a pool is there twice"
+                        : "kernel dispatch error: paged_copy: pools overlap");
     if (page * el > 0x7fffffffu)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: pages of %llu bytes",
                     (unsigned long long)(page * el));

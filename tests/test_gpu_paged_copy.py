@@ -168,3 +168,37 @@ def test_pools_that_overlap(ctx):
     ctx.flush()
     raw[3] = raw[1]
     assert np.array_equal(both.read(np.uint8).reshape(raw.shape), raw)
+
+
+@pytest.mark.parametrize("layers", [1, 20])
+def test_pools_that_overlap_anywhere(ctx, layers):
+    """Pools shifted by whole pages, or into the gaps of others that are too
+    narrow, are refused; those that end where the next begins, or in wide gaps, copied."""
+    page = d.PagedBatch.page_bytes("q4", 1, 16, 64)
+    raw = np.random.default_rng(8).integers(0, 256, (2 * layers + 1) * 4 * 2 * page, np.uint8)
+    buf = ctx.buffer_from(raw)
+    ids = ctx.buffer_from(np.array([1], np.uint32)), ctx.buffer_from(np.array([3], np.uint32))
+
+    def copy(starts, stride, pages=4):
+        """The last layer's values take the last start; the others are apart from both of its pools."""
+        make = lambda k, v: d.PagedBatch(buf.ptr + k, buf.ptr + v, "q4", pages, 16, 1, 64, None, 0, 0, None, page_stride=stride)
+        d.paged_copy(ctx, [make(k, v) for k, v in zip(starts[::2], starts[1::2])], *ids, 1)
+        ctx.flush()
+
+    whole = [4 * page * i for i in range(2 * layers)]
+    turns = [2 * page * 4 * i for i in range(2 * layers)]
+    for bad in (*((whole, s, 0) for s in (1, 2, 3)), *((whole, s, page) for s in (1, 3)), (whole, 3.5, 0),
+                (turns, 0.5, 2 * page), (turns, 1.5, 2 * page), (turns, 2, 2 * page), (turns, 4.5, 2 * page), (turns, 6, 2 * page)):
+        starts, shift, stride = bad
+        n = d.launch_count(ctx)
+        with pytest.raises(d.Dispatch, match="overlap"):
+            copy([*starts[:-1], starts[-2] + int(shift * page)], stride)
+        assert d.launch_count(ctx) == n
+    assert np.array_equal(buf.read(np.uint8), raw)
+    for starts, shift, stride in ((whole, 4, 0), (turns, 1, 2 * page), (turns, 5, 2 * page), (turns, 7, 2 * page)):
+        at = [*starts[:-1], starts[-2] + shift * page]
+        copy(at, stride)
+        for k in at:
+            raw[k + 3 * (stride or page):][:page] = raw[k + (stride or page):][:page]
+        assert np.array_equal(buf.read(np.uint8), raw)
+    copy([0, page], 0, 1)  # (one page each: one behind the other)
