@@ -4176,6 +4176,8 @@ static int paged_pool_check(rt_ctx* c, const rt_paged_batch* b, const char* who,
     if (b->num_pages == 0 || b->num_pages > 0x7fffffffu)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: num_pages=%u", who, b->num_pages);
     const uint32_t unit = b->f16 == RT_PAGES_Q4 ? 16 : 8;
+    if ((uint64_t)b->num_kv_heads * b->page_size > (1ull << 60) / b->head_dim)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: %s: a page exceeds the address space", who);
     page = (uint64_t)b->num_kv_heads * b->page_size * b->head_dim;
     if (b->f16 == RT_PAGES_Q4) page = page / 16 * 9;
     stride = b->page_stride ? b->page_stride : page;

@@ -202,3 +202,18 @@ def test_pools_that_overlap_anywhere(ctx, layers):
             raw[k + 3 * (stride or page):][:page] = raw[k + (stride or page):][:page]
         assert np.array_equal(buf.read(np.uint8), raw)
     copy([0, page], 0, 1)  # (one page each: one behind the other)
+
+
+@pytest.mark.parametrize("kind", ["q4", "f16", "f32"])
+def test_sizes_beyond_64_bits(ctx, kind):
+    """Pages whose bytes do not fit 64 bits are refused, by every call over pages."""
+    buf = ctx.new_buffer(1 << 16)
+    n = d.launch_count(ctx)
+    for heads, ps in ((1 << 25, 1 << 31), (1 << 31, 1 << 31), (1 << 29, 1 << 27), (1 << 31, 1 << 28)):
+        b = d.PagedBatch(buf, buf.ptr + 256, kind, 1, ps, heads, 256, None, 0, 1, buf)
+        for call in (lambda: d.paged_copy(ctx, b, buf, buf, 1), lambda: d.paged_gather_f32(ctx, b, buf, buf),
+                     lambda: d.rope_kv_append_paged_f32(ctx, b, buf, buf, buf, buf, heads, 1e4),
+                     lambda: d.paged_attention_f32(ctx, b, buf, buf.ptr + 4096, heads)):
+            with pytest.raises(d.Dispatch, match="address space"):
+                call()
+    assert d.launch_count(ctx) == n
