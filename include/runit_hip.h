@@ -795,7 +795,8 @@ int rt_paged_gather_f16(rt_ctx* ctx, const rt_paged_batch* batch, uint16_t* k, u
  * layers; pages of one type, size, number and stride, sequences and tables not looked
  * at), page dst[i] becomes what page src[i] is, i < n ≤ 65,535, as if one after another:
  * chains, cycles and pages written twice included.  src and dst are device arrays; an
- * entry with an id ≥ num_pages copies nothing.  No two pools may overlap. */
+ * entry with an id ≥ num_pages copies nothing.  A page has less than 2^31 bytes; no
+ * two pools may overlap. */
 int rt_paged_copy(rt_ctx* ctx, const rt_paged_batch* batches, uint32_t n_batches,
                   const uint32_t* src, const uint32_t* dst, uint32_t n);
 /* Rules on logits (new; the reference's sampler has none).  Row r's list of tokens is

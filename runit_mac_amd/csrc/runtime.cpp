@@ -4400,16 +4400,14 @@ int rt_paged_copy(rt_ctx* c, const rt_paged_batch* batches, uint32_t n_batches, 
     if (page * el > 0x7fffffffu)
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: pages of %llu bytes",
                     (unsigned long long)(page * el));
-    a.src = src, a.dst = dst, a.n = n, a.num_pages = b.num_pages;
+    a.num_pages = b.num_pages;
     a.page_stride = stride * el;
     a.page_bytes = (uint32_t)(page * el);
     a.slices = (a.page_bytes + RT_COPY_SLICE - 1) / RT_COPY_SLICE;
     a.slice_bytes = ((a.page_bytes + a.slices - 1) / a.slices + 15) / 16 * 16;
-    // (2^32 threads a launch; its pools are arguments)
-    if ((uint64_t)n * a.slices > 0xffffffu)
-        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: paged_copy: %u pages of %u bytes are too many", n,
-                    a.page_bytes);
-    const uint32_t most = std::min(RT_COPY_POOLS, 0xffffffu / (std::min(n, RT_COPY_LIST) * a.slices));
+    // entries and pools of a launch (2^32 threads; its pools are arguments; pages are 2^17 slices at most)
+    const uint32_t list = std::min({n, RT_COPY_LIST, 0xffffffu / a.slices});
+    const uint32_t most = std::min(RT_COPY_POOLS, 0xffffffu / (list * a.slices));
     for (uint64_t p = 0; p < 2ull * n_batches; p += most) {
         const uint32_t k = (uint32_t)std::min<uint64_t>(most, 2ull * n_batches - p);
         for (uint32_t i = 0; i < k; ++i) {
@@ -4418,8 +4416,8 @@ int rt_paged_copy(rt_ctx* c, const rt_paged_batch* batches, uint32_t n_batches, 
         }
         a.n_pools = k;
         a.group = a.slices > 1 ? 1 : std::min(k, RT_COPY_SLICE / a.slice_bytes);
-        for (uint32_t e = 0; e < n; e += RT_COPY_LIST) {
-            a.src = src + e, a.dst = dst + e, a.n = std::min(RT_COPY_LIST, n - e);
+        for (uint32_t e = 0; e < n; e += list) {
+            a.src = src + e, a.dst = dst + e, a.n = std::min(list, n - e);
             void* params[] = {&a};
             const int st = launch(c, a.group > 1 ? "k_paged_copy_small" : "k_paged_copy", dim3(a.n * a.slices, (k + a.group - 1) / a.group), dim3(256), 0, params);
             if (st != RT_OK) return st;

@@ -217,3 +217,32 @@ def test_sizes_beyond_64_bits(ctx, kind):
             with pytest.raises(d.Dispatch, match="address space"):
                 call()
     assert d.launch_count(ctx) == n
+
+
+@pytest.mark.parametrize("n", [32_767, 40_000])
+def test_long_lists_of_large_pages(ctx, n):
+    """Pages of 8 MB (512 workgroups each), most entries without one."""
+    p = Pools(ctx, "f32", 2, 16384, 64, 4, 1, seed=n)
+    src, dst = np.full(n, 0xFFFFFFFF, np.uint32), np.zeros(n, np.uint32)
+    for at, s, t in ((7, 0, 1), (1023, 1, 2), (1024, 2, 0), (n - 1, 3, 2)):
+        src[at], dst[at] = s, t
+    p.copy(src, dst)
+    p.check()
+
+
+def test_lists_of_the_largest_pages(ctx):
+    """Pages of 1.2 GB are 73,728 workgroups' each: fewer entries a launch."""
+    p = d.PagedBatch.page_bytes("q4", 1, 1 << 25, 64)
+    bufs = [ctx.new_buffer(2 * p) for _ in range(2)]
+    rows = np.random.default_rng(1).integers(0, 256, (2, 1 << 20), np.uint8)
+    for b, r in zip(bufs, rows):
+        b.write(r), b.write(r[::-1], p - r.size)
+    batch = d.PagedBatch(*bufs, "q4", 2, 1 << 25, 1, 64, None, 0, 0, None)
+    n, src = d.launch_count(ctx), np.full(300, 0xFFFFFFFF, np.uint32)
+    src[299] = 0
+    d.paged_copy(ctx, batch, ctx.buffer_from(src), ctx.buffer_from(np.ones(300, np.uint32)), 300)
+    ctx.flush()
+    assert d.launch_count(ctx) == n + 4  # (2^24 workgroups: 227 entries of a pool)
+    for b, r in zip(bufs, rows):
+        assert np.array_equal(b.read(np.uint8, r.size, p), r) and np.array_equal(b.read(np.uint8, r.size, 2 * p - r.size), r[::-1])
+        b.free()
