@@ -349,7 +349,7 @@ struct Q4Stage {
 };
 template <int HD>
 struct PagedWave<HD, Q4> {
-    static constexpr uint32_t LDS = Q4Stage<HD>::N * Q4Stage<HD>::LEN / 4, BATCH = 16;
+    static constexpr uint32_t LDS = Q4Stage<HD>::N * Q4Stage<HD>::LEN / 4;
     static constexpr bool HALF = true, MAY_NOTE = true;
     static_assert(LDS >= 16 * (HD + 4), "the outputs fit");
 };

@@ -129,13 +129,12 @@ RT_DEV void paged_gather(const PagedGatherArgs& a, const Load& load) {
 template <bool WIDE>
 constexpr uint32_t paged_slot_rows() { return WIDE ? RT_PAGED_WIDE_ROWS : RT_PAGED_ROWS; }
 
-// A wave of a narrow block: its LDS (its columns' outputs, before them what it likes), in floats; chunks
-// that meet at a time.
+// A wave of a narrow block: its LDS (its columns' outputs, before them what it likes), in floats.
 // (HALF: blocks of eight columns or less are computed as eight, in lanes c and c + 8; MAY_NOTE: whether
 // chunks meet in a launch of their own is the host's choice)
 template <int HD, class T>
 struct PagedWave {
-    static constexpr uint32_t LDS = 16 * (HD + 4), BATCH = 16;
+    static constexpr uint32_t LDS = 16 * (HD + 4);
     static constexpr bool HALF = false, MAY_NOTE = false;
 };
 
@@ -824,7 +823,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
     // than 24, the last of each group of about √chunks those of the group first.
     // All loads of sixteen chunks are in flight at once.
     __shared__ uint32_t turn;
-    constexpr uint32_t PW = HD / 2, PT = 16 * PW / (64 * NW), BATCH = PagedWave<HD, T>::BATCH;  // pairs a row, a thread; chunks at a time
+    constexpr uint32_t PW = HD / 2, PT = 16 * PW / (64 * NW), BATCH = 16;  // pairs a row, a thread; chunks at a time
     __shared__ float mc[BATCH][16], lc[BATCH][16];
     auto last_of = [&](uint32_t* counter, uint32_t n) {
         dev_stores_done();
@@ -847,7 +846,7 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
             uint64_t x[PT][BATCH];
             const uint32_t mk = tid & 15, my = tid >> 4;
             uint64_t ml = pair_of(NEG, 0.0f);
-            if (my < BATCH && x0 + my < n && mk < ncl) ml = dev_load((const uint64_t*)a.ml + slot_of(at + (x0 + my) * step) + mk);
+            if (x0 + my < n && mk < ncl) ml = dev_load((const uint64_t*)a.ml + slot_of(at + (x0 + my) * step) + mk);
 #pragma unroll
             for (uint32_t u = 0; u < PT; ++u)
                 if (256 * u < items) {
@@ -857,10 +856,8 @@ RT_DEV void paged_narrow(const PagedAttnArgs& a, const PagedCols<HD, T>& co, con
                         if (x0 + y < n) x[u][y] = dev_load((const uint64_t*)(a.part + slot_of(at + (x0 + y) * step) * HD) + i);
                 }
             if (x0) __syncthreads();
-            if (my < BATCH) {
-                mc[my][mk] = pair_lo(ml);
-                lc[my][mk] = pair_hi(ml);
-            }
+            mc[my][mk] = pair_lo(ml);
+            lc[my][mk] = pair_hi(ml);
             __syncthreads();
 #pragma unroll
             for (uint32_t u = 0; u < PT; ++u)
