@@ -801,9 +801,8 @@ int rt_paged_copy(rt_ctx* ctx, const rt_paged_batch* batches, uint32_t n_batches
                   const uint32_t* src, const uint32_t* dst, uint32_t n);
 /* Rules on logits (new; the reference's sampler has none).  Row r's list of tokens is
  * tokens[token_start[r]] .. token_len[r] of them, the first prompt_len[r] (NULL: 0) of
- * its prompt; its biases likewise.  Lists may overlap and are cut at n_tokens and n_bias, a
- * row's at 2^31 − 1 entries; ids ≥ n are passed over.  A token that is c times in the list, c' times
- * behind the prompt:
+ * its prompt; its biases likewise.  Lists may overlap and are cut at n_tokens and n_bias;
+ * ids ≥ n are passed over.  A token that is c times in the list, c' times behind the prompt:
  *   x → (c > 0: x > 0 ? x / repetition : x · repetition) − frequency · c'
  *         − (c' > 0 ? presence : 0) + Σ bias,
  * in f32, rounded once; then −inf if the row has a mask without the token's bit (bit t % 32 of

@@ -90,8 +90,7 @@ RT_DEV void adjust_logits(const RulesArgs& a) {
     }
     auto list = [&](const uint32_t* start, const uint32_t* len, uint64_t n, uint64_t& at) {
         at = start[row];
-        // (2^31 − 1 entries at most: their places, some threads' steps on, are within 32 bits, counts within 31)
-        return at < n ? min((uint32_t)min((uint64_t)len[row], n - at), 0x7fffffffu) : 0u;
+        return at < n ? (uint32_t)min((uint64_t)len[row], n - at) : 0u;
     };
     uint64_t ta = 0, ba = 0;
     const uint32_t nt = a.tokens ? list(a.token_start, a.token_len, a.n_tokens, ta) : 0;
