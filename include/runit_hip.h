@@ -810,11 +810,11 @@ int rt_paged_copy(rt_ctx* ctx, const rt_paged_batch* batches, uint32_t n_batches
  * are device arrays, NULL with n_tokens, n_bias or mask_rows 0. */
 typedef struct {
     const uint32_t *tokens, *token_start, *token_len, *prompt_len;
-    uint64_t n_tokens;                               /* elements of tokens */
+    uint64_t n_tokens;                               /* elements of tokens, at most 2^32 − 2^16 */
     const float *repetition, *frequency, *presence;  /* [rows]; NULL: 1, 0, 0 */
     const uint32_t *bias_ids, *bias_start, *bias_len;
     const float* bias;
-    uint64_t n_bias;                                 /* elements of bias_ids and bias */
+    uint64_t n_bias;                                 /* of bias_ids and bias, likewise */
     const uint32_t *mask, *mask_row;                 /* [mask_rows][mask_stride], [rows] */
     uint64_t mask_stride;                            /* words; 0: ceil(n / 32) */
     uint32_t mask_rows;

@@ -4450,6 +4450,10 @@ static int adjust_logits(rt_ctx* c, const char* type, uint32_t el, const void* x
     if (r->n_bias && (!r->bias_ids || !r->bias || !r->bias_start || !r->bias_len))
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: %llu biases in no list",
                     (unsigned long long)r->n_bias);
+    // (places within a list step on by some thousands in 32 bits)
+    if (std::max(r->n_tokens, r->n_bias) > 0xffff0000u)
+        return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: %llu tokens, %llu biases are too many",
+                    (unsigned long long)r->n_tokens, (unsigned long long)r->n_bias);
     const uint64_t words = ((uint64_t)n + 31) / 32, stride = r->mask_stride ? r->mask_stride : words;
     if (r->mask_rows && (!r->mask || stride < words))
         return fail(c, RT_ERR_DISPATCH, "kernel dispatch error: adjust_logits: %u masks, %llu of %llu words each",

@@ -324,3 +324,23 @@ def test_refusals(ctx):
     n = d.launch_count(ctx)
     d.adjust_logits_f32(ctx, None, None, 0, 64, rules.upload(ctx))
     assert d.launch_count(ctx) == n
+
+
+@pytest.mark.parametrize("n", [0xFFFF0001, 0xFFFFFFFF, 1 << 32, 1 << 40])
+def test_lists_of_almost_32_bits(ctx, n):
+    """Refused: places within them are 32-bit numbers that step on by thousands."""
+    buf = ctx.buffer_from(np.zeros(64, np.float32))
+    before = d.launch_count(ctx)
+    for kw in (dict(tokens=buf, n_tokens=n, token_start=buf, token_len=buf),
+               dict(bias_ids=buf, bias=buf, n_bias=n, bias_start=buf, bias_len=buf)):
+        for call in (d.adjust_logits_f32, d.adjust_logits_f16):
+            with pytest.raises(d.Dispatch, match="too many"):
+                call(ctx, buf, buf, 1, 16, d.LogitRules(**kw))
+    assert d.launch_count(ctx) == before
+    # (the most that there may be, of which the list takes four)
+    x = ctx.buffer_from(np.zeros(16, np.float32))
+    u = lambda *v: ctx.buffer_from(np.array(v, np.uint32))
+    d.adjust_logits_f32(ctx, x, x, 1, 16, d.LogitRules(tokens=u(3, 4, 3, 9), n_tokens=0xFFFF0000, token_start=u(0), token_len=u(4),
+                                                       frequency=ctx.buffer_from(np.ones(1, np.float32))))
+    ctx.flush()
+    assert list(x.read(np.float32)) == [0, 0, 0, -2, -1, 0, 0, 0, 0, -1, 0, 0, 0, 0, 0, 0]
