@@ -4355,6 +4355,9 @@ int rt_paged_gather_f16(rt_ctx* c, const rt_paged_batch* batch, uint16_t* k, uin
 // turns are apart where the one's begin in the other's gaps.)  In order of their addresses.
 static bool pools_apart(const std::vector<uintptr_t>& pools, uint64_t page, uint64_t stride, uint32_t n) {
     const uint64_t span = (n - 1) * stride + page;
+    bool behind = true;  // (each begins where the one before has ended: no quotients needed)
+    for (size_t i = 1; i < pools.size(); ++i) behind &= pools[i] - pools[i - 1] >= span;
+    if (behind) return true;
     std::vector<uint64_t> in(pools.size());  // from a page's beginning of the first pool on
     for (size_t i = 0; i < pools.size(); ++i) in[i] = (pools[i] - pools[0]) % stride;
     for (size_t i = 0; i < pools.size(); ++i)
