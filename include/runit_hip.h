@@ -763,7 +763,8 @@ typedef struct {
  * [rows][num_kv_heads][head_dim] at the rows' positions (pairs (d, d +
  * head_dim/2), the angles reduced in 64 bits), k and v (as k) stored into the
  * pages (f16: rounded to nearest even; 4 bits: as above).  Rows that several sequences store in one place
- * leave either's elements there: a shared page is copied before it is written. */
+ * leave either's elements there (4 bits: of a group either's codes and either's scale word): a
+ * shared page is copied before it is written. */
 int rt_rope_kv_append_paged_f32(rt_ctx* ctx, const rt_paged_batch* batch, const float* q,
                                 const float* k, const float* v, float* q_out, uint32_t num_heads,
                                 float theta);
@@ -805,9 +806,9 @@ int rt_paged_copy(rt_ctx* ctx, const rt_paged_batch* batches, uint32_t n_batches
  * ids ≥ n are passed over.  A token that is c times in the list, c' times behind the prompt:
  *   x → (c > 0: x > 0 ? x / repetition : x · repetition) − frequency · c'
  *         − (c' > 0 ? presence : 0) + Σ bias,
- * in f32, rounded once; then −inf if the row has a mask without the token's bit (bit t % 32 of
- * word t / 32).  mask_row[r] (NULL: r) is the row's mask; none if ≥ mask_rows.  All pointers
- * are device arrays, NULL with n_tokens, n_bias or mask_rows 0. */
+ * in f32 (f16 logits: rounded to f16 at the end); then −inf if the row has a mask without
+ * the token's bit (bit t % 32 of word t / 32).  mask_row[r] (NULL: r) is the row's mask; none
+ * if ≥ mask_rows.  All pointers are device arrays, NULL with n_tokens, n_bias or mask_rows 0. */
 typedef struct {
     const uint32_t *tokens, *token_start, *token_len, *prompt_len;
     uint64_t n_tokens;                               /* elements of tokens, at most 2^32 − 2^16 */

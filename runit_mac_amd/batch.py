@@ -185,9 +185,10 @@ class _Sequence:
 
 class BatchDecoder:
     """`max_seqs` sequences of up to `max_len` positions over `num_pages` pages
-    of `page_size` positions (f16, f32 or, q4, 4 bits) a layer; passes of up to `max_rows`
-    rows, the logits of up to `max_logits` of them at once, up to `max_top`
-    alternatives.  Longer prompts run in several passes."""
+    of `page_size` positions (f16, f32 or, q4, 4 bits: less memory, faster decoding over long
+    contexts, prompts a little slower) a layer; passes of up to `max_rows` rows, the logits
+    of up to `max_logits` of them at once, up to `max_top` alternatives.  Longer prompts run
+    in several passes."""
 
     def __init__(self, model: DecodeModel, max_seqs: int, num_pages: int, page_size: int = 64,
                  kv: str = "f16", max_len: int | None = None, max_rows: int = 512,

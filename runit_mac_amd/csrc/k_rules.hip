@@ -4,7 +4,7 @@
 // Of a token that its row's list has c times, c' of them behind the prompt, and
 // whose biases sum to b:
 //   x → (c > 0: x > 0 ? x / rep : x·rep) − freq·c' − (c' > 0 ? pres : 0) + b,
-// −∞ where the row's mask has no bit for it; in f32, rounded once.
+// −∞ where the row's mask has no bit for it; in f32, f16 logits rounded to f16 at the end.
 //
 // A workgroup has RT_RULES_SEG tokens of a row.  Its logits are on their way (where
 // all are copied) while it counts the list's tokens among its own in LDS (whole
@@ -14,7 +14,7 @@
 //
 // Bound by the logits' bytes: 120 rows of 152,064 f32 with histories of up to 9,000
 // tokens, up to 300 biases and masks 33.7 µs for 147 MB (4.4 TB/s; a large copy makes
-// 5.1; without lists 29).  Few rows: by trips to memory, 5 rows 3.7 µs, 4.4 a call.  4,096
+// 5.1; without lists 29).  Few rows: by trips to memory, 5 rows 4.1 µs, 4.4 a call.  4,096
 // tokens and 512 threads: with 256 threads 39 µs, with 8,192 tokens 41, one thread
 // adding all biases of its token one after another 68.
 #include "rt_attn.h"

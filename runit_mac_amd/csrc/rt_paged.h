@@ -60,7 +60,10 @@ RT_DEV void paged_turns(uint32_t pos, double log2_theta, float* cs, float* sn) {
 }
 
 // The rows' keys and values as they are in the pages, four elements a thread; zeros
-// where a row has no place.  load(page, KV head, slot, whether a value, first element).
+// where a row has no place.  load(page, KV head, slot, whether a value, first element).  Bound by the
+// trips to memory one behind the other (row starts, length, page id, elements), of which a workgroup
+// has few bytes: 2,068 rows of 4 KV heads of 128 as f16 4.8 µs from f16 pages (8.5 MB, 1.8 TB/s), 4.9 from f32 (13) and
+// from 4 bits (5.4); as f32 6.2–6.5.  Few rows 2 µs, a launch.
 template <class O, class Load>
 RT_DEV void paged_gather(const PagedGatherArgs& a, const Load& load) {
     typedef O o4_t __attribute__((ext_vector_type(4)));
