@@ -11,6 +11,7 @@ choice.
 """
 from __future__ import annotations
 
+from ctypes import c_float
 from dataclasses import dataclass
 
 import numpy as np
@@ -19,6 +20,7 @@ from . import dispatch as d
 from .decode import Arena, DecodeModel, accept_drafts
 
 NO_PAGE = 0xFFFFFFFF
+NO_BIASES = np.zeros(0, np.int64), np.zeros(0, np.float32)
 
 
 class PagePool:
@@ -96,31 +98,32 @@ class Rules:
 
     def checked(self, vocab: int) -> "Rules":
         rep, freq, pres = self.penalties()
-        if not 0 < rep < np.inf or not np.isfinite([freq, pres]).all():
+        if not (0 < rep < np.inf and abs(freq) < np.inf and abs(pres) < np.inf):
             raise ValueError(f"rules: penalties {self.repetition}, {self.frequency}, {self.presence}")
         if not self.prompt_len >= 0 or self.prompt_len % 1:
             raise ValueError(f"rules: prompt_len {self.prompt_len}")
         if any(not 0 <= t < vocab or t % 1 for t in self.bias or ()):
             raise ValueError(f"rules: a bias's token is none of [0, {vocab})")
-        ids, bias = self.biases()
-        if np.isnan(bias).any():
-            raise ValueError("rules: a bias is NaN")
-        left = np.ones(vocab, bool)
-        if self.allowed is not None:
-            left = np.unpackbits(np.ascontiguousarray(self.mask(vocab)).view(np.uint8), bitorder="little")[:vocab] > 0
-        left[ids[bias == -np.inf]] = False
-        if not left.any():
+        left = self.left(vocab) if self.allowed is not None else None
+        if self.bias:
+            ids, bias = self.biases()
+            if np.isnan(bias).any():
+                raise ValueError("rules: a bias is NaN")
+            never = ids[bias == -np.inf]
+            if never.size:
+                left = np.ones(vocab, bool) if left is None else left.copy()
+                left[never] = False
+        if left is not None and not left.any():
             raise ValueError("rules: no token is allowed")
         return self
 
-    def penalties(self) -> np.ndarray:
-        """Repetition, frequency and presence in the 32 bits that the device has."""
-        with np.errstate(over="ignore", under="ignore"):
-            return np.array([self.repetition, self.frequency, self.presence], np.float64).astype(np.float32)
+    def penalties(self) -> tuple:
+        """Repetition, frequency and presence as the 32-bit numbers that they become."""
+        return tuple(c_float(x).value for x in (self.repetition, self.frequency, self.presence))
 
     def penalises(self) -> bool:
         """Whether the sequence's tokens change anything."""
-        return not np.array_equal(self.penalties(), [1, 0, 0])
+        return self.penalties() != (1, 0, 0)
 
     def biases(self) -> tuple[np.ndarray, np.ndarray]:
         """The biases' tokens and, in 32 bits, values."""
@@ -135,14 +138,22 @@ class Rules:
         off = a is not None and not (a[token] if a.dtype == bool else a[token // 32] >> token % 32 & 1)
         return bool(off or np.any(bias[ids == token] == -np.inf))
 
+    def left(self, vocab: int) -> np.ndarray:
+        """The mask's tokens as [vocab] truth values."""
+        a, words = np.asarray(self.allowed), -(-vocab // 32)
+        if a.dtype == np.uint32 and a.shape == (words,):
+            return np.unpackbits(np.ascontiguousarray(a).view(np.uint8), bitorder="little")[:vocab].view(bool)
+        if a.dtype != bool or a.shape != (vocab,):
+            raise ValueError(f"rules: allowed is neither {vocab} truth values nor {words} u32 words")
+        return a
+
     def mask(self, vocab: int) -> np.ndarray:
+        """The mask's tokens as bits in u32 words."""
         a, words = np.asarray(self.allowed), -(-vocab // 32)
         if a.dtype == np.uint32 and a.shape == (words,):
             return a
-        if a.dtype != bool or a.shape != (vocab,):
-            raise ValueError(f"rules: allowed is neither {vocab} truth values nor {words} u32 words")
         bits = np.zeros(32 * words, bool)
-        bits[:vocab] = a
+        bits[:vocab] = self.left(vocab)
         return np.packbits(bits, bitorder="little").view(np.uint32)
 
 
@@ -529,7 +540,8 @@ class BatchDecoder:
         vocab, n = self.model.cfg.vocab, len(rows)
         rules = [r[0] if r else Rules() for r in rows]
         lists = [(r[1] if r else _Tokens()).ids for r in rows]
-        biases, penalties = [r.biases() for r in rules], np.stack([r.penalties() for r in rules]).view(np.uint32)
+        penalties = np.array([r.penalties() for r in rules], np.float32).view(np.uint32)
+        ids, biases = zip(*(r.biases() if r.bias else NO_BIASES for r in rules))
         masks = [r.mask(vocab) for r in rules if r.allowed is not None]
         starts = lambda x: np.concatenate([[0], np.cumsum([len(v) for v in x])[:-1]])
         u32 = lambda v: np.asarray(v, np.int64).astype(np.uint32)
@@ -537,8 +549,8 @@ class BatchDecoder:
             tokens=np.concatenate(lists), token_start=u32(starts(lists)), token_len=u32([len(v) for v in lists]),
             prompt_len=u32([min(r.prompt_len, 0xFFFFFFFF) for r in rules]), repetition=penalties[:, 0],
             frequency=penalties[:, 1], presence=penalties[:, 2],
-            bias_ids=u32(np.concatenate([t for t, _ in biases])), bias=np.concatenate([b for _, b in biases]).view(np.uint32),
-            bias_start=u32(starts([t for t, _ in biases])), bias_len=u32([len(t) for t, _ in biases]),
+            bias_ids=u32(np.concatenate(ids)), bias=np.concatenate(biases).view(np.uint32),
+            bias_start=u32(starts(ids)), bias_len=u32([len(t) for t in ids]),
             mask=np.concatenate(masks) if masks else u32([]),
             mask_row=u32(np.where([r.allowed is not None for r in rules],
                                   np.cumsum([r.allowed is not None for r in rules]) - 1, NO_PAGE)))
