@@ -119,7 +119,7 @@ class Rules:
 
     def penalties(self) -> tuple:
         """Repetition, frequency and presence as the 32-bit numbers that they become."""
-        return tuple(c_float(x).value for x in (self.repetition, self.frequency, self.presence))
+        return c_float(self.repetition).value, c_float(self.frequency).value, c_float(self.presence).value
 
     def penalises(self) -> bool:
         """Whether the sequence's tokens change anything."""
