@@ -350,8 +350,9 @@ class BatchDecoder:
     def step(self, work: dict, top: int | None = None, rules: dict | None = None) -> dict:
         """Appends tokens to sequences ({sequence: tokens}) and returns the
         likeliest next token of each that its `rules` ({sequence: Rules}) leave
-        (ValueError if they leave none with a logit above -inf); with `top`, pairs of it and its TokenScores with that many alternatives,
-        the model's own: without the rules."""
+        (ValueError if they leave none with a logit above -inf); with `top`,
+        pairs of it and its TokenScores with that many alternatives, the model's
+        own: without the rules."""
         work = self._checked(work)
         if any(t.size == 0 for t in work.values()):
             raise ValueError("step: empty sequence of tokens")

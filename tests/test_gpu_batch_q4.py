@@ -233,3 +233,38 @@ def test_rules_leave_no_logit(ctx):
     only.frequency = 1.0
     assert b.step({s: [9, 1], t: [5]}, rules={s: only})[s] == 9
     b.free(), m.free()
+
+
+@pytest.mark.parametrize("kv", ["q4", "f16"])
+@pytest.mark.parametrize("turned", [False, True])
+def test_forks_of_unequal_length_after_a_failure(ctx, kv, turned, monkeypatch):
+    """A fork that was trimmed and its origin write to the page that both hold, and the
+    call's last pass fails: both hold what they held, and go on."""
+    m = DecodeModel(ctx, DecodeConfig(**TINY), seed=71)
+    b = BatchDecoder(m, 2, 20, 16, kv=kv, max_rows=8)
+    rng = np.random.default_rng(72)
+    tokens = lambda n: rng.integers(m.cfg.vocab, size=n)
+    s = b.open()
+    b.step({s: tokens(28)})
+    t = b.fork(s)
+    b.trim(t, 20)
+    before, free = {(x, i): held(b, x, i) for x in (s, t) for i in range(m.cfg.layers)}, b.pool.free
+    same = lambda: all(np.array_equal(y, z[:len(y)]) for (x, i), kv in before.items() for y, z in zip(kv, held(b, x, i)))
+    work = {s: tokens(3), t: tokens(10)}
+    work = dict(reversed(work.items())) if turned else work
+    launch, left = b._launch, [1]
+
+    def failing(*args):
+        if left[0] == 0:
+            raise d.Dispatch("kernel dispatch error: none")
+        left[0] -= 1
+        return launch(*args)
+
+    monkeypatch.setattr(b, "_launch", failing)
+    with pytest.raises(d.Dispatch):
+        b.step(work)
+    assert b.length(s) == 28 and b.length(t) == 20 and b.pool.free == free and same()
+    left[0] = 9
+    b.step(work)
+    assert b.length(s) == 31 and b.length(t) == 30 and same()
+    b.free(), m.free()
